@@ -450,6 +450,87 @@ NF4_API int32_t nf4_peer_arrivals_wait_dev(uint32_t *own_arrivals, uint32_t expe
 NF4_API uint64_t nf4_linear_noalloc_scratch_bytes(void);
 NF4_API int32_t nf4_linear_forward_noalloc_dev(const nf4_linear_args *args, void *stream);
 
+/* ------------------------------------------------- key and value cache -- */
+
+/* A paged cache of a decoder layer's keys and values, beside the quantized projections that make
+ * them.  A page holds `page_size` tokens of every head; which pages a sequence has, and in which order, says
+ * nf4_cache_batch.page_table.  The reference's NF4 path has no counterpart.
+ *   NF4_CACHE_BF16  k, v [num_pages, heads, page_size, head_dim] bf16
+ *   NF4_CACHE_NF4   k, v [num_pages, heads, page_size, head_dim / 2] packed codes, and a scale for every 64 values of
+ *                   a row in k_scales, v_scales [num_pages, heads, page_size, head_dim / 64]: the form and the
+ *                   arithmetic of nf4_quantize_dev (4.5 bits a value), bit for bit.
+ * head_dim is 64, 128 or 256; page_size a multiple of 16, at most 65536; the pools are 16-byte aligned. */
+#define NF4_CACHE_BF16 0
+#define NF4_CACHE_NF4 1
+typedef struct nf4_cache {
+    uint32_t struct_bytes;      /* sizeof(nf4_cache), checked */
+    int32_t form;               /* NF4_CACHE_* */
+    uint32_t num_pages;
+    uint32_t page_size;
+    uint32_t heads;             /* heads of keys and values */
+    uint32_t head_dim;
+    void *k, *v;
+    float *k_scales, *v_scales; /* NULL for NF4_CACHE_BF16 */
+} nf4_cache;
+
+/* The sequences of a call and the rows of its tensors that belong to them.  Rows row_starts[s] ...
+ * row_starts[s + 1] - 1 are the NEWEST tokens of sequence s, which has lengths[s] tokens in the cache with them: row i
+ * of n is token lengths[s] - n + i.  Token t is at place t % page_size of page page_table[s][t / page_size].
+ * page_table, lengths and row_starts are device memory and may be changed between launches of a captured
+ * graph; row_starts does not decrease.  Whatever stands in them, no access leaves the buffers: lengths beyond the table's
+ * pages and row_starts beyond `rows` are cut there.  Rows that belong to no sequence are neither read nor written.
+ * Sequences may share pages (a common prefix); a token that a call appends is in a page of its sequence alone. */
+typedef struct nf4_cache_batch {
+    uint32_t struct_bytes;      /* sizeof(nf4_cache_batch), checked */
+    uint32_t sequences;
+    const int32_t *page_table;  /* [sequences, pages_per_sequence] */
+    const int32_t *lengths;     /* [sequences] */
+    const int32_t *row_starts;  /* [sequences + 1] */
+    uint32_t pages_per_sequence;
+    uint32_t rows;              /* rows of the call's tensors */
+    uint32_t max_rows;          /* most rows of a sequence and most tokens of one, as far as the host knows; 0: it does */
+    uint32_t max_length;        /* not.  They choose kernels and how work is shared out, and bound nothing. */
+} nf4_cache_batch;
+
+/* Writes the rows' keys and values, k and v [rows, heads, head_dim] of io_dtype with ldk and ldv elements from row to row
+ * (0: heads * head_dim), to their places.  NF4_CACHE_NF4 quantizes as it writes; NF4_CACHE_BF16 rounds f32 once.  A row whose
+ * token is negative, or in a page outside [0, num_pages), is not written.  16-byte aligned, the row strides too. */
+NF4_API int32_t nf4_cache_append_dev(const nf4_cache *cache, const nf4_cache_batch *batch, const void *k, uint64_t ldk,
+                                     const void *v, uint64_t ldv, int32_t io_dtype, void *stream);
+
+/* The rows' keys and values as they stand in the cache, dense: k and v [rows, heads, head_dim] of io_dtype (bf16: the f32
+ * value rounded once).  A row whose token is negative, or in a page outside [0, num_pages), becomes NaNs. */
+NF4_API int32_t nf4_cache_read_dev(const nf4_cache *cache, const nf4_cache_batch *batch, void *k, uint64_t ldk, void *v,
+                                   uint64_t ldv, int32_t io_dtype, void *stream);
+
+/* Attention of a call's rows over the cache, which holds their own keys and values already:
+ *     out[i] = sum_t p_it v_t,  p_i = softmax over t <= token of row i of (scale * q_i . k_t),
+ * q and out [rows, q_heads, head_dim] of io_dtype with ldq and ldo elements from row to row (0: q_heads * head_dim).  Query head
+ * h reads head h / (q_heads / heads) of the cache.  A row whose token is negative sees nothing and becomes zeros; a
+ * row that sees a token in a page outside [0, num_pages) becomes NaNs (others of its sequence may, too).  Values of the tokens
+ * that a call's rows see are finite; what stands in other places of their pages does not matter.  One token to a sequence, drafted
+ * tokens, chunks of a prompt and whole prompts are the same call.
+ * bf16 tensors multiply on the tensor cores with f32 sums; f32 tensors in f32 throughout.
+ * workspace: nf4_cache_attention_workspace_bytes() bytes, 256-byte aligned, the first nf4_cache_attention_flag_bytes() of
+ * them zero at the first use; every call leaves them zero.  One workspace serves one stream. */
+typedef struct nf4_attention_args {
+    uint32_t struct_bytes;      /* sizeof(nf4_attention_args), checked */
+    int32_t io_dtype;
+    uint32_t q_heads;           /* a multiple of the cache's heads */
+    float scale;
+    const void *q;
+    uint64_t ldq;
+    void *out;
+    uint64_t ldo;
+    void *workspace;
+    uint64_t workspace_bytes;
+} nf4_attention_args;
+NF4_API uint64_t nf4_cache_attention_workspace_bytes(const nf4_cache *cache, const nf4_cache_batch *batch, uint32_t q_heads,
+                                                     int32_t io_dtype);
+NF4_API uint64_t nf4_cache_attention_flag_bytes(void);
+NF4_API int32_t nf4_cache_attention_dev(const nf4_cache *cache, const nf4_cache_batch *batch, const nf4_attention_args *args,
+                                        void *stream);
+
 /* ------------------------------------------------ resident weight handles -- */
 
 /* An NF4 weight resident in device memory (what Nf4Linear holds in `packed`,

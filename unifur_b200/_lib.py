@@ -16,6 +16,8 @@ LAYOUT_OUT_IN = 0
 LAYOUT_IN_OUT = 1
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
+CACHE_BF16 = 0
+CACHE_NF4 = 1
 
 
 class Nf4Error(RuntimeError):
@@ -59,6 +61,27 @@ class LinearArgs(C.Structure):
         ("workspace", C.c_void_p),
         ("workspace_bytes", C.c_uint64),
     ]
+
+
+class Cache(C.Structure):
+    """``nf4_cache`` (include/nf4_b200.h)."""
+    _fields_ = [("struct_bytes", C.c_uint32), ("form", C.c_int32), ("num_pages", C.c_uint32), ("page_size", C.c_uint32),
+                ("heads", C.c_uint32), ("head_dim", C.c_uint32), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("k_scales", C.c_void_p), ("v_scales", C.c_void_p)]
+
+
+class CacheBatch(C.Structure):
+    """``nf4_cache_batch`` (include/nf4_b200.h)."""
+    _fields_ = [("struct_bytes", C.c_uint32), ("sequences", C.c_uint32), ("page_table", C.c_void_p), ("lengths", C.c_void_p),
+                ("row_starts", C.c_void_p), ("pages_per_sequence", C.c_uint32), ("rows", C.c_uint32), ("max_rows", C.c_uint32),
+                ("max_length", C.c_uint32)]
+
+
+class AttentionArgs(C.Structure):
+    """``nf4_attention_args`` (include/nf4_b200.h)."""
+    _fields_ = [("struct_bytes", C.c_uint32), ("io_dtype", C.c_int32), ("q_heads", C.c_uint32), ("scale", C.c_float),
+                ("q", C.c_void_p), ("ldq", C.c_uint64), ("out", C.c_void_p), ("ldo", C.c_uint64), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_uint64)]
 
 
 _vp, _u64, _i32, _u32, _f32 = C.c_void_p, C.c_uint64, C.c_int32, C.c_uint32, C.c_float
@@ -118,6 +141,11 @@ SIGNATURES = {
     "nf4_peer_arrivals_wait_dev": (_i32, [_vp, _u32, _u32, _vp]),
     "nf4_peer_push_columns_dev": (_i32, [C.POINTER(PeerOutputs), _u64, _u64, _i32, _vp, _vp]),
     "nf4_linear_forward_noalloc_dev": (_i32, [C.POINTER(LinearArgs), _vp]),
+    "nf4_cache_append_dev": (_i32, [C.POINTER(Cache), C.POINTER(CacheBatch), _vp, _u64, _vp, _u64, _i32, _vp]),
+    "nf4_cache_read_dev": (_i32, [C.POINTER(Cache), C.POINTER(CacheBatch), _vp, _u64, _vp, _u64, _i32, _vp]),
+    "nf4_cache_attention_workspace_bytes": (_u64, [C.POINTER(Cache), C.POINTER(CacheBatch), _u32, _i32]),
+    "nf4_cache_attention_flag_bytes": (_u64, []),
+    "nf4_cache_attention_dev": (_i32, [C.POINTER(Cache), C.POINTER(CacheBatch), C.POINTER(AttentionArgs), _vp]),
     "nf4_weight_from_values_host": (_i32, [_vp, _u64, _u64, _i32, _i32, C.POINTER(_vp)]),
     "nf4_weight_from_packed_host": (_i32, [_vp, _vp, _vp, _f32, _u64, _u64, _i32,
                                            C.POINTER(_vp)]),

@@ -23,6 +23,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -139,8 +140,8 @@ bool capturing(cudaStream_t s) {
     return cudaStreamIsCapturing(s, &st) == cudaSuccess && st != cudaStreamCaptureStatusNone;
 }
 
-void zero_flags(const Tensor &ws, const Place &at_) {
-    if (cudaMemsetAsync(ws.mutable_data_ptr(), 0, 256, at_.stream) != cudaSuccess)
+void zero_flags(const Tensor &ws, const Place &at_, uint64_t flags = 256) {
+    if (cudaMemsetAsync(ws.mutable_data_ptr(), 0, flags, at_.stream) != cudaSuccess)
         throw std::runtime_error("clearing the workspace's flag words failed");
 }
 
@@ -154,13 +155,14 @@ struct Kept {
 };
 thread_local std::vector<Kept> t_kept;  // most recently used last
 
-// `bytes` of scratch whose first 256 bytes are zero.  `slot`: which of a call's workspaces (the
-// projections of a grouped call have one each).
-Tensor flagged_workspace(uint64_t bytes, const Place &at_, uint32_t slot) {
-    if (bytes < 256) bytes = 256;
+// `bytes` of scratch whose first `flags` bytes are zero.  `slot`: which of a call's workspaces (the
+// projections of a grouped call have one each, attention one of its own: the words at its start are its kernels').
+constexpr uint32_t kAttentionSlot = 4;
+Tensor flagged_workspace(uint64_t bytes, const Place &at_, uint32_t slot, uint64_t flags = 256) {
+    if (bytes < flags) bytes = flags;
     if (bytes > kKeptBytes || capturing(at_.stream)) {
         Tensor ws = empty({(int64_t)bytes}, at::kByte, at_);
-        zero_flags(ws, at_);
+        zero_flags(ws, at_, flags);
         return ws;
     }
     const int dev = at_.device.index();
@@ -177,7 +179,7 @@ Tensor flagged_workspace(uint64_t bytes, const Place &at_, uint32_t slot) {
     uint64_t cap = 1u << 16;
     while (cap < bytes) cap <<= 1;
     Tensor ws = empty({(int64_t)cap}, at::kByte, at_);
-    zero_flags(ws, at_);
+    zero_flags(ws, at_, flags);
     t_kept.push_back(Kept{dev, at_.stream, slot, ws});
     return ws;
 }
@@ -530,6 +532,173 @@ PyObject *embedding(PyObject *, PyObject *const *v, Py_ssize_t n) {
     });
 }
 
+// ---- key and value cache ----------------------------------------------------------------------
+void require(bool ok, const char *msg) {
+    if (!ok) raise(PyExc_ValueError, msg);
+}
+uint32_t word_arg(PyObject *o) {
+    const uint64_t v = size_arg(o);
+    require(v < 1ull << 31, "a size of the cache's call is 2^31 or more");
+    return (uint32_t)v;
+}
+
+// k, v, k_scales, v_scales, page_table, lengths, row_starts, rows, max_rows, max_length
+constexpr Py_ssize_t kCacheArgs = 10;
+struct CacheCall {
+    nf4_cache cache;
+    nf4_cache_batch batch;
+    const Tensor *k;
+};
+CacheCall cache_call(PyObject *const *v) {
+    CacheCall c;
+    std::memset(&c.cache, 0, sizeof(c.cache));
+    std::memset(&c.batch, 0, sizeof(c.batch));
+    const Tensor &k = tensor(v[0]), &vv = tensor(v[1]);
+    const Tensor *ks = tensor_or_none(v[2]), *vs = tensor_or_none(v[3]);
+    const Tensor &table = tensor(v[4]), &lengths = tensor(v[5]), &starts = tensor(v[6]);
+    require_cuda(k, "the cache");
+    const bool packed = k.scalar_type() == at::kByte;
+    require(packed || k.scalar_type() == at::kBFloat16, "the cache's k is uint8 (NF4) or bfloat16");
+    require(k.dim() == 4 && vv.scalar_type() == k.scalar_type() && vv.sizes() == k.sizes(), "the cache's k and v are 4-D and of one shape and type");
+    require(k.is_contiguous() && vv.is_contiguous(), "the cache's k and v must be contiguous");
+    const int64_t dim = k.size(3) * (packed ? 2 : 1);
+    if (packed) {
+        require(ks && vs && ks->scalar_type() == at::kFloat && vs->scalar_type() == at::kFloat, "a quantized cache has f32 k_scales and v_scales");
+        const std::vector<int64_t> shape{k.size(0), k.size(1), k.size(2), dim / NF4_BLOCK_SIZE};
+        require(dim % NF4_BLOCK_SIZE == 0 && ks->sizes() == at::IntArrayRef(shape) && vs->sizes() == at::IntArrayRef(shape) && ks->is_contiguous() &&
+                    vs->is_contiguous(),
+                "k_scales and v_scales are contiguous and have one scale for every 64 values");
+    } else {
+        require(!ks && !vs, "a bfloat16 cache has no scales");
+    }
+    require(table.scalar_type() == at::kInt && lengths.scalar_type() == at::kInt && starts.scalar_type() == at::kInt,
+            "page_table, lengths and row_starts are int32");
+    require(table.dim() == 2 && lengths.dim() == 1 && starts.dim() == 1 && lengths.size(0) == table.size(0) && starts.size(0) == table.size(0) + 1,
+            "page_table is [sequences, pages], lengths [sequences], row_starts [sequences + 1]");
+    require(table.is_contiguous() && lengths.is_contiguous() && starts.is_contiguous(), "page_table, lengths and row_starts must be contiguous");
+    const c10::Device d = k.device();
+    require(vv.device() == d && (!ks || (ks->device() == d && vs->device() == d)) && table.device() == d && lengths.device() == d && starts.device() == d,
+            "the cache's and the batch's tensors must be on one device");
+    require(k.numel() > 0 && k.size(0) < 1ll << 31 && k.size(1) < 1ll << 31 && k.size(2) < 1ll << 31 && dim < 1ll << 31 && table.size(0) < 1ll << 31 &&
+                table.size(1) < 1ll << 31,
+            "the cache is empty or too large");
+    c.k = &k;
+    c.cache.struct_bytes = sizeof(c.cache);
+    c.cache.form = packed ? NF4_CACHE_NF4 : NF4_CACHE_BF16;
+    c.cache.num_pages = (uint32_t)k.size(0);
+    c.cache.heads = (uint32_t)k.size(1);
+    c.cache.page_size = (uint32_t)k.size(2);
+    c.cache.head_dim = (uint32_t)dim;
+    c.cache.k = k.mutable_data_ptr();
+    c.cache.v = vv.mutable_data_ptr();
+    c.cache.k_scales = ks ? static_cast<float *>(ks->mutable_data_ptr()) : nullptr;
+    c.cache.v_scales = vs ? static_cast<float *>(vs->mutable_data_ptr()) : nullptr;
+    c.batch.struct_bytes = sizeof(c.batch);
+    c.batch.sequences = (uint32_t)table.size(0);
+    c.batch.pages_per_sequence = (uint32_t)table.size(1);
+    c.batch.page_table = ptr_as<int32_t>(&table);
+    c.batch.lengths = ptr_as<int32_t>(&lengths);
+    c.batch.row_starts = ptr_as<int32_t>(&starts);
+    c.batch.rows = word_arg(v[7]);
+    c.batch.max_rows = word_arg(v[8]);
+    c.batch.max_length = word_arg(v[9]);
+    return c;
+}
+
+// Rows of `heads` times the cache's head_dim values; heads 0: as many as there are (query heads).
+struct HeadRows {
+    Tensor t;
+    uint64_t ld;
+    uint32_t heads;
+};
+HeadRows head_rows(const Tensor &t, const CacheCall &c, uint32_t heads, const char *what, bool output) {
+    const int64_t dim = c.cache.head_dim, width = t.dim() == 3 ? t.size(1) * t.size(2) : t.dim() == 2 ? t.size(1) : 0;
+    if ((t.dim() == 3 && t.size(2) != dim) || width == 0 || width % dim != 0 || (heads && width != heads * dim) || t.size(0) != (int64_t)c.batch.rows)
+        raise(PyExc_ValueError, (std::string(what) + " must be [rows, heads, head_dim] or [rows, heads * head_dim]").c_str());
+    if (t.device() != c.k->device()) raise(PyExc_ValueError, (std::string(what) + " must be on the cache's device").c_str());
+    const int64_t whole = 16 / (int64_t)t.element_size();
+    const bool lies = t.numel() == 0 || ((t.dim() == 2 ? t.stride(1) == 1 : t.stride(2) == 1 && (t.size(1) == 1 || t.stride(1) == dim)) &&
+                      (t.size(0) == 1 || (t.stride(0) >= width && t.stride(0) % whole == 0)) && ((uintptr_t)t.const_data_ptr() & 15u) == 0);
+    if (output && !lies) raise(PyExc_ValueError, (std::string(what) + " must have whole, 16-byte aligned rows").c_str());
+    // (a copy starts at an allocation's aligned address, also where t is contiguous at an odd one)
+    HeadRows r{lies ? t : t.clone(at::MemoryFormat::Contiguous), 0, (uint32_t)(width / dim)};
+    r.ld = t.size(0) > 1 ? (uint64_t)r.t.stride(0) : (uint64_t)width;
+    return r;
+}
+
+// cache_append(<cache, batch>, k, v)
+PyObject *cache_append(PyObject *, PyObject *const *v, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        expect(n, kCacheArgs + 2);
+        const CacheCall c = cache_call(v);
+        const Tensor &k = tensor(v[kCacheArgs]), &vv = tensor(v[kCacheArgs + 1]);
+        require(k.scalar_type() == vv.scalar_type(), "k and v must be of one type");
+        const int32_t type = io_dtype(k.scalar_type());
+        Place place(c.k->device());
+        const HeadRows rk = head_rows(k, c, c.cache.heads, "k", false), rv = head_rows(vv, c, c.cache.heads, "v", false);
+        const void *pk = rk.t.const_data_ptr(), *pv = rv.t.const_data_ptr();
+        check(unlocked([&] { return nf4_cache_append_dev(&c.cache, &c.batch, pk, rk.ld, pv, rv.ld, type, place.stream); }));
+        Py_RETURN_NONE;
+    });
+}
+
+// cache_read(<cache, batch>, dtype, k or None, v or None) -> (k, v)
+PyObject *cache_read(PyObject *, PyObject *const *v, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        expect(n, kCacheArgs + 3);
+        const CacheCall c = cache_call(v);
+        if (!THPDtype_Check(v[kCacheArgs])) raise(PyExc_TypeError, "expected a torch dtype");
+        const at::ScalarType type = reinterpret_cast<THPDtype *>(v[kCacheArgs])->scalar_type;
+        const int32_t io = io_dtype(type);
+        Place place(c.k->device());
+        Tensor out[2];
+        uint64_t ld[2];
+        void *p[2];
+        for (int i = 0; i < 2; ++i) {
+            const Tensor *given = tensor_or_none(v[kCacheArgs + 1 + i]);
+            if (given) require(given->scalar_type() == type, "out must be of the dtype asked for");
+            out[i] = given ? *given : empty({(int64_t)c.batch.rows, (int64_t)c.cache.heads, (int64_t)c.cache.head_dim}, type, place);
+            ld[i] = head_rows(out[i], c, c.cache.heads, "out", true).ld;
+            p[i] = out[i].mutable_data_ptr();
+        }
+        check(unlocked([&] { return nf4_cache_read_dev(&c.cache, &c.batch, p[0], ld[0], p[1], ld[1], io, place.stream); }));
+        return pair(std::move(out[0]), std::move(out[1]));
+    });
+}
+
+// cache_attention(<cache, batch>, q, scale, out or None) -> out
+PyObject *cache_attention(PyObject *, PyObject *const *v, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        expect(n, kCacheArgs + 3);
+        const CacheCall c = cache_call(v);
+        const Tensor &q = tensor(v[kCacheArgs]);
+        const Tensor *given = tensor_or_none(v[kCacheArgs + 2]);
+        nf4_attention_args a;
+        std::memset(&a, 0, sizeof(a));
+        a.struct_bytes = sizeof(a);
+        a.io_dtype = io_dtype(q.scalar_type());
+        a.scale = (float)float_arg(v[kCacheArgs + 1]);
+        Place place(c.k->device());
+        const HeadRows rq = head_rows(q, c, 0, "q", false);
+        Tensor out = given ? *given : empty(q.sizes(), q.scalar_type(), place);
+        require(out.scalar_type() == q.scalar_type() && out.sizes() == q.sizes(), "out must have q's shape and type");
+        a.q_heads = rq.heads;
+        a.q = rq.t.const_data_ptr();
+        a.ldq = rq.ld;
+        a.ldo = head_rows(out, c, rq.heads, "out", true).ld;
+        a.out = out.mutable_data_ptr();
+        const uint64_t bytes = nf4_cache_attention_workspace_bytes(&c.cache, &c.batch, a.q_heads, a.io_dtype);
+        Tensor ws;
+        if (bytes) {  // (0: arguments that the call refuses)
+            ws = flagged_workspace(bytes, place, kAttentionSlot, nf4_cache_attention_flag_bytes());
+            a.workspace = ws.mutable_data_ptr();
+            a.workspace_bytes = (uint64_t)ws.numel();
+        }
+        check(unlocked([&] { return nf4_cache_attention_dev(&c.cache, &c.batch, &a, place.stream); }));
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
 PyObject *release_workspaces(PyObject *, PyObject *) {
     t_kept.clear();
     Py_RETURN_NONE;
@@ -541,6 +710,7 @@ PyMethodDef kMethods[] = {
     FAST(linear_forward), FAST(linear_forward_grouped), FAST(qlora_backward), FAST(quantize), FAST(quantize_transposed),
     FAST(quantize_transposed_double),
     FAST(double_quantize), FAST(dequantize), FAST(quantize_dequantize), FAST(embedding),
+    FAST(cache_append), FAST(cache_read), FAST(cache_attention),
     {"release_workspaces", release_workspaces, METH_NOARGS, "Give the calling thread's kept workspaces back."},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -1,0 +1,89 @@
+// The paged key and value cache as the kernels see it, and what the attention kernels share.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "kernels.cuh"
+
+namespace nf4 {
+
+struct CacheView {
+    const void *k, *v;
+    const float *k_scales, *v_scales;
+    uint32_t pages, page_size, heads;
+};
+struct BatchView {
+    const int32_t *table, *lengths, *starts;
+    uint32_t sequences, width, rows;  // width: pages to a sequence
+};
+
+// A sequence of the call: its rows and its tokens, cut to what the buffers hold whatever the device memory says.
+struct Sequence {
+    uint32_t row0, rows, length;
+};
+__device__ __forceinline__ Sequence sequence_of(const CacheView &c, const BatchView &b, uint32_t s) {
+    const int32_t from = max(__ldg(b.starts + s), 0), to = max(__ldg(b.starts + s + 1), 0), len = max(__ldg(b.lengths + s), 0);
+    Sequence q;
+    q.row0 = min((uint32_t)from, b.rows);
+    q.rows = max(min((uint32_t)to, b.rows), q.row0) - q.row0;
+    q.length = (uint32_t)min((uint64_t)len, (uint64_t)b.width * c.page_size);
+    return q;
+}
+
+// kv_cache.cu: a call's arguments looked over, with a message that begins with `what`.  check_rows also fills in the row stride.
+int32_t check_cache(const char *what, const nf4_cache *c, const nf4_cache_batch *b);
+int32_t check_rows(const char *what, const char *name, const void *p, uint64_t *ld, uint64_t width, int32_t io_dtype);
+CacheView view_of(const nf4_cache &c);
+BatchView view_of(const nf4_cache_batch &b);
+
+// Eight values of the cache as they are stored, to f32: of bf16 words, or of a word of codes and their block's scale.
+__device__ __forceinline__ void values_of_bf16(const uint4 &w, float (&v)[8]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(u[i] << 16);
+        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void values_of_codes(uint32_t w, float scale, const float *levels, float (&v)[8]) {
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(levels[(w >> (4 * i)) & 15u], scale);
+}
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// ---- attention ------------------------------------------------------------------------------------
+// A call's arguments as the kernels take them.  The rows that one head of the cache serves are numbered token by token,
+// the query heads of a token side by side: row r is token r / group, query head head * group + r % group.
+struct AttentionView {
+    const void *q;
+    void *out;
+    uint64_t ldq, ldo;
+    uint32_t group;
+    float scale_log2;  // the scale times log2(e): weights are powers of two
+    // Where the keys of a row tile are shared out between several CTAs each leaves its part here: the sums of weights times
+    // values [part][row * heads * group + head][dim], and {largest exponent, sum of weights} beside them.
+    float *part_o;
+    float2 *part_ml;
+    uint32_t parts;
+};
+
+// How many tokens row tile `tile` (of `rows` rows) of a sequence sees: its last row's.
+__device__ __forceinline__ uint32_t visible_end(const Sequence &s, uint32_t group, uint32_t last_row) {
+    const int64_t token = (int64_t)s.length - s.rows + last_row / group;
+    return token < 0 ? 0u : (uint32_t)token + 1;
+}
+
+struct AttentionCall {
+    CacheView cache;
+    BatchView batch;
+    AttentionView view;
+    bool nf4, f32;
+    uint32_t head_dim;
+    uint32_t most_rows, most_tokens;  // of a sequence, as far as the host knows: rows of the call's tensors, tokens
+};
+
+constexpr uint64_t kAttentionFlagBytes = 4096;  // at the start of a workspace, as zeros
+
+}  // namespace nf4
