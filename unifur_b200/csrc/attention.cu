@@ -211,6 +211,8 @@ join_kernel(const BatchView b, const AttentionView a, uint32_t q_heads) {
 }
 
 // ---- how a call is carried out -----------------------------------------------------------------------
+bool takes_decode(const AttentionCall &c) { return !c.f32 && (uint64_t)c.most_rows * c.view.group <= 64; }
+
 struct Plan {
     uint32_t row_tiles, parts;  // CTAs to a head of a sequence: row tiles side by side, and parts of the tokens
 };
@@ -230,6 +232,7 @@ uint64_t part_ml_bytes(const AttentionCall &c, uint32_t parts) {
     return ((uint64_t)parts * c.batch.rows * c.cache.heads * c.view.group * sizeof(float2) + 255) / 256 * 256;
 }
 uint64_t workspace_bytes_of(const AttentionCall &c, const Plan &p) {
+    if (takes_decode(c)) return attention_decode_bytes(c);
     if (p.parts == 1) return kAttentionFlagBytes;
     return kAttentionFlagBytes + part_ml_bytes(c, p.parts) + (uint64_t)p.parts * c.batch.rows * c.cache.heads * c.view.group * c.head_dim * sizeof(float);
 }
@@ -321,6 +324,7 @@ int32_t nf4_cache_attention_dev(const nf4_cache *cache, const nf4_cache_batch *b
     c.view.part_ml = reinterpret_cast<float2 *>(ws);
     c.view.part_o = reinterpret_cast<float *>(ws + part_ml_bytes(c, p.parts));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (takes_decode(c)) return attention_decode(c, static_cast<uint8_t *>(args->workspace), s);
     return c.head_dim == 64 ? launch_of<64>(c, p, s) : c.head_dim == 128 ? launch_of<128>(c, p, s) : launch_of<256>(c, p, s);
 }
 

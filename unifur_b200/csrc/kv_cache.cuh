@@ -86,4 +86,8 @@ struct AttentionCall {
 
 constexpr uint64_t kAttentionFlagBytes = 4096;  // at the start of a workspace, as zeros
 
+// attention_decode.cu: bf16 tensors, few rows to a head of a sequence
+uint64_t attention_decode_bytes(const AttentionCall &c);
+int32_t attention_decode(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream);
+
 }  // namespace nf4
