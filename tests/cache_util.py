@@ -61,6 +61,11 @@ def stored(cache, name):
     return nf4_levels().numpy().astype(np.float64)[codes] * np.repeat(scales.astype(np.float64), 64, -1)
 
 
+def largest(cache):
+    t = cache.v_scales if cache.is_quantized() else cache.v
+    return float(torch.nan_to_num(t.float()).abs().max())
+
+
 def tokens_of(values, batch, page_size, s):
     """A sequence's tokens [tokens, heads, dim] out of stored()."""
     length = int(batch.lengths[s])
@@ -93,13 +98,16 @@ def reference(cache, batch, q, scale):
     return out, spread, reach
 
 
-def tolerance(out, spread, reach, dim, length, f32):
+def tolerance(out, spread, reach, dim, length, f32, high):
     """How far a result may be off.  Relative errors of the weights: twice the scores' errors (e^x), their own rounding, and the
     sums'; they move a result by as much of sum(weight * |value|); then the result is rounded.
     f32: sums of dim and length products, 2^-24 each.  bf16: keys and values enter as f16 (2^-11) or as they are, a query as it is, the
-    weights as bf16 (2^-8) or f16; f32 sums beside that."""
+    weights as bf16 (2^-8) or f16; f32 sums beside that.  f16 is off by up to 2^-25 where a number is below 2^-14, which counts beside
+    `high`, the largest scale (or value) of the cache: weights are kept 2^7 above their size in units of at most 2 high, so that a token
+    is off by 2^-25 2^-7 2 high at most; values are in units of at most 2 high, off by 2^-25 of that."""
     out, reach = np.abs(out), reach[..., None]
     sums = 2.0 ** -24 * (2 * (dim + 4) * reach + 2 * length + 64)
     if f32:
         return 2.0 ** -24 * out + sums * spread
-    return 2.0 ** -8 * out + (2 * 2 * 2.0 ** -11 * reach + 2.0 ** -8 + 2.0 ** -11 + sums) * spread * (1 + 2.0 ** -8)
+    return 2.0 ** -8 * out + (2 * 2 * 2.0 ** -11 * reach + 2.0 ** -8 + 2.0 ** -11 + sums) * spread * (1 + 2.0 ** -8) + \
+        (length * 2.0 ** -31 + 2.0 ** -24) * high

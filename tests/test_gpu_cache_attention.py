@@ -5,7 +5,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
-from cache_util import DEV, batch_of, filled_cache, reference, spoil_unused, tolerance  # noqa: E402
+from cache_util import DEV, batch_of, filled_cache, largest, reference, spoil_unused, tolerance  # noqa: E402
 from unifur_b200 import _lib  # noqa: E402
 from unifur_b200.kv_cache import CacheBatch, PagedKvCache  # noqa: E402
 
@@ -29,8 +29,9 @@ def check(specs, heads, group, dim, page_size, quantized, dtype, seed=0, hints=T
     rows = slice(1, batch.rows - 2)
     assert bool((out[:1] == 7.0).all()) and bool((out[-2:] == 7.0).all()), "rows of no sequence were written"
     off = np.abs(out[rows].cpu().double().numpy() - ref[rows])
-    may = tolerance(ref[rows], spread[rows], reach[rows], dim, max(n for n, _ in specs), dtype == torch.float32)
-    assert np.isfinite(off).all() and (off <= may).all(), (float(off.max()), float((off / np.maximum(may, 1e-300)).max()))
+    may = tolerance(ref[rows], spread[rows], reach[rows], dim, max(n for n, _ in specs), dtype == torch.float32, largest(cache))
+    worst = float((off / np.maximum(may, 1e-300)).max())
+    assert worst <= 1, f"off by {float(off.max())}, {worst} of what it may be"
     assert _lib.load().nf4_device_status(None, None, None) == 0
     return cache, batch, q, got
 
@@ -143,7 +144,7 @@ def test_decode_steps_in_a_graph_and_beside_it(oracle):
         eager.append((a.clone(), y.clone()))
         ref, spread, reach = reference(cache, CacheBatch(table, lengths, starts, n), q.view(n, heads * group, dim), dim ** -0.5)
         off = np.abs(a.view(n, heads * group, dim).cpu().double().numpy() - ref)
-        assert (off <= tolerance(ref, spread, reach, dim, 64, False)).all()
+        assert (off <= tolerance(ref, spread, reach, dim, 64, False, largest(cache))).all()
 
     cache, lengths = begin()
     x = xs[0].clone()

@@ -22,7 +22,7 @@ struct F32Shape {
     static constexpr uint32_t kSmem = 4 * (kRows * kPitch + 2 * kTokens * kPitch + kRows * kPPitch);
 };
 
-template <int D, bool NF4, typename T>
+template <int D, bool NF4>
 __global__ void __launch_bounds__(kThreads)
 attention_f32_kernel(const CacheView c, const BatchView b, const AttentionView a) {
     using S = F32Shape<D>;
@@ -45,13 +45,7 @@ attention_f32_kernel(const CacheView c, const BatchView b, const AttentionView a
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             if (r < n) {
                 const uint32_t token = (uint32_t)((r0 + r) / a.group), h = (uint32_t)((r0 + r) % a.group);
-                const T *p = static_cast<const T *>(a.q) + (uint64_t)(s.row0 + token) * a.ldq + (uint64_t)(head * a.group + h) * D + d;
-                if constexpr (sizeof(T) == 4) {
-                    v = *reinterpret_cast<const float4 *>(p);
-                } else {
-                    const uint2 w = *reinterpret_cast<const uint2 *>(p);
-                    v = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
-                }
+                v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + (uint64_t)(s.row0 + token) * a.ldq + (uint64_t)(head * a.group + h) * D + d);
             }
             *reinterpret_cast<float4 *>(sq + r * S::kPitch + d) = v;
         }
@@ -158,13 +152,10 @@ attention_f32_kernel(const CacheView c, const BatchView b, const AttentionView a
                 continue;
             }
             const float f = sum[i] == 0.f ? 0.f : 1.f / sum[i];
-            T *const out = static_cast<T *>(a.out) + (uint64_t)row * a.ldo + (uint64_t)h * D;
+            float *const out = static_cast<float *>(a.out) + (uint64_t)row * a.ldo + (uint64_t)h * D;
             #pragma unroll
-            for (int j = 0; j < D / 32; ++j) {
-                const float4 v = make_float4(acc[i][4 * j] * f, acc[i][4 * j + 1] * f, acc[i][4 * j + 2] * f, acc[i][4 * j + 3] * f);
-                if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(out + 4 * tx + 32 * j) = v;
-                else *reinterpret_cast<uint2 *>(out + 4 * tx + 32 * j) = make_uint2(bf16_pair(v.x, v.y), bf16_pair(v.z, v.w));
-            }
+            for (int j = 0; j < D / 32; ++j)
+                *reinterpret_cast<float4 *>(out + 4 * tx + 32 * j) = make_float4(acc[i][4 * j] * f, acc[i][4 * j + 1] * f, acc[i][4 * j + 2] * f, acc[i][4 * j + 3] * f);
         }
     }
 }
@@ -211,15 +202,25 @@ join_kernel(const BatchView b, const AttentionView a, uint32_t q_heads) {
 }
 
 // ---- how a call is carried out -----------------------------------------------------------------------
+// Few rows to a head of a sequence: the kernel that streams the cache; its tiles have 16 rows, four of them read the tokens four times.
 bool takes_decode(const AttentionCall &c) { return !c.f32 && (uint64_t)c.most_rows * c.view.group <= 64; }
 
 struct Plan {
-    uint32_t row_tiles, parts;  // CTAs to a head of a sequence: row tiles side by side, and parts of the tokens
+    uint32_t row_tiles, parts;  // f32: CTAs to a head of a sequence, row tiles side by side; parts of the tokens
 };
 
 Plan plan_of(const AttentionCall &c) {
-    const uint64_t tiles = std::max<uint64_t>(1, ((uint64_t)c.most_rows * c.view.group + kRows - 1) / kRows);
     Plan p;
+    if (!c.f32) {
+        p.row_tiles = attention_chunk_tiles(c);
+        // a CTA to an SM, two rounds of them where there are few row tiles; a part has eight steps of 128 tokens at least
+        const uint64_t rows = c.head_dim == 256 ? 128 : 256;
+        const uint64_t ctas = std::max<uint64_t>(1, std::min<uint64_t>(p.row_tiles, ((uint64_t)c.most_rows * c.view.group + rows - 1) / rows * c.batch.sequences) * c.cache.heads);
+        const uint64_t most = std::max<uint64_t>(1, c.most_tokens / 1024);
+        p.parts = (uint32_t)std::min<uint64_t>(std::min<uint64_t>(64, most), std::max<uint64_t>(1, 2 * kNumSMs / ctas));
+        return p;
+    }
+    const uint64_t tiles = std::max<uint64_t>(1, ((uint64_t)c.most_rows * c.view.group + kRows - 1) / kRows);
     p.row_tiles = (uint32_t)std::min<uint64_t>(tiles, 65535 / c.cache.heads);
     // two CTAs to an SM; a part has two token tiles at least
     const uint64_t ctas = (uint64_t)p.row_tiles * c.cache.heads * std::max(1u, c.batch.sequences);
@@ -237,24 +238,24 @@ uint64_t workspace_bytes_of(const AttentionCall &c, const Plan &p) {
     return kAttentionFlagBytes + part_ml_bytes(c, p.parts) + (uint64_t)p.parts * c.batch.rows * c.cache.heads * c.view.group * c.head_dim * sizeof(float);
 }
 
-template <int D, bool NF4, typename T>
+template <int D, bool NF4>
 int32_t launch_f32(const AttentionCall &c, const Plan &p, cudaStream_t stream) {
-    auto kernel = attention_f32_kernel<D, NF4, T>;
+    auto kernel = attention_f32_kernel<D, NF4>;
     NF4_TRY(ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), F32Shape<D>::kSmem));
     count_launch();
-    NF4_TRY(launch_maybe_overlapped(kernel, dim3(p.parts, p.row_tiles * c.cache.heads, c.batch.sequences), dim3(kThreads), F32Shape<D>::kSmem,
-                                    stream, true, c.cache, c.batch, c.view));
+    return launch_maybe_overlapped(kernel, dim3(p.parts, p.row_tiles * c.cache.heads, c.batch.sequences), dim3(kThreads), F32Shape<D>::kSmem,
+                                   stream, true, c.cache, c.batch, c.view);
+}
+template <int D>
+int32_t launch_of(const AttentionCall &c, const Plan &p, cudaStream_t stream) {
+    if (!c.f32) NF4_TRY(attention_chunk(c, stream));
+    else NF4_TRY((c.nf4 ? launch_f32<D, true>(c, p, stream) : launch_f32<D, false>(c, p, stream)));
     if (p.parts == 1) return NF4_OK;
     const uint32_t q_heads = c.cache.heads * c.view.group;
     const uint64_t warps = (uint64_t)c.batch.rows * q_heads;
     count_launch();
-    return launch_maybe_overlapped(join_kernel<D, T>, dim3((unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32))), dim3(kThreads), 0, stream, true,
-                                   c.batch, c.view, q_heads);
-}
-template <int D>
-int32_t launch_of(const AttentionCall &c, const Plan &p, cudaStream_t stream) {
-    if (c.f32) return c.nf4 ? launch_f32<D, true, float>(c, p, stream) : launch_f32<D, false, float>(c, p, stream);
-    return c.nf4 ? launch_f32<D, true, __nv_bfloat16>(c, p, stream) : launch_f32<D, false, __nv_bfloat16>(c, p, stream);
+    return launch_maybe_overlapped(c.f32 ? join_kernel<D, float> : join_kernel<D, __nv_bfloat16>, dim3((unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32))),
+                                   dim3(kThreads), 0, stream, true, c.batch, c.view, q_heads);
 }
 
 AttentionCall call_of(const nf4_cache &cache, const nf4_cache_batch &batch, uint32_t q_heads, int32_t io_dtype) {

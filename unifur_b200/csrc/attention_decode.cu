@@ -8,7 +8,7 @@
 // tokens of a head were several CTAs', the CTA that is done last joins theirs out of the workspace, in the order of the tokens.
 //
 // Mathematics, per group of sixteen tokens t and eight rows r (one MMA tile):
-//   x[t][r] = scale * log2(e) * sum_b ks[t][b] (levels_b[t] . q_b[r]),  w = 2^(x - m[r]),  l[r] += w,
+//   x[t][r] = scale * log2(e) * sum_b ks[t][b] (levels_b[t] . q_b[r]),  w = 2^(x - m[r] + 8),  l[r] += w,
 //   o[d][r] += sum_t levels[t][d] (w[t][r] vs[t][block of d])
 // Tokens are on the MMA's M side in the first product and on its K side in the second, so the weights go from one to the other by a
 // transposition of 8 x 8 tiles (movmatrix) and nothing is padded to sixteen rows.  A quantized cache's codes are
@@ -16,8 +16,8 @@
 // nibbles of two tokens are put side by side first.  Block scales never touch f16 on their own: K's multiply the f32 sums of a
 // block, V's the weights.  The weights enter the second product in f16 (2^-11 of each; bf16 with a bf16 cache: 2^-8, half of the
 // result's own rounding on average), times V's scale divided by a power of two `ref` that no scale so far exceeds.
-// m is the largest exponent seen or up to 8 below it: while no score exceeds m by more than 8, weights stay below 2^8 and nothing
-// has to be rescaled, which spares the maximum over the tokens in nearly every group.
+// m is the largest exponent seen or up to 8 below it: while no score exceeds m by more than 8 nothing has to be
+// rescaled, which spares the maximum over the tokens in nearly every group.
 #include <algorithm>
 
 #include "kv_cache.cuh"
@@ -28,6 +28,9 @@ namespace nf4 {
 
 namespace {
 
+// Weights are 2^(x - m + kRaise), and times V's scales up to 2^15, so that f16 holds those that are 2^-31 of a row's largest; their sum is
+// raised alike.
+constexpr float kRaise = 8.f;
 constexpr uint32_t kGroup = 16;   // tokens to a group: pages are multiples of it
 constexpr uint32_t kStages = 3;   // groups in flight, a warp
 constexpr uint32_t kPassRegs = 16;  // accumulator registers of a thread that go through shared memory at a time
@@ -415,7 +418,7 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
             for (int nt = 0; nt < NT; ++nt)
                 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const float from = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
+                    const float from = m[nt][j] == -INFINITY ? 0.f : m[nt][j] - kRaise;
                     x[nt][j] = exp2_approx(x[nt][j] - from);
                     x[nt][j + 2] = exp2_approx(x[nt][j + 2] - from);
                     l[nt][j] += x[nt][j] + x[nt][j + 2];
