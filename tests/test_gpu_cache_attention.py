@@ -37,7 +37,7 @@ def check(specs, heads, group, dim, page_size, quantized, dtype, seed=0, hints=T
 
 
 @pytest.mark.parametrize("quantized", [True, False])
-@pytest.mark.parametrize("heads,group,dim,page_size", [(4, 7, 128, 64), (2, 4, 64, 16), (1, 8, 256, 48), (3, 1, 128, 32), (2, 16, 64, 128)])
+@pytest.mark.parametrize("heads,group,dim,page_size", [(4, 7, 128, 64), (2, 4, 64, 16), (1, 8, 256, 48), (3, 1, 128, 32), (2, 16, 64, 128), (2, 4, 128, 48)])
 @pytest.mark.parametrize("specs", ONE + FEW)
 def test_few_rows(specs, heads, group, dim, page_size, quantized):
     check(specs, heads, group, dim, page_size, quantized, torch.bfloat16)

@@ -52,8 +52,8 @@ attention_f32_kernel(const CacheView c, const BatchView b, const AttentionView a
         // the tokens that this thread's two rows see, and those that any row of the tile does
         uint32_t sees[2];
         #pragma unroll
-        for (int i = 0; i < 2; ++i) sees[i] = 2 * ty + i < n ? visible_end(s, a.group, (uint32_t)(r0 + 2 * ty + i)) : 0u;
-        const uint32_t end = visible_end(s, a.group, (uint32_t)(r0 + n - 1)), tiles = (end + kTokens - 1) / kTokens;
+        for (int i = 0; i < 2; ++i) sees[i] = 2 * ty + i < n ? visible_end(s, a.by_group, (uint32_t)(r0 + 2 * ty + i)) : 0u;
+        const uint32_t end = visible_end(s, a.by_group, (uint32_t)(r0 + n - 1)), tiles = (end + kTokens - 1) / kTokens;
         const uint32_t tile0 = (uint32_t)((uint64_t)tiles * part / a.parts), tile1 = (uint32_t)((uint64_t)tiles * (part + 1) / a.parts);
         float most[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
         float acc[2][D / 8] = {};
@@ -65,7 +65,7 @@ attention_f32_kernel(const CacheView c, const BatchView b, const AttentionView a
                 float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
                 const uint32_t token = t0 + t;
                 if (token < end) {
-                    const uint32_t at = token / c.page_size;
+                    const uint32_t at = c.by_page.of(token);
                     const int32_t page = __ldg(b.table + (uint64_t)seq * b.width + at);
                     if (page < 0 || (uint32_t)page >= c.pages) {
                         #pragma unroll
@@ -263,6 +263,7 @@ AttentionCall call_of(const nf4_cache &cache, const nf4_cache_batch &batch, uint
     c.cache = view_of(cache);
     c.batch = view_of(batch);
     c.view.group = q_heads / cache.heads;
+    c.view.by_group = FastDiv(c.view.group);
     c.nf4 = cache.form == NF4_CACHE_NF4;
     c.f32 = io_dtype == NF4_DTYPE_F32;
     c.head_dim = cache.head_dim;

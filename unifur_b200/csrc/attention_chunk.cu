@@ -148,7 +148,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     }
     if (NF4) {
         for (uint32_t i = tid; i < 256 * 8; i += kThreads) {  // the table: an entry's copy to a lane
-            const uint32_t byte = i >> 3, entry = c_level_f16_bits[byte & 15u] | c_level_f16_bits[byte >> 4] << 16;
+            const uint32_t byte = i >> 3, entry = level_pair_f16(byte);
             st_shared_u4(table + byte * 128u + (i & 7u) * 16u, make_uint4(entry, entry, entry, entry));
         }
     }
@@ -191,7 +191,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     if (seq < b.sequences) {
         const Sequence s = sequence_of(c, b, seq);
         const uint32_t rows = (uint32_t)min((uint64_t)S::kRows, (uint64_t)s.rows * a.group - r0), live = (rows + 127) / 128;
-        const uint32_t end = visible_end(s, a.group, r0 + rows - 1), all = (end + N - 1) / N;
+        const uint32_t end = visible_end(s, a.by_group, r0 + rows - 1), all = (end + N - 1) / N;
         const uint32_t step0 = (uint32_t)((uint64_t)all * part / a.parts), steps = (uint32_t)((uint64_t)all * (part + 1) / a.parts) - step0;
         const uint32_t t_first = step0 * N, t_end = min(end, t_first + steps * N);  // this CTA's tokens
         const uint32_t q_heads = c.heads * a.group;
@@ -231,7 +231,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             uint32_t most_k = 0, most_v = 0;
             bool bad = false;
             for (uint32_t t = t_first + (NF4 ? tid : tid * kGroup); t < t_end; t += NF4 ? kThreads : kThreads * kGroup) {
-                const uint32_t at = t / c.page_size;
+                const uint32_t at = c.by_page.of(t);
                 const int32_t page = __ldg(b.table + (uint64_t)seq * b.width + at);
                 if (page < 0 || (uint32_t)page >= c.pages) {
                     bad = true;
@@ -261,7 +261,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             const uint32_t tile = warp >> 2, r = tid & 127u, row = r0 + tile * 128 + r;  // this thread's row
             if (tile < live) {
                 const bool real = tile * 128 + r < rows;
-                const uint32_t sees = real ? visible_end(s, a.group, row) : 0u, sees_first = visible_end(s, a.group, r0 + tile * 128);
+                const uint32_t sees = real ? visible_end(s, a.by_group, row) : 0u, sees_first = visible_end(s, a.by_group, r0 + tile * 128);
                 const float factor = fmaxf(fabsf(a.scale_log2) * (NF4 ? s_qpower[tile * 128 + r] * k_power : 1.f), 1.2e-38f);
                 const uint32_t lanes = (warp & 3u) << 21;  // a warp reaches its quarter of tensor memory's lanes
                 const uint32_t ts = tmem + S::kS + tile * N + lanes, to = tmem + S::kO + tile * D + lanes;
@@ -381,7 +381,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                         if (lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 25);
                         break;
                     }
-                    const float unit = reciprocal_of_power(i & 1u ? v_power : k_power);
+                    const float unit = reciprocal_of_power(i & 1u ? v_power : k_power) * (1.f / kLevelUnit);
                     const uint32_t t0 = t_first + (i >> 1) * N;
                     #pragma unroll
                     for (uint32_t pass = 0; pass < N / kPass; ++pass) {
@@ -400,7 +400,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                             #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const uint32_t word = words[k], at = ((e == 0 ? word << 7 : word >> (8 * e - 7)) & 0x7f80u) | lane_word;
-                                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[e]) : "r"(at) : "memory");
+                                asm("ld.shared.u32 %0, [%1];" : "=r"(v[e]) : "r"(at));  // (free to move: the table stands)
                                 v[e] = mul_f16x2(v[e], s2);
                             }
                             const uint32_t chunk = (q & 1u) * 4 + (k ^ order);
@@ -422,7 +422,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                     const uint32_t groups = min(kGroups, (stored - t0 + kGroup - 1) / kGroup);
                     uint32_t place = 0;
                     if (g < groups) {
-                        const uint32_t at = t / c.page_size;
+                        const uint32_t at = c.by_page.of(t);
                         const int32_t page = __ldg(b.table + (uint64_t)seq * b.width + at);
                         if (page >= 0 && (uint32_t)page < c.pages) place = ((uint32_t)page * c.heads + head) * c.page_size + (t - at * c.page_size);
                     }

@@ -44,7 +44,7 @@ int32_t check_rows(const char *what, const char *name, const void *p, uint64_t *
     return NF4_OK;
 }
 
-CacheView view_of(const nf4_cache &c) { return CacheView{c.k, c.v, c.k_scales, c.v_scales, c.num_pages, c.page_size, c.heads}; }
+CacheView view_of(const nf4_cache &c) { return CacheView{c.k, c.v, c.k_scales, c.v_scales, c.num_pages, c.page_size, c.heads, FastDiv(c.page_size)}; }
 BatchView view_of(const nf4_cache_batch &b) {
     return BatchView{b.page_table, b.lengths, b.row_starts, b.sequences, b.pages_per_sequence, b.rows};
 }
@@ -75,7 +75,7 @@ __device__ __forceinline__ int64_t place_of(const CacheView &c, const BatchView 
     *in = true;
     const int64_t token = (int64_t)q.length - q.rows + (row - q.row0);
     if (token < 0) return -1;
-    const uint32_t at = (uint32_t)token / c.page_size;
+    const uint32_t at = c.by_page.of((uint32_t)token);
     const int32_t page = __ldg(b.table + (uint64_t)s * b.width + at);
     if (page < 0 || (uint32_t)page >= c.pages) return -1;
     return (int64_t)page * c.heads * c.page_size + ((uint32_t)token - at * c.page_size);
