@@ -189,15 +189,18 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         // be given CTAs of their own with a quota that is not longer by more, they are.  Quotas of all units over fewer CTAs: with as many
         // fewer as there are heads every head's last CTA may have next to nothing, so that one always serves.
         share.quota = 0;
-        if (!share.whole && items < ctas && b.sequences <= 32) {
+        if (!share.whole && items < ctas && b.sequences <= 32 && units < 1ull << 31) {
+            uint32_t quota[4], need[4];
             #pragma unroll
-            for (uint32_t k = 0; k <= 4; ++k) {
-                const uint64_t quota64 = divided(units - 1, ctas - items * k / 4) + 1;
-                const uint32_t quota = (uint32_t)min(quota64, (uint64_t)0x7fffffffu);
-                uint32_t need = line0.items * ((line0.units + quota - 1) / quota);
-                need = __reduce_add_sync(0xffffffffu, need);
-                if (need <= ctas && !share.quota && quota <= share.per + 2 * W) share.quota = quota;
+            for (uint32_t k = 0; k < 4; ++k) {
+                quota[k] = ((uint32_t)units - 1) / (ctas - items * (k + 1) / 4) + 1;
+                need[k] = line0.items * ((line0.units + quota[k] - 1) / quota[k]);
             }
+            #pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) need[k] = __reduce_add_sync(0xffffffffu, need[k]);
+            #pragma unroll
+            for (uint32_t k = 4; k-- > 0;)
+                if (need[k] <= ctas && quota[k] <= share.per + 2 * W) share.quota = quota[k];
         }
     }
 
