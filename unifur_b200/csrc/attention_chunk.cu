@@ -23,12 +23,15 @@ namespace nf4 {
 
 namespace {
 
-constexpr uint32_t kThreads = 448;  // 146 registers each
+constexpr uint32_t kThreads = 512;
 // Weights are 2^(S c - m + kRaise): up to 2^15, so that f16 holds those that are 2^-32 of a row's largest; their sum is raised alike.
 constexpr float kRaise = 7.f;
 constexpr uint32_t kGroup = 16;  // tokens that are in one page for sure
 // warps 0-3 and 4-7: softmax of a tile; 8-11: codes to f16; 12: copies; 13: MMAs
 constexpr uint32_t kExpandWarp = 8, kCopyWarp = 12, kMmaWarp = 13;
+// Registers: 512 threads are launched with 128 each; the two softmax warpgroups take 160 and leave 96 to the other two (together the
+// same 65536).
+constexpr uint32_t kSoftmaxRegs = 160, kOtherRegs = 96;
 
 template <int D, bool NF4>
 struct Shape {
@@ -258,6 +261,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         const float k_power = NF4 ? power_above(s_most[0]) : 1.f, v_power = NF4 ? power_above(s_most[1]) : 1.f;
 
         if (warp < 8) {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
             const uint32_t tile = warp >> 2, r = tid & 127u, row = r0 + tile * 128 + r;  // this thread's row
             if (tile < live) {
                 const bool real = tile * 128 + r < rows;
@@ -283,11 +287,13 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                         const float from = m == -INFINITY ? 0.f : kRaise - m;
                         float top[2] = {-INFINITY, -INFINITY};
                         sum = make_float2(0.f, 0.f);
+                        uint32_t ahead[2][32];  // 32 scores come while 32 are worked on
+                        tmem_ld32(ts, ahead[0]);
                         #pragma unroll
                         for (uint32_t k = 0; k < N; k += 32) {
-                            uint32_t x[32];
-                            tmem_ld32(ts + k, x);
+                            uint32_t (&x)[32] = ahead[k / 32 & 1];
                             ptx::tmem_wait_ld();
+                            if (k + 32 < N) tmem_ld32(ts + k + 32, ahead[k / 32 + 1 & 1]);
                             if (masked) {
                                 #pragma unroll
                                 for (uint32_t i = 0; i < 32; ++i) x[i] = k + i < lim ? x[i] : 0xff800000u;
@@ -366,6 +372,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                 ptx::tc_fence_before();
             }
         } else {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
             if (NF4 && warp >= kExpandWarp && warp < kExpandWarp + 4) {
                 // ---- codes to f16: a thread has 16 bytes of a token's row, 32 values ----
                 constexpr uint32_t kLanes = D / 32, kPass = 128 / kLanes;
