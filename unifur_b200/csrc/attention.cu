@@ -163,7 +163,7 @@ attention_f32_kernel(const CacheView c, const BatchView b, const AttentionView a
 // ---- the join of parts ------------------------------------------------------------------------------
 // A warp to a row of a query head: parts by their largest exponents, in their order, so that the result does not depend on
 // which was ready first.  Rows of no sequence have no parts and are left alone.
-template <int D, typename T>
+template <int D>
 __global__ void __launch_bounds__(kThreads)
 join_kernel(const BatchView b, const AttentionView a, uint32_t q_heads) {
     ptx::pdl_launch_dependents();
@@ -193,12 +193,9 @@ join_kernel(const BatchView b, const AttentionView a, uint32_t q_heads) {
         }
     }
     const float f = sum == 0.f ? 0.f : 1.f / sum;
-    T *const out = static_cast<T *>(a.out) + (uint64_t)row * a.ldo + (uint64_t)h * D + lane * (D / 32);
+    float *const out = static_cast<float *>(a.out) + (uint64_t)row * a.ldo + (uint64_t)h * D + lane * (D / 32);
     #pragma unroll
-    for (int j = 0; j < D / 32; j += 2) {
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<float2 *>(out + j) = make_float2(acc[j] * f, acc[j + 1] * f);
-        else *reinterpret_cast<uint32_t *>(out + j) = bf16_pair(acc[j] * f, acc[j + 1] * f);
-    }
+    for (int j = 0; j < D / 32; j += 2) *reinterpret_cast<float2 *>(out + j) = make_float2(acc[j] * f, acc[j + 1] * f);
 }
 
 // ---- how a call is carried out -----------------------------------------------------------------------
@@ -206,20 +203,11 @@ join_kernel(const BatchView b, const AttentionView a, uint32_t q_heads) {
 bool takes_decode(const AttentionCall &c) { return !c.f32 && (uint64_t)c.most_rows * c.view.group <= 64; }
 
 struct Plan {
-    uint32_t row_tiles, parts;  // f32: CTAs to a head of a sequence, row tiles side by side; parts of the tokens
+    uint32_t row_tiles, parts;  // CTAs to a head of a sequence: row tiles side by side, and parts of the tokens
 };
 
 Plan plan_of(const AttentionCall &c) {
     Plan p;
-    if (!c.f32) {
-        p.row_tiles = attention_chunk_tiles(c);
-        // a CTA to an SM, two rounds of them where there are few row tiles; a part has eight steps of 128 tokens at least
-        const uint64_t rows = c.head_dim == 256 ? 128 : 256;
-        const uint64_t ctas = std::max<uint64_t>(1, std::min<uint64_t>(p.row_tiles, ((uint64_t)c.most_rows * c.view.group + rows - 1) / rows * c.batch.sequences) * c.cache.heads);
-        const uint64_t most = std::max<uint64_t>(1, c.most_tokens / 1024);
-        p.parts = (uint32_t)std::min<uint64_t>(std::min<uint64_t>(64, most), std::max<uint64_t>(1, 2 * kNumSMs / ctas));
-        return p;
-    }
     const uint64_t tiles = std::max<uint64_t>(1, ((uint64_t)c.most_rows * c.view.group + kRows - 1) / kRows);
     p.row_tiles = (uint32_t)std::min<uint64_t>(tiles, 65535 / c.cache.heads);
     // two CTAs to an SM; a part has two token tiles at least
@@ -233,7 +221,7 @@ uint64_t part_ml_bytes(const AttentionCall &c, uint32_t parts) {
     return ((uint64_t)parts * c.batch.rows * c.cache.heads * c.view.group * sizeof(float2) + 255) / 256 * 256;
 }
 uint64_t workspace_bytes_of(const AttentionCall &c, const Plan &p) {
-    if (takes_decode(c)) return attention_decode_bytes(c);
+    if (!c.f32) return takes_decode(c) ? attention_decode_bytes(c) : attention_chunk_bytes(c);
     if (p.parts == 1) return kAttentionFlagBytes;
     return kAttentionFlagBytes + part_ml_bytes(c, p.parts) + (uint64_t)p.parts * c.batch.rows * c.cache.heads * c.view.group * c.head_dim * sizeof(float);
 }
@@ -248,13 +236,12 @@ int32_t launch_f32(const AttentionCall &c, const Plan &p, cudaStream_t stream) {
 }
 template <int D>
 int32_t launch_of(const AttentionCall &c, const Plan &p, cudaStream_t stream) {
-    if (!c.f32) NF4_TRY(attention_chunk(c, stream));
-    else NF4_TRY((c.nf4 ? launch_f32<D, true>(c, p, stream) : launch_f32<D, false>(c, p, stream)));
+    NF4_TRY((c.nf4 ? launch_f32<D, true>(c, p, stream) : launch_f32<D, false>(c, p, stream)));
     if (p.parts == 1) return NF4_OK;
     const uint32_t q_heads = c.cache.heads * c.view.group;
     const uint64_t warps = (uint64_t)c.batch.rows * q_heads;
     count_launch();
-    return launch_maybe_overlapped(c.f32 ? join_kernel<D, float> : join_kernel<D, __nv_bfloat16>, dim3((unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32))),
+    return launch_maybe_overlapped(join_kernel<D>, dim3((unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32))),
                                    dim3(kThreads), 0, stream, true, c.batch, c.view, q_heads);
 }
 
@@ -326,7 +313,10 @@ int32_t nf4_cache_attention_dev(const nf4_cache *cache, const nf4_cache_batch *b
     c.view.part_ml = reinterpret_cast<float2 *>(ws);
     c.view.part_o = reinterpret_cast<float *>(ws + part_ml_bytes(c, p.parts));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (takes_decode(c)) return attention_decode(c, static_cast<uint8_t *>(args->workspace), s);
+    if (!c.f32) {
+        uint8_t *const workspace = static_cast<uint8_t *>(args->workspace);
+        return takes_decode(c) ? attention_decode(c, workspace, s) : attention_chunk(c, workspace, s);
+    }
     return c.head_dim == 64 ? launch_of<64>(c, p, s) : c.head_dim == 128 ? launch_of<128>(c, p, s) : launch_of<256>(c, p, s);
 }
 

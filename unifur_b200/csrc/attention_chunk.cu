@@ -1,18 +1,22 @@
 // Attention of many rows over the paged cache (chunks of prompts, whole prompts) on the tensor cores.
 //
-// Bound by the MMAs (4 * dim operations for a row and a token) and by the exponentials beside them.  A CTA has 256 rows of one
-// head of the cache (a token's query heads are neighbouring rows), or 128 with a dim of 256, as one or two MMA tiles of 128, and goes over the
-// tokens 128 (or 64) a step.  Keys and values are in shared memory in f16 or bf16 with 128-byte swizzle: brought there by TMA from a bf16
-// cache; looked up by four warps from codes that came by bulk copies, times their block's scale, from a quantized one, once for all
-// of the CTA's rows.  One elected thread issues tcgen05.mma:
+// Bound by the MMAs (4 * dim operations for a row and a token) and by the exponentials beside them.  A row tile is 256 rows of one
+// head of the cache (a token's query heads are neighbouring rows), or 128 with a dim of 256: one or two MMA tiles of 128.  It goes over the
+// tokens that it sees 128 (or 64) a step.  The steps of all sequences, heads and row tiles form one line that the CTAs, one to an SM, share
+// out evenly: a CTA has pieces of the line, and a row tile that is in several CTAs leaves its parts in the workspace for the join.
+//
+// Keys and values are in shared memory in f16 or bf16 with 128-byte swizzle: brought there by TMA from a bf16 cache; looked up by four warps
+// from codes that came by bulk copies, times their block's scale, from a quantized one, once for all of a tile's rows.  One elected thread
+// issues tcgen05.mma:
 //   S = Q K^T   both operands from shared memory, 128 x 128 f32 sums in tensor memory
 //   O += P V    P from tensor memory, where the softmax warps have put it over S; V as it lies, MN-major
 // A softmax thread owns a row: it reads S, keeps the row's largest exponent m and sum l, and writes P = 2^(S c - m + 7) back as f16
 // (bf16 with a bf16 cache).  While one tile's softmax runs, the other's two products do.  m is the largest exponent so far or up to 8
 // below it: O is rescaled only where a row rises above that, by the warps themselves, at a moment when
-// no product is writing it.
-// f16's range: K's and V's scales are divided by the power of two of the largest among the CTA's tokens, a row of Q by its own
-// (exact); the powers come back in f32.  f16 is off by 2^-12 on average, bf16 would be by 2^-9.
+// no product is writing it.  Copies and lookups run ahead into the next piece while a row tile's results are written.
+// f16's range: K's and V's scales are divided by a power of two of a step's largest, a row of Q by its own (exact).  K's comes back as a
+// factor of the step's scores; V's goes into the step's weights, relative to the largest so far (`ref`), which comes back at the end.  f16 is
+// off by 2^-12 on average, bf16 would be by 2^-9.
 #include <algorithm>
 
 #include "kv_cache.cuh"
@@ -110,25 +114,106 @@ __device__ __forceinline__ float power_above(uint32_t most) {
 }
 __device__ __forceinline__ float reciprocal_of_power(float p) { return __uint_as_float(0x7f000000u - __float_as_uint(p)); }
 
-// row_tiles: the most that the call's rows can make of one head
+// How the line of steps is shared out: `per` to a CTA, one more to the first `more` of them.
+struct Share {
+    uint32_t per, more, ctas;
+    __device__ uint32_t start(uint32_t cta) const { return per * cta + min(cta, more); }
+    __device__ uint32_t cta_of(uint32_t u) const {
+        const uint32_t first = (per + 1) * more;
+        return u < first ? u / (per + 1) : more + (u - first) / per;
+    }
+};
+
+// A run of steps of one row tile.
+struct Piece {
+    Sequence s;
+    uint32_t seq, head, r0, rows, live;  // rows of the tile; MMA tiles that have some
+    uint32_t step0, steps, all;          // of the `all` steps that the tile has
+    uint32_t line0;                      // where the tile's steps begin in the line
+};
+
+// Steps' worth of time that a row tile takes beside its steps (its queries in, its results out): counted in the line, or the CTAs that have
+// a prompt's first tiles, of one step each, would be done last.
+constexpr uint32_t kStart = 3;
+
+template <uint32_t R, uint32_t N>
+struct Walker {  // through a CTA's pieces; every warp goes its own way
+    Sequence s;
+    uint32_t seq, head, tile, off, now, end;
+
+    static __device__ __forceinline__ uint32_t tiles_of(const Sequence &s, uint32_t group) { return (uint32_t)(((uint64_t)s.rows * group + R - 1) / R); }
+    // (a tile that sees nothing has one step all the same: its results are zeros)
+    static __device__ __forceinline__ uint32_t steps_of(const Sequence &s, const AttentionView &a, uint32_t tile) {
+        const uint32_t last = (uint32_t)min((uint64_t)(tile + 1) * R, (uint64_t)s.rows * a.group) - 1;
+        return max(1u, (visible_end(s, a.by_group, last) + N - 1) / N);
+    }
+    __device__ __forceinline__ bool next(const CacheView &c, const BatchView &b, const AttentionView &a, Piece &p) {
+        do {
+            if (!one(c, b, a, p)) return false;
+        } while (p.steps == 0);  // (the end of a share that lies ahead of a tile's first step)
+        return true;
+    }
+    __device__ __forceinline__ bool one(const CacheView &c, const BatchView &b, const AttentionView &a, Piece &p) {
+        if (now >= end) return false;
+        while (tile >= tiles_of(s, a.group)) {  // on to the next head, or the next sequence with rows
+            tile = 0;
+            if (s.rows == 0 || ++head >= c.heads) {
+                head = 0;
+                if (++seq >= b.sequences) return false;
+                s = sequence_of(c, b, seq);
+            }
+        }
+        p.s = s;
+        p.seq = seq;
+        p.head = head;
+        p.r0 = tile * R;
+        p.rows = (uint32_t)min((uint64_t)R, (uint64_t)s.rows * a.group - p.r0);
+        p.live = (p.rows + 127) / 128;
+        p.all = steps_of(s, a, tile);
+        p.line0 = now - off;
+        // of the tile's place in the line [line0, line0 + kStart + all) the steps are behind kStart
+        const uint32_t upto = min(p.all + kStart, end - p.line0);
+        p.step0 = off > kStart ? off - kStart : 0u;
+        p.steps = (upto > kStart ? upto - kStart : 0u) - p.step0;
+        now = p.line0 + upto;
+        off = 0;
+        ++tile;
+        return true;
+    }
+};
+
+// What the join has to know of a row tile that several CTAs have: written by the CTA in whose share it begins, rows 0 by the others.
+struct Split {
+    uint32_t row0, r0, rows, head, more;  // more: CTAs behind the first
+};
+
 template <int D, bool NF4>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const CacheView c, const BatchView b,
-                       const AttentionView a, uint32_t row_tiles, const FailureRef failure) {
+                       const AttentionView a, Split *const splits, const FailureRef failure) {
     using S = Shape<D, NF4>;
+    using Walk = Walker<S::kRows, S::kTokens>;
     constexpr uint32_t N = S::kTokens, kBlocks = S::kBlocks;
     extern __shared__ uint8_t smem_any[];
-    __shared__ __align__(8) uint64_t s_bars[19];
-    __shared__ uint32_t s_tmem, s_most[2], s_bad;
+    __shared__ __align__(8) uint64_t s_bars[25];
+    __shared__ uint32_t s_tmem, s_bad[8], s_first[6];  // s_bad: of the last pieces, whether a page was not there
+    __shared__ Share s_share;
+    __shared__ Walk s_walk[8];
+    __shared__ Piece s_piece[8];
     __shared__ float s_qpower[S::kRows];
+    __shared__ float2 s_powers[4];  // of the last steps' K and V
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u;
     const uint32_t base = ptx::smem_addr(smem_any);
     const uint32_t raw0 = (base + 15u) & ~15u, table = (raw0 + S::kRawSlots * S::kRaw + 32767u) & ~32767u;
     const uint32_t q0 = NF4 ? table + 32768u : (base + 1023u) & ~1023u, ring0 = q0 + S::kTiles * S::kQTile;
     const uint32_t bars = ptx::smem_addr(s_bars), full0 = bars, empty0 = bars + 32, raw_full0 = bars + 64, raw_empty0 = bars + 88, s_full0 = bars + 112,
-                   p_ready0 = bars + 128, tail_bar = bars + 144;
+                   p_ready0 = bars + 128, tail_bar = bars + 144, q_ready0 = bars + 152, power0 = bars + 168;
     if (ring0 + S::kSlots * S::kTile > base + S::kSmem) {
-        if (tid == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 22);
+        ptx::pdl_wait();
+        if (tid == 0) {
+            NF4_REPORT_FAILURE(*failure.flag, *failure.host, 22);
+            splits[blockIdx.x].rows = 0;
+        }
         return;
     }
     if (tid == 0) {
@@ -143,11 +228,12 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         for (uint32_t i = 0; i < 2; ++i) {
             ptx::mbar_init(s_full0 + 8 * i, 1);
             ptx::mbar_init(p_ready0 + 8 * i, 4);
+            ptx::mbar_init(q_ready0 + 8 * i, 4);
         }
+        for (uint32_t i = 0; i < 4; ++i) ptx::mbar_init(power0 + 8 * i, 1);
         ptx::mbar_init(tail_bar, 1);
         ptx::fence_mbar_init();
         ptx::fence_proxy_async();
-        s_most[0] = s_most[1] = s_bad = 0;
     }
     if (NF4) {
         for (uint32_t i = tid; i < 256 * 8; i += kThreads) {  // the table: an entry's copy to a lane
@@ -159,119 +245,166 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         ptx::tmem_alloc(ptx::smem_addr(&s_tmem), 512);
         ptx::tmem_relinquish();
     }
-    ptx::tc_fence_before();
-    __syncthreads();
-    ptx::tc_fence_after();
-    const uint32_t tmem = s_tmem;
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
 
-    // ---- which rows: the last tiles, which see most, first ----
-    const uint32_t part = blockIdx.y, head = blockIdx.x % c.heads, want = row_tiles - 1 - blockIdx.x / c.heads;
-    uint32_t seq = b.sequences, r0 = 0;
-    {
+    // ---- this CTA's share of the line, and where in it begins ----
+    if (warp == 0) {
+        // a lane a sequence: its steps, all heads
+        auto steps_of = [&](uint32_t s0, Sequence &s) -> uint32_t {
+            s = Sequence{0, 0, 0};
+            if (s0 + lane < b.sequences) s = sequence_of(c, b, s0 + lane);
+            const uint32_t tiles = Walk::tiles_of(s, a.group);
+            uint32_t sum = 0;
+            if (tiles <= 8)
+                for (uint32_t t = 0; t < tiles; ++t) sum += kStart + Walk::steps_of(s, a, t);
+            for (uint32_t many = __ballot_sync(0xffffffffu, tiles > 8); many; many &= many - 1) {  // with the whole warp
+                const int l = __ffs(many) - 1;
+                const Sequence o{__shfl_sync(0xffffffffu, s.row0, l), __shfl_sync(0xffffffffu, s.rows, l), __shfl_sync(0xffffffffu, s.length, l)};
+                uint32_t part = 0;
+                for (uint32_t t = lane; t < Walk::tiles_of(o, a.group); t += 32) part += kStart + Walk::steps_of(o, a, t);
+                part = __reduce_add_sync(0xffffffffu, part);
+                if ((int)lane == l) sum = part;
+            }
+            return sum * c.heads;
+        };
+        Sequence s0;
+        const uint32_t own0 = steps_of(0, s0);
+        uint32_t total = own0;
+        for (uint32_t k = 32; k < b.sequences; k += 32) {
+            Sequence s;
+            total += steps_of(k, s);
+        }
+        total = __reduce_add_sync(0xffffffffu, total);
+        Share share;
+        share.ctas = min(gridDim.x, (total + kStart + 1) / (kStart + 2));  // two steps at least
+        share.per = share.ctas ? total / share.ctas : 0;
+        share.more = share.ctas ? total - share.per * share.ctas : 0;
+        const uint32_t first = share.start(blockIdx.x), last = blockIdx.x < share.ctas ? share.start(blockIdx.x + 1) : first;
         uint32_t before = 0;
-        for (uint32_t s0 = 0; s0 < b.sequences; s0 += 32) {
-            uint32_t own = 0;
-            if (s0 + lane < b.sequences) own = (uint32_t)(((uint64_t)sequence_of(c, b, s0 + lane).rows * a.group + S::kRows - 1) / S::kRows);
+        for (uint32_t k = 0; first < last && k < b.sequences; k += 32) {
+            Sequence s = s0;
+            const uint32_t own = k ? steps_of(k, s) : own0;
             uint32_t upto = own;
             #pragma unroll
-            for (int k = 1; k < 32; k <<= 1) {
-                const uint32_t o = __shfl_up_sync(0xffffffffu, upto, k);
-                if (lane >= (uint32_t)k) upto += o;
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d);
+                if (lane >= (uint32_t)d) upto += o;
             }
-            const uint32_t past = __ballot_sync(0xffffffffu, before + upto > want);
+            const uint32_t past = __ballot_sync(0xffffffffu, before + upto > first);
             if (past) {
-                const int l0 = __ffs(past) - 1;
-                seq = s0 + l0;
-                r0 = (want - (before + __shfl_sync(0xffffffffu, upto - own, l0))) * S::kRows;
+                const int l = __ffs(past) - 1;
+                const Sequence o{__shfl_sync(0xffffffffu, s.row0, l), __shfl_sync(0xffffffffu, s.rows, l), __shfl_sync(0xffffffffu, s.length, l)};
+                const uint32_t at = first - before - __shfl_sync(0xffffffffu, upto - own, l), of_head = __shfl_sync(0xffffffffu, own, l) / c.heads;
+                const uint32_t head = at / of_head;
+                uint32_t left = at - head * of_head, tile = 0;
+                for (uint32_t t0 = 0;; t0 += 32) {
+                    const uint32_t mine = t0 + lane < Walk::tiles_of(o, a.group) ? kStart + Walk::steps_of(o, a, t0 + lane) : 0u;
+                    uint32_t sum = mine;
+                    #pragma unroll
+                    for (int d = 1; d < 32; d <<= 1) {
+                        const uint32_t v = __shfl_up_sync(0xffffffffu, sum, d);
+                        if (lane >= (uint32_t)d) sum += v;
+                    }
+                    const uint32_t in = __ballot_sync(0xffffffffu, sum > left);
+                    if (in) {
+                        const int t = __ffs(in) - 1;
+                        tile = t0 + t;
+                        left -= __shfl_sync(0xffffffffu, sum - mine, t);
+                        break;
+                    }
+                    if (t0 + 32 >= Walk::tiles_of(o, a.group)) break;  // (not reached: the head has that many steps)
+                    left -= __shfl_sync(0xffffffffu, sum, 31);
+                }
+                if (lane == 0) {
+                    s_first[0] = k + l;
+                    s_first[1] = head;
+                    s_first[2] = tile;
+                    s_first[3] = left;
+                }
                 break;
             }
             before += __shfl_sync(0xffffffffu, upto, 31);
         }
-    }
-    bool ok = true;
-    if (seq < b.sequences) {
-        const Sequence s = sequence_of(c, b, seq);
-        const uint32_t rows = (uint32_t)min((uint64_t)S::kRows, (uint64_t)s.rows * a.group - r0), live = (rows + 127) / 128;
-        const uint32_t end = visible_end(s, a.by_group, r0 + rows - 1), all = (end + N - 1) / N;
-        const uint32_t step0 = (uint32_t)((uint64_t)all * part / a.parts), steps = (uint32_t)((uint64_t)all * (part + 1) / a.parts) - step0;
-        const uint32_t t_first = step0 * N, t_end = min(end, t_first + steps * N);  // this CTA's tokens
-        const uint32_t q_heads = c.heads * a.group;
-
-        // ---- Q to shared memory; the largest scales of the CTA's tokens ----
-        if (steps) {
-            constexpr uint32_t kLanes = D / 8;  // to a row: eight values each
-            const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a scale below zero: the rows change sign, so that c is not)
-            #pragma unroll 4
-            for (uint32_t i = tid; i < live * 128 * kLanes; i += kThreads) {
-                const uint32_t r = i / kLanes, x = i % kLanes;
-                uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                if (r < rows) {
-                    const uint32_t row = r0 + r;
-                    w = __ldg(reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.q) + (uint64_t)(s.row0 + row / a.group) * a.ldq +
-                                                               (uint64_t)(head * a.group + row % a.group) * D) + x);
-                    w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
-                }
-                if (NF4) {
-                    uint32_t u[4] = {w.x, w.y, w.z, w.w}, most = 0;
-                    #pragma unroll
-                    for (int k = 0; k < 4; ++k) most = max(most, max((u[k] << 16) & 0x7fffffffu, u[k] & 0x7fff0000u));
-                    #pragma unroll
-                    for (uint32_t k = 1; k < kLanes; k <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, k));
-                    // the row's largest magnitude is left in [2^11, 2^12)
-                    const int e = most ? min(max((int)(most >> 23) - 127 - 11, -100), 115) : 0;
-                    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-                    #pragma unroll
-                    for (int k = 0; k < 4; ++k) u[k] = pack<true>(__uint_as_float(u[k] << 16) * down, __uint_as_float(u[k] & 0xffff0000u) * down);
-                    w = make_uint4(u[0], u[1], u[2], u[3]);
-                    if (x == 0) s_qpower[r] = __uint_as_float((uint32_t)(127 + e) << 23);
-                }
-                const uint32_t tile = r >> 7, rr = r & 127u;
-                st_shared_u4(q0 + tile * S::kQTile + (x >> 3) * 16384u + rr * 128u + (((x & 7u) ^ (rr & 7u)) << 4), w);
-            }
-            ptx::fence_proxy_async();
-            uint32_t most_k = 0, most_v = 0;
-            bool bad = false;
-            for (uint32_t t = t_first + (NF4 ? tid : tid * kGroup); t < t_end; t += NF4 ? kThreads : kThreads * kGroup) {
-                const uint32_t at = c.by_page.of(t);
-                const int32_t page = __ldg(b.table + (uint64_t)seq * b.width + at);
-                if (page < 0 || (uint32_t)page >= c.pages) {
-                    bad = true;
-                } else if (NF4) {
-                    const uint64_t row = ((uint64_t)page * c.heads + head) * c.page_size + (t - at * c.page_size);
-                    #pragma unroll
-                    for (uint32_t k = 0; k < kBlocks; ++k) {
-                        most_k = max(most_k, __float_as_uint(__ldg(c.k_scales + row * kBlocks + k)));
-                        most_v = max(most_v, __float_as_uint(__ldg(c.v_scales + row * kBlocks + k)));
-                    }
-                }
-            }
-            if (NF4) {
-                most_k = __reduce_max_sync(0xffffffffu, most_k);
-                most_v = __reduce_max_sync(0xffffffffu, most_v);
-                if (lane == 0) {
-                    atomicMax(&s_most[0], most_k);
-                    atomicMax(&s_most[1], most_v);
-                }
-            }
-            if (bad) s_bad = 1;
+        if (lane == 0) {
+            s_first[4] = first;
+            s_first[5] = last;
+            s_share = share;
+            splits[blockIdx.x].rows = 0;
         }
-        __syncthreads();
-        const float k_power = NF4 ? power_above(s_most[0]) : 1.f, v_power = NF4 ? power_above(s_most[1]) : 1.f;
-
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    bool ok = true;
+    if (s_first[4] < s_first[5]) {
+        Walk walk{sequence_of(c, b, s_first[0]), s_first[0], s_first[1], s_first[2], s_first[3], s_first[4], s_first[5]};
+        Piece p;
         if (warp < 8) {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-            const uint32_t tile = warp >> 2, r = tid & 127u, row = r0 + tile * 128 + r;  // this thread's row
-            if (tile < live) {
-                const bool real = tile * 128 + r < rows;
-                const uint32_t sees = real ? visible_end(s, a.by_group, row) : 0u, sees_first = visible_end(s, a.by_group, r0 + tile * 128);
-                const float factor = fmaxf(fabsf(a.scale_log2) * (NF4 ? s_qpower[tile * 128 + r] * k_power : 1.f), 1.2e-38f);
-                const uint32_t lanes = (warp & 3u) << 21;  // a warp reaches its quarter of tensor memory's lanes
-                const uint32_t ts = tmem + S::kS + tile * N + lanes, to = tmem + S::kO + tile * D + lanes;
-                float m = -INFINITY, l = 0.f;
-                for (uint32_t j = 0; j < steps; ++j) {
-                    if (!__all_sync(0xffffffffu, ptx::mbar_wait_suspended(s_full0 + 8 * tile, j & 1u))) {
+            const uint32_t tile = warp >> 2, r = tid & 127u;
+            const uint32_t lanes = (warp & 3u) << 21;  // a warp reaches its quarter of tensor memory's lanes
+            const uint32_t ts = tmem + S::kS + tile * N + lanes, to = tmem + S::kO + tile * D + lanes;
+            const uint32_t q_tile = q0 + tile * S::kQTile;
+            uint32_t scores = 0, step = 0, piece = 0;  // scores of this tile, steps and pieces of the CTA, so far
+            for (; ok && walk.next(c, b, a, p); step += p.steps, ++piece) {
+                if (tile >= p.live) continue;
+                // (what the steps do not need waits in shared memory: registers are short there)
+                if (lane == 0) {
+                    s_walk[warp] = walk;
+                    s_piece[warp] = p;
+                }
+                // ---- Q to shared memory ----
+                constexpr uint32_t kLanes = D / 8, kBatch = kLanes < 16 ? kLanes : 16;  // lanes to a row, eight values each; loads in flight
+                const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a scale below zero: the rows change sign, so that c is not)
+                #pragma unroll 1
+                for (uint32_t i0 = 0; i0 < kLanes; i0 += kBatch) {
+                    uint4 w[kBatch];
+                    #pragma unroll
+                    for (uint32_t k = 0; k < kBatch; ++k) {
+                        const uint32_t i = (i0 + k) * 128 + r, row = p.r0 + tile * 128 + i / kLanes, token = a.by_group.of(row);
+                        w[k] = make_uint4(0u, 0u, 0u, 0u);
+                        if (tile * 128 + i / kLanes < p.rows)
+                            w[k] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.q) + (uint64_t)(p.s.row0 + token) * a.ldq +
+                                                                         (uint64_t)(p.head * a.group + row - token * a.group) * D) + i % kLanes);
+                    }
+                    #pragma unroll
+                    for (uint32_t k = 0; k < kBatch; ++k) {
+                        const uint32_t i = (i0 + k) * 128 + r, rr = i / kLanes, x = i % kLanes;
+                        uint32_t u[4] = {w[k].x ^ flip, w[k].y ^ flip, w[k].z ^ flip, w[k].w ^ flip};
+                        if (NF4) {
+                            uint32_t most = 0;
+                            #pragma unroll
+                            for (int e = 0; e < 4; ++e) most = max(most, max((u[e] << 16) & 0x7fffffffu, u[e] & 0x7fff0000u));
+                            #pragma unroll
+                            for (uint32_t d = 1; d < kLanes; d <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+                            // the row's largest magnitude is left in [2^11, 2^12)
+                            const int e2 = most ? min(max((int)(most >> 23) - 127 - 11, -100), 115) : 0;
+                            const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+                            #pragma unroll
+                            for (int e = 0; e < 4; ++e) u[e] = pack<true>(__uint_as_float(u[e] << 16) * down, __uint_as_float(u[e] & 0xffff0000u) * down);
+                            if (x == 0) s_qpower[tile * 128 + rr] = __uint_as_float((uint32_t)(127 + e2) << 23);
+                        }
+                        st_shared_u4(q_tile + (x >> 3) * 16384u + rr * 128u + (((x & 7u) ^ (rr & 7u)) << 4), make_uint4(u[0], u[1], u[2], u[3]));
+                    }
+                }
+                ptx::fence_proxy_async();
+                if (tile) asm volatile("bar.sync 2, 128;" ::: "memory");  // this tile's warps
+                else asm volatile("bar.sync 1, 128;" ::: "memory");
+                if (lane == 0) ptx::mbar_arrive(q_ready0 + 8 * tile);
+
+                // ---- the steps ----
+                const uint32_t row = p.r0 + tile * 128 + r, t_first = p.step0 * N;
+                const bool real = tile * 128 + r < p.rows;
+                const uint32_t sees = real ? visible_end(p.s, a.by_group, row) : 0u, sees_first = visible_end(p.s, a.by_group, p.r0 + tile * 128);
+                const uint32_t steps = p.steps;
+                const float row_factor = fabsf(a.scale_log2) * (NF4 ? s_qpower[tile * 128 + r] : 1.f);
+                float m = -INFINITY, l = 0.f, ref = 0.f;
+                for (uint32_t j = 0; j < steps; ++j, ++scores) {
+                    bool got = ptx::mbar_wait_suspended(s_full0 + 8 * tile, scores & 1u);
+                    if (NF4) got = got && ptx::mbar_wait_suspended(power0 + 8 * ((step + j) & 3u), ((step + j) >> 2) & 1u);
+                    if (!__all_sync(0xffffffffu, got)) {
                         ok = false;
                         if (lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 23);
                         break;
@@ -279,12 +412,20 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                     ptx::tc_fence_after();
                     const uint32_t t0 = t_first + j * N, lim = sees > t0 ? sees - t0 : 0u;
                     const bool masked = t0 + N > sees_first;
+                    const float2 powers = NF4 ? s_powers[(step + j) & 3u] : make_float2(1.f, 1.f);
+                    const float factor = fmaxf(row_factor * powers.x, 1.2e-38f);
+                    const float ref_was = ref;
+                    if (NF4) ref = fmaxf(ref, powers.y);
+                    // the step's values are in units of powers.y, the sums in units of ref: 2^-less of that (a difference that is no more
+                    // than 2^-60 of the largest is made that)
+                    const int less = NF4 ? min((int)(__float_as_uint(ref) >> 23) - (int)(__float_as_uint(powers.y) >> 23), 60) : 0;
+                    bool grown = NF4 && ref != ref_was && j;
                     // Weights by m as it is, and only then the look at the largest score: where it is out of reach, once or twice a
                     // row, they are made again.  So nothing waits for a maximum, and S need not be held whole.
-                    uint32_t p[N / 2];
+                    uint32_t pw[N / 2];
                     float2 sum;
                     for (;;) {
-                        const float from = m == -INFINITY ? 0.f : kRaise - m;
+                        const float from = m == -INFINITY ? 0.f : kRaise - m - (float)less;
                         float top[2] = {-INFINITY, -INFINITY};
                         sum = make_float2(0.f, 0.f);
                         uint32_t ahead[2][32];  // 32 scores come while 32 are worked on
@@ -304,14 +445,21 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                                 const float2 e = fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), factor, from);
                                 const float2 w = make_float2(exp2_approx(e.x), exp2_approx(e.y));
                                 sum = add2(sum, w);
-                                p[(k + i) / 2] = pack<NF4>(w.x, w.y);
+                                pw[(k + i) / 2] = pack<NF4>(w.x, w.y);
                             }
                         }
                         const float high = fmaxf(top[0], top[1]) * factor;
-                        if (!__any_sync(0xffffffffu, high > m + 8.f)) break;
-                        const float now = fmaxf(m, high), keep = m == -INFINITY ? 0.f : exp2_approx(m - now);
-                        m = now;
-                        l *= keep;
+                        const bool above = __any_sync(0xffffffffu, high > m + 8.f);
+                        if (!above && !grown) break;
+                        float keep = 1.f;
+                        if (above) {
+                            const float now = fmaxf(m, high);
+                            keep = m == -INFINITY ? 0.f : exp2_approx(m - now);
+                            m = now;
+                            l *= keep;
+                        }
+                        if (grown) keep *= ref_was * reciprocal_of_power(ref);
+                        grown = false;
                         if (j) {  // the products so far are done: the scores waited for came behind them
                             #pragma unroll 1
                             for (uint32_t k = 0; k < D; k += 32) {
@@ -323,51 +471,76 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                                 tmem_st32(to + k, v);
                             }
                         }
+                        if (!above) break;
                     }
-                    l += sum.x + sum.y;
+                    l += (sum.x + sum.y) * (NF4 ? __uint_as_float((uint32_t)(127 + less) << 23) : 1.f);
                     #pragma unroll
-                    for (uint32_t k = 0; k < N / 2; k += 32) tmem_st32(ts + k, p + k);
+                    for (uint32_t k = 0; k < N / 2; k += 32) tmem_st32(ts + k, pw + k);
                     ptx::tmem_wait_st();
                     ptx::tc_fence_before();
                     __syncwarp();
                     if (lane == 0) ptx::mbar_arrive(p_ready0 + 8 * tile);
                 }
-                if (ok && steps && !__all_sync(0xffffffffu, ptx::mbar_wait_suspended(s_full0 + 8 * tile, steps & 1u))) {
+                if (ok && !__all_sync(0xffffffffu, ptx::mbar_wait_suspended(s_full0 + 8 * tile, scores & 1u))) {
                     ok = false;
                     if (lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 24);
                 }
+                ++scores;
                 ptx::tc_fence_after();
-                if (s_bad || !ok) l = __uint_as_float(0x7fc00000u);  // NaN
-                const uint32_t out_row = s.row0 + row / a.group, h = head * a.group + row % a.group;
-                const uint64_t at = ((uint64_t)part * b.rows + out_row) * q_heads + h;
-                if (a.parts > 1 && real) a.part_ml[at] = make_float2(m, l);
-                const float f = (a.parts > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l) * v_power;
-                #pragma unroll
-                for (uint32_t k = 0; k < D; k += 32) {
-                    uint32_t v[32];
+                walk = s_walk[warp];
+                p = s_piece[warp];
+
+                // ---- the row's results, through this warp's part of Q's place (its products are done) so that whole rows go out ----
+                if (s_bad[piece & 7u] || !ok) l = __uint_as_float(0x7fc00000u);  // NaN
+                const bool whole = p.steps == p.all;
+                const uint64_t part = (uint64_t)(2 * blockIdx.x + (p.step0 ? 0 : 1)) * S::kRows + tile * 128;
+                if (!whole) a.part_ml[part + r] = make_float2(m, l);
+                const float f = (whole ? l == 0.f ? 0.f : 1.f / l : 1.f) * (NF4 ? ref : 1.f);
+                const uint32_t stage = q_tile + (warp & 3u) * (S::kQTile / 4);
+                constexpr uint32_t kRowBytes = 2 * D, kChunks = D / 8;  // a staged row: bf16 results, or half of a row's f32 sums
+                #pragma unroll 1
+                for (uint32_t half = 0; half < (whole ? 1u : 2u); ++half) {
+                    const uint32_t columns = whole ? D : D / 2;
                     __syncwarp();
-                    if (steps) {
-                        tmem_ld32(to + k, v);
+                    #pragma unroll 1
+                    for (uint32_t k = 0; k < columns; k += 32) {
+                        uint32_t v[32];
+                        tmem_ld32(to + half * columns + k, v);
                         ptx::tmem_wait_ld();
-                    }
-                    #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = steps ? __float_as_uint(__uint_as_float(v[i]) * f) : 0u;
-                    if (!real) continue;
-                    if (a.parts > 1) {
-                        if (!steps) continue;  // (a part without tokens is not read)
-                        uint4 *const o = reinterpret_cast<uint4 *>(a.part_o + at * D + k);
                         #pragma unroll
-                        for (int i = 0; i < 8; ++i) o[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                    } else {
-                        uint4 *const o = reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(a.out) + (uint64_t)out_row * a.ldo + (uint64_t)h * D + k);
-                        #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint32_t w[4];
+                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                        if (whole) {
                             #pragma unroll
-                            for (int e = 0; e < 4; ++e) w[e] = bf16_pair(__uint_as_float(v[8 * i + 2 * e]), __uint_as_float(v[8 * i + 2 * e + 1]));
-                            o[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                            for (uint32_t i = 0; i < 4; ++i) {
+                                uint32_t w[4];
+                                #pragma unroll
+                                for (int e = 0; e < 4; ++e) w[e] = bf16_pair(__uint_as_float(v[8 * i + 2 * e]), __uint_as_float(v[8 * i + 2 * e + 1]));
+                                st_shared_u4(stage + lane * kRowBytes + (((k / 8 + i) ^ (lane & 7u)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+                            }
+                        } else {
+                            #pragma unroll
+                            for (uint32_t i = 0; i < 8; ++i)
+                                st_shared_u4(stage + lane * kRowBytes + (((k / 4 + i) ^ (lane & 7u)) << 4), make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
                         }
                     }
+                    __syncwarp();
+                    #pragma unroll 4
+                    for (uint32_t i = lane; i < 32 * kChunks; i += 32) {
+                        const uint32_t rr = i / kChunks, x = i % kChunks, in_tile = (warp & 3u) * 32 + rr;
+                        if (tile * 128 + in_tile >= p.rows) continue;
+                        const uint4 v = ld_shared_u4(stage + rr * kRowBytes + ((x ^ (rr & 7u)) << 4));
+                        if (whole) {
+                            const uint32_t q_row = p.r0 + tile * 128 + in_tile, token = a.by_group.of(q_row);
+                            *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(a.out) + (uint64_t)(p.s.row0 + token) * a.ldo +
+                                                       (uint64_t)(p.head * a.group + q_row - token * a.group) * D + 8 * x) = v;
+                        } else {
+                            *reinterpret_cast<uint4 *>(a.part_o + (part + in_tile) * D + half * (D / 2) + 4 * x) = v;
+                        }
+                    }
+                }
+                if (!whole && p.step0 == 0 && tid == 0) {
+                    const uint32_t more = s_share.cta_of(p.line0 + kStart + p.all - 1) - blockIdx.x;
+                    splits[blockIdx.x] = Split{p.s.row0, p.r0, p.rows, p.head, more};
                 }
                 ptx::tc_fence_before();
             }
@@ -379,157 +552,207 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                 const uint32_t th = tid - 32 * kExpandWarp, q = th % kLanes, lane_word = table | lane * 4u;
                 // In which order a thread takes its four words: so that eight lanes' 16-byte stores hit all banks
                 const uint32_t order = D == 128 ? (q >> 1) * 2 : D == 256 ? q >> 1 : 0u;
-                for (uint32_t i = 0; i < 2 * steps; ++i) {
-                    const uint32_t rs = i % S::kRawSlots, slot = i % S::kSlots, raw = raw0 + rs * S::kRaw, to = ring0 + slot * S::kTile + (q >> 1) * S::kBox;
-                    bool got = ptx::mbar_wait_suspended(raw_full0 + 8 * rs, (i / S::kRawSlots) & 1u);
-                    if (got && i >= S::kSlots) got = ptx::mbar_wait_suspended(empty0 + 8 * slot, (i / S::kSlots + 1) & 1u);
-                    if (!__all_sync(0xffffffffu, got)) {
+                uint32_t i = 0;  // tiles so far: K's and V's in turn
+                auto wait = [&](uint32_t bar, uint32_t parity) {
+                    if (ok && !__all_sync(0xffffffffu, ptx::mbar_wait_suspended(bar, parity))) {
                         ok = false;
                         if (lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 25);
-                        break;
                     }
-                    const float unit = reciprocal_of_power(i & 1u ? v_power : k_power) * (1.f / kLevelUnit);
-                    const uint32_t t0 = t_first + (i >> 1) * N;
-                    #pragma unroll
-                    for (uint32_t pass = 0; pass < N / kPass; ++pass) {
-                        const uint32_t t = pass * kPass + th / kLanes;
-                        uint4 w = ld_shared_u4(raw + t * (D / 2) + q * 16);
-                        float scale;
-                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale) : "r"(raw + N * (D / 2) + (t * kBlocks + (q >> 1)) * 4) : "memory");
-                        scale = t0 + t < t_end ? scale * unit : 0.f;  // (behind the last token anything may stand)
-                        const uint32_t s2 = pack<true>(scale, scale);
-                        if (order & 2u) w = make_uint4(w.z, w.w, w.x, w.y);
-                        if (order & 1u) w = make_uint4(w.y, w.x, w.w, w.z);
-                        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+                };
+                while (ok && walk.next(c, b, a, p)) {
+                    const uint32_t t_end = min(visible_end(p.s, a.by_group, p.r0 + p.rows - 1), (p.step0 + p.steps) * N);
+                    for (uint32_t j = 0; ok && j < p.steps; ++j) {
+                        const uint32_t t0 = (p.step0 + j) * N;
+                        // the largest scales of the step
+                        float power[2];
                         #pragma unroll
-                        for (uint32_t k = 0; k < 4; ++k) {
-                            uint32_t v[4];
+                        for (uint32_t which = 0; which < 2; ++which) {
+                            const uint32_t rs = (i + which) % S::kRawSlots, from = raw0 + rs * S::kRaw + N * (D / 2);
+                            wait(raw_full0 + 8 * rs, ((i + which) / S::kRawSlots) & 1u);
+                            uint32_t most = 0;
                             #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const uint32_t word = words[k], at = ((e == 0 ? word << 7 : word >> (8 * e - 7)) & 0x7f80u) | lane_word;
-                                asm("ld.shared.u32 %0, [%1];" : "=r"(v[e]) : "r"(at));  // (free to move: the table stands)
-                                v[e] = mul_f16x2(v[e], s2);
+                            for (uint32_t k = 0; k < N * kBlocks / 128; ++k) {
+                                const uint32_t at = 4 * (k * 32 + lane);  // (a token's blocks, or tokens, together)
+                                const uint4 v = ld_shared_u4(from + 4 * at);
+                                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                                #pragma unroll
+                                for (uint32_t e = 0; e < 4; ++e) most = max(most, t0 + (at + e) / kBlocks < t_end ? w[e] : 0u);
                             }
-                            const uint32_t chunk = (q & 1u) * 4 + (k ^ order);
-                            st_shared_u4(to + t * 128 + ((chunk ^ (t & 7u)) << 4), make_uint4(v[0], v[1], v[2], v[3]));
+                            power[which] = power_above(__reduce_max_sync(0xffffffffu, most));
                         }
-                    }
-                    ptx::fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) {
-                        ptx::mbar_arrive(full0 + 8 * slot);
-                        ptx::mbar_arrive(raw_empty0 + 8 * rs);
+                        if (tid == 32 * kExpandWarp) {
+                            s_powers[(i >> 1) & 3u] = make_float2(power[0], power[1]);
+                            ptx::mbar_arrive(power0 + 8 * ((i >> 1) & 3u));
+                        }
+                        #pragma unroll 1
+                        for (uint32_t which = 0; which < 2; ++which, ++i) {
+                            const uint32_t rs = i % S::kRawSlots, slot = i % S::kSlots, raw = raw0 + rs * S::kRaw, dst = ring0 + slot * S::kTile + (q >> 1) * S::kBox;
+                            if (i >= S::kSlots) wait(empty0 + 8 * slot, (i / S::kSlots + 1) & 1u);
+                            if (!ok) break;
+                            const float unit = reciprocal_of_power(which ? power[1] : power[0]) * (1.f / kLevelUnit);
+                            uint4 raws[N / kPass];
+                            uint32_t factors[N / kPass];
+                            #pragma unroll
+                            for (uint32_t pass = 0; pass < N / kPass; ++pass) {
+                                const uint32_t t = pass * kPass + th / kLanes;
+                                raws[pass] = ld_shared_u4(raw + t * (D / 2) + q * 16);
+                                float scale;
+                                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale) : "r"(raw + N * (D / 2) + (t * kBlocks + (q >> 1)) * 4) : "memory");
+                                scale = t0 + t < t_end ? scale * unit : 0.f;  // (behind the last token anything may stand)
+                                factors[pass] = pack<true>(scale, scale);
+                            }
+                            #pragma unroll
+                            for (uint32_t pass = 0; pass < N / kPass; ++pass) {
+                                const uint32_t t = pass * kPass + th / kLanes, s2 = factors[pass];
+                                uint4 w = raws[pass];
+                                if (order & 2u) w = make_uint4(w.z, w.w, w.x, w.y);
+                                if (order & 1u) w = make_uint4(w.y, w.x, w.w, w.z);
+                                const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+                                #pragma unroll
+                                for (uint32_t k = 0; k < 4; ++k) {
+                                    uint32_t v[4];
+                                    #pragma unroll
+                                    for (int e = 0; e < 4; ++e) {
+                                        const uint32_t word = words[k], at = ((e == 0 ? word << 7 : word >> (8 * e - 7)) & 0x7f80u) | lane_word;
+                                        asm("ld.shared.u32 %0, [%1];" : "=r"(v[e]) : "r"(at));  // (free to move: the table stands)
+                                        v[e] = mul_f16x2(v[e], s2);
+                                    }
+                                    const uint32_t chunk = (q & 1u) * 4 + (k ^ order);
+                                    st_shared_u4(dst + t * 128 + ((chunk ^ (t & 7u)) << 4), make_uint4(v[0], v[1], v[2], v[3]));
+                                }
+                            }
+                            ptx::fence_proxy_async();
+                            __syncwarp();
+                            if (lane == 0) {
+                                ptx::mbar_arrive(full0 + 8 * slot);
+                                ptx::mbar_arrive(raw_empty0 + 8 * rs);
+                            }
+                        }
                     }
                 }
             } else if (warp == kCopyWarp) {
                 constexpr uint32_t kGroups = N / kGroup;
-                const uint32_t stored = min(s.length, t_first + steps * N);  // tokens that there are
-                for (uint32_t j = 0; j < steps; ++j) {
-                    const uint32_t t0 = t_first + j * N, g = lane % kGroups, box = lane / kGroups, t = t0 + g * kGroup;
-                    const uint32_t groups = min(kGroups, (stored - t0 + kGroup - 1) / kGroup);
-                    uint32_t place = 0;
-                    if (g < groups) {
-                        const uint32_t at = c.by_page.of(t);
-                        const int32_t page = __ldg(b.table + (uint64_t)seq * b.width + at);
-                        if (page >= 0 && (uint32_t)page < c.pages) place = ((uint32_t)page * c.heads + head) * c.page_size + (t - at * c.page_size);
-                    }
-                    for (uint32_t which = 0; which < 2; ++which) {
-                        const uint32_t i = 2 * j + which;
-                        bool got = true;
-                        if (NF4) {
-                            const uint32_t rs = i % S::kRawSlots, bar = raw_full0 + 8 * rs, to = raw0 + rs * S::kRaw;
-                            if (i >= S::kRawSlots) got = ptx::mbar_wait_suspended(raw_empty0 + 8 * rs, (i / S::kRawSlots + 1) & 1u);
-                            got = __all_sync(0xffffffffu, got);
-                            if (got) {
-                                if (lane == 0) ptx::mbar_arrive_expect_tx(bar, groups * (kGroup * (D / 2) + kGroup * kBlocks * 4));
-                                __syncwarp();
-                                if (box == 0 && g < groups) {
-                                    ptx::bulk_g2s(to + g * kGroup * (D / 2), static_cast<const uint8_t *>(which ? c.v : c.k) + (uint64_t)place * (D / 2), kGroup * (D / 2), bar);
-                                    ptx::bulk_g2s(to + N * (D / 2) + g * kGroup * kBlocks * 4, (which ? c.v_scales : c.k_scales) + (uint64_t)place * kBlocks,
-                                                  kGroup * kBlocks * 4, bar);
+                uint32_t i = 0, tails = 0;
+                for (uint32_t piece = 0; ok && walk.next(c, b, a, p); ++piece) {
+                    if (lane == 0) s_bad[piece & 7u] = 0;  // (the others are at most three pieces behind)
+                    __syncwarp();
+                    const uint32_t stored = min(p.s.length, (p.step0 + p.steps) * N);  // tokens that there are
+                    for (uint32_t j = 0; ok && j < p.steps; ++j) {
+                        const uint32_t t0 = (p.step0 + j) * N, g = lane % kGroups, box = lane / kGroups, t = t0 + g * kGroup;
+                        const uint32_t groups = stored > t0 ? min(kGroups, (stored - t0 + kGroup - 1) / kGroup) : 0u;
+                        uint32_t place = 0;
+                        if (g < groups) {
+                            const uint32_t at = c.by_page.of(t);
+                            const int32_t page = __ldg(b.table + (uint64_t)p.seq * b.width + at);
+                            if (page >= 0 && (uint32_t)page < c.pages) place = ((uint32_t)page * c.heads + p.head) * c.page_size + (t - at * c.page_size);
+                            else s_bad[piece & 7u] = 1;
+                        }
+                        __syncwarp();
+                        for (uint32_t which = 0; which < 2; ++which, ++i) {
+                            bool got = true;
+                            if (NF4) {
+                                const uint32_t rs = i % S::kRawSlots, bar = raw_full0 + 8 * rs, dst = raw0 + rs * S::kRaw;
+                                if (i >= S::kRawSlots) got = ptx::mbar_wait_suspended(raw_empty0 + 8 * rs, (i / S::kRawSlots + 1) & 1u);
+                                got = __all_sync(0xffffffffu, got);
+                                if (got) {
+                                    if (lane == 0) ptx::mbar_arrive_expect_tx(bar, groups * (kGroup * (D / 2) + kGroup * kBlocks * 4));
+                                    __syncwarp();
+                                    if (box == 0 && g < groups) {
+                                        ptx::bulk_g2s(dst + g * kGroup * (D / 2), static_cast<const uint8_t *>(which ? c.v : c.k) + (uint64_t)place * (D / 2), kGroup * (D / 2), bar);
+                                        ptx::bulk_g2s(dst + N * (D / 2) + g * kGroup * kBlocks * 4, (which ? c.v_scales : c.k_scales) + (uint64_t)place * kBlocks,
+                                                      kGroup * kBlocks * 4, bar);
+                                    }
+                                }
+                            } else {
+                                const uint32_t slot = i % S::kSlots, dst = ring0 + slot * S::kTile;
+                                if (i >= S::kSlots) got = ptx::mbar_wait_suspended(empty0 + 8 * slot, (i / S::kSlots + 1) & 1u);
+                                got = __all_sync(0xffffffffu, got);
+                                const bool tail = which && t0 + N > p.s.length;  // values that anything may stand behind: zeros, for weights of zero
+                                const uint32_t bar = tail ? tail_bar : full0 + 8 * slot;
+                                if (got) {
+                                    if (lane == 0) ptx::mbar_arrive_expect_tx(bar, groups * (kGroup * 128) * (D / 64));
+                                    __syncwarp();
+                                    if (g < groups && box < D / 64)
+                                        ptx::tma_load_2d(dst + box * S::kBox + g * (kGroup * 128), which ? &tmap_v : &tmap_k, (int32_t)(64 * box), (int32_t)place, bar);
+                                }
+                                if (got && tail) {
+                                    got = __all_sync(0xffffffffu, ptx::mbar_wait_suspended(tail_bar, tails & 1u));
+                                    ++tails;
+                                    for (uint32_t k = (p.s.length > t0 ? p.s.length - t0 : 0u) * 8 + lane; k < N * 8; k += 32)
+                                        #pragma unroll
+                                        for (uint32_t x = 0; x < D / 64; ++x) st_shared_u4(dst + x * S::kBox + k * 16, make_uint4(0u, 0u, 0u, 0u));
+                                    ptx::fence_proxy_async();
+                                    __syncwarp();
+                                    if (lane == 0) ptx::mbar_arrive(full0 + 8 * slot);
                                 }
                             }
-                        } else {
-                            const uint32_t slot = i % S::kSlots, to = ring0 + slot * S::kTile;
-                            if (i >= S::kSlots) got = ptx::mbar_wait_suspended(empty0 + 8 * slot, (i / S::kSlots + 1) & 1u);
-                            got = __all_sync(0xffffffffu, got);
-                            const bool tail = which && t0 + N > s.length;  // values that anything may stand behind: zeros, for weights of zero
-                            const uint32_t bar = tail ? tail_bar : full0 + 8 * slot;
-                            if (got) {
-                                if (lane == 0) ptx::mbar_arrive_expect_tx(bar, groups * (kGroup * 128) * (D / 64));
-                                __syncwarp();
-                                if (g < groups && box < D / 64)
-                                    ptx::tma_load_2d(to + box * S::kBox + g * (kGroup * 128), which ? &tmap_v : &tmap_k, (int32_t)(64 * box), (int32_t)place, bar);
+                            if (!got) {
+                                ok = false;
+                                if (lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 26);
+                                break;
                             }
-                            if (got && tail) {
-                                got = __all_sync(0xffffffffu, ptx::mbar_wait_suspended(tail_bar, 0));  // (once in a CTA's life)
-                                for (uint32_t k = (s.length - t0) * 8 + lane; k < N * 8; k += 32)
-                                    #pragma unroll
-                                    for (uint32_t x = 0; x < D / 64; ++x) st_shared_u4(to + x * S::kBox + k * 16, make_uint4(0u, 0u, 0u, 0u));
-                                ptx::fence_proxy_async();
-                                __syncwarp();
-                                if (lane == 0) ptx::mbar_arrive(full0 + 8 * slot);
-                            }
-                        }
-                        if (!got) {
-                            ok = false;
-                            if (lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 26);
-                            break;
                         }
                     }
-                    if (!ok) break;
                 }
-            } else if (warp == kMmaWarp && steps) {
+            } else if (warp == kMmaWarp) {
                 constexpr uint32_t fmt = NF4 ? 0 : 1;
                 constexpr uint32_t idesc_s = ptx::f16_idesc(fmt, 128, N, false, false), idesc_o = ptx::f16_idesc(fmt, 128, D, false, true);
+                uint32_t i = 0, weights[2] = {0, 0}, rows_in[2] = {0, 0};  // tiles of K and V, weights and Q's waited for so far
                 auto wait = [&](uint32_t bar, uint32_t parity) {
                     if (!ok) return;
                     ok = __all_sync(0xffffffffu, ptx::mbar_wait_suspended(bar, parity));
                     if (!ok && lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 27);
                 };
-                auto wait_full = [&](uint32_t i) { wait(full0 + 8 * (i % S::kSlots), (i / S::kSlots) & 1u); };
-                auto scores = [&](uint32_t tile, uint32_t i) {  // of the keys in ring place i
-                    const uint64_t qd = ptx::sw128_desc(q0 + tile * S::kQTile), kd = ptx::sw128_desc(ring0 + i % S::kSlots * S::kTile);
+                auto wait_full = [&](uint32_t at) { wait(full0 + 8 * (at % S::kSlots), (at / S::kSlots) & 1u); };
+                auto scores = [&](uint32_t tile, uint32_t at) {  // of the keys in ring place `at`
+                    const uint64_t qd = ptx::sw128_desc(q0 + tile * S::kQTile), kd = ptx::sw128_desc(ring0 + at % S::kSlots * S::kTile);
                     #pragma unroll
                     for (uint32_t k = 0; k < D / 16; ++k)
                         ptx::mma_ss_f16(tmem + S::kS + tile * N, qd + (k >> 2) * (16384 >> 4) + (k & 3u) * 2, kd + (k >> 2) * (S::kBox >> 4) + (k & 3u) * 2, idesc_s, k != 0);
                     ptx::tc_commit(s_full0 + 8 * tile);
                 };
-                auto products = [&](uint32_t tile, uint32_t i, bool add) {
-                    const uint64_t vd = ptx::sw128_desc(ring0 + i % S::kSlots * S::kTile, S::kBox);
+                auto products = [&](uint32_t tile, uint32_t at, bool add) {
+                    const uint64_t vd = ptx::sw128_desc(ring0 + at % S::kSlots * S::kTile, S::kBox);
                     #pragma unroll
                     for (uint32_t k = 0; k < N / 16; ++k) ptx::mma_ts_f16(tmem + S::kO + tile * D, tmem + S::kS + tile * N + 8 * k, vd + 128 * k, idesc_o, add || k != 0);
                 };
-                wait_full(0);
-                ptx::tc_fence_after();
-                if (ok && ptx::elect_one()) {
-                    for (uint32_t t = 0; t < live; ++t) scores(t, 0);
-                    ptx::tc_commit(empty0);
-                }
-                __syncwarp();
-                for (uint32_t j = 0; j < steps && ok; ++j) {
-                    const uint32_t iv = 2 * j + 1, ik = 2 * j + 2;
-                    const bool more = j + 1 < steps;
-                    wait_full(iv);
-                    for (uint32_t t = 0; t < live; ++t) {
-                        wait(p_ready0 + 8 * t, j & 1u);
-                        if (!ok) break;
+                while (ok && walk.next(c, b, a, p)) {
+                    wait_full(i);
+                    for (uint32_t t = 0; t < p.live; ++t) {
+                        wait(q_ready0 + 8 * t, rows_in[t] & 1u);
+                        ++rows_in[t];
                         ptx::tc_fence_after();
-                        if (ptx::elect_one()) {
-                            products(t, iv, j != 0);
-                            if (t + 1 == live) ptx::tc_commit(empty0 + 8 * (iv % S::kSlots));
-                            if (!more) ptx::tc_commit(s_full0 + 8 * t);
+                        if (ok && ptx::elect_one()) {
+                            scores(t, i);
+                            if (t + 1 == p.live) ptx::tc_commit(empty0 + 8 * (i % S::kSlots));
                         }
                         __syncwarp();
-                        if (!more) continue;
-                        if (t == 0) wait_full(ik);
-                        if (!ok) break;
-                        ptx::tc_fence_after();
-                        if (ptx::elect_one()) {
-                            scores(t, ik);
-                            if (t + 1 == live) ptx::tc_commit(empty0 + 8 * (ik % S::kSlots));
+                    }
+                    for (uint32_t j = 0; j < p.steps && ok; ++j, i += 2) {
+                        const uint32_t iv = i + 1, ik = i + 2;
+                        const bool more = j + 1 < p.steps;
+                        wait_full(iv);
+                        for (uint32_t t = 0; t < p.live; ++t) {
+                            wait(p_ready0 + 8 * t, weights[t] & 1u);
+                            ++weights[t];
+                            if (!ok) break;
+                            ptx::tc_fence_after();
+                            if (ptx::elect_one()) {
+                                products(t, iv, j != 0);
+                                if (t + 1 == p.live) ptx::tc_commit(empty0 + 8 * (iv % S::kSlots));
+                                if (!more) ptx::tc_commit(s_full0 + 8 * t);
+                            }
+                            __syncwarp();
+                            if (!more) continue;
+                            if (t == 0) wait_full(ik);
+                            if (!ok) break;
+                            ptx::tc_fence_after();
+                            if (ptx::elect_one()) {
+                                scores(t, ik);
+                                if (t + 1 == p.live) ptx::tc_commit(empty0 + 8 * (ik % S::kSlots));
+                            }
+                            __syncwarp();
                         }
-                        __syncwarp();
                     }
                 }
             }
@@ -544,8 +767,64 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     }
 }
 
+// The row tiles that several CTAs had: a warp to four rows at a time, the parts in the order of the tokens.
+constexpr uint32_t kJoinRows = 4, kJoinWarps = 8;
 template <int D, bool NF4>
-int32_t launch(const AttentionCall &c, cudaStream_t stream) {
+__global__ void __launch_bounds__(32 * kJoinWarps)
+join_pieces_kernel(const AttentionView a, const Split *const splits) {
+    constexpr uint32_t kRows = Shape<D, NF4>::kRows, kWide = D / 32;  // values of a row to a lane
+    ptx::pdl_launch_dependents();
+    ptx::pdl_wait();
+    const Split s = splits[blockIdx.x];
+    const uint32_t r0 = (blockIdx.y * kJoinWarps + threadIdx.x / 32) * kJoinRows, lane = threadIdx.x & 31u;
+    if (r0 >= s.rows) return;
+    auto part = [&](uint32_t i) { return (uint64_t)(2 * (blockIdx.x + i) + (i ? 0 : 1)) * kRows + r0; };
+    float m[kJoinRows], sum[kJoinRows], acc[kJoinRows][kWide];
+    #pragma unroll
+    for (uint32_t r = 0; r < kJoinRows; ++r) {
+        m[r] = -INFINITY;
+        sum[r] = 0.f;
+        #pragma unroll
+        for (uint32_t j = 0; j < kWide; ++j) acc[r][j] = 0.f;
+    }
+    #pragma unroll 2
+    for (uint32_t i = 0; i <= s.more; ++i) {
+        #pragma unroll
+        for (uint32_t r = 0; r < kJoinRows; ++r) {  // (a tile's rows behind its last hold anything; they are not written)
+            const float2 ml = __ldg(a.part_ml + part(i) + r);
+            float v[kWide];
+            const float *const o = a.part_o + (part(i) + r) * D + lane * kWide;
+            #pragma unroll
+            for (uint32_t j = 0; j < kWide; j += 2) {
+                const float2 w = __ldg(reinterpret_cast<const float2 *>(o + j));
+                v[j] = w.x;
+                v[j + 1] = w.y;
+            }
+            const float top = fmaxf(m[r], ml.x), base = top == -INFINITY ? 0.f : top;
+            const float keep = exp2_approx(m[r] - base), f = exp2_approx(ml.x - base);  // (nothing seen: 2^-inf)
+            m[r] = top;
+            sum[r] = fmaf(f, ml.y, sum[r] * keep);
+            #pragma unroll
+            for (uint32_t j = 0; j < kWide; ++j) acc[r][j] = fmaf(f, v[j], acc[r][j] * keep);
+        }
+    }
+    #pragma unroll
+    for (uint32_t r = 0; r < kJoinRows; ++r) {
+        if (r0 + r >= s.rows) break;
+        const float f = sum[r] == 0.f ? 0.f : 1.f / sum[r];
+        const uint32_t q_row = s.r0 + r0 + r, token = a.by_group.of(q_row);
+        __nv_bfloat16 *const out = static_cast<__nv_bfloat16 *>(a.out) + (uint64_t)(s.row0 + token) * a.ldo + (uint64_t)(s.head * a.group + q_row - token * a.group) * D + lane * kWide;
+        #pragma unroll
+        for (uint32_t j = 0; j < kWide; j += 2) *reinterpret_cast<uint32_t *>(out + j) = bf16_pair(acc[r][j] * f, acc[r][j + 1] * f);
+    }
+}
+
+uint64_t rows_of(const AttentionCall &c) { return c.head_dim == 256 ? 128 : 256; }
+uint64_t ml_bytes(const AttentionCall &c) { return 2ull * kNumSMs * rows_of(c) * sizeof(float2); }
+constexpr uint64_t kSplitBytes = (kNumSMs * sizeof(Split) + 255) / 256 * 256;
+
+template <int D, bool NF4>
+int32_t launch(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) {
     using S = Shape<D, NF4>;
     auto kernel = attention_chunk_kernel<D, NF4>;
     NF4_TRY(ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), S::kSmem));
@@ -557,25 +836,31 @@ int32_t launch(const AttentionCall &c, cudaStream_t stream) {
     }
     FailureRef failure;
     NF4_TRY(prefill_failure_ref(&failure));
-    const uint32_t tiles = attention_chunk_tiles(c);
-    if ((uint64_t)tiles * c.cache.heads >= 1ull << 31) return fail(NF4_ERR_UNSUPPORTED, "attention: too many rows in a call");
-    count_launch();
-    return launch_maybe_overlapped(kernel, dim3(tiles * c.cache.heads, c.view.parts), dim3(kThreads), S::kSmem, stream, true, map_k, map_v, c.cache, c.batch,
-                                   c.view, tiles, failure);
+    // the line is counted in 32 bits
+    const uint64_t tiles = ((uint64_t)c.batch.rows * c.view.group / S::kRows + c.batch.sequences) * c.cache.heads;
+    const uint64_t steps = ((uint64_t)c.batch.width * c.cache.page_size + S::kTokens - 1) / S::kTokens;
+    if (tiles * (steps + 1 + kStart) >= 1ull << 31) return fail(NF4_ERR_UNSUPPORTED, "attention: rows times tokens are too many for a call; split it");
+    Split *const splits = reinterpret_cast<Split *>(workspace + kAttentionFlagBytes);
+    AttentionView view = c.view;
+    view.part_ml = reinterpret_cast<float2 *>(workspace + kAttentionFlagBytes + kSplitBytes);
+    view.part_o = reinterpret_cast<float *>(workspace + kAttentionFlagBytes + kSplitBytes + ml_bytes(c));
+    const uint32_t ctas = persistent_ctas();
+    count_launch(2);
+    NF4_TRY(launch_maybe_overlapped(kernel, dim3(ctas), dim3(kThreads), S::kSmem, stream, true, map_k, map_v, c.cache, c.batch, view, splits, failure));
+    return launch_maybe_overlapped(join_pieces_kernel<D, NF4>, dim3(ctas, S::kRows / (kJoinRows * kJoinWarps)), dim3(32 * kJoinWarps), 0, stream, true, view, static_cast<const Split *>(splits));
 }
 
 }  // namespace
 
-uint32_t attention_chunk_tiles(const AttentionCall &c) {
-    const uint32_t rows = c.head_dim == 256 ? 128 : 256;
-    return (uint32_t)((uint64_t)c.batch.rows * c.view.group / rows) + c.batch.sequences;
+uint64_t attention_chunk_bytes(const AttentionCall &c) {
+    return kAttentionFlagBytes + kSplitBytes + ml_bytes(c) + 2ull * kNumSMs * rows_of(c) * c.head_dim * sizeof(float);
 }
 
-int32_t attention_chunk(const AttentionCall &c, cudaStream_t stream) {
+int32_t attention_chunk(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) {
     switch (c.head_dim) {
-        case 64: return c.nf4 ? launch<64, true>(c, stream) : launch<64, false>(c, stream);
-        case 128: return c.nf4 ? launch<128, true>(c, stream) : launch<128, false>(c, stream);
-        default: return c.nf4 ? launch<256, true>(c, stream) : launch<256, false>(c, stream);
+        case 64: return c.nf4 ? launch<64, true>(c, workspace, stream) : launch<64, false>(c, workspace, stream);
+        case 128: return c.nf4 ? launch<128, true>(c, workspace, stream) : launch<128, false>(c, workspace, stream);
+        default: return c.nf4 ? launch<256, true>(c, workspace, stream) : launch<256, false>(c, workspace, stream);
     }
 }
 

@@ -114,9 +114,8 @@ constexpr uint64_t kAttentionFlagBytes = 4096;  // at the start of a workspace, 
 uint64_t attention_decode_bytes(const AttentionCall &c);
 int32_t attention_decode(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream);
 
-// attention_chunk.cu: bf16 tensors, many rows.  Row tiles that the call's rows can make of one head, whatever row_starts says; parts
-// as c.view has them.
-uint32_t attention_chunk_tiles(const AttentionCall &c);
-int32_t attention_chunk(const AttentionCall &c, cudaStream_t stream);
+// attention_chunk.cu: bf16 tensors, many rows
+uint64_t attention_chunk_bytes(const AttentionCall &c);
+int32_t attention_chunk(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream);
 
 }  // namespace nf4
