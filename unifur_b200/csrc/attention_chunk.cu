@@ -11,7 +11,9 @@
 //   S = Q K^T   both operands from shared memory, 128 x 128 f32 sums in tensor memory
 //   O += P V    P from tensor memory, where the softmax warps have put it over S; V as it lies, MN-major
 // A softmax thread owns a row: it reads S, keeps the row's largest exponent m and sum l, and writes P = 2^(S c - m + 7) back as f16
-// (bf16 with a bf16 cache).  While one tile's softmax runs, the other's two products do.  m is the largest exponent so far or up to 8
+// (bf16 with a bf16 cache).  While one tile's softmax runs, the other's two products do.  (64 tokens a step and two places for S, so that a step's scores are
+// there when the last one's weights are done, were tried: a first product of 64 columns takes as long as one of 128, A's rows being read for half
+// the work, and 128 tokens of two tiles took 6100 cycles instead of 4270.)  m is the largest exponent so far or up to 8
 // below it: O is rescaled only where a row rises above that, by the warps themselves, at a moment when
 // no product is writing it.  Copies and lookups run ahead into the next piece while a row tile's results are written.
 // f16's range: K's and V's scales are divided by a power of two of a step's largest, a row of Q by its own (exact).  K's comes back as a
@@ -41,13 +43,17 @@ template <int D, bool NF4>
 struct Shape {
     static constexpr uint32_t kTiles = D == 256 ? 1 : 2, kRows = 128 * kTiles;
     static constexpr uint32_t kTokens = D == 256 ? 64 : 128;          // of a step
+    // S's places to a tile: with a dim of 256 there is room for two, so that the next step's scores come while weights are made
+    static constexpr uint32_t kPlaces = D == 256 ? 2 : 1;
     static constexpr uint32_t kBlocks = D / 64;
     static constexpr uint32_t kQTile = 128 * D * 2, kTile = kTokens * D * 2, kBox = kTokens * 128;
-    static constexpr uint32_t kRaw = NF4 ? kTokens * (D / 2 + 4 * kBlocks) : 0, kRawSlots = 3;
-    static constexpr uint32_t kSlots = NF4 ? (D == 64 ? 4 : 3) : 4;
+    static constexpr uint32_t kScales = kTokens * kBlocks * 4;
+    // a tile's codes and scales, and with K's the V's scales of the step: their power goes to the softmax ahead of V
+    static constexpr uint32_t kRaw = NF4 ? kTokens * D / 2 + 2 * kScales : 0, kRawSlots = D == 64 ? 5 : 2;
+    static constexpr uint32_t kSlots = D == 64 ? (NF4 ? 6 : 8) : NF4 ? 3 : 4;
     // codes, then the table on a multiple of its 32 KB, then Q, then the ring (bf16: Q, then the ring)
     static constexpr uint32_t kSmem = (NF4 ? 65536 : 2048) - 1024 + kTiles * kQTile + kSlots * kTile;
-    static constexpr uint32_t kS = 0, kO = 256;                       // columns of tensor memory
+    static constexpr uint32_t kS = 0, kO = 256;                       // columns of tensor memory: the tiles' S's, then O's
 };
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *r) {
@@ -103,6 +109,11 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint4 ld_shared_u4(uint32_t addr) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 ld_shared_f2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
     return v;
 }
 __device__ __forceinline__ void st_shared_u4(uint32_t addr, uint4 v) {
@@ -182,32 +193,57 @@ struct Walker {  // through a CTA's pieces; every warp goes its own way
     }
 };
 
+// A quantized cache's keys and values expanded to f16 once for all row tiles, by a kernel ahead: a step's tokens of a head are a tile of
+// kTokens rows, zeros behind the sequence's last token.
+struct Dense {
+    uint32_t capacity;        // tiles to a head that there is room for; 0: codes are expanded where they are used
+    const uint32_t *bases;    // [sequences] a sequence's first tile, and behind them [sequences]: all tiles
+    const float2 *powers;     // [tile][head] what K's and V's scales are divided by
+};
+
 // What the join has to know of a row tile that several CTAs have: written by the CTA in whose share it begins, rows 0 by the others.
 struct Split {
     uint32_t row0, r0, rows, head, more;  // more: CTAs behind the first
 };
 
+// In which order a piece's tiles of K and V come: K 0, V 0, K 1, V 1, ...; with two places for S K 0, K 1, V 0, K 2, V 1, ..., V n - 1.
+template <uint32_t kPlaces>
+struct Turn {
+    uint32_t values, step;
+    __device__ __forceinline__ Turn(uint32_t turn, uint32_t steps) {
+        if (kPlaces == 1) {
+            values = turn & 1u;
+            step = turn / 2;
+            return;
+        }
+        const bool last = turn + 1 == 2 * steps;
+        values = last || (turn && !(turn & 1u)) ? 1 : 0;
+        step = last ? steps - 1 : values ? turn / 2 - 1 : (turn + 1) / 2;
+    }
+};
+
 template <int D, bool NF4>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const CacheView c, const BatchView b,
-                       const AttentionView a, Split *const splits, const FailureRef failure) {
+                       const AttentionView a, const Dense dense, Split *const splits, const FailureRef failure) {
     using S = Shape<D, NF4>;
     using Walk = Walker<S::kRows, S::kTokens>;
-    constexpr uint32_t N = S::kTokens, kBlocks = S::kBlocks;
+    constexpr uint32_t N = S::kTokens, kBlocks = S::kBlocks, kPlaces = S::kPlaces;
     extern __shared__ uint8_t smem_any[];
-    __shared__ __align__(8) uint64_t s_bars[25];
+    __shared__ __align__(8) uint64_t s_bars[39];
     __shared__ uint32_t s_tmem, s_bad[8], s_first[6];  // s_bad: of the last pieces, whether a page was not there
     __shared__ Share s_share;
     __shared__ Walk s_walk[8];
     __shared__ Piece s_piece[8];
     __shared__ float s_qpower[S::kRows];
-    __shared__ float2 s_powers[4];  // of the last steps' K and V
+    __shared__ float2 s_powers[8];  // of the last steps' K and V (who writes them is at most four steps ahead of who reads)
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u;
     const uint32_t base = ptx::smem_addr(smem_any);
     const uint32_t raw0 = (base + 15u) & ~15u, table = (raw0 + S::kRawSlots * S::kRaw + 32767u) & ~32767u;
     const uint32_t q0 = NF4 ? table + 32768u : (base + 1023u) & ~1023u, ring0 = q0 + S::kTiles * S::kQTile;
-    const uint32_t bars = ptx::smem_addr(s_bars), full0 = bars, empty0 = bars + 32, raw_full0 = bars + 64, raw_empty0 = bars + 88, s_full0 = bars + 112,
-                   p_ready0 = bars + 128, tail_bar = bars + 144, q_ready0 = bars + 152, power0 = bars + 168;
+    // s_full, p_ready: of a tile's two places
+    const uint32_t bars = ptx::smem_addr(s_bars), full0 = bars, empty0 = bars + 64, raw_full0 = bars + 128, raw_empty0 = bars + 168, s_full0 = bars + 208,
+                   p_ready0 = bars + 240, pv_done0 = bars + 272, q_ready0 = bars + 288, tail_bar = bars + 304;
     if (ring0 + S::kSlots * S::kTile > base + S::kSmem) {
         ptx::pdl_wait();
         if (tid == 0) {
@@ -221,16 +257,18 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             ptx::mbar_init(full0 + 8 * i, NF4 ? 4 : 1);
             ptx::mbar_init(empty0 + 8 * i, 1);
         }
-        for (uint32_t i = 0; i < 3; ++i) {
+        for (uint32_t i = 0; i < S::kRawSlots; ++i) {
             ptx::mbar_init(raw_full0 + 8 * i, 1);
             ptx::mbar_init(raw_empty0 + 8 * i, 4);
         }
-        for (uint32_t i = 0; i < 2; ++i) {
+        for (uint32_t i = 0; i < 4; ++i) {
             ptx::mbar_init(s_full0 + 8 * i, 1);
             ptx::mbar_init(p_ready0 + 8 * i, 4);
+        }
+        for (uint32_t i = 0; i < 2; ++i) {
+            ptx::mbar_init(pv_done0 + 8 * i, 1);
             ptx::mbar_init(q_ready0 + 8 * i, 4);
         }
-        for (uint32_t i = 0; i < 4; ++i) ptx::mbar_init(power0 + 8 * i, 1);
         ptx::mbar_init(tail_bar, 1);
         ptx::fence_mbar_init();
         ptx::fence_proxy_async();
@@ -338,6 +376,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     ptx::tc_fence_after();
     const uint32_t tmem = s_tmem;
     bool ok = true;
+    const bool expanded = NF4 && dense.capacity && __ldg(dense.bases + b.sequences) <= dense.capacity;  // (more tokens than the host knew of: not)
     if (s_first[4] < s_first[5]) {
         Walk walk{sequence_of(c, b, s_first[0]), s_first[0], s_first[1], s_first[2], s_first[3], s_first[4], s_first[5]};
         Piece p;
@@ -345,9 +384,9 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
             const uint32_t tile = warp >> 2, r = tid & 127u;
             const uint32_t lanes = (warp & 3u) << 21;  // a warp reaches its quarter of tensor memory's lanes
-            const uint32_t ts = tmem + S::kS + tile * N + lanes, to = tmem + S::kO + tile * D + lanes;
+            const uint32_t ts0 = tmem + S::kS + kPlaces * tile * N + lanes, to = tmem + S::kO + tile * D + lanes;
             const uint32_t q_tile = q0 + tile * S::kQTile;
-            uint32_t scores = 0, step = 0, piece = 0;  // scores of this tile, steps and pieces of the CTA, so far
+            uint32_t scores = 0, step = 0, piece = 0;  // steps of this tile, steps and pieces of the CTA, so far
             for (; ok && walk.next(c, b, a, p); step += p.steps, ++piece) {
                 if (tile >= p.live) continue;
                 // (what the steps do not need waits in shared memory: registers are short there)
@@ -402,9 +441,8 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                 const float row_factor = fabsf(a.scale_log2) * (NF4 ? s_qpower[tile * 128 + r] : 1.f);
                 float m = -INFINITY, l = 0.f, ref = 0.f;
                 for (uint32_t j = 0; j < steps; ++j, ++scores) {
-                    bool got = ptx::mbar_wait_suspended(s_full0 + 8 * tile, scores & 1u);
-                    if (NF4) got = got && ptx::mbar_wait_suspended(power0 + 8 * ((step + j) & 3u), ((step + j) >> 2) & 1u);
-                    if (!__all_sync(0xffffffffu, got)) {
+                    const uint32_t place = kPlaces * tile + scores % kPlaces, ts = ts0 + scores % kPlaces * N;
+                    if (!__all_sync(0xffffffffu, ptx::mbar_wait_suspended(s_full0 + 8 * place, (scores / kPlaces) & 1u))) {
                         ok = false;
                         if (lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 23);
                         break;
@@ -412,7 +450,8 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                     ptx::tc_fence_after();
                     const uint32_t t0 = t_first + j * N, lim = sees > t0 ? sees - t0 : 0u;
                     const bool masked = t0 + N > sees_first;
-                    const float2 powers = NF4 ? s_powers[(step + j) & 3u] : make_float2(1.f, 1.f);
+                    // (written before the keys' arrival was made known, which the scores are behind)
+                    const float2 powers = NF4 ? ld_shared_f2(ptx::smem_addr(s_powers + ((step + j) & 7u))) : make_float2(1.f, 1.f);
                     const float factor = fmaxf(row_factor * powers.x, 1.2e-38f);
                     const float ref_was = ref;
                     if (NF4) ref = fmaxf(ref, powers.y);
@@ -460,7 +499,13 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                         }
                         if (grown) keep *= ref_was * reciprocal_of_power(ref);
                         grown = false;
-                        if (j) {  // the products so far are done: the scores waited for came behind them
+                        if (j) {  // once the products so far are done
+                            if (!__all_sync(0xffffffffu, ptx::mbar_wait_suspended(pv_done0 + 8 * tile, (scores - 1) & 1u))) {
+                                ok = false;
+                                if (lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 28);
+                                break;
+                            }
+                            ptx::tc_fence_after();
                             #pragma unroll 1
                             for (uint32_t k = 0; k < D; k += 32) {
                                 uint32_t v[32];
@@ -473,19 +518,24 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                         }
                         if (!above) break;
                     }
+                    if (!ok) break;
                     l += (sum.x + sum.y) * (NF4 ? __uint_as_float((uint32_t)(127 + less) << 23) : 1.f);
                     #pragma unroll
                     for (uint32_t k = 0; k < N / 2; k += 32) tmem_st32(ts + k, pw + k);
                     ptx::tmem_wait_st();
                     ptx::tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(p_ready0 + 8 * tile);
+                    if (lane == 0) ptx::mbar_arrive(p_ready0 + 8 * place);
                 }
-                if (ok && !__all_sync(0xffffffffu, ptx::mbar_wait_suspended(s_full0 + 8 * tile, scores & 1u))) {
+                // With two places for S the products may be two steps behind (the last scores came behind those of three steps ago), and a
+                // parity tells only the last round from the one before it: both are waited for in turn.
+                bool done = ok;
+                if (done && kPlaces > 1 && scores > 1) done = ptx::mbar_wait_suspended(pv_done0 + 8 * tile, (scores - 2) & 1u);
+                if (done) done = ptx::mbar_wait_suspended(pv_done0 + 8 * tile, (scores - 1) & 1u);
+                if (ok && !__all_sync(0xffffffffu, done)) {
                     ok = false;
                     if (lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 24);
                 }
-                ++scores;
                 ptx::tc_fence_after();
                 walk = s_walk[warp];
                 p = s_piece[warp];
@@ -546,50 +596,48 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             }
         } else {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-            if (NF4 && warp >= kExpandWarp && warp < kExpandWarp + 4) {
+            if (NF4 && !expanded && warp >= kExpandWarp && warp < kExpandWarp + 4) {
                 // ---- codes to f16: a thread has 16 bytes of a token's row, 32 values ----
                 constexpr uint32_t kLanes = D / 32, kPass = 128 / kLanes;
                 const uint32_t th = tid - 32 * kExpandWarp, q = th % kLanes, lane_word = table | lane * 4u;
                 // In which order a thread takes its four words: so that eight lanes' 16-byte stores hit all banks
                 const uint32_t order = D == 128 ? (q >> 1) * 2 : D == 256 ? q >> 1 : 0u;
-                uint32_t i = 0;  // tiles so far: K's and V's in turn
+                uint32_t i = 0, step = 0;  // tiles and steps so far
                 auto wait = [&](uint32_t bar, uint32_t parity) {
                     if (ok && !__all_sync(0xffffffffu, ptx::mbar_wait_suspended(bar, parity))) {
                         ok = false;
                         if (lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 25);
                     }
                 };
-                while (ok && walk.next(c, b, a, p)) {
+                for (; ok && walk.next(c, b, a, p); step += p.steps) {
                     const uint32_t t_end = min(visible_end(p.s, a.by_group, p.r0 + p.rows - 1), (p.step0 + p.steps) * N);
-                    for (uint32_t j = 0; ok && j < p.steps; ++j) {
-                        const uint32_t t0 = (p.step0 + j) * N;
-                        // the largest scales of the step
-                        float power[2];
-                        #pragma unroll
-                        for (uint32_t which = 0; which < 2; ++which) {
-                            const uint32_t rs = (i + which) % S::kRawSlots, from = raw0 + rs * S::kRaw + N * (D / 2);
-                            wait(raw_full0 + 8 * rs, ((i + which) / S::kRawSlots) & 1u);
+                    #pragma unroll 1
+                    for (uint32_t turn = 0; ok && turn < 2 * p.steps; ++turn, ++i) {
+                        const Turn<kPlaces> of(turn, p.steps);
+                        const uint32_t which = of.values, j = of.step, t0 = (p.step0 + j) * N;
+                        const uint32_t rs = i % S::kRawSlots, slot = i % S::kSlots, raw = raw0 + rs * S::kRaw, dst = ring0 + slot * S::kTile + (q >> 1) * S::kBox;
+                        wait(raw_full0 + 8 * rs, (i / S::kRawSlots) & 1u);
+                        // the power above the tile's largest scale
+                        auto power_of = [&](uint32_t from) {
                             uint32_t most = 0;
                             #pragma unroll
-                            for (uint32_t k = 0; k < N * kBlocks / 128; ++k) {
-                                const uint32_t at = 4 * (k * 32 + lane);  // (a token's blocks, or tokens, together)
-                                const uint4 v = ld_shared_u4(from + 4 * at);
-                                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-                                #pragma unroll
-                                for (uint32_t e = 0; e < 4; ++e) most = max(most, t0 + (at + e) / kBlocks < t_end ? w[e] : 0u);
+                            for (uint32_t k = 0; k < N * kBlocks / 64; ++k) {
+                                const uint32_t at = 2 * (k * 32 + lane);  // (a token's blocks, or tokens, together)
+                                const float2 v = ld_shared_f2(from + 4 * at);
+                                most = max(most, t0 + at / kBlocks < t_end ? __float_as_uint(v.x) : 0u);
+                                most = max(most, t0 + (at + 1) / kBlocks < t_end ? __float_as_uint(v.y) : 0u);
                             }
-                            power[which] = power_above(__reduce_max_sync(0xffffffffu, most));
+                            return power_above(__reduce_max_sync(0xffffffffu, most));
+                        };
+                        const float power = power_of(raw + N * (D / 2));
+                        if (!which) {
+                            const float v_power = power_of(raw + N * (D / 2) + S::kScales);
+                            if (tid == 32 * kExpandWarp) s_powers[(step + j) & 7u] = make_float2(power, v_power);
                         }
-                        if (tid == 32 * kExpandWarp) {
-                            s_powers[(i >> 1) & 3u] = make_float2(power[0], power[1]);
-                            ptx::mbar_arrive(power0 + 8 * ((i >> 1) & 3u));
-                        }
-                        #pragma unroll 1
-                        for (uint32_t which = 0; which < 2; ++which, ++i) {
-                            const uint32_t rs = i % S::kRawSlots, slot = i % S::kSlots, raw = raw0 + rs * S::kRaw, dst = ring0 + slot * S::kTile + (q >> 1) * S::kBox;
-                            if (i >= S::kSlots) wait(empty0 + 8 * slot, (i / S::kSlots + 1) & 1u);
-                            if (!ok) break;
-                            const float unit = reciprocal_of_power(which ? power[1] : power[0]) * (1.f / kLevelUnit);
+                        if (i >= S::kSlots) wait(empty0 + 8 * slot, (i / S::kSlots + 1) & 1u);
+                        if (!ok) break;
+                        {
+                            const float unit = reciprocal_of_power(power) * (1.f / kLevelUnit);
                             uint4 raws[N / kPass];
                             uint32_t factors[N / kPass];
                             #pragma unroll
@@ -632,127 +680,153 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                 }
             } else if (warp == kCopyWarp) {
                 constexpr uint32_t kGroups = N / kGroup;
-                uint32_t i = 0, tails = 0;
-                for (uint32_t piece = 0; ok && walk.next(c, b, a, p); ++piece) {
+                uint32_t i = 0, tails = 0, step = 0;
+                for (uint32_t piece = 0; ok && walk.next(c, b, a, p); ++piece, step += p.steps) {
                     if (lane == 0) s_bad[piece & 7u] = 0;  // (the others are at most three pieces behind)
                     __syncwarp();
+                    const uint32_t tile0 = expanded ? __ldg(dense.bases + p.seq) + p.step0 : 0u;
                     const uint32_t stored = min(p.s.length, (p.step0 + p.steps) * N);  // tokens that there are
-                    for (uint32_t j = 0; ok && j < p.steps; ++j) {
+                    #pragma unroll 1
+                    for (uint32_t turn = 0; ok && turn < 2 * p.steps; ++turn, ++i) {
+                        const Turn<kPlaces> of(turn, p.steps);
+                        const uint32_t which = of.values, j = of.step;
                         const uint32_t t0 = (p.step0 + j) * N, g = lane % kGroups, box = lane / kGroups, t = t0 + g * kGroup;
                         const uint32_t groups = stored > t0 ? min(kGroups, (stored - t0 + kGroup - 1) / kGroup) : 0u;
+                        const uint32_t rs = i % S::kRawSlots, slot = i % S::kSlots;
                         uint32_t place = 0;
-                        if (g < groups) {
+                        if (expanded) {
+                            if (!which) {
+                                const float2 powers = __ldg(dense.powers + (uint64_t)(tile0 + j) * c.heads + p.head);
+                                if (powers.x == 0.f) s_bad[piece & 7u] = 1;  // (a page that there is not)
+                                if (lane == 0) s_powers[(step + j) & 7u] = powers;
+                            }
+                        } else if (g < groups) {
                             const uint32_t at = c.by_page.of(t);
                             const int32_t page = __ldg(b.table + (uint64_t)p.seq * b.width + at);
                             if (page >= 0 && (uint32_t)page < c.pages) place = ((uint32_t)page * c.heads + p.head) * c.page_size + (t - at * c.page_size);
                             else s_bad[piece & 7u] = 1;
                         }
                         __syncwarp();
-                        for (uint32_t which = 0; which < 2; ++which, ++i) {
-                            bool got = true;
-                            if (NF4) {
-                                const uint32_t rs = i % S::kRawSlots, bar = raw_full0 + 8 * rs, dst = raw0 + rs * S::kRaw;
-                                if (i >= S::kRawSlots) got = ptx::mbar_wait_suspended(raw_empty0 + 8 * rs, (i / S::kRawSlots + 1) & 1u);
-                                got = __all_sync(0xffffffffu, got);
-                                if (got) {
-                                    if (lane == 0) ptx::mbar_arrive_expect_tx(bar, groups * (kGroup * (D / 2) + kGroup * kBlocks * 4));
-                                    __syncwarp();
-                                    if (box == 0 && g < groups) {
-                                        ptx::bulk_g2s(dst + g * kGroup * (D / 2), static_cast<const uint8_t *>(which ? c.v : c.k) + (uint64_t)place * (D / 2), kGroup * (D / 2), bar);
-                                        ptx::bulk_g2s(dst + N * (D / 2) + g * kGroup * kBlocks * 4, (which ? c.v_scales : c.k_scales) + (uint64_t)place * kBlocks,
-                                                      kGroup * kBlocks * 4, bar);
-                                    }
-                                }
-                            } else {
-                                const uint32_t slot = i % S::kSlots, dst = ring0 + slot * S::kTile;
-                                if (i >= S::kSlots) got = ptx::mbar_wait_suspended(empty0 + 8 * slot, (i / S::kSlots + 1) & 1u);
-                                got = __all_sync(0xffffffffu, got);
-                                const bool tail = which && t0 + N > p.s.length;  // values that anything may stand behind: zeros, for weights of zero
-                                const uint32_t bar = tail ? tail_bar : full0 + 8 * slot;
-                                if (got) {
-                                    if (lane == 0) ptx::mbar_arrive_expect_tx(bar, groups * (kGroup * 128) * (D / 64));
-                                    __syncwarp();
-                                    if (g < groups && box < D / 64)
-                                        ptx::tma_load_2d(dst + box * S::kBox + g * (kGroup * 128), which ? &tmap_v : &tmap_k, (int32_t)(64 * box), (int32_t)place, bar);
-                                }
-                                if (got && tail) {
-                                    got = __all_sync(0xffffffffu, ptx::mbar_wait_suspended(tail_bar, tails & 1u));
-                                    ++tails;
-                                    for (uint32_t k = (p.s.length > t0 ? p.s.length - t0 : 0u) * 8 + lane; k < N * 8; k += 32)
-                                        #pragma unroll
-                                        for (uint32_t x = 0; x < D / 64; ++x) st_shared_u4(dst + x * S::kBox + k * 16, make_uint4(0u, 0u, 0u, 0u));
-                                    ptx::fence_proxy_async();
-                                    __syncwarp();
-                                    if (lane == 0) ptx::mbar_arrive(full0 + 8 * slot);
-                                }
+                        bool got = true;
+                        if (NF4 && !expanded) {
+                            if (i >= S::kRawSlots) got = ptx::mbar_wait_suspended(raw_empty0 + 8 * rs, (i / S::kRawSlots + 1) & 1u);
+                        } else if (i >= S::kSlots) {
+                            got = ptx::mbar_wait_suspended(empty0 + 8 * slot, (i / S::kSlots + 1) & 1u);
+                        }
+                        got = __all_sync(0xffffffffu, got);
+                        const uint32_t dst = ring0 + slot * S::kTile;
+                        if (!got) {
+                        } else if (NF4 && expanded) {
+                            const uint32_t bar = full0 + 8 * slot;
+                            if (lane == 0) {
+                                ptx::mbar_arrive_expect_tx(bar, S::kTile);
+                                const int32_t row = (int32_t)(((tile0 + j) * c.heads + p.head) * N);
+                                #pragma unroll
+                                for (uint32_t x = 0; x < D / 64; ++x) ptx::tma_load_2d(dst + x * S::kBox, which ? &tmap_v : &tmap_k, (int32_t)(64 * x), row, bar);
+                                for (int e = 0; e < 3; ++e) ptx::mbar_arrive(bar);  // (for the four warps that expand)
                             }
-                            if (!got) {
-                                ok = false;
-                                if (lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 26);
-                                break;
+                        } else if (NF4) {
+                            const uint32_t bar = raw_full0 + 8 * rs, raw = raw0 + rs * S::kRaw;
+                            if (lane == 0) ptx::mbar_arrive_expect_tx(bar, groups * (kGroup * (D / 2) + (which ? 1u : 2u) * kGroup * kBlocks * 4));
+                            __syncwarp();
+                            if (box == 0 && g < groups) {
+                                ptx::bulk_g2s(raw + g * kGroup * (D / 2), static_cast<const uint8_t *>(which ? c.v : c.k) + (uint64_t)place * (D / 2), kGroup * (D / 2), bar);
+                                ptx::bulk_g2s(raw + N * (D / 2) + g * kGroup * kBlocks * 4, (which ? c.v_scales : c.k_scales) + (uint64_t)place * kBlocks, kGroup * kBlocks * 4, bar);
+                                if (!which)
+                                    ptx::bulk_g2s(raw + N * (D / 2) + S::kScales + g * kGroup * kBlocks * 4, c.v_scales + (uint64_t)place * kBlocks, kGroup * kBlocks * 4, bar);
                             }
+                        } else {
+                            const bool tail = which && t0 + N > p.s.length;  // values that anything may stand behind: zeros, for weights of zero
+                            const uint32_t bar = tail ? tail_bar : full0 + 8 * slot;
+                            if (lane == 0) ptx::mbar_arrive_expect_tx(bar, groups * (kGroup * 128) * (D / 64));
+                            __syncwarp();
+                            if (g < groups && box < D / 64)
+                                ptx::tma_load_2d(dst + box * S::kBox + g * (kGroup * 128), which ? &tmap_v : &tmap_k, (int32_t)(64 * box), (int32_t)place, bar);
+                            if (tail) {
+                                got = __all_sync(0xffffffffu, ptx::mbar_wait_suspended(tail_bar, tails & 1u));
+                                ++tails;
+                                for (uint32_t k = (p.s.length > t0 ? p.s.length - t0 : 0u) * 8 + lane; k < N * 8; k += 32)
+                                    #pragma unroll
+                                    for (uint32_t x = 0; x < D / 64; ++x) st_shared_u4(dst + x * S::kBox + k * 16, make_uint4(0u, 0u, 0u, 0u));
+                                ptx::fence_proxy_async();
+                                __syncwarp();
+                                if (lane == 0) ptx::mbar_arrive(full0 + 8 * slot);
+                            }
+                        }
+                        if (!got) {
+                            ok = false;
+                            if (lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 26);
                         }
                     }
                 }
             } else if (warp == kMmaWarp) {
                 constexpr uint32_t fmt = NF4 ? 0 : 1;
                 constexpr uint32_t idesc_s = ptx::f16_idesc(fmt, 128, N, false, false), idesc_o = ptx::f16_idesc(fmt, 128, D, false, true);
-                uint32_t i = 0, weights[2] = {0, 0}, rows_in[2] = {0, 0};  // tiles of K and V, weights and Q's waited for so far
+                uint32_t i = 0, made[2] = {0, 0}, used[2] = {0, 0}, rows_in[2] = {0, 0};  // tiles of K and V, scores, weights and Q's so far
                 auto wait = [&](uint32_t bar, uint32_t parity) {
                     if (!ok) return;
                     ok = __all_sync(0xffffffffu, ptx::mbar_wait_suspended(bar, parity));
                     if (!ok && lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 27);
                 };
                 auto wait_full = [&](uint32_t at) { wait(full0 + 8 * (at % S::kSlots), (at / S::kSlots) & 1u); };
-                auto scores = [&](uint32_t tile, uint32_t at) {  // of the keys in ring place `at`
+                // (these two by the elected thread)
+                auto scores = [&](uint32_t tile, uint32_t at, uint32_t n) {  // of the keys in ring place `at`, to the place of the tile's n-th
                     const uint64_t qd = ptx::sw128_desc(q0 + tile * S::kQTile), kd = ptx::sw128_desc(ring0 + at % S::kSlots * S::kTile);
                     #pragma unroll
                     for (uint32_t k = 0; k < D / 16; ++k)
-                        ptx::mma_ss_f16(tmem + S::kS + tile * N, qd + (k >> 2) * (16384 >> 4) + (k & 3u) * 2, kd + (k >> 2) * (S::kBox >> 4) + (k & 3u) * 2, idesc_s, k != 0);
-                    ptx::tc_commit(s_full0 + 8 * tile);
+                        ptx::mma_ss_f16(tmem + S::kS + (kPlaces * tile + n % kPlaces) * N, qd + (k >> 2) * (16384 >> 4) + (k & 3u) * 2, kd + (k >> 2) * (S::kBox >> 4) + (k & 3u) * 2,
+                                        idesc_s, k != 0);
+                    ptx::tc_commit(s_full0 + 8 * (kPlaces * tile + n % kPlaces));
                 };
-                auto products = [&](uint32_t tile, uint32_t at, bool add) {
+                auto products = [&](uint32_t tile, uint32_t at, uint32_t n, bool add) {
                     const uint64_t vd = ptx::sw128_desc(ring0 + at % S::kSlots * S::kTile, S::kBox);
                     #pragma unroll
-                    for (uint32_t k = 0; k < N / 16; ++k) ptx::mma_ts_f16(tmem + S::kO + tile * D, tmem + S::kS + tile * N + 8 * k, vd + 128 * k, idesc_o, add || k != 0);
+                    for (uint32_t k = 0; k < N / 16; ++k)
+                        ptx::mma_ts_f16(tmem + S::kO + tile * D, tmem + S::kS + (kPlaces * tile + n % kPlaces) * N + 8 * k, vd + 128 * k, idesc_o, add || k != 0);
+                    ptx::tc_commit(pv_done0 + 8 * tile);
                 };
                 while (ok && walk.next(c, b, a, p)) {
-                    wait_full(i);
-                    for (uint32_t t = 0; t < p.live; ++t) {
-                        wait(q_ready0 + 8 * t, rows_in[t] & 1u);
-                        ++rows_in[t];
-                        ptx::tc_fence_after();
-                        if (ok && ptx::elect_one()) {
-                            scores(t, i);
-                            if (t + 1 == p.live) ptx::tc_commit(empty0 + 8 * (i % S::kSlots));
-                        }
-                        __syncwarp();
-                    }
-                    for (uint32_t j = 0; j < p.steps && ok; ++j, i += 2) {
-                        const uint32_t iv = i + 1, ik = i + 2;
-                        const bool more = j + 1 < p.steps;
-                        wait_full(iv);
+                    for (uint32_t j = 0; j < min(kPlaces, p.steps) && ok; ++j, ++i) {  // the first scores
+                        wait_full(i);
                         for (uint32_t t = 0; t < p.live; ++t) {
-                            wait(p_ready0 + 8 * t, weights[t] & 1u);
-                            ++weights[t];
+                            if (j == 0) {
+                                wait(q_ready0 + 8 * t, rows_in[t] & 1u);
+                                ++rows_in[t];
+                            }
+                            ptx::tc_fence_after();
+                            if (ok && ptx::elect_one()) {
+                                scores(t, i, made[t]);
+                                if (t + 1 == p.live) ptx::tc_commit(empty0 + 8 * (i % S::kSlots));
+                            }
+                            ++made[t];
+                            __syncwarp();
+                        }
+                    }
+                    for (uint32_t j = 0; j < p.steps && ok; ++j) {
+                        const bool more = j + kPlaces < p.steps;
+                        wait_full(i);
+                        for (uint32_t t = 0; t < p.live; ++t) {
+                            wait(p_ready0 + 8 * (kPlaces * t + used[t] % kPlaces), (used[t] / kPlaces) & 1u);
                             if (!ok) break;
                             ptx::tc_fence_after();
                             if (ptx::elect_one()) {
-                                products(t, iv, j != 0);
-                                if (t + 1 == p.live) ptx::tc_commit(empty0 + 8 * (iv % S::kSlots));
-                                if (!more) ptx::tc_commit(s_full0 + 8 * t);
+                                products(t, i, used[t], j != 0);
+                                if (t + 1 == p.live) ptx::tc_commit(empty0 + 8 * (i % S::kSlots));
                             }
+                            ++used[t];
                             __syncwarp();
                             if (!more) continue;
-                            if (t == 0) wait_full(ik);
+                            if (t == 0) wait_full(i + 1);
                             if (!ok) break;
                             ptx::tc_fence_after();
                             if (ptx::elect_one()) {
-                                scores(t, ik);
-                                if (t + 1 == p.live) ptx::tc_commit(empty0 + 8 * (ik % S::kSlots));
+                                scores(t, i + 1, made[t]);
+                                if (t + 1 == p.live) ptx::tc_commit(empty0 + 8 * ((i + 1) % S::kSlots));
                             }
+                            ++made[t];
                             __syncwarp();
                         }
+                        i += more ? 2 : 1;
                     }
                 }
             }
@@ -764,6 +838,91 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     if (warp == kMmaWarp) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc(tmem, 512);
+    }
+}
+
+// ---- a quantized cache expanded once --------------------------------------------------------------
+// Where several row tiles of a head go over the same tokens.  A CTA has a tile of N tokens of one head: the power of two
+// above its largest scale, then levels times scales in f16, eight values to a thread at a time.  Bound by what it writes.
+template <int D>
+__global__ void __launch_bounds__(256)
+expand_kernel(const CacheView c, const BatchView b, uint4 *const k_out, uint4 *const v_out, uint32_t *const bases, float2 *const powers) {
+    constexpr uint32_t N = Shape<D, true>::kTokens, kBlocks = D / 64, kGroups = D / 8;  // eight values each
+    __shared__ uint32_t s_pairs[256], s_most[2], s_place[N], s_bad;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u;
+    s_pairs[tid] = level_pair_f16(tid);
+    if (tid < 2) s_most[tid] = 0;
+    if (tid == 2) s_bad = 0;
+    ptx::pdl_launch_dependents();
+    ptx::pdl_wait();
+    // which sequence the tile is of (every warp finds it); the first CTA writes down where each begins
+    const uint32_t head = blockIdx.x % c.heads, want = blockIdx.x / c.heads;
+    uint32_t seq = b.sequences, tile = 0, before = 0;
+    Sequence s{0, 0, 0};
+    for (uint32_t s0 = 0; s0 < b.sequences && (seq == b.sequences || blockIdx.x == 0); s0 += 32) {
+        Sequence o{0, 0, 0};
+        if (s0 + lane < b.sequences) o = sequence_of(c, b, s0 + lane);
+        const uint32_t own = s0 + lane < b.sequences ? max(1u, (o.length + N - 1) / N) : 0u;
+        uint32_t upto = own;
+        #pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= (uint32_t)d) upto += v;
+        }
+        if (blockIdx.x == 0 && tid < 32 && s0 + lane < b.sequences) bases[s0 + lane] = before + upto - own;
+        const uint32_t past = __ballot_sync(0xffffffffu, before + upto > want);
+        if (past && seq == b.sequences) {
+            const int l = __ffs(past) - 1;
+            seq = s0 + l;
+            tile = want - before - __shfl_sync(0xffffffffu, upto - own, l);
+            s = Sequence{__shfl_sync(0xffffffffu, o.row0, l), __shfl_sync(0xffffffffu, o.rows, l), __shfl_sync(0xffffffffu, o.length, l)};
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (blockIdx.x == 0 && tid == 0) bases[b.sequences] = before;
+    if (seq == b.sequences) return;
+    __syncthreads();
+    const uint32_t t0 = tile * N, tokens = s.length > t0 ? min(N, s.length - t0) : 0u;
+    if (tid < N) {
+        uint32_t place = 0;
+        if (tid < tokens) {
+            const uint32_t at = c.by_page.of(t0 + tid);
+            const int32_t page = __ldg(b.table + (uint64_t)seq * b.width + at);
+            if (page < 0 || (uint32_t)page >= c.pages) s_bad = 1;
+            else place = ((uint32_t)page * c.heads + head) * c.page_size + (t0 + tid - at * c.page_size);
+            uint32_t most[2] = {0, 0};
+            #pragma unroll
+            for (uint32_t k = 0; k < kBlocks; ++k) {
+                most[0] = max(most[0], __float_as_uint(__ldg(c.k_scales + (uint64_t)place * kBlocks + k)));
+                most[1] = max(most[1], __float_as_uint(__ldg(c.v_scales + (uint64_t)place * kBlocks + k)));
+            }
+            atomicMax(&s_most[0], most[0]);
+            atomicMax(&s_most[1], most[1]);
+        }
+        s_place[tid] = place;
+    }
+    __syncthreads();
+    const float power[2] = {power_above(s_most[0]), power_above(s_most[1])};
+    const uint64_t out0 = ((uint64_t)want * c.heads + head) * N * kGroups;
+    if (tid == 0) powers[(uint64_t)want * c.heads + head] = s_bad ? make_float2(0.f, 0.f) : make_float2(power[0], power[1]);
+    #pragma unroll
+    for (uint32_t which = 0; which < 2; ++which) {
+        const uint32_t *const codes = static_cast<const uint32_t *>(which ? c.v : c.k);
+        const float *const scales = which ? c.v_scales : c.k_scales;
+        const float unit = reciprocal_of_power(power[which]) * (1.f / kLevelUnit);
+        #pragma unroll 4
+        for (uint32_t i = tid; i < N * kGroups; i += 256) {
+            const uint32_t t = i / kGroups, g = i % kGroups;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (t < tokens) {
+                const uint64_t row = s_place[t];
+                const uint32_t w = __ldg(codes + row * kGroups + g);
+                const float scale = __ldg(scales + row * kBlocks + g / 8) * unit;
+                const uint32_t s2 = pack<true>(scale, scale);
+                v = make_uint4(mul_f16x2(s_pairs[w & 255u], s2), mul_f16x2(s_pairs[w >> 8 & 255u], s2), mul_f16x2(s_pairs[w >> 16 & 255u], s2), mul_f16x2(s_pairs[w >> 24], s2));
+            }
+            (which ? v_out : k_out)[out0 + i] = v;
+        }
     }
 }
 
@@ -820,8 +979,36 @@ join_pieces_kernel(const AttentionView a, const Split *const splits) {
 }
 
 uint64_t rows_of(const AttentionCall &c) { return c.head_dim == 256 ? 128 : 256; }
-uint64_t ml_bytes(const AttentionCall &c) { return 2ull * kNumSMs * rows_of(c) * sizeof(float2); }
-constexpr uint64_t kSplitBytes = (kNumSMs * sizeof(Split) + 255) / 256 * 256;
+uint64_t tokens_of(const AttentionCall &c) { return c.head_dim == 256 ? 64 : 128; }
+
+// Tiles to a head to be expanded ahead: where the host's bounds say that three row tiles or more of a head go over most tokens (with two
+// the expansion in place, which is slower by half a step, costs what the kernel ahead does), up to 2 GB.
+uint64_t dense_tiles(const AttentionCall &c) {
+    if (!c.nf4 || (uint64_t)c.most_rows * c.view.group <= 2 * rows_of(c)) return 0;
+    const uint64_t tiles = (uint64_t)c.batch.sequences * std::max<uint64_t>(1, (c.most_tokens + tokens_of(c) - 1) / tokens_of(c));
+    return tiles * c.cache.heads * tokens_of(c) * c.head_dim * 4 <= 1ull << 31 && tiles * c.cache.heads * tokens_of(c) < 1ull << 31 ? tiles : 0;
+}
+
+struct Layout {  // of the workspace
+    uint64_t splits, ml, o, bases, powers, k, v, bytes;
+    explicit Layout(const AttentionCall &c) {
+        uint64_t at = kAttentionFlagBytes;
+        auto take = [&](uint64_t n) {
+            const uint64_t from = at;
+            at += (n + 255) / 256 * 256;
+            return from;
+        };
+        const uint64_t tiles = dense_tiles(c), dense = tiles * c.cache.heads * tokens_of(c) * c.head_dim * 2;
+        splits = take(kNumSMs * sizeof(Split));
+        ml = take(2ull * kNumSMs * rows_of(c) * sizeof(float2));
+        o = take(2ull * kNumSMs * rows_of(c) * c.head_dim * sizeof(float));
+        bases = take(tiles ? (c.batch.sequences + 1ull) * sizeof(uint32_t) : 0);
+        powers = take(tiles * c.cache.heads * sizeof(float2));
+        k = take(dense);
+        v = take(dense);
+        bytes = at;
+    }
+};
 
 template <int D, bool NF4>
 int32_t launch(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) {
@@ -840,20 +1027,38 @@ int32_t launch(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) 
     const uint64_t tiles = ((uint64_t)c.batch.rows * c.view.group / S::kRows + c.batch.sequences) * c.cache.heads;
     const uint64_t steps = ((uint64_t)c.batch.width * c.cache.page_size + S::kTokens - 1) / S::kTokens;
     if (tiles * (steps + 1 + kStart) >= 1ull << 31) return fail(NF4_ERR_UNSUPPORTED, "attention: rows times tokens are too many for a call; split it");
-    Split *const splits = reinterpret_cast<Split *>(workspace + kAttentionFlagBytes);
+    const Layout at(c);
+    Split *const splits = reinterpret_cast<Split *>(workspace + at.splits);
     AttentionView view = c.view;
-    view.part_ml = reinterpret_cast<float2 *>(workspace + kAttentionFlagBytes + kSplitBytes);
-    view.part_o = reinterpret_cast<float *>(workspace + kAttentionFlagBytes + kSplitBytes + ml_bytes(c));
+    view.part_ml = reinterpret_cast<float2 *>(workspace + at.ml);
+    view.part_o = reinterpret_cast<float *>(workspace + at.o);
+    Dense dense{};
+    if constexpr (NF4) {
+        dense.capacity = (uint32_t)dense_tiles(c);
+        if (dense.capacity) {
+            uint32_t *const bases = reinterpret_cast<uint32_t *>(workspace + at.bases);
+            float2 *const powers = reinterpret_cast<float2 *>(workspace + at.powers);
+            const uint64_t dense_rows = (uint64_t)dense.capacity * c.cache.heads * S::kTokens;
+            NF4_TRY(make_map(&map_k, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, workspace + at.k, dense_rows, D, 2 * D, S::kTokens, 64, CU_TENSOR_MAP_SWIZZLE_128B));
+            NF4_TRY(make_map(&map_v, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, workspace + at.v, dense_rows, D, 2 * D, S::kTokens, 64, CU_TENSOR_MAP_SWIZZLE_128B));
+            dense.bases = bases;
+            dense.powers = powers;
+            count_launch();
+            NF4_TRY(launch_maybe_overlapped(expand_kernel<D>, dim3(dense.capacity * c.cache.heads), dim3(256), 0, stream, true, c.cache, c.batch,
+                                            reinterpret_cast<uint4 *>(workspace + at.k), reinterpret_cast<uint4 *>(workspace + at.v), bases, powers));
+        }
+    }
     const uint32_t ctas = persistent_ctas();
     count_launch(2);
-    NF4_TRY(launch_maybe_overlapped(kernel, dim3(ctas), dim3(kThreads), S::kSmem, stream, true, map_k, map_v, c.cache, c.batch, view, splits, failure));
-    return launch_maybe_overlapped(join_pieces_kernel<D, NF4>, dim3(ctas, S::kRows / (kJoinRows * kJoinWarps)), dim3(32 * kJoinWarps), 0, stream, true, view, static_cast<const Split *>(splits));
+    NF4_TRY(launch_maybe_overlapped(kernel, dim3(ctas), dim3(kThreads), S::kSmem, stream, true, map_k, map_v, c.cache, c.batch, view, dense, splits, failure));
+    return launch_maybe_overlapped(join_pieces_kernel<D, NF4>, dim3(ctas, S::kRows / (kJoinRows * kJoinWarps)), dim3(32 * kJoinWarps), 0, stream, true, view,
+                                   static_cast<const Split *>(splits));
 }
 
 }  // namespace
 
 uint64_t attention_chunk_bytes(const AttentionCall &c) {
-    return kAttentionFlagBytes + kSplitBytes + ml_bytes(c) + 2ull * kNumSMs * rows_of(c) * c.head_dim * sizeof(float);
+    return Layout(c).bytes;
 }
 
 int32_t attention_chunk(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) {
