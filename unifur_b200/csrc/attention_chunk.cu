@@ -50,7 +50,7 @@ struct Shape {
     static constexpr uint32_t kScales = kTokens * kBlocks * 4;
     // a tile's codes and scales, and with K's the V's scales of the step: their power goes to the softmax ahead of V
     static constexpr uint32_t kRaw = NF4 ? kTokens * D / 2 + 2 * kScales : 0, kRawSlots = D == 64 ? 5 : 2;
-    static constexpr uint32_t kSlots = D == 64 ? (NF4 ? 6 : 8) : NF4 ? 3 : 4;
+    static constexpr uint32_t kSlots = D == 64 ? (NF4 ? 6 : 7) : NF4 ? 3 : 5;  // of the ring; one more where the table is not needed
     // codes, then the table on a multiple of its 32 KB, then Q, then the ring (bf16: Q, then the ring)
     static constexpr uint32_t kSmem = (NF4 ? 65536 : 2048) - 1024 + kTiles * kQTile + kSlots * kTile;
     static constexpr uint32_t kS = 0, kO = 256;                       // columns of tensor memory: the tiles' S's, then O's
@@ -93,6 +93,24 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
         : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+// 2^e of two numbers up to 2^8 (below 2^-126 that) without the exponential unit: e = i + f with f in [-1/2, 1/2], 2^f by the polynomial of degree
+// 3 that is least off (7.5e-5, a third of an f16's rounding on average; found by weighted least squares), i added to its exponent.
+__device__ __forceinline__ float2 exp2_by_fma(float2 e) {
+    const float2 one = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23: adding it leaves i in the low bits
+    e = make_float2(fmaxf(e.x, -126.f), fmaxf(e.y, -126.f));
+    const float2 t = add2(e, one), i = add2(t, make_float2(-12582912.f, -12582912.f));
+    const float2 f = add2(e, make_float2(-i.x, -i.y));
+    float2 p = fma2(f, make_float2(0.05517167f, 0.05517167f), make_float2(0.24261112f, 0.24261112f));
+    p = fma2(p, f, make_float2(0.69326099f, 0.69326099f));
+    p = fma2(p, f, make_float2(0.99992807f, 0.99992807f));
+    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)), __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
 }
 template <bool F16>
 __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -206,6 +224,17 @@ struct Split {
     uint32_t row0, r0, rows, head, more;  // more: CTAs behind the first
 };
 
+// A place in the ring of tiles, and the parity of its barriers' round.
+struct Ring {
+    uint32_t slot = 0, round = 0;
+    __device__ __forceinline__ void on(uint32_t slots) {
+        if (++slot == slots) {
+            slot = 0;
+            ++round;
+        }
+    }
+};
+
 // In which order a piece's tiles of K and V come: K 0, V 0, K 1, V 1, ...; with two places for S K 0, K 1, V 0, K 2, V 1, ..., V n - 1.
 template <uint32_t kPlaces>
 struct Turn {
@@ -225,25 +254,28 @@ struct Turn {
 template <int D, bool NF4>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const CacheView c, const BatchView b,
-                       const AttentionView a, const Dense dense, Split *const splits, const FailureRef failure) {
+                       const AttentionView a, const Dense dense, uint32_t box_rows, Split *const splits, const FailureRef failure) {
     using S = Shape<D, NF4>;
     using Walk = Walker<S::kRows, S::kTokens>;
+    // A bf16 cache's pages may be of sixteen tokens, and a warp asks for boxes one after another: four warps share the asking, a tile's
+    // columns between two of them (with one, 137 cycles to a box of 2 KB, the MMAs waited for copies)
+    constexpr uint32_t kCopies = !NF4 && D >= 128 ? 2 : 1;
     constexpr uint32_t N = S::kTokens, kBlocks = S::kBlocks, kPlaces = S::kPlaces;
     extern __shared__ uint8_t smem_any[];
-    __shared__ __align__(8) uint64_t s_bars[39];
-    __shared__ uint32_t s_tmem, s_bad[8], s_first[6];  // s_bad: of the last pieces, whether a page was not there
+    __shared__ __align__(8) uint64_t s_bars[42];
+    __shared__ uint32_t s_tmem, s_bad[8], s_first[6];  // s_bad: of the last eight pieces, its number + 1 where a page was not there
     __shared__ Share s_share;
     __shared__ Walk s_walk[8];
     __shared__ Piece s_piece[8];
-    __shared__ float s_qpower[S::kRows];
+    __shared__ float s_qpower[NF4 ? S::kRows : 1];
     __shared__ float2 s_powers[8];  // of the last steps' K and V (who writes them is at most four steps ahead of who reads)
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u;
     const uint32_t base = ptx::smem_addr(smem_any);
     const uint32_t raw0 = (base + 15u) & ~15u, table = (raw0 + S::kRawSlots * S::kRaw + 32767u) & ~32767u;
     const uint32_t q0 = NF4 ? table + 32768u : (base + 1023u) & ~1023u, ring0 = q0 + S::kTiles * S::kQTile;
-    // s_full, p_ready: of a tile's two places
+    // s_full, p_ready: of a tile's places; pv_done: products that a rescaling waits for
     const uint32_t bars = ptx::smem_addr(s_bars), full0 = bars, empty0 = bars + 64, raw_full0 = bars + 128, raw_empty0 = bars + 168, s_full0 = bars + 208,
-                   p_ready0 = bars + 240, pv_done0 = bars + 272, q_ready0 = bars + 288, tail_bar = bars + 304;
+                   p_ready0 = bars + 240, pv_done0 = bars + 272, q_ready0 = bars + 288, tail0 = bars + 304, o_done0 = bars + 320;
     if (ring0 + S::kSlots * S::kTile > base + S::kSmem) {
         ptx::pdl_wait();
         if (tid == 0) {
@@ -253,8 +285,9 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         return;
     }
     if (tid == 0) {
-        for (uint32_t i = 0; i < S::kSlots; ++i) {
-            ptx::mbar_init(full0 + 8 * i, NF4 ? 4 : 1);
+        static_assert(S::kSlots + 1 <= 8);
+        for (uint32_t i = 0; i < 8; ++i) {  // (a place more than kSlots may be in use)
+            ptx::mbar_init(full0 + 8 * i, NF4 ? 4 : kCopies);
             ptx::mbar_init(empty0 + 8 * i, 1);
         }
         for (uint32_t i = 0; i < S::kRawSlots; ++i) {
@@ -268,16 +301,19 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         for (uint32_t i = 0; i < 2; ++i) {
             ptx::mbar_init(pv_done0 + 8 * i, 1);
             ptx::mbar_init(q_ready0 + 8 * i, 4);
+            ptx::mbar_init(o_done0 + 8 * i, 1);
         }
-        ptx::mbar_init(tail_bar, 1);
+        for (uint32_t i = 0; i < 2; ++i) ptx::mbar_init(tail0 + 8 * i, 1);
         ptx::fence_mbar_init();
         ptx::fence_proxy_async();
     }
+    if (tid < 8) s_bad[tid] = 0;
     if (NF4) {
         for (uint32_t i = tid; i < 256 * 8; i += kThreads) {  // the table: an entry's copy to a lane
             const uint32_t byte = i >> 3, entry = level_pair_f16(byte);
             st_shared_u4(table + byte * 128u + (i & 7u) * 16u, make_uint4(entry, entry, entry, entry));
         }
+        ptx::fence_proxy_async();  // (copies may come to this place instead)
     }
     if (warp == kMmaWarp) {
         ptx::tmem_alloc(ptx::smem_addr(&s_tmem), 512);
@@ -377,6 +413,8 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     const uint32_t tmem = s_tmem;
     bool ok = true;
     const bool expanded = NF4 && dense.capacity && __ldg(dense.bases + b.sequences) <= dense.capacity;  // (more tokens than the host knew of: not)
+    const uint32_t slots = S::kSlots + (expanded ? 1u : 0u);
+    auto place_of = [&](uint32_t slot) -> uint32_t { return slot < S::kSlots ? ring0 + slot * S::kTile : table; };
     if (s_first[4] < s_first[5]) {
         Walk walk{sequence_of(c, b, s_first[0]), s_first[0], s_first[1], s_first[2], s_first[3], s_first[4], s_first[5]};
         Piece p;
@@ -386,7 +424,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             const uint32_t lanes = (warp & 3u) << 21;  // a warp reaches its quarter of tensor memory's lanes
             const uint32_t ts0 = tmem + S::kS + kPlaces * tile * N + lanes, to = tmem + S::kO + tile * D + lanes;
             const uint32_t q_tile = q0 + tile * S::kQTile;
-            uint32_t scores = 0, step = 0, piece = 0;  // steps of this tile, steps and pieces of the CTA, so far
+            uint32_t scores = 0, finished = 0, step = 0, piece = 0;  // steps and pieces of this tile, steps and pieces of the CTA, so far
             for (; ok && walk.next(c, b, a, p); step += p.steps, ++piece) {
                 if (tile >= p.live) continue;
                 // (what the steps do not need waits in shared memory: registers are short there)
@@ -413,11 +451,11 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                         const uint32_t i = (i0 + k) * 128 + r, rr = i / kLanes, x = i % kLanes;
                         uint32_t u[4] = {w[k].x ^ flip, w[k].y ^ flip, w[k].z ^ flip, w[k].w ^ flip};
                         if (NF4) {
-                            uint32_t most = 0;
+                            constexpr uint32_t kSize = 0x7fff7fffu;  // (bf16 magnitudes go by their bits)
+                            uint32_t two = __vmaxu2(__vmaxu2(u[0] & kSize, u[1] & kSize), __vmaxu2(u[2] & kSize, u[3] & kSize));
                             #pragma unroll
-                            for (int e = 0; e < 4; ++e) most = max(most, max((u[e] << 16) & 0x7fffffffu, u[e] & 0x7fff0000u));
-                            #pragma unroll
-                            for (uint32_t d = 1; d < kLanes; d <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+                            for (uint32_t d = 1; d < kLanes; d <<= 1) two = __vmaxu2(two, __shfl_xor_sync(0xffffffffu, two, d));
+                            const uint32_t most = max(two << 16, two & 0xffff0000u);
                             // the row's largest magnitude is left in [2^11, 2^12)
                             const int e2 = most ? min(max((int)(most >> 23) - 127 - 11, -100), 115) : 0;
                             const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
@@ -482,7 +520,8 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                             for (uint32_t i = 0; i < 32; i += 2) {
                                 top[(i >> 1) & 1] = fmaxf(fmaxf(top[(i >> 1) & 1], __uint_as_float(x[i])), __uint_as_float(x[i + 1]));
                                 const float2 e = fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), factor, from);
-                                const float2 w = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+                                // the exponential unit gives 16 a clock, which is what the MMAs take as long for: a quarter goes by the FMA pipe
+                                const float2 w = i % 8 == 6 ? exp2_by_fma(e) : make_float2(exp2_approx(e.x), exp2_approx(e.y));
                                 sum = add2(sum, w);
                                 pw[(k + i) / 2] = pack<NF4>(w.x, w.y);
                             }
@@ -499,8 +538,8 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                         }
                         if (grown) keep *= ref_was * reciprocal_of_power(ref);
                         grown = false;
-                        if (j) {  // once the products so far are done
-                            if (!__all_sync(0xffffffffu, ptx::mbar_wait_suspended(pv_done0 + 8 * tile, (scores - 1) & 1u))) {
+                        if (j) {  // once the products so far are done: the last step's were, with one place, ahead of these scores
+                            if (kPlaces > 1 && !__all_sync(0xffffffffu, ptx::mbar_wait_suspended(pv_done0 + 8 * tile, (scores - 1) & 1u))) {
                                 ok = false;
                                 if (lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 28);
                                 break;
@@ -527,64 +566,66 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                     __syncwarp();
                     if (lane == 0) ptx::mbar_arrive(p_ready0 + 8 * place);
                 }
-                // With two places for S the products may be two steps behind (the last scores came behind those of three steps ago), and a
-                // parity tells only the last round from the one before it: both are waited for in turn.
-                bool done = ok;
-                if (done && kPlaces > 1 && scores > 1) done = ptx::mbar_wait_suspended(pv_done0 + 8 * tile, (scores - 2) & 1u);
-                if (done) done = ptx::mbar_wait_suspended(pv_done0 + 8 * tile, (scores - 1) & 1u);
-                if (ok && !__all_sync(0xffffffffu, done)) {
+                if (ok && !__all_sync(0xffffffffu, ptx::mbar_wait_suspended(o_done0 + 8 * tile, finished & 1u))) {
                     ok = false;
                     if (lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 24);
                 }
+                ++finished;
                 ptx::tc_fence_after();
                 walk = s_walk[warp];
                 p = s_piece[warp];
 
                 // ---- the row's results, through this warp's part of Q's place (its products are done) so that whole rows go out ----
-                if (s_bad[piece & 7u] || !ok) l = __uint_as_float(0x7fc00000u);  // NaN
+                if (s_bad[piece & 7u] == piece + 1 || !ok) l = __uint_as_float(0x7fc00000u);  // NaN
                 const bool whole = p.steps == p.all;
                 const uint64_t part = (uint64_t)(2 * blockIdx.x + (p.step0 ? 0 : 1)) * S::kRows + tile * 128;
                 if (!whole) a.part_ml[part + r] = make_float2(m, l);
-                const float f = (whole ? l == 0.f ? 0.f : 1.f / l : 1.f) * (NF4 ? ref : 1.f);
+                // (m is -inf where nothing was seen: weights by the FMA pipe are 2^-126 there)
+                const float f = (whole ? l == 0.f || (m == -INFINITY && l == l) ? 0.f : 1.f / l : 1.f) * (NF4 ? ref : 1.f);
                 const uint32_t stage = q_tile + (warp & 3u) * (S::kQTile / 4);
                 constexpr uint32_t kRowBytes = 2 * D, kChunks = D / 8;  // a staged row: bf16 results, or half of a row's f32 sums
                 #pragma unroll 1
                 for (uint32_t half = 0; half < (whole ? 1u : 2u); ++half) {
                     const uint32_t columns = whole ? D : D / 2;
                     __syncwarp();
-                    #pragma unroll 1
-                    for (uint32_t k = 0; k < columns; k += 32) {
-                        uint32_t v[32];
-                        tmem_ld32(to + half * columns + k, v);
+                    uint32_t v[2][32];
+                    tmem_ld32(to + half * columns, v[0]);
+                    #pragma unroll
+                    for (uint32_t k = 0; k < D; k += 32) {
+                        if (k >= columns) break;
+                        uint32_t (&x)[32] = v[k / 32 & 1];
                         ptx::tmem_wait_ld();
+                        if (k + 32 < columns) tmem_ld32(to + half * columns + k + 32, v[k / 32 + 1 & 1]);
                         #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                        for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * f);
                         if (whole) {
                             #pragma unroll
                             for (uint32_t i = 0; i < 4; ++i) {
                                 uint32_t w[4];
                                 #pragma unroll
-                                for (int e = 0; e < 4; ++e) w[e] = bf16_pair(__uint_as_float(v[8 * i + 2 * e]), __uint_as_float(v[8 * i + 2 * e + 1]));
+                                for (int e = 0; e < 4; ++e) w[e] = bf16_pair(__uint_as_float(x[8 * i + 2 * e]), __uint_as_float(x[8 * i + 2 * e + 1]));
                                 st_shared_u4(stage + lane * kRowBytes + (((k / 8 + i) ^ (lane & 7u)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
                             }
                         } else {
                             #pragma unroll
                             for (uint32_t i = 0; i < 8; ++i)
-                                st_shared_u4(stage + lane * kRowBytes + (((k / 4 + i) ^ (lane & 7u)) << 4), make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+                                st_shared_u4(stage + lane * kRowBytes + (((k / 4 + i) ^ (lane & 7u)) << 4), make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]));
                         }
                     }
                     __syncwarp();
-                    #pragma unroll 4
-                    for (uint32_t i = lane; i < 32 * kChunks; i += 32) {
-                        const uint32_t rr = i / kChunks, x = i % kChunks, in_tile = (warp & 3u) * 32 + rr;
-                        if (tile * 128 + in_tile >= p.rows) continue;
-                        const uint4 v = ld_shared_u4(stage + rr * kRowBytes + ((x ^ (rr & 7u)) << 4));
+                    const uint32_t first = tile * 128 + (warp & 3u) * 32, here = p.rows > first ? min(32u, p.rows - first) : 0u;  // the warp's rows
+                    const uint32_t x = lane % kChunks;
+                    #pragma unroll 8
+                    for (uint32_t i = 0; i < kChunks; ++i) {
+                        const uint32_t rr = i * (32 / kChunks) + lane / kChunks;
+                        const uint4 w = ld_shared_u4(stage + rr * kRowBytes + ((x ^ (rr & 7u)) << 4));
                         if (whole) {
-                            const uint32_t q_row = p.r0 + tile * 128 + in_tile, token = a.by_group.of(q_row);
-                            *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(a.out) + (uint64_t)(p.s.row0 + token) * a.ldo +
-                                                       (uint64_t)(p.head * a.group + q_row - token * a.group) * D + 8 * x) = v;
-                        } else {
-                            *reinterpret_cast<uint4 *>(a.part_o + (part + in_tile) * D + half * (D / 2) + 4 * x) = v;
+                            const uint32_t q_row = p.r0 + first + rr, token = a.by_group.of(q_row);
+                            if (rr < here)
+                                *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(a.out) + (uint64_t)(p.s.row0 + token) * a.ldo +
+                                                           (uint64_t)(p.head * a.group + q_row - token * a.group) * D + 8 * x) = w;
+                        } else if (rr < here) {
+                            *reinterpret_cast<uint4 *>(a.part_o + (part + (warp & 3u) * 32 + rr) * D + half * (D / 2) + 4 * x) = w;
                         }
                     }
                 }
@@ -603,6 +644,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                 // In which order a thread takes its four words: so that eight lanes' 16-byte stores hit all banks
                 const uint32_t order = D == 128 ? (q >> 1) * 2 : D == 256 ? q >> 1 : 0u;
                 uint32_t i = 0, step = 0;  // tiles and steps so far
+                Ring ring;
                 auto wait = [&](uint32_t bar, uint32_t parity) {
                     if (ok && !__all_sync(0xffffffffu, ptx::mbar_wait_suspended(bar, parity))) {
                         ok = false;
@@ -612,10 +654,10 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                 for (; ok && walk.next(c, b, a, p); step += p.steps) {
                     const uint32_t t_end = min(visible_end(p.s, a.by_group, p.r0 + p.rows - 1), (p.step0 + p.steps) * N);
                     #pragma unroll 1
-                    for (uint32_t turn = 0; ok && turn < 2 * p.steps; ++turn, ++i) {
+                    for (uint32_t turn = 0; ok && turn < 2 * p.steps; ++turn, ++i, ring.on(slots)) {
                         const Turn<kPlaces> of(turn, p.steps);
                         const uint32_t which = of.values, j = of.step, t0 = (p.step0 + j) * N;
-                        const uint32_t rs = i % S::kRawSlots, slot = i % S::kSlots, raw = raw0 + rs * S::kRaw, dst = ring0 + slot * S::kTile + (q >> 1) * S::kBox;
+                        const uint32_t rs = i % S::kRawSlots, slot = ring.slot, raw = raw0 + rs * S::kRaw, dst = place_of(slot) + (q >> 1) * S::kBox;
                         wait(raw_full0 + 8 * rs, (i / S::kRawSlots) & 1u);
                         // the power above the tile's largest scale
                         auto power_of = [&](uint32_t from) {
@@ -634,7 +676,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                             const float v_power = power_of(raw + N * (D / 2) + S::kScales);
                             if (tid == 32 * kExpandWarp) s_powers[(step + j) & 7u] = make_float2(power, v_power);
                         }
-                        if (i >= S::kSlots) wait(empty0 + 8 * slot, (i / S::kSlots + 1) & 1u);
+                        if (ring.round) wait(empty0 + 8 * slot, (ring.round + 1) & 1u);
                         if (!ok) break;
                         {
                             const float unit = reciprocal_of_power(power) * (1.f / kLevelUnit);
@@ -678,43 +720,44 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                         }
                     }
                 }
-            } else if (warp == kCopyWarp) {
-                constexpr uint32_t kGroups = N / kGroup;
+            } else if (NF4 ? warp == kCopyWarp : warp < kExpandWarp + 2 * kCopies) {
+                const uint32_t own = NF4 ? 0u : (warp - kExpandWarp) & 1u, part = NF4 ? 0u : (warp - kExpandWarp) >> 1;  // bf16: K or V, and which columns
+                const uint32_t unit = NF4 ? kGroup : box_rows, units = N / unit;  // tokens that come together, being in one page
                 uint32_t i = 0, tails = 0, step = 0;
+                Ring ring;
                 for (uint32_t piece = 0; ok && walk.next(c, b, a, p); ++piece, step += p.steps) {
-                    if (lane == 0) s_bad[piece & 7u] = 0;  // (the others are at most three pieces behind)
-                    __syncwarp();
                     const uint32_t tile0 = expanded ? __ldg(dense.bases + p.seq) + p.step0 : 0u;
                     const uint32_t stored = min(p.s.length, (p.step0 + p.steps) * N);  // tokens that there are
                     #pragma unroll 1
-                    for (uint32_t turn = 0; ok && turn < 2 * p.steps; ++turn, ++i) {
+                    for (uint32_t turn = 0; ok && turn < 2 * p.steps; ++turn, ++i, ring.on(slots)) {
                         const Turn<kPlaces> of(turn, p.steps);
                         const uint32_t which = of.values, j = of.step;
-                        const uint32_t t0 = (p.step0 + j) * N, g = lane % kGroups, box = lane / kGroups, t = t0 + g * kGroup;
-                        const uint32_t groups = stored > t0 ? min(kGroups, (stored - t0 + kGroup - 1) / kGroup) : 0u;
-                        const uint32_t rs = i % S::kRawSlots, slot = i % S::kSlots;
+                        if (!NF4 && which != own) continue;
+                        const uint32_t t0 = (p.step0 + j) * N, g = lane % units, box = lane / units, t = t0 + g * unit;
+                        const uint32_t groups = stored > t0 ? min(units, (stored - t0 + unit - 1) / unit) : 0u;
+                        const uint32_t rs = i % S::kRawSlots, slot = ring.slot;
                         uint32_t place = 0;
                         if (expanded) {
                             if (!which) {
                                 const float2 powers = __ldg(dense.powers + (uint64_t)(tile0 + j) * c.heads + p.head);
-                                if (powers.x == 0.f) s_bad[piece & 7u] = 1;  // (a page that there is not)
+                                if (powers.x == 0.f) s_bad[piece & 7u] = piece + 1;  // (a page that there is not)
                                 if (lane == 0) s_powers[(step + j) & 7u] = powers;
                             }
                         } else if (g < groups) {
                             const uint32_t at = c.by_page.of(t);
                             const int32_t page = __ldg(b.table + (uint64_t)p.seq * b.width + at);
                             if (page >= 0 && (uint32_t)page < c.pages) place = ((uint32_t)page * c.heads + p.head) * c.page_size + (t - at * c.page_size);
-                            else s_bad[piece & 7u] = 1;
+                            else s_bad[piece & 7u] = piece + 1;
                         }
                         __syncwarp();
                         bool got = true;
                         if (NF4 && !expanded) {
                             if (i >= S::kRawSlots) got = ptx::mbar_wait_suspended(raw_empty0 + 8 * rs, (i / S::kRawSlots + 1) & 1u);
-                        } else if (i >= S::kSlots) {
-                            got = ptx::mbar_wait_suspended(empty0 + 8 * slot, (i / S::kSlots + 1) & 1u);
+                        } else if (ring.round) {
+                            got = ptx::mbar_wait_suspended(empty0 + 8 * slot, (ring.round + 1) & 1u);
                         }
                         got = __all_sync(0xffffffffu, got);
-                        const uint32_t dst = ring0 + slot * S::kTile;
+                        const uint32_t dst = place_of(slot);
                         if (!got) {
                         } else if (NF4 && expanded) {
                             const uint32_t bar = full0 + 8 * slot;
@@ -737,17 +780,20 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                             }
                         } else {
                             const bool tail = which && t0 + N > p.s.length;  // values that anything may stand behind: zeros, for weights of zero
-                            const uint32_t bar = tail ? tail_bar : full0 + 8 * slot;
-                            if (lane == 0) ptx::mbar_arrive_expect_tx(bar, groups * (kGroup * 128) * (D / 64));
+                            const uint32_t bar = tail ? tail0 + 8 * part : full0 + 8 * slot;
+                            constexpr uint32_t kColumns = D / 64 / kCopies;  // boxes of 64
+                            if (lane == 0) ptx::mbar_arrive_expect_tx(bar, groups * (unit * 128) * kColumns);
                             __syncwarp();
-                            if (g < groups && box < D / 64)
-                                ptx::tma_load_2d(dst + box * S::kBox + g * (kGroup * 128), which ? &tmap_v : &tmap_k, (int32_t)(64 * box), (int32_t)place, bar);
+                            if (g < groups && box < kColumns) {
+                                const uint32_t x = part * kColumns + box;
+                                ptx::tma_load_2d(dst + x * S::kBox + g * (unit * 128), which ? &tmap_v : &tmap_k, (int32_t)(64 * x), (int32_t)place, bar);
+                            }
                             if (tail) {
-                                got = __all_sync(0xffffffffu, ptx::mbar_wait_suspended(tail_bar, tails & 1u));
+                                got = __all_sync(0xffffffffu, ptx::mbar_wait_suspended(bar, tails & 1u));
                                 ++tails;
                                 for (uint32_t k = (p.s.length > t0 ? p.s.length - t0 : 0u) * 8 + lane; k < N * 8; k += 32)
                                     #pragma unroll
-                                    for (uint32_t x = 0; x < D / 64; ++x) st_shared_u4(dst + x * S::kBox + k * 16, make_uint4(0u, 0u, 0u, 0u));
+                                    for (uint32_t x = 0; x < kColumns; ++x) st_shared_u4(dst + (part * kColumns + x) * S::kBox + k * 16, make_uint4(0u, 0u, 0u, 0u));
                                 ptx::fence_proxy_async();
                                 __syncwarp();
                                 if (lane == 0) ptx::mbar_arrive(full0 + 8 * slot);
@@ -759,19 +805,29 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                         }
                     }
                 }
+            } else if (warp == kMmaWarp + 1) {
+                // (idle otherwise) the L2 asked for the queries of all of the CTA's pieces
+                while (walk.next(c, b, a, p))
+                    for (uint32_t i = lane; i < p.rows * (D / 64); i += 32) {
+                        const uint32_t row = p.r0 + i / (D / 64), token = a.by_group.of(row);
+                        const __nv_bfloat16 *const q = static_cast<const __nv_bfloat16 *>(a.q) + (uint64_t)(p.s.row0 + token) * a.ldq +
+                                                       (uint64_t)(p.head * a.group + row - token * a.group) * D + i % (D / 64) * 64;
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
+                    }
             } else if (warp == kMmaWarp) {
                 constexpr uint32_t fmt = NF4 ? 0 : 1;
                 constexpr uint32_t idesc_s = ptx::f16_idesc(fmt, 128, N, false, false), idesc_o = ptx::f16_idesc(fmt, 128, D, false, true);
-                uint32_t i = 0, made[2] = {0, 0}, used[2] = {0, 0}, rows_in[2] = {0, 0};  // tiles of K and V, scores, weights and Q's so far
+                uint32_t made[2] = {0, 0}, used[2] = {0, 0}, rows_in[2] = {0, 0};  // scores, weights and Q's so far
+                Ring ring;  // the next tile of K or V
                 auto wait = [&](uint32_t bar, uint32_t parity) {
                     if (!ok) return;
                     ok = __all_sync(0xffffffffu, ptx::mbar_wait_suspended(bar, parity));
                     if (!ok && lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 27);
                 };
-                auto wait_full = [&](uint32_t at) { wait(full0 + 8 * (at % S::kSlots), (at / S::kSlots) & 1u); };
+                auto wait_full = [&](const Ring &at) { wait(full0 + 8 * at.slot, at.round & 1u); };
                 // (these two by the elected thread)
                 auto scores = [&](uint32_t tile, uint32_t at, uint32_t n) {  // of the keys in ring place `at`, to the place of the tile's n-th
-                    const uint64_t qd = ptx::sw128_desc(q0 + tile * S::kQTile), kd = ptx::sw128_desc(ring0 + at % S::kSlots * S::kTile);
+                    const uint64_t qd = ptx::sw128_desc(q0 + tile * S::kQTile), kd = ptx::sw128_desc(place_of(at));
                     #pragma unroll
                     for (uint32_t k = 0; k < D / 16; ++k)
                         ptx::mma_ss_f16(tmem + S::kS + (kPlaces * tile + n % kPlaces) * N, qd + (k >> 2) * (16384 >> 4) + (k & 3u) * 2, kd + (k >> 2) * (S::kBox >> 4) + (k & 3u) * 2,
@@ -779,15 +835,15 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                     ptx::tc_commit(s_full0 + 8 * (kPlaces * tile + n % kPlaces));
                 };
                 auto products = [&](uint32_t tile, uint32_t at, uint32_t n, bool add) {
-                    const uint64_t vd = ptx::sw128_desc(ring0 + at % S::kSlots * S::kTile, S::kBox);
+                    const uint64_t vd = ptx::sw128_desc(place_of(at), S::kBox);
                     #pragma unroll
                     for (uint32_t k = 0; k < N / 16; ++k)
                         ptx::mma_ts_f16(tmem + S::kO + tile * D, tmem + S::kS + (kPlaces * tile + n % kPlaces) * N + 8 * k, vd + 128 * k, idesc_o, add || k != 0);
-                    ptx::tc_commit(pv_done0 + 8 * tile);
+                    if (kPlaces > 1) ptx::tc_commit(pv_done0 + 8 * tile);
                 };
                 while (ok && walk.next(c, b, a, p)) {
-                    for (uint32_t j = 0; j < min(kPlaces, p.steps) && ok; ++j, ++i) {  // the first scores
-                        wait_full(i);
+                    for (uint32_t j = 0; j < min(kPlaces, p.steps) && ok; ++j, ring.on(slots)) {  // the first scores
+                        wait_full(ring);
                         for (uint32_t t = 0; t < p.live; ++t) {
                             if (j == 0) {
                                 wait(q_ready0 + 8 * t, rows_in[t] & 1u);
@@ -795,8 +851,8 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                             }
                             ptx::tc_fence_after();
                             if (ok && ptx::elect_one()) {
-                                scores(t, i, made[t]);
-                                if (t + 1 == p.live) ptx::tc_commit(empty0 + 8 * (i % S::kSlots));
+                                scores(t, ring.slot, made[t]);
+                                if (t + 1 == p.live) ptx::tc_commit(empty0 + 8 * ring.slot);
                             }
                             ++made[t];
                             __syncwarp();
@@ -804,29 +860,31 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                     }
                     for (uint32_t j = 0; j < p.steps && ok; ++j) {
                         const bool more = j + kPlaces < p.steps;
-                        wait_full(i);
+                        const Ring v = ring;
+                        ring.on(slots);
+                        const Ring k = ring;
+                        if (more) ring.on(slots);
+                        wait_full(v);  // (both ahead of the weights: what is looked at while they are made costs nothing)
+                        if (more) wait_full(k);
                         for (uint32_t t = 0; t < p.live; ++t) {
                             wait(p_ready0 + 8 * (kPlaces * t + used[t] % kPlaces), (used[t] / kPlaces) & 1u);
                             if (!ok) break;
                             ptx::tc_fence_after();
                             if (ptx::elect_one()) {
-                                products(t, i, used[t], j != 0);
-                                if (t + 1 == p.live) ptx::tc_commit(empty0 + 8 * (i % S::kSlots));
+                                products(t, v.slot, used[t], j != 0);
+                                if (t + 1 == p.live) ptx::tc_commit(empty0 + 8 * v.slot);
+                                if (j + 1 == p.steps) ptx::tc_commit(o_done0 + 8 * t);
                             }
                             ++used[t];
                             __syncwarp();
                             if (!more) continue;
-                            if (t == 0) wait_full(i + 1);
-                            if (!ok) break;
-                            ptx::tc_fence_after();
                             if (ptx::elect_one()) {
-                                scores(t, i + 1, made[t]);
-                                if (t + 1 == p.live) ptx::tc_commit(empty0 + 8 * ((i + 1) % S::kSlots));
+                                scores(t, k.slot, made[t]);
+                                if (t + 1 == p.live) ptx::tc_commit(empty0 + 8 * k.slot);
                             }
                             ++made[t];
                             __syncwarp();
                         }
-                        i += more ? 2 : 1;
                     }
                 }
             }
@@ -1017,9 +1075,11 @@ int32_t launch(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) 
     NF4_TRY(ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), S::kSmem));
     const uint64_t pool = (uint64_t)c.cache.pages * c.cache.heads * c.cache.page_size;
     CUtensorMap map_k{}, map_v{};
+    uint32_t box_rows = kGroup;  // tokens of a page that come in one copy
     if (!NF4) {
-        NF4_TRY(make_map(&map_k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, c.cache.k, pool, D, 2 * D, kGroup, 64, CU_TENSOR_MAP_SWIZZLE_128B));
-        NF4_TRY(make_map(&map_v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, c.cache.v, pool, D, 2 * D, kGroup, 64, CU_TENSOR_MAP_SWIZZLE_128B));
+        while (box_rows < S::kTokens && c.cache.page_size % (2 * box_rows) == 0) box_rows *= 2;
+        NF4_TRY(make_map(&map_k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, c.cache.k, pool, D, 2 * D, box_rows, 64, CU_TENSOR_MAP_SWIZZLE_128B));
+        NF4_TRY(make_map(&map_v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, c.cache.v, pool, D, 2 * D, box_rows, 64, CU_TENSOR_MAP_SWIZZLE_128B));
     }
     FailureRef failure;
     NF4_TRY(prefill_failure_ref(&failure));
@@ -1050,7 +1110,7 @@ int32_t launch(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) 
     }
     const uint32_t ctas = persistent_ctas();
     count_launch(2);
-    NF4_TRY(launch_maybe_overlapped(kernel, dim3(ctas), dim3(kThreads), S::kSmem, stream, true, map_k, map_v, c.cache, c.batch, view, dense, splits, failure));
+    NF4_TRY(launch_maybe_overlapped(kernel, dim3(ctas), dim3(kThreads), S::kSmem, stream, true, map_k, map_v, c.cache, c.batch, view, dense, box_rows, splits, failure));
     return launch_maybe_overlapped(join_pieces_kernel<D, NF4>, dim3(ctas, S::kRows / (kJoinRows * kJoinWarps)), dim3(32 * kJoinWarps), 0, stream, true, view,
                                    static_cast<const Split *>(splits));
 }
