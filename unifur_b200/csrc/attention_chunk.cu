@@ -94,24 +94,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return r;
 }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 r;
-    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return r;
-}
-// 2^e of two numbers up to 2^8 (below 2^-126 that) without the exponential unit: e = i + f with f in [-1/2, 1/2], 2^f by the polynomial of degree
-// 3 that is least off (7.5e-5, a third of an f16's rounding on average; found by weighted least squares), i added to its exponent.
-__device__ __forceinline__ float2 exp2_by_fma(float2 e) {
-    const float2 one = make_float2(12582912.f, 12582912.f);  // 1.5 * 2^23: adding it leaves i in the low bits
-    e = make_float2(fmaxf(e.x, -126.f), fmaxf(e.y, -126.f));
-    const float2 t = add2(e, one), i = add2(t, make_float2(-12582912.f, -12582912.f));
-    const float2 f = add2(e, make_float2(-i.x, -i.y));
-    float2 p = fma2(f, make_float2(0.05517167f, 0.05517167f), make_float2(0.24261112f, 0.24261112f));
-    p = fma2(p, f, make_float2(0.69326099f, 0.69326099f));
-    p = fma2(p, f, make_float2(0.99992807f, 0.99992807f));
-    return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)), __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
-}
 template <bool F16>
 __device__ __forceinline__ uint32_t pack(float a, float b) {
     uint32_t r;
@@ -163,7 +145,7 @@ struct Piece {
 
 // Steps' worth of time that a row tile takes beside its steps (its queries in, its results out): counted in the line, or the CTAs that have
 // a prompt's first tiles, of one step each, would be done last.
-constexpr uint32_t kStart = 3;
+constexpr uint32_t kStart = 4;
 
 template <uint32_t R, uint32_t N>
 struct Walker {  // through a CTA's pieces; every warp goes its own way
@@ -520,8 +502,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                             for (uint32_t i = 0; i < 32; i += 2) {
                                 top[(i >> 1) & 1] = fmaxf(fmaxf(top[(i >> 1) & 1], __uint_as_float(x[i])), __uint_as_float(x[i + 1]));
                                 const float2 e = fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), factor, from);
-                                // the exponential unit gives 16 a clock, which is what the MMAs take as long for: a quarter goes by the FMA pipe
-                                const float2 w = i % 8 == 6 ? exp2_by_fma(e) : make_float2(exp2_approx(e.x), exp2_approx(e.y));
+                                const float2 w = make_float2(exp2_approx(e.x), exp2_approx(e.y));
                                 sum = add2(sum, w);
                                 pw[(k + i) / 2] = pack<NF4>(w.x, w.y);
                             }
@@ -580,8 +561,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                 const bool whole = p.steps == p.all;
                 const uint64_t part = (uint64_t)(2 * blockIdx.x + (p.step0 ? 0 : 1)) * S::kRows + tile * 128;
                 if (!whole) a.part_ml[part + r] = make_float2(m, l);
-                // (m is -inf where nothing was seen: weights by the FMA pipe are 2^-126 there)
-                const float f = (whole ? l == 0.f || (m == -INFINITY && l == l) ? 0.f : 1.f / l : 1.f) * (NF4 ? ref : 1.f);
+                const float f = (whole ? l == 0.f ? 0.f : 1.f / l : 1.f) * (NF4 ? ref : 1.f);
                 const uint32_t stage = q_tile + (warp & 3u) * (S::kQTile / 4);
                 constexpr uint32_t kRowBytes = 2 * D, kChunks = D / 8;  // a staged row: bf16 results, or half of a row's f32 sums
                 #pragma unroll 1
@@ -864,8 +844,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                         ring.on(slots);
                         const Ring k = ring;
                         if (more) ring.on(slots);
-                        wait_full(v);  // (both ahead of the weights: what is looked at while they are made costs nothing)
-                        if (more) wait_full(k);
+                        wait_full(v);
                         for (uint32_t t = 0; t < p.live; ++t) {
                             wait(p_ready0 + 8 * (kPlaces * t + used[t] % kPlaces), (used[t] / kPlaces) & 1u);
                             if (!ok) break;
@@ -878,6 +857,9 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                             ++used[t];
                             __syncwarp();
                             if (!more) continue;
+                            if (t == 0) wait_full(k);
+                            if (!ok) break;
+                            ptx::tc_fence_after();
                             if (ptx::elect_one()) {
                                 scores(t, k.slot, made[t]);
                                 if (t + 1 == p.live) ptx::tc_commit(empty0 + 8 * k.slot);
