@@ -52,9 +52,9 @@ BatchView view_of(const nf4_cache_batch &b) {
 namespace {
 
 constexpr int kThreads = 256;
-// Rows to a thread at most, all asked for before the first is used.  Measured with 1, 2, 4 and 8: 7,300 rows of four heads of 128 quantized in
-// 22.4, 19.7, 20.5 and 26.7 us (2.5 TB/s; the last: three or four CTAs to an SM, which is uneven), 26,900 read in 27.7, 19.4, 15.8
-// and 15.0 us (4.5 TB/s; bound by instructions as much as by HBM).
+// Rows to a thread at most, all asked for before the first is used.  Measured with 1, 2, 4 and 8 for both: 7,300 rows of four heads of 128
+// quantized and then read back as f32 in 22.4, 19.7, 20.5 and 26.7 us, 26,900 read as bf16 in 27.7, 19.4, 15.8 and 15.0 us (4.5 TB/s;
+// bound by instructions as much as by HBM).
 constexpr uint32_t kAppendBatch = 2, kReadBatch = 4;
 constexpr uint32_t kMostRows = 4 * kThreads / 16;    // of a CTA: a row has 16 groups at least
 constexpr uint32_t kStarts = 1024;                   // row_starts that a CTA holds; of more, every second, third, ...
