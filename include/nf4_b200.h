@@ -478,7 +478,8 @@ typedef struct nf4_cache {
  * of n is token lengths[s] - n + i.  Token t is at place t % page_size of page page_table[s][t / page_size].
  * page_table, lengths and row_starts are device memory and may be changed between launches of a captured
  * graph; row_starts does not decrease.  Whatever stands in them, no access leaves the buffers: lengths beyond the table's
- * pages and row_starts beyond `rows` are cut there.  Rows that belong to no sequence are neither read nor written.
+ * pages and row_starts beyond `rows` are cut there.  Rows that belong to no sequence are not written, and what stands in them does not
+ * matter.
  * Sequences may share pages (a common prefix); a token that a call appends is in a page of its sequence alone. */
 typedef struct nf4_cache_batch {
     uint32_t struct_bytes;      /* sizeof(nf4_cache_batch), checked */
@@ -509,7 +510,7 @@ NF4_API int32_t nf4_cache_read_dev(const nf4_cache *cache, const nf4_cache_batch
  * h reads head h / (q_heads / heads) of the cache.  A row whose token is negative sees nothing and becomes zeros; a
  * row that sees a token in a page outside [0, num_pages) becomes NaNs (others of its sequence may, too).  Values of the tokens
  * that a call's rows see are finite; what stands in other places of their pages does not matter.  One token to a sequence, drafted
- * tokens, chunks of a prompt and whole prompts are the same call.
+ * tokens, chunks of a prompt and whole prompts are the same call.  out does not overlap q.
  * bf16 tensors multiply on the tensor cores with f32 sums; f32 tensors in f32 throughout.
  * workspace: nf4_cache_attention_workspace_bytes() bytes, 256-byte aligned, the first nf4_cache_attention_flag_bytes() of
  * them zero at the first use; every call leaves them zero.  One workspace serves one stream. */

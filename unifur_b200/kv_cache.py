@@ -2,7 +2,7 @@
 
 No counterpart on the reference's NF4 path: these are the operators between the projections that
 ``linear_forward_grouped`` makes of a layer's input and the one that takes the attention's result.  Every computation is a
-call into ``libnf4b200.so``; ``torch`` holds the memory.
+call into ``libnf4b200.so``; ``torch`` holds the memory.  They serve: nothing here has a gradient.
 """
 from __future__ import annotations
 
@@ -21,7 +21,7 @@ class CacheBatch:
     Rows ``row_starts[s]`` to ``row_starts[s + 1]`` are the newest tokens of sequence ``s``, which has ``lengths[s]`` tokens in
     the cache with them; token ``t`` is at place ``t % page_size`` of page ``page_table[s][t // page_size]``.  All three are
     int32 tensors on the cache's device (``[sequences, pages]``, ``[sequences]``, ``[sequences + 1]``); their values may change
-    between replays of a captured graph.  ``rows``: rows of the call's tensors; those of no sequence are neither read nor written.
+    between replays of a captured graph.  ``rows``: rows of the call's tensors; those of no sequence are not written.
     ``max_rows``, ``max_length``: the most rows and tokens of a sequence where the program knows them; they choose kernels and
     how work is shared out, and results hold without them.  Sequences may share the pages of a common prefix, but a token that a
     call appends is in a page of its sequence alone."""
