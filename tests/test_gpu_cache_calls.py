@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from cache_util import DEV, batch_of, filled_cache, largest, reference, spoil_unused, tolerance
+from unifur_b200 import _lib
 from unifur_b200.kv_cache import CacheBatch, PagedKvCache
 
 pytestmark = pytest.mark.gpu
@@ -194,3 +195,79 @@ def test_a_pool_beyond_32_bits(quantized):
         q = rows_of(batch, 2 * heads, dim, dtype)
         assert torch.equal(big.attention(q, there), small.attention(q, batch))
         assert all(torch.equal(a, b) for a, b in zip(big.read(there, dtype), small.read(batch, dtype)))
+
+
+# ---- the kernel for many rows, which a wide page table without hints stands for (one launch more than the kernel that streams the cache, or two) ----
+
+def wide(specs, page_size, tokens=1 << 16, **more):
+    return batch_of(specs, page_size, width=tokens // page_size, hints=False, **more)
+
+
+def many(cache, batch, q, **more):
+    before = _lib.launch_count()
+    out = cache.attention(q, batch, **more)
+    assert _lib.launch_count() - before >= 2
+    return out
+
+
+CHUNKS = [[(130, 130)], [(300, 40), (65, 64), (1, 1)], [(1000, 129), (257, 257)], [(20, 33), (128, 128)], [(513, 300), (0, 7)]]
+
+
+@pytest.mark.parametrize("quantized", [True, False])
+@pytest.mark.parametrize("heads,group,dim,page_size", [(2, 7, 128, 64), (1, 4, 64, 16), (1, 3, 256, 48), (2, 2, 128, 80)])
+@pytest.mark.parametrize("specs", CHUNKS)
+def test_many_rows(specs, heads, group, dim, page_size, quantized):
+    batch, pages = wide(specs, page_size, tokens=1 << 20 if dim == 64 else page_size * 1024, spare_rows=(1, 2))
+    cache = filled_cache(pages, page_size, heads, dim, quantized)
+    spoil_unused(cache, batch)
+    q = rows_of(batch, heads * group, dim)
+    out = torch.full_like(q, 7.0)
+    many(cache, batch, q, out=out)
+    check(cache, batch, q, out)
+    assert (out[:1] == 7).all() and (out[-2:] == 7).all()
+
+
+@pytest.mark.parametrize("quantized", [True, False])
+@pytest.mark.parametrize("k_std,v_std,q_std,scale", [(1e4, 1.0, 1e-4, None), (1e-6, 1e6, 1e6, 0.1), (1.0, 1e-6, 1.0, 0.0), (1.0, 1.0, 1.0, -0.3), (1.0, 1.0, 30.0, None)])
+@pytest.mark.parametrize("n", [70, 300])
+def test_magnitudes_of_many_rows(n, quantized, k_std, v_std, q_std, scale):
+    batch, pages = wide([(700, n)], 16, tokens=1 << 20)
+    cache = filled_cache(pages, 16, 1, 128, quantized, k_std=k_std, v_std=v_std)
+    q = (rows_of(batch, 2, 128, F32) * q_std).bfloat16()
+    check(cache, batch, q, many(cache, batch, q, scale=scale), scale)
+
+
+@pytest.mark.parametrize("quantized", [True, False])
+@pytest.mark.parametrize("n", [90, 600])
+def test_many_rows_and_a_page_that_there_is_not(n, quantized):
+    """That sequence's rows behind it are NaNs, another's are right."""
+    batch, pages = wide([(700, n), (300, 64)], 16, tokens=1 << 20)
+    cache = filled_cache(pages, 16, 2, 64, quantized)
+    q = rows_of(batch, 4, 64)
+    want = many(cache, batch, q)
+    batch.page_table[0, 2] = pages
+    got = many(cache, batch, q)
+    assert got[:n].isnan().all() and torch.equal(got[n:], want[n:])
+
+
+def test_more_tokens_than_the_hint_says():
+    """The room for expanded keys and values follows the hint; with more tokens they are expanded where they are used."""
+    batch, pages = batch_of([(3000, 700), (2000, 300)], 64)
+    cache = filled_cache(pages, 64, 2, 128, True)
+    q = rows_of(batch, 32, 128)
+    batch.max_rows, batch.max_length = 100000, 100
+    check(cache, batch, q, many(cache, batch, q))
+
+
+@pytest.mark.parametrize("quantized", [True, False])
+@pytest.mark.parametrize("n,dim", [(40, 128), (9, 256), (300, 64)])
+def test_both_kernels_agree(n, dim, quantized):
+    """The same batch with a narrow and with a wide page table."""
+    specs = [(700, n), (31, 3), (300, 1)]
+    narrow, pages = batch_of(specs, 16)
+    table = torch.full((3, 4096), -1, dtype=torch.int32, device=DEV)
+    table[:, :narrow.page_table.shape[1]] = narrow.page_table
+    cache = filled_cache(pages, 16, 1, dim, quantized)
+    q = rows_of(narrow, 8, dim)
+    for batch in (narrow, CacheBatch(table, narrow.lengths, narrow.row_starts, narrow.rows)):
+        check(cache, batch, q, cache.attention(q, batch))

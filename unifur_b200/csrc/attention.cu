@@ -250,8 +250,26 @@ join_kernel(const BatchView b, const AttentionView a, uint32_t q_heads) {
 }
 
 // ---- how a call is carried out -----------------------------------------------------------------------
-// Few rows to a head of a sequence: the kernel that streams the cache; its tiles have 16 rows, four of them read the tokens four times.
-bool takes_decode(const AttentionCall &c) { return !c.f32 && (uint64_t)c.most_rows * c.view.group <= 64; }
+// Which of two kernels: the one that streams the cache reads a head's tokens once for every 16 rows, the one for many rows once for
+// every 256 (128 with a dim of 256).  By what each takes, in tenths of a microsecond on an SM: a row tile's start, and 128 tokens of
+// it; the second kernel's own start, its joins and the expansion ahead of it are 15 to 20 us more.  Measured on both sides (us, first / second):
+// 16 sequences of 8192 tokens, 8 heads of 128, NF4: 16 rows 62 / 166, 48 rows 161 / 166, 64 rows 211 / 166; bf16: 16 rows 92 / 126, 32 rows
+// 177 / 127; one such sequence, NF4: 96 rows 34 / 43, 128 rows 46 / 43; 4 sequences of 512, 4 heads, NF4: 384 rows 24 / 31, 768 rows 44 / 35; 8
+// of 4096, 4 heads of 256, NF4: 16 rows 40 / 62, 32 rows 69 / 64; 8 heads of 64, NF4: 64 rows 54 / 52, bf16: 64 rows 40 / 43.
+bool takes_decode(const AttentionCall &c) {
+    if (c.f32) return false;
+    const int of_dim = c.head_dim == 64 ? 0 : c.head_dim == 128 ? 1 : 2;
+    static constexpr double kStream[2][3] = {{5, 11, 32}, {7, 9, 45}}, kMany[2][3] = {{13, 18, 40}, {19, 25, 58}};  // [NF4][dim]
+    // row tiles of all sequences: by the most rows of one, or by all rows where that says less
+    auto tiles = [&](uint64_t rows) -> double {
+        const uint64_t group = c.view.group, all = (uint64_t)c.batch.rows * group / rows + c.batch.sequences;
+        return (double)std::min<uint64_t>(all, c.batch.sequences * (((uint64_t)c.most_rows * group + rows - 1) / rows));
+    };
+    const double steps = c.most_tokens / 128 + 1, heads = c.cache.heads;
+    const double stream = tiles(16) * heads * (32 + steps * kStream[c.nf4][of_dim]);
+    const double many = tiles(c.head_dim == 256 ? 128 : 256) * heads * (90 + steps * kMany[c.nf4][of_dim]) + kNumSMs * (c.nf4 ? 200 : 150);
+    return stream <= many;
+}
 
 struct Plan {
     uint32_t row_tiles, parts;  // CTAs to a head of a sequence: row tiles side by side, and parts of the tokens
