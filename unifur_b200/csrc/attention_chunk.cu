@@ -336,8 +336,9 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
         share.ctas = min(gridDim.x, (total + kStart + 1) / (kStart + 2));  // two steps at least
         share.per = share.ctas ? total / share.ctas : 0;
         share.more = share.ctas ? total - share.per * share.ctas : 0;
-        const uint32_t first = share.start(blockIdx.x), last = blockIdx.x < share.ctas ? share.start(blockIdx.x + 1) : first;
-        uint32_t before = 0;
+        const uint32_t first = share.start(blockIdx.x);
+        uint32_t last = blockIdx.x < share.ctas ? share.start(blockIdx.x + 1) : first, before = 0;
+        bool found = false;
         for (uint32_t k = 0; first < last && k < b.sequences; k += 32) {
             Sequence s = s0;
             const uint32_t own = k ? steps_of(k, s) : own0;
@@ -352,7 +353,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                 const int l = __ffs(past) - 1;
                 const Sequence o{__shfl_sync(0xffffffffu, s.row0, l), __shfl_sync(0xffffffffu, s.rows, l), __shfl_sync(0xffffffffu, s.length, l)};
                 const uint32_t at = first - before - __shfl_sync(0xffffffffu, upto - own, l), of_head = __shfl_sync(0xffffffffu, own, l) / c.heads;
-                const uint32_t head = at / of_head;
+                const uint32_t head = of_head ? at / of_head : c.heads;
                 uint32_t left = at - head * of_head, tile = 0;
                 for (uint32_t t0 = 0;; t0 += 32) {
                     const uint32_t mine = t0 + lane < Walk::tiles_of(o, a.group) ? kStart + Walk::steps_of(o, a, t0 + lane) : 0u;
@@ -367,9 +368,10 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                         const int t = __ffs(in) - 1;
                         tile = t0 + t;
                         left -= __shfl_sync(0xffffffffu, sum - mine, t);
+                        found = head < c.heads;
                         break;
                     }
-                    if (t0 + 32 >= Walk::tiles_of(o, a.group)) break;  // (not reached: the head has that many steps)
+                    if (t0 + 32 >= Walk::tiles_of(o, a.group)) break;  // (not reached where row starts do not decrease: the head has that many steps)
                     left -= __shfl_sync(0xffffffffu, sum, 31);
                 }
                 if (lane == 0) {
@@ -382,6 +384,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             }
             before += __shfl_sync(0xffffffffu, upto, 31);
         }
+        if (!found) last = first;  // (row starts that decrease, whose rows are more than the line is counted for: no access by what is not there)
         if (lane == 0) {
             s_first[4] = first;
             s_first[5] = last;
@@ -610,7 +613,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                     }
                 }
                 if (!whole && p.step0 == 0 && tid == 0) {
-                    const uint32_t more = s_share.cta_of(p.line0 + kStart + p.all - 1) - blockIdx.x;
+                    const uint32_t more = min(s_share.cta_of(p.line0 + kStart + p.all - 1) - blockIdx.x, gridDim.x - 1 - blockIdx.x);
                     splits[blockIdx.x] = Split{p.s.row0, p.r0, p.rows, p.head, more};
                 }
                 ptx::tc_fence_before();
@@ -897,7 +900,8 @@ expand_kernel(const CacheView c, const BatchView b, uint4 *const k_out, uint4 *c
     ptx::pdl_wait();
     // which sequence the tile is of (every warp finds it); the first CTA writes down where each begins
     const uint32_t head = blockIdx.x % c.heads, want = blockIdx.x / c.heads;
-    uint32_t seq = b.sequences, tile = 0, before = 0;
+    uint32_t seq = b.sequences, tile = 0;
+    uint64_t before = 0;
     Sequence s{0, 0, 0};
     for (uint32_t s0 = 0; s0 < b.sequences && (seq == b.sequences || blockIdx.x == 0); s0 += 32) {
         Sequence o{0, 0, 0};
@@ -909,17 +913,17 @@ expand_kernel(const CacheView c, const BatchView b, uint4 *const k_out, uint4 *c
             const uint32_t v = __shfl_up_sync(0xffffffffu, upto, d);
             if (lane >= (uint32_t)d) upto += v;
         }
-        if (blockIdx.x == 0 && tid < 32 && s0 + lane < b.sequences) bases[s0 + lane] = before + upto - own;
+        if (blockIdx.x == 0 && tid < 32 && s0 + lane < b.sequences) bases[s0 + lane] = (uint32_t)before + upto - own;
         const uint32_t past = __ballot_sync(0xffffffffu, before + upto > want);
         if (past && seq == b.sequences) {
             const int l = __ffs(past) - 1;
             seq = s0 + l;
-            tile = want - before - __shfl_sync(0xffffffffu, upto - own, l);
+            tile = want - (uint32_t)before - __shfl_sync(0xffffffffu, upto - own, l);
             s = Sequence{__shfl_sync(0xffffffffu, o.row0, l), __shfl_sync(0xffffffffu, o.rows, l), __shfl_sync(0xffffffffu, o.length, l)};
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    if (blockIdx.x == 0 && tid == 0) bases[b.sequences] = before;
+    if (blockIdx.x == 0 && tid == 0) bases[b.sequences] = (uint32_t)min(before, (uint64_t)0xffffffffu);
     if (seq == b.sequences) return;
     __syncthreads();
     const uint32_t t0 = tile * N, tokens = s.length > t0 ? min(N, s.length - t0) : 0u;

@@ -93,9 +93,9 @@ struct AttentionView {
     uint32_t parts;
 };
 
-// How many tokens row tile `tile` (of `rows` rows) of a sequence sees: its last row's.
-__device__ __forceinline__ uint32_t visible_end(const Sequence &s, const FastDiv &by_group, uint32_t last_row) {
-    const int32_t token = (int32_t)s.length - (int32_t)s.rows + (int32_t)by_group.of(last_row);
+// How many tokens a row sees; of a tile's rows the last sees most.
+__device__ __forceinline__ uint32_t visible_end(const Sequence &s, const FastDiv &by_group, uint32_t row) {
+    const int32_t token = (int32_t)s.length - (int32_t)s.rows + (int32_t)by_group.of(row);
     return (uint32_t)max(token, -1) + 1;
 }
 
