@@ -529,6 +529,9 @@ typedef struct nf4_attention_args {
 NF4_API uint64_t nf4_cache_attention_workspace_bytes(const nf4_cache *cache, const nf4_cache_batch *batch, uint32_t q_heads,
                                                      int32_t io_dtype);
 NF4_API uint64_t nf4_cache_attention_flag_bytes(void);
+/* Of those, how many the call relies on: all, or 0.  For a host that allocates a workspace per call. */
+NF4_API uint64_t nf4_cache_attention_call_flag_bytes(const nf4_cache *cache, const nf4_cache_batch *batch, uint32_t q_heads,
+                                                     int32_t io_dtype);
 NF4_API int32_t nf4_cache_attention_dev(const nf4_cache *cache, const nf4_cache_batch *batch, const nf4_attention_args *args,
                                         void *stream);
 

@@ -103,6 +103,19 @@ def test_workspace_grows_with_the_call_and_holds_the_flags(lib):
     assert max(sizes) < 1 << 30
 
 
+def test_flags_that_a_call_relies_on(lib):
+    """Those of the kernel that streams the cache, which single tokens and short contexts take in bf16; none with f32 tensors."""
+    def flags(io, **changed):
+        cache, batch, _ = arguments(batch__pages_per_sequence=1024, **changed)
+        return lib.nf4_cache_attention_call_flag_bytes(ctypes.byref(cache), ctypes.byref(batch), 28, io)
+
+    most = lib.nf4_cache_attention_flag_bytes()
+    assert flags(0, batch__rows=1) == most and flags(0, batch__rows=300, batch__max_length=128) == most
+    assert flags(0, batch__rows=4000, batch__max_length=16384) == 0
+    assert flags(1, batch__rows=1) == 0
+    assert flags(0, batch__rows=1, cache__page_size=24) == most  # (refused by the call itself)
+
+
 def test_host_tensors_are_refused(lib):
     from unifur_b200 import _lib
     from unifur_b200.kv_cache import CacheBatch, PagedKvCache

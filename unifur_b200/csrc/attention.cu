@@ -350,6 +350,12 @@ extern "C" {
 
 uint64_t nf4_cache_attention_flag_bytes(void) { return kAttentionFlagBytes; }
 
+uint64_t nf4_cache_attention_call_flag_bytes(const nf4_cache *cache, const nf4_cache_batch *batch, uint32_t q_heads, int32_t io_dtype) {
+    const char *const what = "nf4_cache_attention_call_flag_bytes";
+    if (check_cache(what, cache, batch) != NF4_OK || check_heads(what, *cache, *batch, q_heads) != NF4_OK) return kAttentionFlagBytes;
+    return takes_decode(call_of(*cache, *batch, q_heads, io_dtype)) ? kAttentionFlagBytes : 0;
+}
+
 uint64_t nf4_cache_attention_workspace_bytes(const nf4_cache *cache, const nf4_cache_batch *batch, uint32_t q_heads, int32_t io_dtype) {
     const char *const what = "nf4_cache_attention_workspace_bytes";
     if (check_cache(what, cache, batch) != NF4_OK || check_heads(what, *cache, *batch, q_heads) != NF4_OK) return 0;

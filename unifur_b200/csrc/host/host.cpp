@@ -690,7 +690,8 @@ PyObject *cache_attention(PyObject *, PyObject *const *v, Py_ssize_t n) {
         const uint64_t bytes = nf4_cache_attention_workspace_bytes(&c.cache, &c.batch, a.q_heads, a.io_dtype);
         Tensor ws;
         if (bytes) {  // (0: arguments that the call refuses)
-            ws = flagged_workspace(bytes, place, kAttentionSlot, nf4_cache_attention_flag_bytes());
+            const uint64_t flags = nf4_cache_attention_call_flag_bytes(&c.cache, &c.batch, a.q_heads, a.io_dtype);
+            ws = flags ? flagged_workspace(bytes, place, kAttentionSlot, flags) : empty({(int64_t)bytes}, at::kByte, place);
             a.workspace = ws.mutable_data_ptr();
             a.workspace_bytes = (uint64_t)ws.numel();
         }
