@@ -1,5 +1,6 @@
 // Attention of a call's rows over the paged cache: the entry points, the kernel for f32 tensors, and the join of parts.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_cache.cuh"
 #include "ptx.cuh"
@@ -9,19 +10,20 @@ namespace nf4 {
 namespace {
 
 // ---- f32 throughout ---------------------------------------------------------------------------------
-// A CTA has a tile of 64 rows of one head of the cache and goes over its tokens 32 at a time (16 with a dim of 256): four rows to a
-// thread, by every eighth token for the scores and by dim / 8 values for the results, weights from one to the other through shared
-// memory, with the running largest exponent and sum of a softmax that is never held whole.  A row's scores are eight neighbouring lanes'.
-// FMAs are done in pairs.  Bound by shared memory: 8 reads of 16 bytes to 32 pairs of FMAs for the scores, 3 to 16 for the results (of 64).  (Two
-// rows to a thread, 256 threads: 6 to 16 and 4 to 8.)
+// A CTA has a tile of 16, 32 or 64 rows of one head of the cache (as many as there are, or 64) and goes over its tokens 32 at a time (16 with a
+// dim of 256): one, two or four rows to a thread, by every eighth token for the scores and by dim / 8 values for the results, weights from one to the
+// other through shared memory, with the running largest exponent and sum of a softmax that is never held whole.  A row's scores are
+// eight neighbouring lanes'.  FMAs are done in pairs.  Bound by shared memory, which gives registers 128 bytes a clock: with four rows 8 reads of
+// 16 bytes to 32 pairs of FMAs for the scores and 5 to 32 for the results (of 128), 24 to 30 TFLOP/s for long prompts; with one row 5 to 4 and 5
+// to 8 (16 sequences of 4096 tokens, 7 rows of four heads of 128: 180 us, 280 with tiles of 64 rows).
 constexpr int kThreads = 256, kF32Threads = 128;
-constexpr uint32_t kRows = 64;
 
 constexpr uint32_t tokens_of_tile(uint32_t dim) { return dim == 256 ? 16 : 32; }
 
-template <int D>
+// R: rows to a thread
+template <int D, int R>
 struct F32Shape {
-    static constexpr uint32_t kTokens = tokens_of_tile(D), kPitch = D + 4, kPPitch = kRows + 4;
+    static constexpr uint32_t kRows = 16 * R, kTokens = tokens_of_tile(D), kPitch = D + 4, kPPitch = kRows + 4;
     static constexpr uint32_t kSmem = 4 * (kRows * kPitch + 2 * kTokens * kPitch + kTokens * kPPitch);
 };
 
@@ -33,11 +35,30 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     return r;
 }
 
-template <int D, bool NF4>
+template <int R>
+__device__ __forceinline__ void put(float *to, const float (&v)[R]) {
+    if constexpr (R == 4) *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
+    else if constexpr (R == 2) *reinterpret_cast<float2 *>(to) = make_float2(v[0], v[1]);
+    else *to = v[0];
+}
+template <int R>
+__device__ __forceinline__ void get(const float *from, float (&v)[R]) {
+    if constexpr (R == 4) {
+        const float4 w = *reinterpret_cast<const float4 *>(from);
+        v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
+    } else if constexpr (R == 2) {
+        const float2 w = *reinterpret_cast<const float2 *>(from);
+        v[0] = w.x; v[1] = w.y;
+    } else {
+        v[0] = *from;
+    }
+}
+
+template <int D, bool NF4, int R>
 __global__ void __launch_bounds__(kF32Threads)
 attention_f32_kernel(const CacheView c, const BatchView b, const AttentionView a) {
-    using S = F32Shape<D>;
-    constexpr uint32_t kTokens = S::kTokens, kOwn = kTokens / 8;  // kOwn: tokens of a tile that a thread has scores of
+    using S = F32Shape<D, R>;
+    constexpr uint32_t kRows = S::kRows, kTokens = S::kTokens, kOwn = kTokens / 8;  // kOwn: tokens of a tile that a thread has scores of
     extern __shared__ __align__(16) float smem[];
     float *const sq = smem, *const sk = sq + kRows * S::kPitch, *const sv = sk + kTokens * S::kPitch, *const sp = sv + kTokens * S::kPitch;
     __shared__ float s_levels[16];
@@ -61,16 +82,16 @@ attention_f32_kernel(const CacheView c, const BatchView b, const AttentionView a
             }
             *reinterpret_cast<float4 *>(sq + r * S::kPitch + d) = v;
         }
-        // the tokens that this thread's four rows see, and those that any row of the tile does
-        uint32_t sees[4];
+        // the tokens that this thread's rows see, and those that any row of the tile does
+        uint32_t sees[R];
         #pragma unroll
-        for (int i = 0; i < 4; ++i) sees[i] = 4 * ty + i < n ? visible_end(s, a.by_group, r0 + 4 * ty + i) : 0u;
+        for (int i = 0; i < R; ++i) sees[i] = R * ty + i < n ? visible_end(s, a.by_group, r0 + R * ty + i) : 0u;
         const uint32_t end = visible_end(s, a.by_group, r0 + n - 1), tiles = (end + kTokens - 1) / kTokens;
         const uint32_t tile0 = (uint32_t)((uint64_t)tiles * part / a.parts), tile1 = (uint32_t)((uint64_t)tiles * (part + 1) / a.parts);
-        float most[4], sum[4] = {};
-        float2 acc[4][D / 16] = {};
+        float most[R], sum[R] = {};
+        float2 acc[R][D / 16] = {};
         #pragma unroll
-        for (int i = 0; i < 4; ++i) most[i] = -INFINITY;
+        for (int i = 0; i < R; ++i) most[i] = -INFINITY;
         // a tile's keys and values, kLoads groups of eight to a thread, asked for while the tile before is worked on
         constexpr uint32_t kLoads = 2 * kTokens * (D / 8) / kF32Threads;
         uint4 raw[kLoads];
@@ -120,30 +141,31 @@ attention_f32_kernel(const CacheView c, const BatchView b, const AttentionView a
                     values_of_bf16(raw[l], v);
                 }
                 float *const to = (which ? sv : sk) + t * S::kPitch + 8 * g;
-                *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
-                *reinterpret_cast<float4 *>(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                const uint32_t half = g & 4u;  // (which comes first: so that eight lanes' stores hit all banks)
+                *reinterpret_cast<float4 *>(to + half) = half ? make_float4(v[4], v[5], v[6], v[7]) : make_float4(v[0], v[1], v[2], v[3]);
+                *reinterpret_cast<float4 *>(to + (half ^ 4u)) = half ? make_float4(v[0], v[1], v[2], v[3]) : make_float4(v[4], v[5], v[6], v[7]);
             }
             if (tile + 1 < tile1) ask(tile + 1);
             __syncthreads();
-            float2 pairs[4][kOwn] = {};  // the scores' sums over even and odd places
+            float2 pairs[R][kOwn] = {};  // the scores' sums over even and odd places
             #pragma unroll 4
             for (uint32_t d = 0; d < D; d += 4) {
-                float4 q[4], k[kOwn];
+                float4 q[R], k[kOwn];
                 #pragma unroll
-                for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const float4 *>(sq + (4 * ty + i) * S::kPitch + d);
+                for (int i = 0; i < R; ++i) q[i] = *reinterpret_cast<const float4 *>(sq + (R * ty + i) * S::kPitch + d);
                 #pragma unroll
                 for (int j = 0; j < kOwn; ++j) k[j] = *reinterpret_cast<const float4 *>(sk + (tx + 8 * j) * S::kPitch + d);
                 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < R; ++i)
                     #pragma unroll
                     for (int j = 0; j < kOwn; ++j) {
                         pairs[i][j] = fma2(make_float2(q[i].x, q[i].y), make_float2(k[j].x, k[j].y), pairs[i][j]);
                         pairs[i][j] = fma2(make_float2(q[i].z, q[i].w), make_float2(k[j].z, k[j].w), pairs[i][j]);
                     }
             }
-            float x[kOwn][4];
+            float x[kOwn][R];
             #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < R; ++i) {
                 float top = most[i];
                 #pragma unroll
                 for (int j = 0; j < kOwn; ++j) {
@@ -169,30 +191,30 @@ attention_f32_kernel(const CacheView c, const BatchView b, const AttentionView a
                 }
             }
             #pragma unroll
-            for (int j = 0; j < kOwn; ++j) *reinterpret_cast<float4 *>(sp + (tx + 8 * j) * S::kPPitch + 4 * ty) = make_float4(x[j][0], x[j][1], x[j][2], x[j][3]);
+            for (int j = 0; j < kOwn; ++j) put<R>(sp + (tx + 8 * j) * S::kPPitch + R * ty, x[j]);
             __syncwarp();  // (a row's weights are written and read by the same eight lanes)
             #pragma unroll 4
             for (uint32_t t = 0; t < kTokens; ++t) {
-                const float4 w = *reinterpret_cast<const float4 *>(sp + t * S::kPPitch + 4 * ty);
+                float w[R];
+                get<R>(sp + t * S::kPPitch + R * ty, w);
                 #pragma unroll
                 for (int j = 0; j < D / 32; ++j) {
                     const float4 v = *reinterpret_cast<const float4 *>(sv + t * S::kPitch + 4 * tx + 32 * j);
                     #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float wi = i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w;
-                        acc[i][2 * j] = fma2(make_float2(wi, wi), make_float2(v.x, v.y), acc[i][2 * j]);
-                        acc[i][2 * j + 1] = fma2(make_float2(wi, wi), make_float2(v.z, v.w), acc[i][2 * j + 1]);
+                    for (int i = 0; i < R; ++i) {
+                        acc[i][2 * j] = fma2(make_float2(w[i], w[i]), make_float2(v.x, v.y), acc[i][2 * j]);
+                        acc[i][2 * j + 1] = fma2(make_float2(w[i], w[i]), make_float2(v.z, v.w), acc[i][2 * j + 1]);
                     }
                 }
             }
         }
         #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < R; ++i) {
             sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
             sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
             sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 4);
-            if (4 * ty + i >= n) continue;
-            const uint32_t r = r0 + 4 * ty + i, token = a.by_group.of(r), row = s.row0 + token, h = head * a.group + (r - token * a.group);
+            if (R * ty + i >= n) continue;
+            const uint32_t r = r0 + R * ty + i, token = a.by_group.of(r), row = s.row0 + token, h = head * a.group + (r - token * a.group);
             if (a.parts > 1) {
                 const uint64_t at = ((uint64_t)part * b.rows + row) * q_heads + h;
                 if (tx == 0) a.part_ml[at] = make_float2(most[i], sum[i]);
@@ -273,17 +295,20 @@ bool takes_decode(const AttentionCall &c) {
 
 struct Plan {
     uint32_t row_tiles, parts;  // CTAs to a head of a sequence: row tiles side by side, and parts of the tokens
+    uint32_t rows;              // to a thread: 1, 2 or 4
 };
 
 Plan plan_of(const AttentionCall &c) {
     Plan p;
-    const uint64_t tiles = std::max<uint64_t>(1, ((uint64_t)c.most_rows * c.view.group + kRows - 1) / kRows);
+    const uint64_t rows = (uint64_t)c.most_rows * c.view.group;
+    p.rows = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    const uint64_t tiles = std::max<uint64_t>(1, (rows + 16 * p.rows - 1) / (16 * p.rows));
     p.row_tiles = (uint32_t)std::min<uint64_t>(tiles, 65535 / c.cache.heads);
-    // four CTAs to an SM as near as parts of equally many token tiles come to it (measured with two, three, four and six: 29, 26, 23 and 27 us
-    // for three prompts of 100 rows over 700 tokens, two heads of 64)
+    // four CTAs to an SM, of fewer rows eight, as near as parts of equally many token tiles come to it (measured with two, three, four and six: 29, 26,
+    // 23 and 27 us for three prompts of 100 rows over 700 tokens, two heads of 64; with four, six and eight of 16 rows 209, 256 and 180 us)
     const uint64_t ctas = (uint64_t)p.row_tiles * c.cache.heads * std::max(1u, c.batch.sequences);
     const uint64_t tokens = tokens_of_tile(c.head_dim), token_tiles = std::max<uint64_t>(1, (c.most_tokens + tokens - 1) / tokens);
-    const uint64_t parts = std::min<uint64_t>(std::min<uint64_t>(64, token_tiles), std::max<uint64_t>(1, 4 * kNumSMs / ctas));
+    const uint64_t parts = std::min<uint64_t>(std::min<uint64_t>(64, token_tiles), std::max<uint64_t>(1, (p.rows == 4 ? 4 : 8) * kNumSMs / ctas));
     const uint64_t tiles_of_part = (token_tiles + parts - 1) / parts;
     p.parts = (uint32_t)((token_tiles + tiles_of_part - 1) / tiles_of_part);
     return p;
@@ -298,17 +323,22 @@ uint64_t workspace_bytes_of(const AttentionCall &c, const Plan &p) {
     return kAttentionFlagBytes + part_ml_bytes(c, p.parts) + (uint64_t)p.parts * c.batch.rows * c.cache.heads * c.view.group * c.head_dim * sizeof(float);
 }
 
-template <int D, bool NF4>
+template <int D, bool NF4, int R>
 int32_t launch_f32(const AttentionCall &c, const Plan &p, cudaStream_t stream) {
-    auto kernel = attention_f32_kernel<D, NF4>;
-    NF4_TRY(ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), F32Shape<D>::kSmem));
+    auto kernel = attention_f32_kernel<D, NF4, R>;
+    constexpr uint32_t kSmem = F32Shape<D, R>::kSmem;
+    NF4_TRY(ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), kSmem));
     count_launch();
-    return launch_maybe_overlapped(kernel, dim3(p.parts, p.row_tiles * c.cache.heads, c.batch.sequences), dim3(kF32Threads), F32Shape<D>::kSmem,
+    return launch_maybe_overlapped(kernel, dim3(p.parts, p.row_tiles * c.cache.heads, c.batch.sequences), dim3(kF32Threads), kSmem,
                                    stream, true, c.cache, c.batch, c.view);
 }
 template <int D>
 int32_t launch_of(const AttentionCall &c, const Plan &p, cudaStream_t stream) {
-    NF4_TRY((c.nf4 ? launch_f32<D, true>(c, p, stream) : launch_f32<D, false>(c, p, stream)));
+    auto launch = [&](auto nf4) {
+        constexpr bool kNf4 = decltype(nf4)::value;
+        return p.rows == 1 ? launch_f32<D, kNf4, 1>(c, p, stream) : p.rows == 2 ? launch_f32<D, kNf4, 2>(c, p, stream) : launch_f32<D, kNf4, 4>(c, p, stream);
+    };
+    NF4_TRY((c.nf4 ? launch(std::true_type()) : launch(std::false_type())));
     if (p.parts == 1) return NF4_OK;
     const uint32_t q_heads = c.cache.heads * c.view.group;
     const uint64_t warps = (uint64_t)c.batch.rows * q_heads;
