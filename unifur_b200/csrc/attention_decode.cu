@@ -1,4 +1,4 @@
-// Attention of few rows over the paged cache (decode steps, drafted tokens): up to sixteen rows of a head at a time.
+// Attention of few rows, or over few tokens, of the paged cache (decode steps, drafted tokens, short prompts): up to sixteen rows of a head at a time.
 //
 // Bound by the bytes of the cache, and for a quantized one by its lookups as well.  A CTA has an SM to itself; the units
 // (16 or 32 tokens) of all sequences, heads and row tiles form one line that the CTAs share out evenly, whatever the sequences'
