@@ -10,20 +10,21 @@ namespace nf4 {
 namespace {
 
 // ---- f32 throughout ---------------------------------------------------------------------------------
-// A CTA has a tile of 16, 32 or 64 rows of one head of the cache (as many as there are, or 64) and goes over its tokens 32 at a time (16 with a
-// dim of 256): one, two or four rows to a thread, by every eighth token for the scores and by dim / 8 values for the results, weights from one to the
-// other through shared memory, with the running largest exponent and sum of a softmax that is never held whole.  A row's scores are
-// eight neighbouring lanes'.  FMAs are done in pairs.  Bound by shared memory, which gives registers 128 bytes a clock: with four rows 8 reads of
-// 16 bytes to 32 pairs of FMAs for the scores and 5 to 32 for the results (of 128), 24 to 30 TFLOP/s for long prompts; with one row 5 to 4 and 5
-// to 8 (16 sequences of 4096 tokens, 7 rows of four heads of 128: 180 us, 280 with tiles of 64 rows).
-constexpr int kThreads = 256, kF32Threads = 128;
+// A CTA has a tile of 64 rows of one head of the cache (32 in the same four warps, 16 or 8 in one, where there are no more) and goes over its
+// tokens 32 at a time (16 with one warp or a dim of 256, 8 with both): four or two rows to a thread, by every eighth token for the scores and by
+// dim / 8 values for the results, weights from one to the other through shared memory, with the running largest exponent and sum of a
+// softmax that is never held whole.  A row's scores are eight neighbouring lanes'.  FMAs are done in pairs.  Bound by shared
+// memory, which gives registers 128 bytes a clock, so that 16 bytes to a lane take four whatever is broadcast: with four rows 8 such reads
+// to 32 pairs of FMAs for the scores and 5 to 32 for the results (of 128), 24 to 32 TFLOP/s over long prompts.  (16 sequences of 4096 tokens, 7 rows of
+// four heads of 128: 110 us; with tiles of 64 rows 280, of 16 rows in four warps, one to a thread, 174.)
+constexpr int kThreads = 256;
 
-constexpr uint32_t tokens_of_tile(uint32_t dim) { return dim == 256 ? 16 : 32; }
+constexpr uint32_t tokens_of_tile(uint32_t dim, uint32_t warps) { return (dim == 256 ? 16 : 32) / (warps == 1 ? 2 : 1); }
 
-// R: rows to a thread
-template <int D, int R>
+// R: rows to a thread; W: warps, of 4 R rows each
+template <int D, int R, int W>
 struct F32Shape {
-    static constexpr uint32_t kRows = 16 * R, kTokens = tokens_of_tile(D), kPitch = D + 4, kPPitch = kRows + 4;
+    static constexpr uint32_t kThreads = 32 * W, kRows = 4 * R * W, kTokens = tokens_of_tile(D, W), kPitch = D + 4, kPPitch = kRows + 4;
     static constexpr uint32_t kSmem = 4 * (kRows * kPitch + 2 * kTokens * kPitch + kTokens * kPPitch);
 };
 
@@ -38,27 +39,24 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 template <int R>
 __device__ __forceinline__ void put(float *to, const float (&v)[R]) {
     if constexpr (R == 4) *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
-    else if constexpr (R == 2) *reinterpret_cast<float2 *>(to) = make_float2(v[0], v[1]);
-    else *to = v[0];
+    else *reinterpret_cast<float2 *>(to) = make_float2(v[0], v[1]);
 }
 template <int R>
 __device__ __forceinline__ void get(const float *from, float (&v)[R]) {
     if constexpr (R == 4) {
         const float4 w = *reinterpret_cast<const float4 *>(from);
         v[0] = w.x; v[1] = w.y; v[2] = w.z; v[3] = w.w;
-    } else if constexpr (R == 2) {
+    } else {
         const float2 w = *reinterpret_cast<const float2 *>(from);
         v[0] = w.x; v[1] = w.y;
-    } else {
-        v[0] = *from;
     }
 }
 
-template <int D, bool NF4, int R>
-__global__ void __launch_bounds__(kF32Threads)
+template <int D, bool NF4, int R, int W>
+__global__ void __launch_bounds__(32 * W)
 attention_f32_kernel(const CacheView c, const BatchView b, const AttentionView a) {
-    using S = F32Shape<D, R>;
-    constexpr uint32_t kRows = S::kRows, kTokens = S::kTokens, kOwn = kTokens / 8;  // kOwn: tokens of a tile that a thread has scores of
+    using S = F32Shape<D, R, W>;
+    constexpr uint32_t kCtaThreads = S::kThreads, kRows = S::kRows, kTokens = S::kTokens, kOwn = kTokens / 8;  // kOwn: tokens of a tile that a thread has scores of
     extern __shared__ __align__(16) float smem[];
     float *const sq = smem, *const sk = sq + kRows * S::kPitch, *const sv = sk + kTokens * S::kPitch, *const sp = sv + kTokens * S::kPitch;
     __shared__ float s_levels[16];
@@ -73,7 +71,7 @@ attention_f32_kernel(const CacheView c, const BatchView b, const AttentionView a
     for (uint32_t r0 = blockIdx.y / c.heads * kRows; r0 < rows; r0 += gridDim.y / c.heads * kRows) {
         const uint32_t n = min(kRows, rows - r0);
         __syncthreads();
-        for (uint32_t i = tid; i < kRows * (D / 4); i += kF32Threads) {
+        for (uint32_t i = tid; i < kRows * (D / 4); i += kCtaThreads) {
             const uint32_t r = i / (D / 4), d = 4 * (i % (D / 4));
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             if (r < n) {
@@ -93,7 +91,7 @@ attention_f32_kernel(const CacheView c, const BatchView b, const AttentionView a
         #pragma unroll
         for (int i = 0; i < R; ++i) most[i] = -INFINITY;
         // a tile's keys and values, kLoads groups of eight to a thread, asked for while the tile before is worked on
-        constexpr uint32_t kLoads = 2 * kTokens * (D / 8) / kF32Threads;
+        constexpr uint32_t kLoads = 2 * kTokens * (D / 8) / kCtaThreads;
         uint4 raw[kLoads];
         float scale[kLoads];
         uint32_t state = 0;  // two bits to a group: 1 behind the last token, 2 in a page that there is not
@@ -101,7 +99,7 @@ attention_f32_kernel(const CacheView c, const BatchView b, const AttentionView a
             state = 0;
             #pragma unroll
             for (uint32_t l = 0; l < kLoads; ++l) {
-                const uint32_t i = tid + l * kF32Threads, which = i / (kTokens * (D / 8)), j = i % (kTokens * (D / 8)), g = j % (D / 8);
+                const uint32_t i = tid + l * kCtaThreads, which = i / (kTokens * (D / 8)), j = i % (kTokens * (D / 8)), g = j % (D / 8);
                 const uint32_t token = tile * kTokens + j / (D / 8);
                 if (token >= end) {
                     state |= 1u << 2 * l;
@@ -129,7 +127,7 @@ attention_f32_kernel(const CacheView c, const BatchView b, const AttentionView a
             __syncthreads();
             #pragma unroll
             for (uint32_t l = 0; l < kLoads; ++l) {
-                const uint32_t i = tid + l * kF32Threads, which = i / (kTokens * (D / 8)), j = i % (kTokens * (D / 8)), t = j / (D / 8), g = j % (D / 8);
+                const uint32_t i = tid + l * kCtaThreads, which = i / (kTokens * (D / 8)), j = i % (kTokens * (D / 8)), t = j / (D / 8), g = j % (D / 8);
                 const uint32_t is = state >> 2 * l & 3u;
                 float v[8];
                 if (is) {
@@ -234,41 +232,56 @@ attention_f32_kernel(const CacheView c, const BatchView b, const AttentionView a
 }
 
 // ---- the join of parts ------------------------------------------------------------------------------
-// A warp to a row of a query head: parts by their largest exponents, in their order, so that the result does not depend on
-// which was ready first.  Rows of no sequence have no parts and are left alone.
+// A CTA to a row of a query head: a warp takes every eighth part, in their order, by the largest exponent so far; then the warps' sums
+// are joined in theirs, so that the result does not depend on which was ready first.  Rows of no sequence have no parts and are left
+// alone.  (A warp to a row took 20 us for 64 parts, a chain of their loads.)
 template <int D>
 __global__ void __launch_bounds__(kThreads)
 join_kernel(const BatchView b, const AttentionView a, uint32_t q_heads) {
+    constexpr uint32_t W = kThreads / 32;
+    __shared__ float2 s_ml[W];
+    __shared__ float s_acc[W][D];
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
-    const uint32_t i = blockIdx.x * (kThreads / 32) + threadIdx.x / 32, all = b.rows * q_heads;  // (below 2^31)
-    const uint32_t lane = threadIdx.x & 31u;
-    if (i >= all) return;
+    const uint32_t i = blockIdx.x, all = b.rows * q_heads, lane = threadIdx.x & 31u, warp = threadIdx.x / 32;  // (below 2^31)
     const uint32_t row = i / q_heads, h = i - row * q_heads;
     if ((int32_t)row < __ldg(b.starts) || (int32_t)row >= __ldg(b.starts + b.sequences)) return;
-    float top = -INFINITY;
-    for (uint32_t p = lane; p < a.parts; p += 32) top = fmaxf(top, __ldg(&a.part_ml[(uint64_t)p * all + i].x));
-    #pragma unroll
-    for (int k = 1; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, acc[D / 32] = {};
-    #pragma unroll 8
-    for (uint32_t p = 0; p < a.parts; ++p) {
+    float top = -INFINITY, sum = 0.f, acc[D / 32] = {};
+    #pragma unroll 4
+    for (uint32_t p = warp; p < a.parts; p += W) {
         const float2 ml = __ldg(a.part_ml + (uint64_t)p * all + i);
-        const float f = ml.y == 0.f ? 0.f : exp2f(ml.x - base);  // (a NaN stays one)
-        sum = fmaf(f, ml.y, sum);
         const float *const o = a.part_o + ((uint64_t)p * all + i) * D + lane * (D / 32);
+        float2 v[D / 64];
         #pragma unroll
-        for (int j = 0; j < D / 32; j += 2) {
-            const float2 v = ml.y == 0.f ? make_float2(0.f, 0.f) : __ldg(reinterpret_cast<const float2 *>(o + j));
-            acc[j] = fmaf(f, v.x, acc[j]);
-            acc[j + 1] = fmaf(f, v.y, acc[j + 1]);
+        for (int j = 0; j < D / 64; ++j) v[j] = __ldg(reinterpret_cast<const float2 *>(o) + j);
+        const float now = fmaxf(top, ml.x), base = now == -INFINITY ? 0.f : now;
+        const float keep = exp2f(top - base), f = ml.y == 0.f ? 0.f : exp2f(ml.x - base);  // (a NaN stays one)
+        top = now;
+        sum = fmaf(f, ml.y, sum * keep);
+        #pragma unroll
+        for (int j = 0; j < D / 64; ++j) {
+            acc[2 * j] = fmaf(f, ml.y == 0.f ? 0.f : v[j].x, acc[2 * j] * keep);
+            acc[2 * j + 1] = fmaf(f, ml.y == 0.f ? 0.f : v[j].y, acc[2 * j + 1] * keep);
         }
     }
-    const float f = sum == 0.f ? 0.f : 1.f / sum;
-    float *const out = static_cast<float *>(a.out) + (uint64_t)row * a.ldo + (uint64_t)h * D + lane * (D / 32);
+    if (lane == 0) s_ml[warp] = make_float2(top, sum);
     #pragma unroll
-    for (int j = 0; j < D / 32; j += 2) *reinterpret_cast<float2 *>(out + j) = make_float2(acc[j] * f, acc[j + 1] * f);
+    for (int j = 0; j < D / 32; ++j) s_acc[warp][lane * (D / 32) + j] = acc[j];
+    __syncthreads();
+    if (threadIdx.x >= D) return;
+    top = -INFINITY;
+    #pragma unroll
+    for (uint32_t w = 0; w < W; ++w) top = fmaxf(top, s_ml[w].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    float value = 0.f;
+    sum = 0.f;
+    #pragma unroll
+    for (uint32_t w = 0; w < W; ++w) {
+        const float f = exp2f(s_ml[w].x - base);
+        sum = fmaf(f, s_ml[w].y, sum);
+        value = fmaf(f, s_acc[w][threadIdx.x], value);
+    }
+    static_cast<float *>(a.out)[(uint64_t)row * a.ldo + (uint64_t)h * D + threadIdx.x] = sum == 0.f ? 0.f : value * (1.f / sum);
 }
 
 // ---- how a call is carried out -----------------------------------------------------------------------
@@ -295,20 +308,23 @@ bool takes_decode(const AttentionCall &c) {
 
 struct Plan {
     uint32_t row_tiles, parts;  // CTAs to a head of a sequence: row tiles side by side, and parts of the tokens
-    uint32_t rows;              // to a thread: 1, 2 or 4
+    uint32_t rows, warps;       // rows to a thread, warps of a CTA
 };
 
 Plan plan_of(const AttentionCall &c) {
     Plan p;
     const uint64_t rows = (uint64_t)c.most_rows * c.view.group;
-    p.rows = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    const uint64_t tiles = std::max<uint64_t>(1, (rows + 16 * p.rows - 1) / (16 * p.rows));
+    p.warps = rows <= 16 ? 1 : 4;
+    p.rows = rows <= 8 || (rows > 16 && rows <= 32) ? 2 : 4;
+    const uint64_t of_tile = 4 * p.rows * p.warps, tiles = std::max<uint64_t>(1, (rows + of_tile - 1) / of_tile);
     p.row_tiles = (uint32_t)std::min<uint64_t>(tiles, 65535 / c.cache.heads);
-    // four CTAs to an SM, of fewer rows eight, as near as parts of equally many token tiles come to it (measured with two, three, four and six: 29, 26,
-    // 23 and 27 us for three prompts of 100 rows over 700 tokens, two heads of 64; with four, six and eight of 16 rows 209, 256 and 180 us)
+    // four CTAs to an SM, of 32 rows eight, of one warp sixteen, as near as parts of equally many token tiles come to it (measured with two, three, four
+    // and six: 29, 26, 23 and 27 us for three prompts of 100 rows over 700 tokens, two heads of 64; of one warp with 10, 16 and 24: 70, 53 and 68
+    // us for 16 sequences of 4096 tokens, four heads of 64); 256 parts at most (with 32, 64, 128 and 256 one row over 65536 tokens took 711, 364, 226
+    // and 132 us)
     const uint64_t ctas = (uint64_t)p.row_tiles * c.cache.heads * std::max(1u, c.batch.sequences);
-    const uint64_t tokens = tokens_of_tile(c.head_dim), token_tiles = std::max<uint64_t>(1, (c.most_tokens + tokens - 1) / tokens);
-    const uint64_t parts = std::min<uint64_t>(std::min<uint64_t>(64, token_tiles), std::max<uint64_t>(1, (p.rows == 4 ? 4 : 8) * kNumSMs / ctas));
+    const uint64_t tokens = tokens_of_tile(c.head_dim, p.warps), token_tiles = std::max<uint64_t>(1, (c.most_tokens + tokens - 1) / tokens);
+    const uint64_t parts = std::min<uint64_t>(std::min<uint64_t>(256, token_tiles), std::max<uint64_t>(1, (p.warps == 1 ? 16 : p.rows == 4 ? 4 : 8) * kNumSMs / ctas));
     const uint64_t tiles_of_part = (token_tiles + parts - 1) / parts;
     p.parts = (uint32_t)((token_tiles + tiles_of_part - 1) / tiles_of_part);
     return p;
@@ -323,28 +339,27 @@ uint64_t workspace_bytes_of(const AttentionCall &c, const Plan &p) {
     return kAttentionFlagBytes + part_ml_bytes(c, p.parts) + (uint64_t)p.parts * c.batch.rows * c.cache.heads * c.view.group * c.head_dim * sizeof(float);
 }
 
-template <int D, bool NF4, int R>
+template <int D, bool NF4, int R, int W>
 int32_t launch_f32(const AttentionCall &c, const Plan &p, cudaStream_t stream) {
-    auto kernel = attention_f32_kernel<D, NF4, R>;
-    constexpr uint32_t kSmem = F32Shape<D, R>::kSmem;
+    auto kernel = attention_f32_kernel<D, NF4, R, W>;
+    constexpr uint32_t kSmem = F32Shape<D, R, W>::kSmem;
     NF4_TRY(ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), kSmem));
     count_launch();
-    return launch_maybe_overlapped(kernel, dim3(p.parts, p.row_tiles * c.cache.heads, c.batch.sequences), dim3(kF32Threads), kSmem,
+    return launch_maybe_overlapped(kernel, dim3(p.parts, p.row_tiles * c.cache.heads, c.batch.sequences), dim3(32 * W), kSmem,
                                    stream, true, c.cache, c.batch, c.view);
 }
 template <int D>
 int32_t launch_of(const AttentionCall &c, const Plan &p, cudaStream_t stream) {
     auto launch = [&](auto nf4) {
         constexpr bool kNf4 = decltype(nf4)::value;
-        return p.rows == 1 ? launch_f32<D, kNf4, 1>(c, p, stream) : p.rows == 2 ? launch_f32<D, kNf4, 2>(c, p, stream) : launch_f32<D, kNf4, 4>(c, p, stream);
+        if (p.warps == 1) return p.rows == 2 ? launch_f32<D, kNf4, 2, 1>(c, p, stream) : launch_f32<D, kNf4, 4, 1>(c, p, stream);
+        return p.rows == 2 ? launch_f32<D, kNf4, 2, 4>(c, p, stream) : launch_f32<D, kNf4, 4, 4>(c, p, stream);
     };
     NF4_TRY((c.nf4 ? launch(std::true_type()) : launch(std::false_type())));
     if (p.parts == 1) return NF4_OK;
     const uint32_t q_heads = c.cache.heads * c.view.group;
-    const uint64_t warps = (uint64_t)c.batch.rows * q_heads;
     count_launch();
-    return launch_maybe_overlapped(join_kernel<D>, dim3((unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32))),
-                                   dim3(kThreads), 0, stream, true, c.batch, c.view, q_heads);
+    return launch_maybe_overlapped(join_kernel<D>, dim3(c.batch.rows * q_heads), dim3(kThreads), 0, stream, true, c.batch, c.view, q_heads);
 }
 
 AttentionCall call_of(const nf4_cache &cache, const nf4_cache_batch &batch, uint32_t q_heads, int32_t io_dtype) {
