@@ -534,6 +534,10 @@ NF4_API uint64_t nf4_cache_attention_call_flag_bytes(const nf4_cache *cache, con
                                                      int32_t io_dtype);
 NF4_API int32_t nf4_cache_attention_dev(const nf4_cache *cache, const nf4_cache_batch *batch, const nf4_attention_args *args,
                                         void *stream);
+/* Where, in the kernel for many rows, one of the 128 threads of a row tile's softmax puts the 16-byte chunk `chunk` (below head_dim / 8) of what it
+ * brings of the queries and takes of the results (results 0), or of the results of its own row (results 1): bytes from the start of the tile's
+ * place in shared memory, or a negative status.  For inspection and tests. */
+NF4_API int32_t nf4_cache_attention_row_place(uint32_t head_dim, uint32_t thread, uint32_t chunk, int32_t results);
 
 /* ------------------------------------------------ resident weight handles -- */
 

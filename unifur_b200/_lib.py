@@ -147,6 +147,7 @@ SIGNATURES = {
     "nf4_cache_attention_flag_bytes": (_u64, []),
     "nf4_cache_attention_call_flag_bytes": (_u64, [C.POINTER(Cache), C.POINTER(CacheBatch), _u32, _i32]),
     "nf4_cache_attention_dev": (_i32, [C.POINTER(Cache), C.POINTER(CacheBatch), C.POINTER(AttentionArgs), _vp]),
+    "nf4_cache_attention_row_place": (_i32, [_u32, _u32, _u32, _i32]),
     "nf4_weight_from_values_host": (_i32, [_vp, _u64, _u64, _i32, _i32, C.POINTER(_vp)]),
     "nf4_weight_from_packed_host": (_i32, [_vp, _vp, _vp, _f32, _u64, _u64, _i32,
                                            C.POINTER(_vp)]),

@@ -56,6 +56,19 @@ struct Shape {
     static constexpr uint32_t kS = 0, kO = 256;                       // columns of tensor memory: the tiles' S's, then O's
 };
 
+// A tile's 128 rows of queries, as the MMA reads them, and in their place later the tile's results: a box of 128 rows to every 64 values (128
+// bytes), 16-byte chunks swizzled.  Each of the tile's four warps has the 32 rows whose softmax is its own, for both, so that a warp which
+// writes its next queries has nothing to wait for from one that still reads its results out.
+__host__ __device__ constexpr uint32_t chunk_place(uint32_t row, uint32_t x) { return (x >> 3) * 16384u + row * 128u + (((x & 7u) ^ (row & 7u)) << 4); }
+// The n-th chunk (of dim / 8) that a lane of one of the four warps brings of the queries, and that it takes of the results.
+struct RowChunk {
+    uint32_t row, x;
+};
+__host__ __device__ constexpr RowChunk chunk_of(uint32_t dim, uint32_t warp, uint32_t lane, uint32_t n) {
+    const uint32_t lanes = dim / 8;  // of a row
+    return RowChunk{warp * 32 + n * (32 / lanes) + lane / lanes, lane % lanes};
+}
+
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *r) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
@@ -425,15 +438,16 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                     uint4 w[kBatch];
                     #pragma unroll
                     for (uint32_t k = 0; k < kBatch; ++k) {
-                        const uint32_t i = (i0 + k) * 128 + r, row = p.r0 + tile * 128 + i / kLanes, token = a.by_group.of(row);
+                        const RowChunk own = chunk_of(D, warp & 3u, lane, i0 + k);
+                        const uint32_t row = p.r0 + tile * 128 + own.row, token = a.by_group.of(row);
                         w[k] = make_uint4(0u, 0u, 0u, 0u);
-                        if (tile * 128 + i / kLanes < p.rows)
+                        if (tile * 128 + own.row < p.rows)
                             w[k] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.q) + (uint64_t)(p.s.row0 + token) * a.ldq +
-                                                                         (uint64_t)(p.head * a.group + row - token * a.group) * D) + i % kLanes);
+                                                                         (uint64_t)(p.head * a.group + row - token * a.group) * D) + own.x);
                     }
                     #pragma unroll
                     for (uint32_t k = 0; k < kBatch; ++k) {
-                        const uint32_t i = (i0 + k) * 128 + r, rr = i / kLanes, x = i % kLanes;
+                        const RowChunk own = chunk_of(D, warp & 3u, lane, i0 + k);
                         uint32_t u[4] = {w[k].x ^ flip, w[k].y ^ flip, w[k].z ^ flip, w[k].w ^ flip};
                         if (NF4) {
                             constexpr uint32_t kSize = 0x7fff7fffu;  // (bf16 magnitudes go by their bits)
@@ -446,14 +460,13 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                             const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
                             #pragma unroll
                             for (int e = 0; e < 4; ++e) u[e] = pack<true>(__uint_as_float(u[e] << 16) * down, __uint_as_float(u[e] & 0xffff0000u) * down);
-                            if (x == 0) s_qpower[tile * 128 + rr] = __uint_as_float((uint32_t)(127 + e2) << 23);
+                            if (own.x == 0) s_qpower[tile * 128 + own.row] = __uint_as_float((uint32_t)(127 + e2) << 23);
                         }
-                        st_shared_u4(q_tile + (x >> 3) * 16384u + rr * 128u + (((x & 7u) ^ (rr & 7u)) << 4), make_uint4(u[0], u[1], u[2], u[3]));
+                        st_shared_u4(q_tile + chunk_place(own.row, own.x), make_uint4(u[0], u[1], u[2], u[3]));
                     }
                 }
                 ptx::fence_proxy_async();
-                if (tile) asm volatile("bar.sync 2, 128;" ::: "memory");  // this tile's warps
-                else asm volatile("bar.sync 1, 128;" ::: "memory");
+                __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(q_ready0 + 8 * tile);
 
                 // ---- the steps ----
@@ -559,14 +572,13 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                 walk = s_walk[warp];
                 p = s_piece[warp];
 
-                // ---- the row's results, through this warp's part of Q's place (its products are done) so that whole rows go out ----
+                // ---- the row's results, through the place of this warp's rows of Q (the products are done) so that whole rows go out ----
                 if (s_bad[piece & 7u] == piece + 1 || !ok) l = __uint_as_float(0x7fc00000u);  // NaN
                 const bool whole = p.steps == p.all;
                 const uint64_t part = (uint64_t)(2 * blockIdx.x + (p.step0 ? 0 : 1)) * S::kRows + tile * 128;
                 if (!whole) a.part_ml[part + r] = make_float2(m, l);
                 const float f = (whole ? l == 0.f ? 0.f : 1.f / l : 1.f) * (NF4 ? ref : 1.f);
-                const uint32_t stage = q_tile + (warp & 3u) * (S::kQTile / 4);
-                constexpr uint32_t kRowBytes = 2 * D, kChunks = D / 8;  // a staged row: bf16 results, or half of a row's f32 sums
+                constexpr uint32_t kChunks = D / 8;  // of a staged row: bf16 results, or half of a row's f32 sums
                 #pragma unroll 1
                 for (uint32_t half = 0; half < (whole ? 1u : 2u); ++half) {
                     const uint32_t columns = whole ? D : D / 2;
@@ -587,31 +599,31 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                                 uint32_t w[4];
                                 #pragma unroll
                                 for (int e = 0; e < 4; ++e) w[e] = bf16_pair(__uint_as_float(x[8 * i + 2 * e]), __uint_as_float(x[8 * i + 2 * e + 1]));
-                                st_shared_u4(stage + lane * kRowBytes + (((k / 8 + i) ^ (lane & 7u)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+                                st_shared_u4(q_tile + chunk_place(r, k / 8 + i), make_uint4(w[0], w[1], w[2], w[3]));
                             }
                         } else {
                             #pragma unroll
                             for (uint32_t i = 0; i < 8; ++i)
-                                st_shared_u4(stage + lane * kRowBytes + (((k / 4 + i) ^ (lane & 7u)) << 4), make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]));
+                                st_shared_u4(q_tile + chunk_place(r, k / 4 + i), make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]));
                         }
                     }
                     __syncwarp();
-                    const uint32_t first = tile * 128 + (warp & 3u) * 32, here = p.rows > first ? min(32u, p.rows - first) : 0u;  // the warp's rows
-                    const uint32_t x = lane % kChunks;
                     #pragma unroll 8
                     for (uint32_t i = 0; i < kChunks; ++i) {
-                        const uint32_t rr = i * (32 / kChunks) + lane / kChunks;
-                        const uint4 w = ld_shared_u4(stage + rr * kRowBytes + ((x ^ (rr & 7u)) << 4));
+                        const RowChunk own = chunk_of(D, warp & 3u, lane, i);
+                        const uint4 w = ld_shared_u4(q_tile + chunk_place(own.row, own.x));
+                        const bool here = tile * 128 + own.row < p.rows;
                         if (whole) {
-                            const uint32_t q_row = p.r0 + first + rr, token = a.by_group.of(q_row);
-                            if (rr < here)
+                            const uint32_t q_row = p.r0 + tile * 128 + own.row, token = a.by_group.of(q_row);
+                            if (here)
                                 *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(a.out) + (uint64_t)(p.s.row0 + token) * a.ldo +
-                                                           (uint64_t)(p.head * a.group + q_row - token * a.group) * D + 8 * x) = w;
-                        } else if (rr < here) {
-                            *reinterpret_cast<uint4 *>(a.part_o + (part + (warp & 3u) * 32 + rr) * D + half * (D / 2) + 4 * x) = w;
+                                                           (uint64_t)(p.head * a.group + q_row - token * a.group) * D + 8 * own.x) = w;
+                        } else if (here) {
+                            *reinterpret_cast<uint4 *>(a.part_o + (part + own.row) * D + half * (D / 2) + 4 * own.x) = w;
                         }
                     }
                 }
+                __syncwarp();  // (the next queries come to the same place)
                 if (!whole && p.step0 == 0 && tid == 0) {
                     const uint32_t more = min(s_share.cta_of(p.line0 + kStart + p.all - 1) - blockIdx.x, gridDim.x - 1 - blockIdx.x);
                     splits[blockIdx.x] = Split{p.s.row0, p.r0, p.rows, p.head, more};
@@ -1116,3 +1128,18 @@ int32_t attention_chunk(const AttentionCall &c, uint8_t *workspace, cudaStream_t
 }
 
 }  // namespace nf4
+
+using namespace nf4;
+
+extern "C" {
+
+int32_t nf4_cache_attention_row_place(uint32_t head_dim, uint32_t thread, uint32_t chunk, int32_t results) {
+    const char *const what = "nf4_cache_attention_row_place";
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256) return fail(NF4_ERR_UNSUPPORTED, "%s: head_dim is %u; 64, 128 and 256 are supported", what, head_dim);
+    if (thread >= 128 || chunk >= head_dim / 8) return fail(NF4_ERR_INVALID_ARG, "%s: no such thread or chunk", what);
+    if (results) return (int32_t)chunk_place(thread, chunk);
+    const RowChunk own = chunk_of(head_dim, thread / 32, thread % 32, chunk);
+    return (int32_t)chunk_place(own.row, own.x);
+}
+
+}  // extern "C"
