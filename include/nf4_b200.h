@@ -511,7 +511,11 @@ NF4_API int32_t nf4_cache_read_dev(const nf4_cache *cache, const nf4_cache_batch
  * row that sees a token in a page outside [0, num_pages) becomes NaNs (others of its sequence may, too).  Values of the tokens
  * that a call's rows see are finite; what stands in other places of their pages does not matter.  One token to a sequence, drafted
  * tokens, chunks of a prompt and whole prompts are the same call.  out does not overlap q.
- * bf16 tensors multiply on the tensor cores with f32 sums; f32 tensors in f32 throughout.
+ * bf16 tensors multiply on the tensor cores with f32 sums; f32 tensors in f32 throughout.  With bf16 tensors an NF4 cache's keys and values
+ * take part in f16, in units that the largest of them set, so that what is much smaller is off by a part of that: with many rows a key or
+ * value by up to 2^-37 of the largest of its head among the 128 tokens of the sequence that it stands with (64 with a head_dim of 256), also
+ * where the row does not see that one; and a token's part of a result by up to 2^-31 of the largest value that the row, or one of the 15
+ * behind it, sees.
  * workspace: nf4_cache_attention_workspace_bytes() bytes, 256-byte aligned, the first nf4_cache_attention_flag_bytes() of
  * them zero at the first use; every call leaves them zero.  One workspace serves one stream. */
 typedef struct nf4_attention_args {

@@ -16,9 +16,11 @@
 // the work, and 128 tokens of two tiles took 6100 cycles instead of 4270.)  m is the largest exponent so far or up to 8
 // below it: O is rescaled only where a row rises above that, by the warps themselves, at a moment when
 // no product is writing it.  Copies and lookups run ahead into the next piece while a row tile's results are written.
-// f16's range: K's and V's scales are divided by a power of two of a step's largest, a row of Q by its own (exact).  K's comes back as a
-// factor of the step's scores; V's goes into the step's weights, relative to the largest so far (`ref`), which comes back at the end.  f16 is
-// off by 2^-12 on average, bf16 would be by 2^-9.
+// f16's range: K's and V's scales are divided by a power of two that brings a step's largest next to the upper end of it, a row of Q by its own
+// (exact).  K's comes back as a factor of the step's scores; V's goes into the step's weights, relative to the largest so far (`ref`), which
+// comes back at the end.  f16 is off by 2^-12 on average, bf16 would be by 2^-9.  A step's tokens share the power, those that a row does not see
+// among them: a value has all of its bits down to 2^-29 of the step's largest scale, and is off by 2^-37 of that below.  (The sums are f32 and
+// take any size.)
 #include <algorithm>
 
 #include "kv_cache.cuh"
@@ -132,10 +134,9 @@ __device__ __forceinline__ float2 ld_shared_f2(uint32_t addr) {
 __device__ __forceinline__ void st_shared_u4(uint32_t addr, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-// A power of two (as a float) that no scale up to `most` (bits) exceeds, between 2^-100 and 2^126.
-__device__ __forceinline__ float power_above(uint32_t most) {
-    return __uint_as_float(min(max((most & 0x7f800000u) + 0x00800000u, 27u << 23), 253u << 23));
-}
+// The power of two that scales up to `most` (bits) are divided by, to be below 2^15: 2^-126 or more.
+constexpr int kTop = 15;
+__device__ __forceinline__ float power_for(uint32_t most) { return __uint_as_float((uint32_t)max((int)(most >> 23) + 1 - kTop, 1) << 23); }
 __device__ __forceinline__ float reciprocal_of_power(float p) { return __uint_as_float(0x7f000000u - __float_as_uint(p)); }
 
 // How the line of steps is shared out: `per` to a CTA, one more to the first `more` of them.
@@ -654,7 +655,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                         const uint32_t which = of.values, j = of.step, t0 = (p.step0 + j) * N;
                         const uint32_t rs = i % S::kRawSlots, slot = ring.slot, raw = raw0 + rs * S::kRaw, dst = place_of(slot) + (q >> 1) * S::kBox;
                         wait(raw_full0 + 8 * rs, (i / S::kRawSlots) & 1u);
-                        // the power above the tile's largest scale
+                        // the power for the tile's largest scale
                         auto power_of = [&](uint32_t from) {
                             uint32_t most = 0;
                             #pragma unroll
@@ -664,7 +665,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                                 most = max(most, t0 + at / kBlocks < t_end ? __float_as_uint(v.x) : 0u);
                                 most = max(most, t0 + (at + 1) / kBlocks < t_end ? __float_as_uint(v.y) : 0u);
                             }
-                            return power_above(__reduce_max_sync(0xffffffffu, most));
+                            return power_for(__reduce_max_sync(0xffffffffu, most));
                         };
                         const float power = power_of(raw + N * (D / 2));
                         if (!which) {
@@ -898,7 +899,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
 
 // ---- a quantized cache expanded once --------------------------------------------------------------
 // Where several row tiles of a head go over the same tokens.  A CTA has a tile of N tokens of one head: the power of two
-// above its largest scale, then levels times scales in f16, eight values to a thread at a time.  Bound by what it writes.
+// for its largest scale, then levels times scales in f16, eight values to a thread at a time.  Bound by what it writes.
 template <int D>
 __global__ void __launch_bounds__(256)
 expand_kernel(const CacheView c, const BatchView b, uint4 *const k_out, uint4 *const v_out, uint32_t *const bases, float2 *const powers) {
@@ -958,7 +959,7 @@ expand_kernel(const CacheView c, const BatchView b, uint4 *const k_out, uint4 *c
         s_place[tid] = place;
     }
     __syncthreads();
-    const float power[2] = {power_above(s_most[0]), power_above(s_most[1])};
+    const float power[2] = {power_for(s_most[0]), power_for(s_most[1])};
     const uint64_t out0 = ((uint64_t)want * c.heads + head) * N * kGroups;
     if (tid == 0) powers[(uint64_t)want * c.heads + head] = s_bad ? make_float2(0.f, 0.f) : make_float2(power[0], power[1]);
     #pragma unroll

@@ -15,7 +15,7 @@
 // looked up in a table of pairs of f16 levels, a copy to a lane, as in the decode GEMV: a byte of K holds neighbouring d, and for V the
 // nibbles of two tokens are put side by side first.  Block scales never touch f16 on their own: K's multiply the f32 sums of a
 // block, V's the weights.  The weights enter the second product in f16 (2^-11 of each; bf16 with a bf16 cache: 2^-8, half of the
-// result's own rounding on average), times V's scale divided by a power of two `ref` that no scale so far exceeds.
+// result's own rounding on average), times V's scale divided by a power of two `ref` that no scale so far exceeds, of the tokens that some row of the tile sees.
 // m is the largest exponent seen or up to 8 below it: while no score exceeds m by more than 8 nothing has to be
 // rescaled, which spares the maximum over the tokens in nearly every group.
 #include <algorithm>
@@ -296,7 +296,8 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         const uint32_t n = share.whole ? line.units : (uint32_t)min((uint64_t)(line.units - off), end - now);
         const uint64_t item_first = now - off;
         const uint32_t r0 = tile * S::kRows, rows = min((uint64_t)S::kRows, (uint64_t)s.rows * a.group - r0);
-        const uint32_t limit = min(s.length, (off + n) * kUnit);  // the first token that is not this share's
+        // the first token that is not this share's, or that none of the tile's rows sees
+        const uint32_t limit = min(visible_end(s, a.by_group, r0 + rows - 1), (off + n) * kUnit);
         const uint32_t here = limit > off * kUnit ? (limit - off * kUnit + kUnit - 1) / kUnit : 0u;  // units with tokens
         const uint32_t mine = warp < here ? (here - warp + W - 1) / W : 0u;
 
@@ -403,7 +404,7 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
             for (int j = 0; j < 2; ++j) {
                 factor[nt][j] = __shfl_sync(0xffffffffu, f, 4 * (2 * t4 + j));
                 const uint32_t col = 8 * nt + 2 * t4 + j;
-                sees[nt][j] = min(col < rows ? visible_end(s, a.by_group, r0 + col) : s.length, limit);
+                sees[nt][j] = col < rows ? min(visible_end(s, a.by_group, r0 + col), limit) : limit;
             }
         }
 
