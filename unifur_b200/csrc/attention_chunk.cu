@@ -10,7 +10,7 @@
 // issues tcgen05.mma:
 //   S = Q K^T   both operands from shared memory, 128 x 128 f32 sums in tensor memory
 //   O += P V    P from tensor memory, where the softmax warps have put it over S; V as it lies, MN-major
-// A softmax thread owns a row: it reads S, keeps the row's largest exponent m and sum l, and writes P = 2^(S c - m + 7) back as f16
+// A softmax thread owns a row: it reads S, keeps the row's largest exponent m and sum l, and writes P = 2^(S c - m + raise) back as f16
 // (bf16 with a bf16 cache).  While one tile's softmax runs, the other's two products do.  (64 tokens a step and two places for S, so that a step's scores are
 // there when the last one's weights are done, were tried: a first product of 64 columns takes as long as one of 128, A's rows being read for half
 // the work, and 128 tokens of two tiles took 6100 cycles instead of 4270.)  m is the largest exponent so far or up to 8
@@ -32,8 +32,13 @@ namespace nf4 {
 namespace {
 
 constexpr uint32_t kThreads = 512;
-// Weights are 2^(S c - m + kRaise): up to 2^15, so that f16 holds those that are 2^-32 of a row's largest; their sum is raised alike.
-constexpr float kRaise = 7.f;
+// Weights are 2^(S c - m + raise).  In f16 up to 2^15, so that it holds those that are 2^-32 of a row's largest; their sum is raised alike, and where
+// sums go to the workspace both are lowered by that again, so that no value overflows them that would not overflow a sum of weights up to
+// one.  bf16 has the range: weights up to one.
+template <bool NF4>
+constexpr float kRaise = NF4 ? 7.f : -8.f;
+template <bool NF4>
+constexpr float kLower = NF4 ? 1.f / 32768.f : 1.f;
 constexpr uint32_t kGroup = 16;  // tokens that are in one page for sure
 // warps 0-3 and 4-7: softmax of a tile; 8-11: codes to f16; 12: copies; 13: MMAs
 constexpr uint32_t kExpandWarp = 8, kCopyWarp = 12, kMmaWarp = 13;
@@ -501,7 +506,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                     uint32_t pw[N / 2];
                     float2 sum;
                     for (;;) {
-                        const float from = m == -INFINITY ? 0.f : kRaise - m - (float)less;
+                        const float from = m == -INFINITY ? 0.f : kRaise<NF4> - m - (float)less;
                         float top[2] = {-INFINITY, -INFINITY};
                         sum = make_float2(0.f, 0.f);
                         uint32_t ahead[2][32];  // 32 scores come while 32 are worked on
@@ -577,8 +582,8 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                 if (s_bad[piece & 7u] == piece + 1 || !ok) l = __uint_as_float(0x7fc00000u);  // NaN
                 const bool whole = p.steps == p.all;
                 const uint64_t part = (uint64_t)(2 * blockIdx.x + (p.step0 ? 0 : 1)) * S::kRows + tile * 128;
-                if (!whole) a.part_ml[part + r] = make_float2(m, l);
-                const float f = (whole ? l == 0.f ? 0.f : 1.f / l : 1.f) * (NF4 ? ref : 1.f);
+                if (!whole) a.part_ml[part + r] = make_float2(m, l * kLower<NF4>);
+                const float f = (whole ? l == 0.f ? 0.f : 1.f / l : kLower<NF4>) * (NF4 ? ref : 1.f);
                 constexpr uint32_t kChunks = D / 8;  // of a staged row: bf16 results, or half of a row's f32 sums
                 #pragma unroll 1
                 for (uint32_t half = 0; half < (whole ? 1u : 2u); ++half) {

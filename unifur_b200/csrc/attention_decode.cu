@@ -8,7 +8,7 @@
 // tokens of a head were several CTAs', the CTA that is done last joins theirs out of the workspace, in the order of the tokens.
 //
 // Mathematics, per group of sixteen tokens t and eight rows r (one MMA tile):
-//   x[t][r] = scale * log2(e) * sum_b ks[t][b] (levels_b[t] . q_b[r]),  w = 2^(x - m[r] + 8),  l[r] += w,
+//   x[t][r] = scale * log2(e) * sum_b ks[t][b] (levels_b[t] . q_b[r]),  w = 2^(x - m[r] + raise),  l[r] += w,
 //   o[d][r] += sum_t levels[t][d] (w[t][r] vs[t][block of d])
 // Tokens are on the MMA's M side in the first product and on its K side in the second, so the weights go from one to the other by a
 // transposition of 8 x 8 tiles (movmatrix) and nothing is padded to sixteen rows.  A quantized cache's codes are
@@ -28,9 +28,12 @@ namespace nf4 {
 
 namespace {
 
-// Weights are 2^(x - m + kRaise), and times V's scales up to 2^15, so that f16 holds those that are 2^-31 of a row's largest; their sum is
-// raised alike.
-constexpr float kRaise = 8.f;
+// Weights are 2^(x - m + raise).  With a quantized cache raised by 8, and times V's scales up to 2^15, so that f16 holds those that are 2^-31 of a
+// row's largest; they are up to 2^16, which sums and results lose again (kLower) before V's power of two comes back, so that no value overflows
+// them that would not overflow a sum of weights up to one.  bf16 has the range: weights up to one.
+template <bool NF4>
+constexpr float kRaise = NF4 ? 8.f : -8.f;
+constexpr float kLower = 1.f / 65536.f;
 constexpr float kNothing = -3e38f;  // the largest exponent of a row that has seen no token: all but the lowest number, so that weights of -inf are zeros
 constexpr uint32_t kGroup = 16;   // tokens to a group: pages are multiples of it
 
@@ -545,7 +548,7 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
             for (int nt = 0; nt < NT; ++nt)
                 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const float from = kRaise - m[nt][j];
+                    const float from = kRaise<NF4> - m[nt][j];
                     #pragma unroll
                     for (uint32_t u = 0; u < G; ++u) {
                         x[u][nt][j] = exp2_approx(x[u][nt][j] + from);
@@ -709,7 +712,14 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         };
         if (__any_sync(0xffffffffu, lost) || !ok) l[0][0] = l[0][1] = l[NT - 1][0] = l[NT - 1][1] = __uint_as_float(0x7fc00000u);  // NaN, and the results with it
         const bool divided = c0 != c1;
-        meet(NF4 ? ref * (1.f / kLevelUnit) : 1.f, !divided);
+        if (NF4) {
+            #pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                l[nt][0] *= kLower;
+                l[nt][1] *= kLower;
+            }
+        }
+        meet(NF4 ? ref * (kLower / kLevelUnit) : 1.f, !divided);
         if (divided) {
             if (tid == 0) {  // (behind the barrier that `meet` ends with: its release is for what all threads stored)
                 uint32_t done;
