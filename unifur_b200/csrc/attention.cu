@@ -293,6 +293,7 @@ join_kernel(const BatchView b, const AttentionView a, uint32_t q_heads) {
 // of 4096, 4 heads of 256, NF4: 16 rows 40 / 62, 32 rows 69 / 64; 8 heads of 64, NF4: 64 rows 54 / 52, bf16: 64 rows 40 / 43.
 bool takes_decode(const AttentionCall &c) {
     if (c.f32) return false;
+    if (!attention_chunk_counts(c)) return true;  // (the other counts in 64 bits)
     const int of_dim = c.head_dim == 64 ? 0 : c.head_dim == 128 ? 1 : 2;
     static constexpr double kStream[2][3] = {{5, 11, 32}, {7, 9, 45}}, kMany[2][3] = {{13, 18, 40}, {19, 25, 58}};  // [NF4][dim]
     // row tiles of all sequences: by the most rows of one, or by all rows where that says less

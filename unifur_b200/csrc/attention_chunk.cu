@@ -1087,10 +1087,6 @@ int32_t launch(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) 
     }
     FailureRef failure;
     NF4_TRY(prefill_failure_ref(&failure));
-    // the line is counted in 32 bits
-    const uint64_t tiles = ((uint64_t)c.batch.rows * c.view.group / S::kRows + c.batch.sequences) * c.cache.heads;
-    const uint64_t steps = ((uint64_t)c.batch.width * c.cache.page_size + S::kTokens - 1) / S::kTokens;
-    if (tiles * (steps + 1 + kStart) >= 1ull << 31) return fail(NF4_ERR_UNSUPPORTED, "attention: rows times tokens are too many for a call; split it");
     const Layout at(c);
     Split *const splits = reinterpret_cast<Split *>(workspace + at.splits);
     AttentionView view = c.view;
@@ -1123,6 +1119,13 @@ int32_t launch(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) 
 
 uint64_t attention_chunk_bytes(const AttentionCall &c) {
     return Layout(c).bytes;
+}
+
+// The line of steps is counted in 32 bits, and what the page table has room for bounds it.
+bool attention_chunk_counts(const AttentionCall &c) {
+    const uint64_t tiles = ((uint64_t)c.batch.rows * c.view.group / rows_of(c) + c.batch.sequences) * c.cache.heads;
+    const uint64_t steps = ((uint64_t)c.batch.width * c.cache.page_size + tokens_of(c) - 1) / tokens_of(c);
+    return tiles * (steps + 1 + kStart) < 1ull << 31;
 }
 
 int32_t attention_chunk(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) {

@@ -114,7 +114,8 @@ constexpr uint64_t kAttentionFlagBytes = 4096;  // at the start of a workspace, 
 uint64_t attention_decode_bytes(const AttentionCall &c);
 int32_t attention_decode(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream);
 
-// attention_chunk.cu: bf16 tensors, many rows
+// attention_chunk.cu: bf16 tensors, many rows; where it can count the call's steps
+bool attention_chunk_counts(const AttentionCall &c);
 uint64_t attention_chunk_bytes(const AttentionCall &c);
 int32_t attention_chunk(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream);
 
