@@ -1,7 +1,7 @@
 // Attention of few rows, or over few tokens, of the paged cache (decode steps, drafted tokens, short prompts): up to sixteen rows of a head at a time.
 //
 // Bound by the bytes of the cache, and for a quantized one by its lookups as well.  A CTA has an SM to itself; the units
-// (16 or 32 tokens) of all sequences, heads and row tiles form one line that the CTAs share out evenly, whatever the sequences'
+// (16 or 32 tokens) of all sequences, heads and row tiles, and their starts, form one line that the CTAs share out evenly, whatever the sequences'
 // lengths.  In a CTA every warp takes every W-th unit of its share, which it has brought to shared memory by TMA into a
 // ring of its own (two or three units in flight: no barrier between warps while tokens stream), with its own running largest exponent,
 // sum and accumulator.  At the end of a head's share the warps' results are joined through shared memory, and where the
@@ -51,6 +51,10 @@ struct Shape {
     static constexpr uint32_t kScaleTile = NF4 ? kGroup * kBlocks * 4 : 0;  // its scales, likewise
     static constexpr uint32_t kFit = 98304 / (kWarps * kPer * 2 * kTile), kStages = !NF4 || kFit > 3 ? 3 : kFit;
     static constexpr uint32_t kAcc = D / 16 * 4 * NT;                  // accumulator registers of a thread
+    // A head's start and end in a CTA (its queries, the first copies, the warps' results) take about as long as two units of every warp: 3.7 us
+    // where a unit in the stream takes 0.155 (128, NF4), 2.6 and 0.2 (128, bf16).  63 sequences of one token beside one of 120,000 (four heads) take 33
+    // and 62 us; 387 and 654 when only units counted, the CTAs that had the single tokens being last by far.
+    static constexpr uint32_t kStart = 2 * kWarps;
     // accumulator registers of a thread that go through shared memory at a time: what the space ahead of the table holds
     static constexpr uint32_t kPassRegs = kAcc >= 32 && NF4 && kWarps <= 12 ? 32 : 16;
     static constexpr uint32_t kMerge = kWarps * kPassRegs * 32 * 4;    // where the warps' results meet
@@ -99,15 +103,15 @@ __device__ __forceinline__ uint64_t divided(uint64_t a, uint64_t b) {  // a / b,
     return (a | b) >> 32 ? a / b : (uint64_t)((uint32_t)a / (uint32_t)b);
 }
 
-// How the units of the line (kPer groups each) are shared out.  quota 0: `per` to a CTA, one more to the first `more` of them, whatever head
-// they are of.  Otherwise a CTA has units of one head only, and a head as many CTAs as it takes for none to have more than `quota`.
+// How the line is shared out: of every head and row tile its start, which counts as much as kStart units, and behind it its units (kPer groups
+// each).  quota 0: `per` places to a CTA, one more to the first `more` of them, whatever head they are of.  Otherwise a CTA has units of one head only, and a head as many CTAs as it takes for none to have more than `quota`.
 struct Share {
     uint64_t per;
     uint32_t more, quota;
     bool whole;  // quota 0: heads are not divided
     __device__ uint64_t start(uint32_t cta) const { return per * cta + min(cta, more); }
     __device__ uint32_t cta_of(uint64_t u) const {
-        const uint64_t first = (per + 1) * more;  // units of the CTAs that have one more
+        const uint64_t first = (per + 1) * more;  // places of the CTAs that have one more
         return u < first ? (uint32_t)divided(u, per + 1) : more + (uint32_t)divided(u - first, per);
     }
 };
@@ -116,7 +120,7 @@ struct Line {  // a sequence's part of the line
     Sequence s;
     uint32_t units;  // to a head and row tile
     uint32_t tiles, items;  // row tiles, and heads times row tiles
-    __device__ uint64_t all() const { return (uint64_t)units * items; }
+    __device__ uint64_t all(uint32_t start) const { return (uint64_t)(units + start) * items; }
 };
 __device__ __forceinline__ Line line_of(const CacheView &c, const BatchView &b, uint32_t group, uint32_t rows_of_tile, uint32_t tokens_of_unit, uint32_t s) {
     Line l{{0, 0, 0}, 0, 0, 0};
@@ -133,7 +137,7 @@ __global__ void __launch_bounds__(Shape<D, NF4, NT>::kThreads, 1)
 attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const CacheView c, const BatchView b,
                         const AttentionView a, uint32_t *const counters, float *const parts, const FailureRef failure) {
     using S = Shape<D, NF4, NT>;
-    constexpr uint32_t W = S::kWarps, kBlocks = S::kBlocks, kStages = S::kStages, G = S::kPer, kUnit = G * kGroup;
+    constexpr uint32_t W = S::kWarps, kBlocks = S::kBlocks, kStages = S::kStages, G = S::kPer, kUnit = G * kGroup, kStart = S::kStart;
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ __align__(8) uint64_t s_bars[W * kStages];
     __shared__ float2 s_ml[W][S::kRows];
@@ -169,25 +173,25 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     const Line line0 = line_of(c, b, a.group, S::kRows, kUnit, lane);  // of the first 32 sequences
     Share share;
     {
-        uint64_t units = line0.all();
-        uint32_t items = line0.items;
+        uint64_t units = line0.all(0);
+        uint32_t items = line0.items, longest = line0.items ? line0.units : 0u;
         for (uint32_t s = lane + 32; s < b.sequences; s += 32) {
             const Line l = line_of(c, b, a.group, S::kRows, kUnit, s);
-            units += l.all();
+            units += l.all(0);
             items += l.items;
+            longest = max(longest, l.items ? l.units : 0u);
         }
         #pragma unroll
-        for (int k = 1; k < 32; k <<= 1) {
-            units += __shfl_xor_sync(0xffffffffu, units, k);
-            items += __shfl_xor_sync(0xffffffffu, items, k);
-        }
+        for (int k = 1; k < 32; k <<= 1) units += __shfl_xor_sync(0xffffffffu, units, k);
+        items = __reduce_add_sync(0xffffffffu, items);
+        longest = __reduce_max_sync(0xffffffffu, longest);
         if (units == 0) return;  // nothing to do
         const uint32_t ctas = (uint32_t)min((uint64_t)gridDim.x, units);
         if (blockIdx.x >= ctas) return;
-        share.per = divided(units, ctas);
-        share.more = (uint32_t)(units - share.per * ctas);
-        // a head whose tokens are two units to a warp is not worth dividing: the join costs about as much
-        share.whole = units <= (uint64_t)items * (2 * W);
+        const uint64_t each = divided(units, ctas);
+        // heads whose tokens are two units to a warp are not worth dividing: the join costs about as much.  It goes by the longest, which its CTA may
+        // come to last (200 sequences of one token beside one of 5000, four heads of 128, NF4: 33 us; undivided, as they were by their mean, 46).
+        share.whole = longest <= 2 * W;
         // A CTA with two heads' units starts and ends twice, which takes about as long as two units of every warp.  So where the heads can
         // be given CTAs of their own with a quota that is not longer by more, they are.  Quotas of all units over fewer CTAs: with as many
         // fewer as there are heads every head's last CTA may have next to nothing, so that one always serves.
@@ -203,11 +207,16 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
             for (uint32_t k = 0; k < 4; ++k) need[k] = __reduce_add_sync(0xffffffffu, need[k]);
             #pragma unroll
             for (uint32_t k = 4; k-- > 0;)
-                if (need[k] <= ctas && quota[k] <= share.per + 2 * W) share.quota = quota[k];
+                if (need[k] <= ctas && quota[k] <= each + 2 * W) share.quota = quota[k];
+        }
+        if (!share.quota) {
+            const uint64_t places = units + (uint64_t)items * kStart;
+            share.per = divided(places, ctas);
+            share.more = (uint32_t)(places - share.per * ctas);
         }
     }
 
-    // the sequence that this CTA begins in, and how far into it: first, in the line (units, or with a quota CTAs)
+    // the sequence that this CTA begins in, and how far into it: first, in the line (places, or with a quota CTAs)
     uint64_t first = share.quota ? blockIdx.x : share.start(blockIdx.x), end = share.quota ? 0 : share.start(blockIdx.x + 1);
     uint32_t seq = b.sequences;
     Line line = line0;
@@ -216,7 +225,7 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         uint64_t before = 0;
         for (uint32_t s0 = 0; s0 < b.sequences; s0 += 32) {
             const Line l = s0 ? line_of(c, b, a.group, S::kRows, kUnit, s0 + lane) : line0;
-            const uint64_t own = share.quota ? (uint64_t)l.items * ((l.units + share.quota - 1) / share.quota) : l.all();
+            const uint64_t own = share.quota ? (uint64_t)l.items * ((l.units + share.quota - 1) / share.quota) : l.all(kStart);
             uint64_t upto = own;
             #pragma unroll
             for (int k = 1; k < 32; k <<= 1) {
@@ -241,23 +250,28 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     }
     if (seq >= b.sequences) return;  // (with a quota the last CTAs may have nothing)
     uint64_t now;
-    uint32_t item, off, c0, c1;  // c0, c1: the CTAs that a head's units are shared by
+    uint32_t item, off, c0, c1;  // off: the first of a head's units that is this CTA's; c0, c1: the CTAs that they are shared by
+    uint32_t lead;               // places of the head's start that are this CTA's too
     if (share.quota) {
         const uint32_t ways = (line.units + share.quota - 1) / share.quota, way = (uint32_t)at % ways;
         item = (uint32_t)at / ways;
         // `ways` shares that differ by one at most; the line is this share
         const uint32_t each = line.units / ways, rest = line.units - each * ways;
         off = way * each + min(way, rest);
+        lead = 0;
         now = off;
         end = off + each + (way < rest ? 1 : 0);
         c0 = blockIdx.x - way;
         c1 = c0 + ways - 1;
     } else {
         now = first;
-        item = (uint32_t)divided(at, line.units);
-        off = (uint32_t)(at - (uint64_t)item * line.units);
-        if (share.whole && off) {  // a head belongs to the CTA in whose share it begins
-            now += line.units - off;
+        item = (uint32_t)divided(at, line.units + kStart);
+        const uint32_t in = (uint32_t)(at - (uint64_t)item * (line.units + kStart));  // how far into the head
+        off = in > kStart ? in - kStart : 0u;
+        lead = in > kStart ? 0u : kStart - in;
+        if (share.whole && in) {  // a head belongs to the CTA in whose share it begins
+            now += line.units + kStart - in;
+            lead = kStart;
             off = 0;
             ++item;
         }
@@ -296,6 +310,8 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         if (seq >= b.sequences) break;
         const Sequence s = line.s;
         const uint32_t head = line.tiles == 1 ? item : item / line.tiles, tile = item - head * line.tiles;
+        now += lead;
+        if (!share.whole && now >= end) break;  // the share ends ahead of the head's units
         const uint32_t n = share.whole ? line.units : (uint32_t)min((uint64_t)(line.units - off), end - now);
         const uint64_t item_first = now - off;
         const uint32_t r0 = tile * S::kRows, rows = min((uint64_t)S::kRows, (uint64_t)s.rows * a.group - r0);
@@ -769,6 +785,7 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         }
         now += n;
         off = 0;
+        lead = kStart;
         ++item;
     }
     if (!ok) ptx::let_flights_land();
