@@ -151,6 +151,7 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     float2 *const merge = reinterpret_cast<float2 *>(smem);
     const uint32_t bars = ptx::smem_addr(s_bars) + 8 * kStages * warp;
     if (NF4 && table + 65536u + S::kRing > base + S::kSmem) {
+        ptx::pdl_wait();
         if (tid == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 20);
         return;
     }
