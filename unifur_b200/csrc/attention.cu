@@ -16,7 +16,7 @@ namespace {
 // softmax that is never held whole.  A row's scores are eight neighbouring lanes'.  FMAs are done in pairs.  Bound by shared
 // memory, which gives registers 128 bytes a clock, so that 16 bytes to a lane take four whatever is broadcast: with four rows 8 such reads
 // to 32 pairs of FMAs for the scores and 5 to 32 for the results (of 128), 24 to 32 TFLOP/s over long prompts.  (16 sequences of 4096 tokens, 7 rows of
-// four heads of 128: 110 us; with tiles of 64 rows 280, of 16 rows in four warps, one to a thread, 174.)
+// four heads of 128, the cache in L2: 110 us; with tiles of 64 rows 280, of 16 rows in four warps, one to a thread, 174.)
 constexpr int kThreads = 256;
 
 constexpr uint32_t tokens_of_tile(uint32_t dim, uint32_t warps) { return (dim == 256 ? 16 : 32) / (warps == 1 ? 2 : 1); }
@@ -288,9 +288,10 @@ join_kernel(const BatchView b, const AttentionView a, uint32_t q_heads) {
 // Which of two kernels: the one that streams the cache reads a head's tokens once for every 16 rows, the one for many rows once for
 // every 256 (128 with a dim of 256).  By what each takes, in tenths of a microsecond on an SM: a row tile's start, and 128 tokens of
 // it; the second kernel's own start, its joins and the expansion ahead of it are 15 to 20 us more.  Measured on both sides (us, first / second):
-// 16 sequences of 8192 tokens, 8 heads of 128, NF4: 16 rows 62 / 166, 48 rows 161 / 166, 64 rows 211 / 166; bf16: 16 rows 92 / 126, 32 rows
-// 177 / 127; one such sequence, NF4: 96 rows 34 / 43, 128 rows 46 / 43; 4 sequences of 512, 4 heads, NF4: 384 rows 24 / 31, 768 rows 44 / 35; 8
-// of 4096, 4 heads of 256, NF4: 16 rows 40 / 62, 32 rows 69 / 64; 8 heads of 64, NF4: 64 rows 54 / 52, bf16: 64 rows 40 / 43.
+// 16 sequences of 8192 tokens, 8 heads of 128, NF4: 16 rows 61 / 161, 48 rows 159 / 162, 64 rows 207 / 162; bf16: 16 rows 95 / 123, 32 rows
+// 173 / 124; one such sequence, NF4: 96 rows 28 / 37, 128 rows 36 / 37, 192 rows 48 / 40; 4 sequences of 512, 4 heads, NF4: 384 rows 24 / 26, 768
+// rows 43 / 34, bf16: 256 rows 24 / 23, 384 rows 29 / 23; 8 of 4096, 4 heads of 256, NF4: 16 rows 41 / 57, 32 rows 67 / 57; 8 heads of 64, NF4: 64
+// rows 50 / 48, 96 rows 68 / 48, bf16: 64 rows 41 / 40, 96 rows 56 / 40.
 bool takes_decode(const AttentionCall &c) {
     if (c.f32) return false;
     if (!attention_chunk_counts(c)) return true;  // (the other counts in 64 bits)

@@ -101,7 +101,8 @@ class PagedKvCache:
         ``softmax(scale * q . k) v`` over each row's token and all before it.  ``q`` is ``[rows, q_heads, head_dim]`` or ``[rows,
         q_heads * head_dim]``, bf16 or f32, rows at any stride; ``q_heads`` is a multiple of the cache's heads, which serve
         neighbouring query heads.  ``scale`` is ``1 / sqrt(head_dim)`` if it is not given.  A row that sees nothing becomes
-        zeros; rows of no sequence are left as ``out`` has them, and without ``out`` undefined."""
+        zeros, one that sees a token in a page that there is not NaNs (others of its sequence may, too); rows of no sequence are left as ``out``
+        has them, and without ``out`` undefined.  ``out`` does not overlap ``q``."""
         if scale is None:
             scale = 1.0 / math.sqrt(self.head_dim())
         return _lib.host().cache_attention(*self._args(), *batch._args(), q, scale, out)
