@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from cache_util import batch_of, filled_cache, reference
+from cache_util import batch_of, filled_cache, reference, stored, tokens_of
 
 F32, BF16 = torch.float32, torch.bfloat16
 
@@ -44,32 +44,24 @@ def test_the_limit_sees_a_unit_left_out(length, lost, q_std):
     scale = 128 ** -0.5
     ref, _, _ = reference(cache, batch, q, scale)
     limit = most_off(cache, batch, q, scale, 128, length, BF16)
-    codes = torch.stack((cache.k & 15, cache.k >> 4), -1).flatten(-2).long()
-    from unifur_b200.quantize import nf4_levels
+    k, v = (tokens_of(stored(cache, name), batch, 64, 0) for name in ("k", "v"))
+    x = np.einsum("hgd,thd->hgt", q[0].double().numpy().reshape(2, 4, 128), k) * scale
 
-    at = torch.arange(length)
-    page = batch.page_table[0, at // 64].long()
-    k, v = ((nf4_levels().double()[torch.stack((t & 15, t >> 4), -1).flatten(-2).long()] * s.double().repeat_interleave(64, -1))[page, :, at % 64]
-            for t, s in ((cache.k, cache.k_scales), (cache.v, cache.v_scales)))
-    assert codes.shape[-1] == 128
-    q2 = q[0].double().view(2, 4, 128)
+    def off(weights):  # with tokens that count as much as this, the rows' largest error
+        w = np.exp(x - x.max(-1, keepdims=True)) * weights
+        return worst((np.einsum("hgt,thd->hgd", w, v) / w.sum(-1, keepdims=True)).reshape(1, 8, 128), ref)
 
-    def result(weights):  # of each token, beside its own
-        x = torch.einsum("hgd,thd->hgt", q2, k) * scale
-        w = torch.exp(x - x.amax(-1, keepdim=True)) * weights
-        return (torch.einsum("hgt,thd->hgd", w, v) / w.sum(-1, keepdim=True)).reshape(1, 8, 128).numpy()
-
-    one = torch.ones(length, dtype=torch.float64)
-    assert worst(result(one), ref) < 1e-12
-    x = torch.einsum("hgd,thd->hgt", q2, k).amax(0).amax(0)
-    first = int(x.argmax()) // lost * lost if q_std > 1 else 32  # (sharp scores: the unit that has the largest)
+    one = np.ones(length)
+    assert off(one) < 1e-12
+    first = int(x[0, 0].argmax()) // lost * lost if q_std > 1 else 32  # (sharp scores: the unit that has the largest)
+    planted = []
     for factor in (0.0, 2.0) if q_std == 1 else (0.0,):  # (twice what has all the weight is the same)
-        planted = one.clone()
-        planted[first:first + lost] = factor
-        assert worst(result(planted), ref) > limit
-    planted = one.clone()
-    planted[length // 2:] = 1.5
-    assert q_std > 1 or worst(result(planted), ref) > limit
+        planted.append(one.copy())
+        planted[-1][first:first + lost] = factor
+    if q_std == 1:
+        planted.append(np.where(np.arange(length) < length // 2, 1.0, 1.5))
+    for weights in planted:
+        assert off(weights) > limit, (off(weights), limit)
     assert worst(0.6 * ref, ref) > limit
 
 
