@@ -543,6 +543,56 @@ NF4_API int32_t nf4_cache_attention_dev(const nf4_cache *cache, const nf4_cache_
  * place in shared memory, or a negative status.  For inspection and tests. */
 NF4_API int32_t nf4_cache_attention_row_place(uint32_t head_dim, uint32_t thread, uint32_t chunk, int32_t results);
 
+/* The same with the positions' rotation on the way: neighbouring values (pairs) or the two halves of a head's first `rotary_dim`
+ * values are turned by the angles of the row's position,
+ *     a' = a cos - b sin,  b' = b cos + a sin,
+ * with pair i's cosine at table[position][i] and its sine at table[position][rotary_dim / 2 + i] (f32, 16-byte aligned): the two are values i and
+ * rotary_dim / 2 + i of a head (pairs 0), or values 2 i and 2 i + 1 (pairs 1).  Products and sums are f32, each rounded; what is stored or written is rounded
+ * once from there (NF4_CACHE_NF4: the codes and scale of the f32 values).  rotary_dim is a multiple of 16, at most head_dim; the values behind it
+ * stay as they are.  positions: [rows], or NULL for each row's place in its sequence. */
+typedef struct nf4_rotation {
+    uint32_t struct_bytes;      /* sizeof(nf4_rotation), checked */
+    uint32_t rotary_dim;
+    int32_t pairs;
+    uint32_t table_positions;   /* rows of the table */
+    const float *table;         /* [table_positions, rotary_dim], device memory */
+    const int32_t *positions;   /* [rows] device memory, or NULL */
+} nf4_rotation;
+
+/* Writes the rows' rotated keys and their values to their places as nf4_cache_append_dev does, and the rows' rotated queries, q [rows, q_heads,
+ * head_dim] of io_dtype with ldq elements from row to row, to q_out (ldo; q itself where ldo is ldq, else memory that q does not overlap).  q_heads 0:
+ * there are no queries, q and q_out are not looked at.  A row whose position is outside the table is not written to the cache and its queries become
+ * NaNs; queries of a row whose token is in no page are turned all the same. */
+NF4_API int32_t nf4_cache_append_rotated_dev(const nf4_cache *cache, const nf4_cache_batch *batch, const nf4_rotation *rotation,
+                                             const void *k, uint64_t ldk, const void *v, uint64_t ldv, const void *q, uint64_t ldq,
+                                             uint32_t q_heads, void *q_out, uint64_t ldo, int32_t io_dtype, void *stream);
+
+/* Trees of drafted tokens.  A sequence's rows in a call are the nodes of a tree (or of several), appended to the cache like any new tokens; node i is its
+ * row i, behind its context of lengths[s] - n tokens.  Which nodes a row sees say masks [rows, mask_words]: bit j % 32 of word j / 32 stands
+ * for node j of the row's sequence; nodes from 32 * mask_words on are seen by none.
+ * nf4_cache_tree_dev makes masks and positions of the nodes' parents (parents[row]: the number of an earlier node of the sequence; whatever else
+ * stands there makes the row a root): a row's mask is itself and its ancestors, its position the context's length and its depth,
+ * a root's the context's length.  masks or positions may be NULL.  Rows of no sequence are left as they are. */
+NF4_API int32_t nf4_cache_tree_dev(const nf4_cache *cache, const nf4_cache_batch *batch, const int32_t *parents, uint32_t *masks,
+                                   uint32_t mask_words, int32_t *positions, void *stream);
+
+/* nf4_cache_attention_dev for such rows: row i sees its sequence's context, and the nodes that its mask has, whether they come before it or not.
+ * A row that sees nothing becomes zeros, as does a row whose own token is negative (a node with a negative token is seen by none).  Values of all tokens
+ * of the sequences that have rows are finite, those of nodes that a row's mask hides among them.  All else is as there, with these three for its workspace. */
+NF4_API uint64_t nf4_cache_tree_attention_workspace_bytes(const nf4_cache *cache, const nf4_cache_batch *batch, uint32_t q_heads,
+                                                          int32_t io_dtype);
+NF4_API uint64_t nf4_cache_tree_attention_call_flag_bytes(const nf4_cache *cache, const nf4_cache_batch *batch, uint32_t q_heads,
+                                                          int32_t io_dtype);
+NF4_API int32_t nf4_cache_tree_attention_dev(const nf4_cache *cache, const nf4_cache_batch *batch, const uint32_t *masks, uint32_t mask_words,
+                                             const nf4_attention_args *args, void *stream);
+
+/* Keeps a path of each tree: nodes kept[s][0], kept[s][1], ... kept[s][counts[s] - 1] of sequence s move to the places behind its context, in
+ * this order, and lengths_out[s] becomes its context's length and counts[s].  kept [sequences, most_kept] increases along a path (ancestors are
+ * earlier nodes): a path ends ahead of the first entry that is not above the one before it, or that is no node.  A token that is, or would
+ * come, where there is no page is not moved.  lengths_out may be the batch's lengths, or NULL (other layers' caches, before the lengths change). */
+NF4_API int32_t nf4_cache_keep_dev(const nf4_cache *cache, const nf4_cache_batch *batch, const int32_t *kept, uint32_t most_kept,
+                                   const int32_t *counts, int32_t *lengths_out, void *stream);
+
 /* ------------------------------------------------ resident weight handles -- */
 
 /* An NF4 weight resident in device memory (what Nf4Linear holds in `packed`,

@@ -84,6 +84,12 @@ class AttentionArgs(C.Structure):
                 ("workspace_bytes", C.c_uint64)]
 
 
+class RotationArgs(C.Structure):
+    """``nf4_rotation`` (include/nf4_b200.h)."""
+    _fields_ = [("struct_bytes", C.c_uint32), ("rotary_dim", C.c_uint32), ("pairs", C.c_int32), ("table_positions", C.c_uint32),
+                ("table", C.c_void_p), ("positions", C.c_void_p)]
+
+
 _vp, _u64, _i32, _u32, _f32 = C.c_void_p, C.c_uint64, C.c_int32, C.c_uint32, C.c_float
 
 # name -> (restype, argtypes)
@@ -148,6 +154,13 @@ SIGNATURES = {
     "nf4_cache_attention_call_flag_bytes": (_u64, [C.POINTER(Cache), C.POINTER(CacheBatch), _u32, _i32]),
     "nf4_cache_attention_dev": (_i32, [C.POINTER(Cache), C.POINTER(CacheBatch), C.POINTER(AttentionArgs), _vp]),
     "nf4_cache_attention_row_place": (_i32, [_u32, _u32, _u32, _i32]),
+    "nf4_cache_append_rotated_dev": (_i32, [C.POINTER(Cache), C.POINTER(CacheBatch), C.POINTER(RotationArgs), _vp, _u64, _vp, _u64, _vp, _u64, _u32,
+                                            _vp, _u64, _i32, _vp]),
+    "nf4_cache_tree_dev": (_i32, [C.POINTER(Cache), C.POINTER(CacheBatch), _vp, _vp, _u32, _vp, _vp]),
+    "nf4_cache_tree_attention_workspace_bytes": (_u64, [C.POINTER(Cache), C.POINTER(CacheBatch), _u32, _i32]),
+    "nf4_cache_tree_attention_call_flag_bytes": (_u64, [C.POINTER(Cache), C.POINTER(CacheBatch), _u32, _i32]),
+    "nf4_cache_tree_attention_dev": (_i32, [C.POINTER(Cache), C.POINTER(CacheBatch), _vp, _u32, C.POINTER(AttentionArgs), _vp]),
+    "nf4_cache_keep_dev": (_i32, [C.POINTER(Cache), C.POINTER(CacheBatch), _vp, _u32, _vp, _vp, _vp]),
     "nf4_weight_from_values_host": (_i32, [_vp, _u64, _u64, _i32, _i32, C.POINTER(_vp)]),
     "nf4_weight_from_packed_host": (_i32, [_vp, _vp, _vp, _f32, _u64, _u64, _i32,
                                            C.POINTER(_vp)]),

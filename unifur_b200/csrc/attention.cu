@@ -52,7 +52,8 @@ __device__ __forceinline__ void get(const float *from, float (&v)[R]) {
     }
 }
 
-template <int D, bool NF4, int R, int W>
+// TREE: rows are nodes of trees, which see their sequence's tokens ahead of the nodes and those nodes that their masks have
+template <int D, bool NF4, int R, int W, bool TREE>
 __global__ void __launch_bounds__(32 * W)
 attention_f32_kernel(const CacheView c, const BatchView b, const AttentionView a) {
     using S = F32Shape<D, R, W>;
@@ -80,11 +81,19 @@ attention_f32_kernel(const CacheView c, const BatchView b, const AttentionView a
             }
             *reinterpret_cast<float4 *>(sq + r * S::kPitch + d) = v;
         }
-        // the tokens that this thread's rows see, and those that any row of the tile does
+        // the tokens that this thread's rows see (TREE: the rows' numbers, kBlind where they see nothing), and those that any row of the tile does
+        constexpr uint32_t kBlind = 0xffffffffu;
         uint32_t sees[R];
         #pragma unroll
-        for (int i = 0; i < R; ++i) sees[i] = R * ty + i < n ? visible_end(s, a.by_group, r0 + R * ty + i) : 0u;
-        const uint32_t end = visible_end(s, a.by_group, r0 + n - 1), tiles = (end + kTokens - 1) / kTokens;
+        for (int i = 0; i < R; ++i) {
+            if (TREE) {
+                const uint32_t token = a.by_group.of(r0 + min(R * ty + i, n - 1));
+                sees[i] = R * ty + i < n && first_node(s) + (int32_t)token >= 0 ? s.row0 + token : kBlind;
+            } else {
+                sees[i] = R * ty + i < n ? visible_end(s, a.by_group, r0 + R * ty + i) : 0u;
+            }
+        }
+        const uint32_t end = seen_end<TREE>(s, a.by_group, r0 + n - 1), tiles = (end + kTokens - 1) / kTokens;
         const uint32_t tile0 = (uint32_t)((uint64_t)tiles * part / a.parts), tile1 = (uint32_t)((uint64_t)tiles * (part + 1) / a.parts);
         float most[R], sum[R] = {};
         float2 acc[R][D / 16] = {};
@@ -165,9 +174,14 @@ attention_f32_kernel(const CacheView c, const BatchView b, const AttentionView a
             #pragma unroll
             for (int i = 0; i < R; ++i) {
                 float top = most[i];
+                uint32_t window = ~0u;  // TREE: bit k: the row sees token t0 + k
+                if (TREE) {
+                    if ((int32_t)(t0 + kTokens) > first_node(s) && sees[i] != kBlind) window = seen_nodes(a, sees[i], (int32_t)t0 - first_node(s));
+                    window = sees[i] == kBlind ? 0u : window & low_bits(end - t0);
+                }
                 #pragma unroll
                 for (int j = 0; j < kOwn; ++j) {
-                    x[j][i] = t0 + tx + 8 * j < sees[i] ? (pairs[i][j].x + pairs[i][j].y) * a.scale_log2 : -INFINITY;
+                    x[j][i] = (TREE ? window >> (tx + 8 * j) & 1u : t0 + tx + 8 * j < sees[i]) ? (pairs[i][j].x + pairs[i][j].y) * a.scale_log2 : -INFINITY;
                     top = fmaxf(top, x[j][i]);
                 }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -343,7 +357,7 @@ uint64_t workspace_bytes_of(const AttentionCall &c, const Plan &p) {
 
 template <int D, bool NF4, int R, int W>
 int32_t launch_f32(const AttentionCall &c, const Plan &p, cudaStream_t stream) {
-    auto kernel = attention_f32_kernel<D, NF4, R, W>;
+    auto kernel = c.tree ? attention_f32_kernel<D, NF4, R, W, true> : attention_f32_kernel<D, NF4, R, W, false>;
     constexpr uint32_t kSmem = F32Shape<D, R, W>::kSmem;
     NF4_TRY(ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), kSmem));
     count_launch();
@@ -364,8 +378,9 @@ int32_t launch_of(const AttentionCall &c, const Plan &p, cudaStream_t stream) {
     return launch_maybe_overlapped(join_kernel<D>, dim3(c.batch.rows * q_heads), dim3(kThreads), 0, stream, true, c.batch, c.view, q_heads);
 }
 
-AttentionCall call_of(const nf4_cache &cache, const nf4_cache_batch &batch, uint32_t q_heads, int32_t io_dtype) {
+AttentionCall call_of(const nf4_cache &cache, const nf4_cache_batch &batch, uint32_t q_heads, int32_t io_dtype, bool tree) {
     AttentionCall c{};
+    c.tree = tree;
     c.cache = view_of(cache);
     c.batch = view_of(batch);
     c.view.group = q_heads / cache.heads;
@@ -387,41 +402,34 @@ int32_t check_heads(const char *what, const nf4_cache &cache, const nf4_cache_ba
     return NF4_OK;
 }
 
-}  // namespace
-
-}  // namespace nf4
-
-using namespace nf4;
-
-extern "C" {
-
-uint64_t nf4_cache_attention_flag_bytes(void) { return kAttentionFlagBytes; }
-
-uint64_t nf4_cache_attention_call_flag_bytes(const nf4_cache *cache, const nf4_cache_batch *batch, uint32_t q_heads, int32_t io_dtype) {
-    const char *const what = "nf4_cache_attention_call_flag_bytes";
+uint64_t call_flag_bytes(const char *what, const nf4_cache *cache, const nf4_cache_batch *batch, uint32_t q_heads, int32_t io_dtype, bool tree) {
     if (check_cache(what, cache, batch) != NF4_OK || check_heads(what, *cache, *batch, q_heads) != NF4_OK) return kAttentionFlagBytes;
-    return takes_decode(call_of(*cache, *batch, q_heads, io_dtype)) ? kAttentionFlagBytes : 0;
+    return takes_decode(call_of(*cache, *batch, q_heads, io_dtype, tree)) ? kAttentionFlagBytes : 0;
 }
 
-uint64_t nf4_cache_attention_workspace_bytes(const nf4_cache *cache, const nf4_cache_batch *batch, uint32_t q_heads, int32_t io_dtype) {
-    const char *const what = "nf4_cache_attention_workspace_bytes";
+uint64_t workspace_bytes(const char *what, const nf4_cache *cache, const nf4_cache_batch *batch, uint32_t q_heads, int32_t io_dtype, bool tree) {
     if (check_cache(what, cache, batch) != NF4_OK || check_heads(what, *cache, *batch, q_heads) != NF4_OK) return 0;
-    const AttentionCall c = call_of(*cache, *batch, q_heads, io_dtype);
+    const AttentionCall c = call_of(*cache, *batch, q_heads, io_dtype, tree);
     return workspace_bytes_of(c, plan_of(c));
 }
 
-int32_t nf4_cache_attention_dev(const nf4_cache *cache, const nf4_cache_batch *batch, const nf4_attention_args *args, void *stream) {
-    const char *const what = "nf4_cache_attention_dev";
+// tree: the rows are nodes that see what their masks say
+int32_t attention(const char *what, const nf4_cache *cache, const nf4_cache_batch *batch, const uint32_t *masks, uint32_t mask_words, bool tree,
+                  const nf4_attention_args *args, void *stream) {
     NF4_TRY(check_cache(what, cache, batch));
     if (!args || args->struct_bytes != sizeof(nf4_attention_args)) return fail(NF4_ERR_INVALID_ARG, "%s: args is null or its struct_bytes wrong", what);
     NF4_TRY(check_heads(what, *cache, *batch, args->q_heads));
     if (!(args->scale - args->scale == 0.0f)) return fail(NF4_ERR_INVALID_ARG, "%s: scale is not finite", what);
+    if (mask_words > 1u << 26) return fail(NF4_ERR_UNSUPPORTED, "%s: masks of %u words; 2^26 are supported", what, mask_words);
     if (!batch->rows || !batch->sequences) return NF4_OK;
+    if (tree && mask_words && !masks) return fail(NF4_ERR_INVALID_ARG, "%s: masks is null", what);
     const uint64_t width = (uint64_t)args->q_heads * cache->head_dim;
     uint64_t ldq = args->ldq, ldo = args->ldo;
     NF4_TRY(check_rows(what, "q", args->q, &ldq, width, args->io_dtype));
     NF4_TRY(check_rows(what, "out", args->out, &ldo, width, args->io_dtype));
-    AttentionCall c = call_of(*cache, *batch, args->q_heads, args->io_dtype);
+    AttentionCall c = call_of(*cache, *batch, args->q_heads, args->io_dtype, tree);
+    c.view.masks = masks;
+    c.view.words = mask_words;
     c.view.q = args->q;
     c.view.out = args->out;
     c.view.ldq = ldq;
@@ -443,6 +451,38 @@ int32_t nf4_cache_attention_dev(const nf4_cache *cache, const nf4_cache_batch *b
         return takes_decode(c) ? attention_decode(c, workspace, s) : attention_chunk(c, workspace, s);
     }
     return c.head_dim == 64 ? launch_of<64>(c, p, s) : c.head_dim == 128 ? launch_of<128>(c, p, s) : launch_of<256>(c, p, s);
+}
+
+}  // namespace
+
+}  // namespace nf4
+
+using namespace nf4;
+
+extern "C" {
+
+uint64_t nf4_cache_attention_flag_bytes(void) { return kAttentionFlagBytes; }
+
+uint64_t nf4_cache_attention_call_flag_bytes(const nf4_cache *cache, const nf4_cache_batch *batch, uint32_t q_heads, int32_t io_dtype) {
+    return call_flag_bytes("nf4_cache_attention_call_flag_bytes", cache, batch, q_heads, io_dtype, false);
+}
+uint64_t nf4_cache_tree_attention_call_flag_bytes(const nf4_cache *cache, const nf4_cache_batch *batch, uint32_t q_heads, int32_t io_dtype) {
+    return call_flag_bytes("nf4_cache_tree_attention_call_flag_bytes", cache, batch, q_heads, io_dtype, true);
+}
+
+uint64_t nf4_cache_attention_workspace_bytes(const nf4_cache *cache, const nf4_cache_batch *batch, uint32_t q_heads, int32_t io_dtype) {
+    return workspace_bytes("nf4_cache_attention_workspace_bytes", cache, batch, q_heads, io_dtype, false);
+}
+uint64_t nf4_cache_tree_attention_workspace_bytes(const nf4_cache *cache, const nf4_cache_batch *batch, uint32_t q_heads, int32_t io_dtype) {
+    return workspace_bytes("nf4_cache_tree_attention_workspace_bytes", cache, batch, q_heads, io_dtype, true);
+}
+
+int32_t nf4_cache_attention_dev(const nf4_cache *cache, const nf4_cache_batch *batch, const nf4_attention_args *args, void *stream) {
+    return attention("nf4_cache_attention_dev", cache, batch, nullptr, 0, false, args, stream);
+}
+int32_t nf4_cache_tree_attention_dev(const nf4_cache *cache, const nf4_cache_batch *batch, const uint32_t *masks, uint32_t mask_words,
+                                     const nf4_attention_args *args, void *stream) {
+    return attention("nf4_cache_tree_attention_dev", cache, batch, masks, mask_words, true, args, stream);
 }
 
 }  // extern "C"

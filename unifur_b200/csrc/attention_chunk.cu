@@ -40,24 +40,27 @@ constexpr float kRaise = NF4 ? 7.f : -8.f;
 template <bool NF4>
 constexpr float kLower = NF4 ? 1.f / 32768.f : 1.f;
 constexpr uint32_t kGroup = 16;  // tokens that are in one page for sure
-// warps 0-3 and 4-7: softmax of a tile; 8-11: codes to f16; 12: copies; 13: MMAs
-constexpr uint32_t kExpandWarp = 8, kCopyWarp = 12, kMmaWarp = 13;
-// Registers: 512 threads are launched with 128 each; the two softmax warpgroups take 160 and leave 96 to the other two (together the
-// same 65536).
-constexpr uint32_t kSoftmaxRegs = 160, kOtherRegs = 96;
+// warps 0-3 and 4-7: softmax of a tile; 8-11: codes to f16 (trees: 4-11); 12: copies; 13: MMAs
+constexpr uint32_t kCopyWarp = 12, kMmaWarp = 13;
 
-template <int D, bool NF4>
+// TREE: rows are nodes of trees, which see their sequence's tokens ahead of the nodes and those nodes that their masks have.  A tree has few rows, mostly
+// one MMA tile of a head.
+template <int D, bool NF4, bool TREE>
 struct Shape {
-    static constexpr uint32_t kTiles = D == 256 ? 1 : 2, kRows = 128 * kTiles;
+    static constexpr uint32_t kTiles = D == 256 || TREE ? 1 : 2, kRows = 128 * kTiles;
     static constexpr uint32_t kTokens = D == 256 ? 64 : 128;          // of a step
-    // S's places to a tile: with a dim of 256 there is room for two, so that the next step's scores come while weights are made
-    static constexpr uint32_t kPlaces = D == 256 ? 2 : 1;
+    // S's places to a tile: with one tile there is room for two, so that the next step's scores come while weights are made
+    static constexpr uint32_t kPlaces = kTiles == 1 ? 2 : 1;
+    static constexpr uint32_t kSoftmaxWarps = TREE ? 4 : 8, kExpandWarp = TREE && NF4 ? 4 : 8, kExpandWarps = kCopyWarp - kExpandWarp;
+    // Registers: 512 threads are launched with 128 each; the two softmax warpgroups take 160 and leave 96 to the other two (together the
+    // same 65536), or one takes 200 and leaves 104 to three.
+    static constexpr uint32_t kSoftmaxRegs = TREE ? 200 : 160, kOtherRegs = TREE ? 104 : 96;
     static constexpr uint32_t kBlocks = D / 64;
     static constexpr uint32_t kQTile = 128 * D * 2, kTile = kTokens * D * 2, kBox = kTokens * 128;
     static constexpr uint32_t kScales = kTokens * kBlocks * 4;
     // a tile's codes and scales, and with K's the V's scales of the step: their power goes to the softmax ahead of V
     static constexpr uint32_t kRaw = NF4 ? kTokens * D / 2 + 2 * kScales : 0, kRawSlots = D == 64 ? 5 : 2;
-    static constexpr uint32_t kSlots = D == 64 ? (NF4 ? 6 : 7) : NF4 ? 3 : 5;  // of the ring; one more where the table is not needed
+    static constexpr uint32_t kSlots = D == 64 ? (NF4 && !TREE ? 6 : 7) : (NF4 ? 3 : 5) + (D == 128 && TREE ? 1 : 0);  // of the ring; one more where the table is not needed
     // codes, then the table on a multiple of its 32 KB, then Q, then the ring (bf16: Q, then the ring)
     static constexpr uint32_t kSmem = (NF4 ? 65536 : 2048) - 1024 + kTiles * kQTile + kSlots * kTile;
     static constexpr uint32_t kS = 0, kO = 256;                       // columns of tensor memory: the tiles' S's, then O's
@@ -166,7 +169,7 @@ struct Piece {
 // a prompt's first tiles, of one step each, would be done last.
 constexpr uint32_t kStart = 4;
 
-template <uint32_t R, uint32_t N>
+template <uint32_t R, uint32_t N, bool TREE>
 struct Walker {  // through a CTA's pieces; every warp goes its own way
     Sequence s;
     uint32_t seq, head, tile, off, now, end;
@@ -175,7 +178,7 @@ struct Walker {  // through a CTA's pieces; every warp goes its own way
     // (a tile that sees nothing has one step all the same: its results are zeros)
     static __device__ __forceinline__ uint32_t steps_of(const Sequence &s, const AttentionView &a, uint32_t tile) {
         const uint32_t last = (uint32_t)min((uint64_t)(tile + 1) * R, (uint64_t)s.rows * a.group) - 1;
-        return max(1u, (visible_end(s, a.by_group, last) + N - 1) / N);
+        return max(1u, (seen_end<TREE>(s, a.by_group, last) + N - 1) / N);
     }
     __device__ __forceinline__ bool next(const CacheView &c, const BatchView &b, const AttentionView &a, Piece &p) {
         do {
@@ -252,12 +255,13 @@ struct Turn {
     }
 };
 
-template <int D, bool NF4>
+template <int D, bool NF4, bool TREE>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const CacheView c, const BatchView b,
                        const AttentionView a, const Dense dense, uint32_t box_rows, Split *const splits, const FailureRef failure) {
-    using S = Shape<D, NF4>;
-    using Walk = Walker<S::kRows, S::kTokens>;
+    using S = Shape<D, NF4, TREE>;
+    using Walk = Walker<S::kRows, S::kTokens, TREE>;
+    constexpr uint32_t kExpandWarp = S::kExpandWarp, kExpandWarps = S::kExpandWarps, kSoftmaxRegs = S::kSoftmaxRegs, kOtherRegs = S::kOtherRegs;
     // A bf16 cache's pages may be of sixteen tokens, and a warp asks for boxes one after another: four warps share the asking, a tile's
     // columns between two of them (with one, 137 cycles to a box of 2 KB, the MMAs waited for copies)
     constexpr uint32_t kCopies = !NF4 && D >= 128 ? 2 : 1;
@@ -288,12 +292,12 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     if (tid == 0) {
         static_assert(S::kSlots + 1 <= 8);
         for (uint32_t i = 0; i < 8; ++i) {  // (a place more than kSlots may be in use)
-            ptx::mbar_init(full0 + 8 * i, NF4 ? 4 : kCopies);
+            ptx::mbar_init(full0 + 8 * i, NF4 ? kExpandWarps : kCopies);
             ptx::mbar_init(empty0 + 8 * i, 1);
         }
         for (uint32_t i = 0; i < S::kRawSlots; ++i) {
             ptx::mbar_init(raw_full0 + 8 * i, 1);
-            ptx::mbar_init(raw_empty0 + 8 * i, 4);
+            ptx::mbar_init(raw_empty0 + 8 * i, kExpandWarps);
         }
         for (uint32_t i = 0; i < 4; ++i) {
             ptx::mbar_init(s_full0 + 8 * i, 1);
@@ -422,7 +426,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     if (s_first[4] < s_first[5]) {
         Walk walk{sequence_of(c, b, s_first[0]), s_first[0], s_first[1], s_first[2], s_first[3], s_first[4], s_first[5]};
         Piece p;
-        if (warp < 8) {
+        if (warp < S::kSoftmaxWarps) {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
             const uint32_t tile = warp >> 2, r = tid & 127u;
             const uint32_t lanes = (warp & 3u) << 21;  // a warp reaches its quarter of tensor memory's lanes
@@ -478,8 +482,13 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                 // ---- the steps ----
                 const uint32_t row = p.r0 + tile * 128 + r, t_first = p.step0 * N;
                 const bool real = tile * 128 + r < p.rows;
-                const uint32_t sees = real ? visible_end(p.s, a.by_group, row) : 0u, sees_first = visible_end(p.s, a.by_group, p.r0 + tile * 128);
-                const uint32_t steps = p.steps;
+                const uint32_t token = a.by_group.of(real ? row : p.r0);
+                const int32_t nodes0 = first_node(p.s);
+                const bool blind = !real || (TREE && nodes0 + (int32_t)token < 0);  // a row that sees nothing
+                const uint32_t sees = blind ? 0u : seen_end<TREE>(p.s, a.by_group, row);
+                const uint32_t sees_first = TREE ? (uint32_t)max(nodes0, 0) : visible_end(p.s, a.by_group, p.r0 + tile * 128);
+                const bool idle = TREE && (warp & 3u) * 32 >= p.rows;  // none of the warp's rows is one: its part of S is never looked at
+                const uint32_t steps = p.steps, p_row = p.s.row0 + token;
                 const float row_factor = fabsf(a.scale_log2) * (NF4 ? s_qpower[tile * 128 + r] : 1.f);
                 float m = -INFINITY, l = 0.f, ref = 0.f;
                 for (uint32_t j = 0; j < steps; ++j, ++scores) {
@@ -488,6 +497,10 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                         ok = false;
                         if (lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 23);
                         break;
+                    }
+                    if (idle) {
+                        if (lane == 0) ptx::mbar_arrive(p_ready0 + 8 * place);
+                        continue;
                     }
                     ptx::tc_fence_after();
                     const uint32_t t0 = t_first + j * N, lim = sees > t0 ? sees - t0 : 0u;
@@ -517,8 +530,10 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                             ptx::tmem_wait_ld();
                             if (k + 32 < N) tmem_ld32(ts + k + 32, ahead[k / 32 + 1 & 1]);
                             if (masked) {
+                                uint32_t seen = 0;
+                                if (TREE) seen = seen_nodes(a, p_row, (int32_t)(t0 + k) - nodes0) & low_bits(lim > k ? lim - k : 0u);
                                 #pragma unroll
-                                for (uint32_t i = 0; i < 32; ++i) x[i] = k + i < lim ? x[i] : 0xff800000u;
+                                for (uint32_t i = 0; i < 32; ++i) x[i] = (TREE ? seen >> i & 1u : k + i < lim) ? x[i] : 0xff800000u;
                             }
                             #pragma unroll
                             for (uint32_t i = 0; i < 32; i += 2) {
@@ -638,9 +653,9 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             }
         } else {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-            if (NF4 && !expanded && warp >= kExpandWarp && warp < kExpandWarp + 4) {
+            if (NF4 && !expanded && warp >= kExpandWarp && warp < kExpandWarp + kExpandWarps) {
                 // ---- codes to f16: a thread has 16 bytes of a token's row, 32 values ----
-                constexpr uint32_t kLanes = D / 32, kPass = 128 / kLanes;
+                constexpr uint32_t kLanes = D / 32, kPass = 32 * kExpandWarps / kLanes;
                 const uint32_t th = tid - 32 * kExpandWarp, q = th % kLanes, lane_word = table | lane * 4u;
                 // In which order a thread takes its four words: so that eight lanes' 16-byte stores hit all banks
                 const uint32_t order = D == 128 ? (q >> 1) * 2 : D == 256 ? q >> 1 : 0u;
@@ -653,7 +668,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                     }
                 };
                 for (; ok && walk.next(c, b, a, p); step += p.steps) {
-                    const uint32_t t_end = min(visible_end(p.s, a.by_group, p.r0 + p.rows - 1), (p.step0 + p.steps) * N);
+                    const uint32_t t_end = min(seen_end<TREE>(p.s, a.by_group, p.r0 + p.rows - 1), (p.step0 + p.steps) * N);
                     #pragma unroll 1
                     for (uint32_t turn = 0; ok && turn < 2 * p.steps; ++turn, ++i, ring.on(slots)) {
                         const Turn<kPlaces> of(turn, p.steps);
@@ -721,7 +736,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                         }
                     }
                 }
-            } else if (NF4 ? warp == kCopyWarp : warp < kExpandWarp + 2 * kCopies) {
+            } else if (NF4 ? warp == kCopyWarp : warp >= kExpandWarp && warp < kExpandWarp + 2 * kCopies) {
                 const uint32_t own = NF4 ? 0u : (warp - kExpandWarp) & 1u, part = NF4 ? 0u : (warp - kExpandWarp) >> 1;  // bf16: K or V, and which columns
                 const uint32_t unit = NF4 ? kGroup : box_rows, units = N / unit;  // tokens that come together, being in one page
                 uint32_t i = 0, tails = 0, step = 0;
@@ -767,7 +782,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                                 const int32_t row = (int32_t)(((tile0 + j) * c.heads + p.head) * N);
                                 #pragma unroll
                                 for (uint32_t x = 0; x < D / 64; ++x) ptx::tma_load_2d(dst + x * S::kBox, which ? &tmap_v : &tmap_k, (int32_t)(64 * x), row, bar);
-                                for (int e = 0; e < 3; ++e) ptx::mbar_arrive(bar);  // (for the four warps that expand)
+                                for (uint32_t e = 1; e < kExpandWarps; ++e) ptx::mbar_arrive(bar);  // (for the warps that expand)
                             }
                         } else if (NF4) {
                             const uint32_t bar = raw_full0 + 8 * rs, raw = raw0 + rs * S::kRaw;
@@ -908,7 +923,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
 template <int D>
 __global__ void __launch_bounds__(256)
 expand_kernel(const CacheView c, const BatchView b, uint4 *const k_out, uint4 *const v_out, uint32_t *const bases, float2 *const powers) {
-    constexpr uint32_t N = Shape<D, true>::kTokens, kBlocks = D / 64, kGroups = D / 8;  // eight values each
+    constexpr uint32_t N = Shape<D, true, false>::kTokens, kBlocks = D / 64, kGroups = D / 8;  // eight values each
     __shared__ uint32_t s_pairs[256], s_most[2], s_place[N], s_bad;
     const uint32_t tid = threadIdx.x, lane = tid & 31u;
     s_pairs[tid] = level_pair_f16(tid);
@@ -990,10 +1005,10 @@ expand_kernel(const CacheView c, const BatchView b, uint4 *const k_out, uint4 *c
 
 // The row tiles that several CTAs had: a warp to four rows at a time, the parts in the order of the tokens.
 constexpr uint32_t kJoinRows = 4, kJoinWarps = 8;
-template <int D, bool NF4>
+template <int D, uint32_t kRows>
 __global__ void __launch_bounds__(32 * kJoinWarps)
 join_pieces_kernel(const AttentionView a, const Split *const splits) {
-    constexpr uint32_t kRows = Shape<D, NF4>::kRows, kWide = D / 32;  // values of a row to a lane
+    constexpr uint32_t kWide = D / 32;  // values of a row to a lane
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
     const Split s = splits[blockIdx.x];
@@ -1040,7 +1055,7 @@ join_pieces_kernel(const AttentionView a, const Split *const splits) {
     }
 }
 
-uint64_t rows_of(const AttentionCall &c) { return c.head_dim == 256 ? 128 : 256; }
+uint64_t rows_of(const AttentionCall &c) { return c.head_dim == 256 || c.tree ? 128 : 256; }
 uint64_t tokens_of(const AttentionCall &c) { return c.head_dim == 256 ? 64 : 128; }
 
 // Tiles to a head to be expanded ahead: where the host's bounds say that three row tiles or more of a head go over most tokens (with two
@@ -1072,10 +1087,10 @@ struct Layout {  // of the workspace
     }
 };
 
-template <int D, bool NF4>
+template <int D, bool NF4, bool TREE>
 int32_t launch(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) {
-    using S = Shape<D, NF4>;
-    auto kernel = attention_chunk_kernel<D, NF4>;
+    using S = Shape<D, NF4, TREE>;
+    auto kernel = attention_chunk_kernel<D, NF4, TREE>;
     NF4_TRY(ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), S::kSmem));
     const uint64_t pool = (uint64_t)c.cache.pages * c.cache.heads * c.cache.page_size;
     CUtensorMap map_k{}, map_v{};
@@ -1111,8 +1126,16 @@ int32_t launch(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) 
     const uint32_t ctas = persistent_ctas();
     count_launch(2);
     NF4_TRY(launch_maybe_overlapped(kernel, dim3(ctas), dim3(kThreads), S::kSmem, stream, true, map_k, map_v, c.cache, c.batch, view, dense, box_rows, splits, failure));
-    return launch_maybe_overlapped(join_pieces_kernel<D, NF4>, dim3(ctas, S::kRows / (kJoinRows * kJoinWarps)), dim3(32 * kJoinWarps), 0, stream, true, view,
+    return launch_maybe_overlapped(join_pieces_kernel<D, S::kRows>, dim3(ctas, S::kRows / (kJoinRows * kJoinWarps)), dim3(32 * kJoinWarps), 0, stream, true, view,
                                    static_cast<const Split *>(splits));
+}
+template <bool TREE>
+int32_t launch_of(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) {
+    switch (c.head_dim) {
+        case 64: return c.nf4 ? launch<64, true, TREE>(c, workspace, stream) : launch<64, false, TREE>(c, workspace, stream);
+        case 128: return c.nf4 ? launch<128, true, TREE>(c, workspace, stream) : launch<128, false, TREE>(c, workspace, stream);
+        default: return c.nf4 ? launch<256, true, TREE>(c, workspace, stream) : launch<256, false, TREE>(c, workspace, stream);
+    }
 }
 
 }  // namespace
@@ -1129,11 +1152,7 @@ bool attention_chunk_counts(const AttentionCall &c) {
 }
 
 int32_t attention_chunk(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) {
-    switch (c.head_dim) {
-        case 64: return c.nf4 ? launch<64, true>(c, workspace, stream) : launch<64, false>(c, workspace, stream);
-        case 128: return c.nf4 ? launch<128, true>(c, workspace, stream) : launch<128, false>(c, workspace, stream);
-        default: return c.nf4 ? launch<256, true>(c, workspace, stream) : launch<256, false>(c, workspace, stream);
-    }
+    return c.tree ? launch_of<true>(c, workspace, stream) : launch_of<false>(c, workspace, stream);
 }
 
 }  // namespace nf4

@@ -132,7 +132,8 @@ __device__ __forceinline__ Line line_of(const CacheView &c, const BatchView &b, 
     return l;
 }
 
-template <int D, bool NF4, int NT>
+// TREE: rows are nodes of trees, which see their sequence's tokens ahead of the nodes and those nodes that their masks have
+template <int D, bool NF4, int NT, bool TREE>
 __global__ void __launch_bounds__(Shape<D, NF4, NT>::kThreads, 1)
 attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const CacheView c, const BatchView b,
                         const AttentionView a, uint32_t *const counters, float *const parts, const FailureRef failure) {
@@ -317,7 +318,7 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
         const uint64_t item_first = now - off;
         const uint32_t r0 = tile * S::kRows, rows = min((uint64_t)S::kRows, (uint64_t)s.rows * a.group - r0);
         // the first token that is not this share's, or that none of the tile's rows sees
-        const uint32_t limit = min(visible_end(s, a.by_group, r0 + rows - 1), (off + n) * kUnit);
+        const uint32_t limit = min(seen_end<TREE>(s, a.by_group, r0 + rows - 1), (off + n) * kUnit);
         const uint32_t here = limit > off * kUnit ? (limit - off * kUnit + kUnit - 1) / kUnit : 0u;  // units with tokens
         const uint32_t mine = warp < here ? (here - warp + W - 1) / W : 0u;
 
@@ -396,8 +397,9 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
 
         // ---- the queries as the first product's B operand ----
         float factor[NT][2];       // of columns 2 t4 and 2 t4 + 1: scale, log2(e), and the power of two the row was divided by
-        uint32_t sees[NT][2];
-        const uint32_t sees_first = min(visible_end(s, a.by_group, r0), limit);
+        uint32_t sees[NT][2];      // the first token that the columns' rows do not see; TREE: the rows' numbers, kBlind where they see nothing
+        constexpr uint32_t kBlind = 0xffffffffu;
+        const uint32_t sees_first = min(TREE ? (uint32_t)max(first_node(s), 0) : visible_end(s, a.by_group, r0), limit);
         #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float f = a.scale_log2;
@@ -424,7 +426,12 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
             for (int j = 0; j < 2; ++j) {
                 factor[nt][j] = __shfl_sync(0xffffffffu, f, 4 * (2 * t4 + j));
                 const uint32_t col = 8 * nt + 2 * t4 + j;
-                sees[nt][j] = col < rows ? min(visible_end(s, a.by_group, r0 + col), limit) : limit;
+                if (TREE) {
+                    const uint32_t token = a.by_group.of(r0 + min(col, rows - 1));
+                    sees[nt][j] = col < rows && first_node(s) + (int32_t)token >= 0 ? s.row0 + token : kBlind;
+                } else {
+                    sees[nt][j] = col < rows ? min(visible_end(s, a.by_group, r0 + col), limit) : limit;
+                }
             }
         }
 
@@ -516,6 +523,14 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
                     for (int e = 0; e < 4; ++e) x[u][nt][e] *= factor[nt][e & 1];
             }
             if (t0 + G * kGroup > sees_first) {  // some row does not see all of it
+                uint32_t window[NT][2];  // TREE: bit i: the column's row sees token t0 + i
+                if (TREE) {
+                    #pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        #pragma unroll
+                        for (int j = 0; j < 2; ++j)
+                            window[nt][j] = sees[nt][j] == kBlind ? 0u : seen_nodes(a, sees[nt][j], (int32_t)t0 - first_node(s)) & low_bits(limit - t0);
+                }
                 #pragma unroll
                 for (uint32_t u = 0; u < G; ++u) {
                     const uint32_t tok = t0 + u * kGroup + (NF4 ? krow : g);
@@ -524,7 +539,10 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
                         #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
                             #pragma unroll
-                            for (int j = 0; j < 2; ++j) x[u][nt][2 * h + j] = tok + 8 * h < sees[nt][j] ? x[u][nt][2 * h + j] : -INFINITY;
+                            for (int j = 0; j < 2; ++j) {
+                                const bool seen = TREE ? window[nt][j] >> (tok + 8 * h - t0) & 1u : tok + 8 * h < sees[nt][j];
+                                x[u][nt][2 * h + j] = seen ? x[u][nt][2 * h + j] : -INFINITY;
+                            }
                         #pragma unroll
                         for (uint32_t kb = 0; NF4 && kb < kBlocks; ++kb) vs[u][h][kb] = tok + 8 * h < limit ? vs[u][h][kb] : 0.f;  // (anything may stand there)
                     }
@@ -792,11 +810,11 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     if (!ok) ptx::let_flights_land();
 }
 
-template <int D, bool NF4, int NT>
+template <int D, bool NF4, int NT, bool TREE>
 int32_t launch(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) {
     using S = Shape<D, NF4, NT>;
     static_assert(kNumSMs * 4 <= kAttentionFlagBytes);
-    auto kernel = attention_decode_kernel<D, NF4, NT>;
+    auto kernel = attention_decode_kernel<D, NF4, NT, TREE>;
     NF4_TRY(ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), S::kSmem));
     const uint64_t rows = (uint64_t)c.cache.pages * c.cache.heads * c.cache.page_size;
     CUtensorMap map_k, map_v;
@@ -815,12 +833,12 @@ int32_t launch(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) 
                                    reinterpret_cast<uint32_t *>(workspace), reinterpret_cast<float *>(workspace + kAttentionFlagBytes), failure);
 }
 
-template <int NT>
+template <int NT, bool TREE>
 int32_t launch_of(const AttentionCall &c, uint8_t *ws, cudaStream_t s) {
     switch (c.head_dim) {
-        case 64: return c.nf4 ? launch<64, true, NT>(c, ws, s) : launch<64, false, NT>(c, ws, s);
-        case 128: return c.nf4 ? launch<128, true, NT>(c, ws, s) : launch<128, false, NT>(c, ws, s);
-        default: return c.nf4 ? launch<256, true, NT>(c, ws, s) : launch<256, false, NT>(c, ws, s);
+        case 64: return c.nf4 ? launch<64, true, NT, TREE>(c, ws, s) : launch<64, false, NT, TREE>(c, ws, s);
+        case 128: return c.nf4 ? launch<128, true, NT, TREE>(c, ws, s) : launch<128, false, NT, TREE>(c, ws, s);
+        default: return c.nf4 ? launch<256, true, NT, TREE>(c, ws, s) : launch<256, false, NT, TREE>(c, ws, s);
     }
 }
 
@@ -834,7 +852,8 @@ uint64_t attention_decode_bytes(const AttentionCall &c) {
 }
 
 int32_t attention_decode(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) {
-    return one_tile(c) ? launch_of<1>(c, workspace, stream) : launch_of<2>(c, workspace, stream);
+    if (c.tree) return one_tile(c) ? launch_of<1, true>(c, workspace, stream) : launch_of<2, true>(c, workspace, stream);
+    return one_tile(c) ? launch_of<1, false>(c, workspace, stream) : launch_of<2, false>(c, workspace, stream);
 }
 
 }  // namespace nf4

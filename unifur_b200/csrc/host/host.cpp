@@ -666,11 +666,105 @@ PyObject *cache_read(PyObject *, PyObject *const *v, Py_ssize_t n) {
     });
 }
 
-// cache_attention(<cache, batch>, q, scale, out or None) -> out
-PyObject *cache_attention(PyObject *, PyObject *const *v, Py_ssize_t n) {
+// An int32 tensor of the call that kernels read or write as it lies.
+int32_t *words_of(const Tensor &t, const CacheCall &c, at::IntArrayRef shape, const char *what) {
+    if (t.scalar_type() != at::kInt || t.sizes() != shape || !t.is_contiguous()) raise(PyExc_ValueError, (std::string(what) + " is contiguous int32 of the batch's shape").c_str());
+    if (t.device() != c.k->device()) raise(PyExc_ValueError, (std::string(what) + " must be on the cache's device").c_str());
+    return t.numel() ? static_cast<int32_t *>(t.mutable_data_ptr()) : nullptr;
+}
+
+// cache_append_rotated(<cache, batch>, k, v, table, pairs, positions or None, q or None, out or None) -> q rotated, or None
+PyObject *cache_append_rotated(PyObject *, PyObject *const *v, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        expect(n, kCacheArgs + 7);
+        const CacheCall c = cache_call(v);
+        PyObject *const *const own = v + kCacheArgs;
+        const Tensor &k = tensor(own[0]), &vv = tensor(own[1]), &table = tensor(own[2]);
+        const Tensor *positions = tensor_or_none(own[4]), *q = tensor_or_none(own[5]), *given = tensor_or_none(own[6]);
+        require(k.scalar_type() == vv.scalar_type() && (!q || q->scalar_type() == k.scalar_type()), "k, v and q must be of one type");
+        require(table.dim() == 2 && table.scalar_type() == at::kFloat && table.is_contiguous(), "the rotation's table is contiguous f32 [positions, rotary_dim]");
+        require(table.device() == c.k->device(), "the rotation's table must be on the cache's device");
+        require(table.size(0) < 1ll << 31 && table.size(1) < 1ll << 31, "the rotation's table is too large");
+        require(q || !given, "out without q");
+        const int32_t type = io_dtype(k.scalar_type());
+        Place place(c.k->device());
+        nf4_rotation r;
+        std::memset(&r, 0, sizeof(r));
+        r.struct_bytes = sizeof(r);
+        r.rotary_dim = (uint32_t)table.size(1);
+        r.pairs = PyObject_IsTrue(own[3]) == 1;
+        r.table_positions = (uint32_t)table.size(0);
+        r.table = ptr_as<float>(&table);
+        if (positions) r.positions = words_of(*positions, c, {(int64_t)c.batch.rows}, "positions");
+        const HeadRows rk = head_rows(k, c, c.cache.heads, "k", false), rv = head_rows(vv, c, c.cache.heads, "v", false);
+        const void *pk = rk.t.const_data_ptr(), *pv = rv.t.const_data_ptr(), *pq = nullptr;
+        HeadRows rq{Tensor(), 0, 0};
+        Tensor out;
+        uint64_t ldo = 0;
+        void *po = nullptr;
+        if (q) {
+            rq = head_rows(*q, c, 0, "q", false);
+            pq = rq.t.const_data_ptr();
+            out = given ? *given : empty(q->sizes(), q->scalar_type(), place);
+            require(out.scalar_type() == q->scalar_type() && out.sizes() == q->sizes(), "out must have q's shape and type");
+            ldo = head_rows(out, c, rq.heads, "out", true).ld;
+            po = out.mutable_data_ptr();
+        }
+        check(unlocked([&] {
+            return nf4_cache_append_rotated_dev(&c.cache, &c.batch, &r, pk, rk.ld, pv, rv.ld, pq, rq.ld, rq.heads, po, ldo, type, place.stream);
+        }));
+        if (!q) Py_RETURN_NONE;
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
+// cache_tree(<cache, batch>, parents, masks, positions)
+PyObject *cache_tree(PyObject *, PyObject *const *v, Py_ssize_t n) {
     return guarded([&]() -> PyObject * {
         expect(n, kCacheArgs + 3);
         const CacheCall c = cache_call(v);
+        const Tensor &masks = tensor(v[kCacheArgs + 1]);
+        const int64_t rows = c.batch.rows;
+        const int32_t *parents = words_of(tensor(v[kCacheArgs]), c, {rows}, "parents");
+        require(masks.dim() == 2 && masks.size(1) < 1ll << 31, "masks is [rows, words]");
+        uint32_t *m = reinterpret_cast<uint32_t *>(words_of(masks, c, {rows, masks.size(1)}, "masks"));
+        int32_t *p = words_of(tensor(v[kCacheArgs + 2]), c, {rows}, "positions");
+        Place place(c.k->device());
+        check(unlocked([&] { return nf4_cache_tree_dev(&c.cache, &c.batch, parents, m, (uint32_t)masks.size(1), p, place.stream); }));
+        Py_RETURN_NONE;
+    });
+}
+
+// cache_keep(<cache, batch>, kept, counts, lengths)
+PyObject *cache_keep(PyObject *, PyObject *const *v, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        expect(n, kCacheArgs + 3);
+        const CacheCall c = cache_call(v);
+        const Tensor &kept = tensor(v[kCacheArgs]);
+        const int64_t sequences = c.batch.sequences;
+        require(kept.dim() == 2 && kept.size(1) < 1ll << 31, "kept is [sequences, nodes]");
+        const int32_t *path = words_of(kept, c, {sequences, kept.size(1)}, "kept"), *counts = words_of(tensor(v[kCacheArgs + 1]), c, {sequences}, "counts");
+        int32_t *lengths = words_of(tensor(v[kCacheArgs + 2]), c, {sequences}, "out");
+        Place place(c.k->device());
+        check(unlocked([&] { return nf4_cache_keep_dev(&c.cache, &c.batch, path, (uint32_t)kept.size(1), counts, lengths, place.stream); }));
+        Py_RETURN_NONE;
+    });
+}
+
+// cache_attention(<cache, batch>, q, scale, out or None[, masks]) -> out; with masks the rows are nodes of trees
+PyObject *cache_attention(PyObject *, PyObject *const *v, Py_ssize_t n) {
+    return guarded([&]() -> PyObject * {
+        const bool tree = n == kCacheArgs + 4;
+        if (!tree) expect(n, kCacheArgs + 3);
+        const CacheCall c = cache_call(v);
+        const uint32_t *masks = nullptr;
+        uint32_t words = 0;
+        if (tree) {
+            const Tensor &m = tensor(v[kCacheArgs + 3]);
+            require(m.dim() == 2 && m.size(1) < 1ll << 31, "masks is [rows, words]");
+            masks = reinterpret_cast<const uint32_t *>(words_of(m, c, {(int64_t)c.batch.rows, m.size(1)}, "masks"));
+            words = (uint32_t)m.size(1);
+        }
         const Tensor &q = tensor(v[kCacheArgs]);
         const Tensor *given = tensor_or_none(v[kCacheArgs + 2]);
         nf4_attention_args a;
@@ -687,15 +781,19 @@ PyObject *cache_attention(PyObject *, PyObject *const *v, Py_ssize_t n) {
         a.ldq = rq.ld;
         a.ldo = head_rows(out, c, rq.heads, "out", true).ld;
         a.out = out.mutable_data_ptr();
-        const uint64_t bytes = nf4_cache_attention_workspace_bytes(&c.cache, &c.batch, a.q_heads, a.io_dtype);
+        const uint64_t bytes = tree ? nf4_cache_tree_attention_workspace_bytes(&c.cache, &c.batch, a.q_heads, a.io_dtype)
+                                    : nf4_cache_attention_workspace_bytes(&c.cache, &c.batch, a.q_heads, a.io_dtype);
         Tensor ws;
         if (bytes) {  // (0: arguments that the call refuses)
-            const uint64_t flags = nf4_cache_attention_call_flag_bytes(&c.cache, &c.batch, a.q_heads, a.io_dtype);
+            const uint64_t flags = tree ? nf4_cache_tree_attention_call_flag_bytes(&c.cache, &c.batch, a.q_heads, a.io_dtype)
+                                        : nf4_cache_attention_call_flag_bytes(&c.cache, &c.batch, a.q_heads, a.io_dtype);
             ws = flags ? flagged_workspace(bytes, place, kAttentionSlot, flags) : empty({(int64_t)bytes}, at::kByte, place);
             a.workspace = ws.mutable_data_ptr();
             a.workspace_bytes = (uint64_t)ws.numel();
         }
-        check(unlocked([&] { return nf4_cache_attention_dev(&c.cache, &c.batch, &a, place.stream); }));
+        check(unlocked([&] {
+            return tree ? nf4_cache_tree_attention_dev(&c.cache, &c.batch, masks, words, &a, place.stream) : nf4_cache_attention_dev(&c.cache, &c.batch, &a, place.stream);
+        }));
         return THPVariable_Wrap(std::move(out));
     });
 }
@@ -711,7 +809,7 @@ PyMethodDef kMethods[] = {
     FAST(linear_forward), FAST(linear_forward_grouped), FAST(qlora_backward), FAST(quantize), FAST(quantize_transposed),
     FAST(quantize_transposed_double),
     FAST(double_quantize), FAST(dequantize), FAST(quantize_dequantize), FAST(embedding),
-    FAST(cache_append), FAST(cache_read), FAST(cache_attention),
+    FAST(cache_append), FAST(cache_append_rotated), FAST(cache_read), FAST(cache_attention), FAST(cache_tree), FAST(cache_keep),
     {"release_workspaces", release_workspaces, METH_NOARGS, "Give the calling thread's kept workspaces back."},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

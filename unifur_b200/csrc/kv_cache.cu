@@ -74,45 +74,18 @@ struct Move {
 };
 
 // Where a CTA's rows have their token in the cache, for head 0 and counted in rows of a head.
-constexpr int64_t kNowhere = -1, kNoRow = -2;  // in no page; the row belongs to no sequence
 struct Places {
     int32_t starts[kStarts];
     int64_t of[kMostRows];
 };
-
-__device__ __forceinline__ int64_t place_of(const CacheView &c, const BatchView &b, const Places &p, uint32_t step, uint32_t row) {
-    // the first sequence that starts behind the row: among the starts that are held, then among those between two of them
-    uint32_t low = 0, high = (b.sequences + step - 1) / step;
-    while (low < high) {
-        const uint32_t mid = (low + high) / 2;
-        if (p.starts[mid] <= (int32_t)row) low = mid + 1;
-        else high = mid;
-    }
-    if (low == 0) return kNoRow;
-    high = min(low * step, b.sequences);
-    low = (low - 1) * step + 1;
-    while (low < high) {
-        const uint32_t mid = (low + high) / 2;
-        if (__ldg(b.starts + mid) <= (int32_t)row) low = mid + 1;
-        else high = mid;
-    }
-    const uint32_t s = low - 1;
-    const Sequence q = sequence_of(c, b, s);
-    if (row - q.row0 >= q.rows) return kNoRow;
-    const int64_t token = (int64_t)q.length - q.rows + (row - q.row0);
-    if (token < 0) return kNowhere;
-    const uint32_t at = c.by_page.of((uint32_t)token);
-    const int32_t page = __ldg(b.table + (uint64_t)s * b.width + at);
-    if (page < 0 || (uint32_t)page >= c.pages) return kNowhere;
-    return (int64_t)page * c.heads * c.page_size + ((uint32_t)token - at * c.page_size);
-}
 
 // The whole CTA finds its rows' places, once for all of a row's groups.
 __device__ __forceinline__ void find_places(const CacheView &c, const BatchView &b, const Move &m, uint32_t row0, Places &p) {
     const uint32_t tid = threadIdx.x, step = (b.sequences + kStarts - 1) / kStarts;
     for (uint32_t i = tid; i * step < b.sequences; i += kThreads) p.starts[i] = __ldg(b.starts + i * step);
     __syncthreads();
-    if (tid < m.rows()) p.of[tid] = row0 + tid < b.rows ? place_of(c, b, p, step, row0 + tid) : kNoRow;
+    int64_t token;
+    if (tid < m.rows()) p.of[tid] = row0 + tid < b.rows ? place_of_row(c, b, p.starts, step, row0 + tid, token) : kNoRow;
     __syncthreads();
 }
 

@@ -67,6 +67,35 @@ __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// The token of a call's row, and where the cache has it (for head 0, counted in rows of a head).  The first sequence that starts behind
+// the row is looked for among `held` of the batch's starts, every step-th, then among those between two of them.
+constexpr int64_t kNowhere = -1, kNoRow = -2;  // in no page; the row belongs to no sequence
+__device__ __forceinline__ int64_t place_of_row(const CacheView &c, const BatchView &b, const int32_t *held, uint32_t step, uint32_t row, int64_t &token) {
+    uint32_t low = 0, high = (b.sequences + step - 1) / step;
+    while (low < high) {
+        const uint32_t mid = (low + high) / 2;
+        if (held[mid] <= (int32_t)row) low = mid + 1;
+        else high = mid;
+    }
+    if (low == 0) return kNoRow;
+    high = min(low * step, b.sequences);
+    low = (low - 1) * step + 1;
+    while (low < high) {
+        const uint32_t mid = (low + high) / 2;
+        if (__ldg(b.starts + mid) <= (int32_t)row) low = mid + 1;
+        else high = mid;
+    }
+    const uint32_t s = low - 1;
+    const Sequence q = sequence_of(c, b, s);
+    if (row - q.row0 >= q.rows) return kNoRow;
+    token = (int64_t)q.length - q.rows + (row - q.row0);
+    if (token < 0) return kNowhere;
+    const uint32_t at = c.by_page.of((uint32_t)token);
+    const int32_t page = __ldg(b.table + (uint64_t)s * b.width + at);
+    if (page < 0 || (uint32_t)page >= c.pages) return kNowhere;
+    return (int64_t)page * c.heads * c.page_size + ((uint32_t)token - at * c.page_size);
+}
+
 // ---- attention ------------------------------------------------------------------------------------
 // f16 holds the levels times kLevelUnit: it rounds each, always the same way, and a sum over many tokens keeps the rounding
 // errors' mean, which at 131072 tokens was 4.5e-3 of the result.  In this unit (found by search over [1, 2)) that mean is 1.7e-6 of a
@@ -91,6 +120,8 @@ struct AttentionView {
     float *part_o;
     float2 *part_ml;
     uint32_t parts;
+    const uint32_t *masks;  // of trees: [rows][words], else null
+    uint32_t words;
 };
 
 // How many tokens a row sees; of a tile's rows the last sees most.
@@ -99,11 +130,30 @@ __device__ __forceinline__ uint32_t visible_end(const Sequence &s, const FastDiv
     return (uint32_t)max(token, -1) + 1;
 }
 
+// Of trees: the first token of the nodes, and 32 bits of what a row sees, of the nodes from number `first` on (the tokens ahead of the nodes are seen).
+__device__ __forceinline__ int32_t first_node(const Sequence &s) { return (int32_t)s.length - (int32_t)s.rows; }
+__device__ __forceinline__ uint32_t seen_nodes(const AttentionView &a, uint32_t row, int32_t first) {
+    const int32_t w = first >> 5;
+    if (w < -1) return ~0u;
+    const uint32_t *const of_row = a.masks + (uint64_t)row * a.words;
+    const uint32_t lo = w < 0 ? ~0u : (uint32_t)w < a.words ? __ldg(of_row + w) : 0u;
+    const uint32_t hi = (uint32_t)(w + 1) < a.words ? __ldg(of_row + w + 1) : 0u;
+    return __funnelshift_r(lo, hi, (uint32_t)first & 31u);
+}
+// The low `n` bits (all from 32 on).
+__device__ __forceinline__ uint32_t low_bits(uint32_t n) { return n >= 32 ? ~0u : (1u << n) - 1; }
+
+// How many tokens a row sees, or may see of a tree.
+template <bool TREE>
+__device__ __forceinline__ uint32_t seen_end(const Sequence &s, const FastDiv &by_group, uint32_t row) {
+    return TREE ? s.length : visible_end(s, by_group, row);
+}
+
 struct AttentionCall {
     CacheView cache;
     BatchView batch;
     AttentionView view;
-    bool nf4, f32;
+    bool nf4, f32, tree;
     uint32_t head_dim;
     uint32_t most_rows, most_tokens;  // of a sequence, as far as the host knows: rows of the call's tensors, tokens
 };

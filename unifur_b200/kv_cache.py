@@ -37,6 +37,26 @@ class CacheBatch:
         return (self.page_table, self.lengths, self.row_starts, self.rows, self.max_rows, self.max_length)
 
 
+class Rotation:
+    """The rotation of keys and queries by the angles of their positions.
+
+    ``table``: contiguous f32 ``[positions, rotary_dim]`` on the cache's device, a position's cosines and behind them its sines.
+    The first ``rotary_dim`` values of a head are turned (a multiple of 16): pair ``i`` is its values ``i`` and ``i + rotary_dim /
+    2``, or, with ``pairs``, the neighbours ``2 i`` and ``2 i + 1``."""
+
+    __slots__ = ("table", "pairs")
+
+    def __init__(self, table: torch.Tensor, pairs: bool = False):
+        self.table, self.pairs = table, pairs
+
+    @staticmethod
+    def new(positions: int, rotary_dim: int, device, base: float = 10000.0, pairs: bool = False) -> "Rotation":
+        """Pair ``i`` turns by ``position / base ** (2 i / rotary_dim)``, worked out in 64 bits."""
+        angles = torch.arange(positions, dtype=torch.float64)[:, None] * base ** (
+            -2.0 * torch.arange(rotary_dim // 2, dtype=torch.float64) / rotary_dim)
+        return Rotation(torch.cat((angles.cos(), angles.sin()), 1).float().to(device), pairs)
+
+
 class PagedKvCache:
     """Keys and values in pages of ``page_size`` tokens (a multiple of 16).
 
@@ -88,6 +108,16 @@ class PagedKvCache:
         not, is not written."""
         _lib.host().cache_append(*self._args(), *batch._args(), k, v)
 
+    def append_rotated(self, k: torch.Tensor, v: torch.Tensor, batch: CacheBatch, rotation: Rotation,
+                       positions: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
+                       out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+        """``append`` of keys that are turned by the angles of their positions on the way, and the queries ``q`` (``[rows, q_heads,
+        head_dim]`` or ``[rows, q_heads * head_dim]``, of ``k``'s type) turned by the same, which are returned (in ``out``, which may
+        be ``q``).  ``positions`` (int32 ``[rows]``) are each row's place in its sequence if they are not given.  Keys are quantized, and
+        queries rounded, from f32 products and sums that are rounded one by one.  A row whose position is outside the table is not
+        written to the cache, and its queries become NaNs."""
+        return _lib.host().cache_append_rotated(*self._args(), *batch._args(), k, v, rotation.table, rotation.pairs, positions, q, out)
+
     def read(self, batch: CacheBatch, dtype: torch.dtype = torch.float32,
              out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
         """The rows' keys and values as the cache has them, ``[rows, heads, head_dim]`` in ``dtype`` (f32 or bf16).  Rows without a
@@ -106,3 +136,38 @@ class PagedKvCache:
         if scale is None:
             scale = 1.0 / math.sqrt(self.head_dim())
         return _lib.host().cache_attention(*self._args(), *batch._args(), q, scale, out)
+
+    # ---- trees of drafted tokens: a sequence's rows are the nodes of a tree (or of several), appended like any new tokens ----
+
+    def tree_masks(self, parents: torch.Tensor, batch: CacheBatch,
+                   out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """What ``tree_attention`` and ``append_rotated`` take of trees given by each node's parent: ``parents`` (int32 ``[rows]``) is the
+        number of an earlier node of the row's sequence, anything else (-1) makes it a root.  Returns masks (int32 ``[rows, words]``, bit
+        ``j % 32`` of word ``j / 32`` for node ``j``: the node itself and its ancestors) and positions (int32 ``[rows]``: the
+        context's length and the node's depth).  There are as many words as ``max_rows`` (or ``rows``) needs, or as ``out`` has: nodes behind
+        them are seen by none.  Rows of no sequence are left as ``out`` has them, and without ``out`` undefined."""
+        if out is None:
+            words = ((batch.max_rows or batch.rows) + 31) // 32
+            out = (torch.empty(batch.rows, words, dtype=torch.int32, device=self.k.device),
+                   torch.empty(batch.rows, dtype=torch.int32, device=self.k.device))
+        _lib.host().cache_tree(*self._args(), *batch._args(), parents, *out)
+        return out
+
+    def tree_attention(self, q: torch.Tensor, masks: torch.Tensor, batch: CacheBatch, scale: Optional[float] = None,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """``attention`` of the nodes of trees: each row sees its sequence's context (what is cached ahead of the sequence's rows) and those
+        of its nodes that ``masks`` (int32 ``[rows, words]``, as ``tree_masks`` makes them) has for it, whether they come before it or not.
+        A row that sees nothing becomes zeros.  Values of all the sequences' tokens are finite, of hidden nodes too."""
+        if scale is None:
+            scale = 1.0 / math.sqrt(self.head_dim())
+        return _lib.host().cache_attention(*self._args(), *batch._args(), q, scale, out, masks)
+
+    def keep(self, kept: torch.Tensor, counts: torch.Tensor, batch: CacheBatch, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Keeps a path of each sequence's tree: nodes ``kept[s][:counts[s]]`` (int32 ``[sequences, nodes]`` and ``[sequences]``), which
+        increase along it, move to the places behind the context.  Returns the sequences' new lengths, the context's and ``counts`` (in ``out``,
+        which may be ``batch.lengths`` where no other cache is still to be moved).  A path ends ahead of the first entry that is not above the
+        one before it, or that is no node."""
+        if out is None:
+            out = torch.empty_like(batch.lengths)
+        _lib.host().cache_keep(*self._args(), *batch._args(), kept, counts, out)
+        return out
