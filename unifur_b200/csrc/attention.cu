@@ -308,7 +308,7 @@ join_kernel(const BatchView b, const AttentionView a, uint32_t q_heads) {
 // rows 50 / 48, 96 rows 68 / 48, bf16: 64 rows 41 / 40, 96 rows 56 / 40.
 bool takes_decode(const AttentionCall &c) {
     if (c.f32) return false;
-    if (!attention_chunk_counts(c)) return true;  // (the other counts in 64 bits)
+    if (!(c.tree ? attention_tree_counts(c) : attention_chunk_counts(c))) return true;  // (the other counts in 64 bits)
     const int of_dim = c.head_dim == 64 ? 0 : c.head_dim == 128 ? 1 : 2;
     static constexpr double kStream[2][3] = {{5, 11, 32}, {7, 9, 45}}, kMany[2][3] = {{13, 18, 40}, {19, 25, 58}};  // [NF4][dim]
     // row tiles of all sequences: by the most rows of one, or by all rows where that says less
@@ -350,7 +350,7 @@ uint64_t part_ml_bytes(const AttentionCall &c, uint32_t parts) {
     return ((uint64_t)parts * c.batch.rows * c.cache.heads * c.view.group * sizeof(float2) + 255) / 256 * 256;
 }
 uint64_t workspace_bytes_of(const AttentionCall &c, const Plan &p) {
-    if (!c.f32) return takes_decode(c) ? attention_decode_bytes(c) : attention_chunk_bytes(c);
+    if (!c.f32) return takes_decode(c) ? attention_decode_bytes(c) : c.tree ? attention_tree_bytes(c) : attention_chunk_bytes(c);
     if (p.parts == 1) return kAttentionFlagBytes;
     return kAttentionFlagBytes + part_ml_bytes(c, p.parts) + (uint64_t)p.parts * c.batch.rows * c.cache.heads * c.view.group * c.head_dim * sizeof(float);
 }
@@ -448,7 +448,7 @@ int32_t attention(const char *what, const nf4_cache *cache, const nf4_cache_batc
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (!c.f32) {
         uint8_t *const workspace = static_cast<uint8_t *>(args->workspace);
-        return takes_decode(c) ? attention_decode(c, workspace, s) : attention_chunk(c, workspace, s);
+        return takes_decode(c) ? attention_decode(c, workspace, s) : c.tree ? attention_tree(c, workspace, s) : attention_chunk(c, workspace, s);
     }
     return c.head_dim == 64 ? launch_of<64>(c, p, s) : c.head_dim == 128 ? launch_of<128>(c, p, s) : launch_of<256>(c, p, s);
 }

@@ -23,8 +23,7 @@
 // take any size.)
 #include <algorithm>
 
-#include "kv_cache.cuh"
-#include "ptx.cuh"
+#include "attention_steps.cuh"
 #include "tmap.cuh"
 
 namespace nf4 {
@@ -32,35 +31,25 @@ namespace nf4 {
 namespace {
 
 constexpr uint32_t kThreads = 512;
-// Weights are 2^(S c - m + raise).  In f16 up to 2^15, so that it holds those that are 2^-32 of a row's largest; their sum is raised alike, and where
-// sums go to the workspace both are lowered by that again, so that no value overflows them that would not overflow a sum of weights up to
-// one.  bf16 has the range: weights up to one.
-template <bool NF4>
-constexpr float kRaise = NF4 ? 7.f : -8.f;
-template <bool NF4>
-constexpr float kLower = NF4 ? 1.f / 32768.f : 1.f;
-constexpr uint32_t kGroup = 16;  // tokens that are in one page for sure
-// warps 0-3 and 4-7: softmax of a tile; 8-11: codes to f16 (trees: 4-11); 12: copies; 13: MMAs
-constexpr uint32_t kCopyWarp = 12, kMmaWarp = 13;
+constexpr uint32_t kStart = 4;  // (see Walker)
+// warps 0-3 and 4-7: softmax of a tile; 8-11: codes to f16; 12: copies; 13: MMAs
+constexpr uint32_t kExpandWarp = 8, kCopyWarp = 12, kMmaWarp = 13;
+// Registers: 512 threads are launched with 128 each; the two softmax warpgroups take 160 and leave 96 to the other two (together the
+// same 65536).
+constexpr uint32_t kSoftmaxRegs = 160, kOtherRegs = 96;
 
-// TREE: rows are nodes of trees, which see their sequence's tokens ahead of the nodes and those nodes that their masks have.  A tree has few rows, mostly
-// one MMA tile of a head.
-template <int D, bool NF4, bool TREE>
+template <int D, bool NF4>
 struct Shape {
-    static constexpr uint32_t kTiles = D == 256 || TREE ? 1 : 2, kRows = 128 * kTiles;
+    static constexpr uint32_t kTiles = D == 256 ? 1 : 2, kRows = 128 * kTiles;
     static constexpr uint32_t kTokens = D == 256 ? 64 : 128;          // of a step
-    // S's places to a tile: with one tile there is room for two, so that the next step's scores come while weights are made
-    static constexpr uint32_t kPlaces = kTiles == 1 ? 2 : 1;
-    static constexpr uint32_t kSoftmaxWarps = TREE ? 4 : 8, kExpandWarp = TREE && NF4 ? 4 : 8, kExpandWarps = kCopyWarp - kExpandWarp;
-    // Registers: 512 threads are launched with 128 each; the two softmax warpgroups take 160 and leave 96 to the other two (together the
-    // same 65536), or one takes 200 and leaves 104 to three.
-    static constexpr uint32_t kSoftmaxRegs = TREE ? 200 : 160, kOtherRegs = TREE ? 104 : 96;
+    // S's places to a tile: with a dim of 256 there is room for two, so that the next step's scores come while weights are made
+    static constexpr uint32_t kPlaces = D == 256 ? 2 : 1;
     static constexpr uint32_t kBlocks = D / 64;
     static constexpr uint32_t kQTile = 128 * D * 2, kTile = kTokens * D * 2, kBox = kTokens * 128;
     static constexpr uint32_t kScales = kTokens * kBlocks * 4;
     // a tile's codes and scales, and with K's the V's scales of the step: their power goes to the softmax ahead of V
     static constexpr uint32_t kRaw = NF4 ? kTokens * D / 2 + 2 * kScales : 0, kRawSlots = D == 64 ? 5 : 2;
-    static constexpr uint32_t kSlots = D == 64 ? (NF4 && !TREE ? 6 : 7) : (NF4 ? 3 : 5) + (D == 128 && TREE ? 1 : 0);  // of the ring; one more where the table is not needed
+    static constexpr uint32_t kSlots = D == 64 ? (NF4 ? 6 : 7) : NF4 ? 3 : 5;  // of the ring; one more where the table is not needed
     // codes, then the table on a multiple of its 32 KB, then Q, then the ring (bf16: Q, then the ring)
     static constexpr uint32_t kSmem = (NF4 ? 65536 : 2048) - 1024 + kTiles * kQTile + kSlots * kTile;
     static constexpr uint32_t kS = 0, kO = 256;                       // columns of tensor memory: the tiles' S's, then O's
@@ -69,7 +58,6 @@ struct Shape {
 // A tile's 128 rows of queries, as the MMA reads them, and in their place later the tile's results: a box of 128 rows to every 64 values (128
 // bytes), 16-byte chunks swizzled.  Each of the tile's four warps has the 32 rows whose softmax is its own, for both, so that a warp which
 // writes its next queries has nothing to wait for from one that still reads its results out.
-__host__ __device__ constexpr uint32_t chunk_place(uint32_t row, uint32_t x) { return (x >> 3) * 16384u + row * 128u + (((x & 7u) ^ (row & 7u)) << 4); }
 // The n-th chunk (of dim / 8) that a lane of one of the four warps brings of the queries, and that it takes of the results.
 struct RowChunk {
     uint32_t row, x;
@@ -79,189 +67,12 @@ __host__ __device__ constexpr RowChunk chunk_of(uint32_t dim, uint32_t warp, uin
     return RowChunk{warp * 32 + n * (32 / lanes) + lane / lanes, lane % lanes};
 }
 
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
-        "%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-          "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
-        "%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
-        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
-        "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ float exp2_approx(float v) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-    return r;
-}
-// Two at a time: half the instructions of the FMA pipe
-__device__ __forceinline__ float2 fma2(float2 a, float b, float c) {
-    float2 r;
-    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%5, %5};\n\tfma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b), "f"(c));
-    return r;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 r;
-    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
-        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-template <bool F16>
-__device__ __forceinline__ uint32_t pack(float a, float b) {
-    uint32_t r;
-    if (F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-    return r;
-}
-__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ uint4 ld_shared_u4(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ float2 ld_shared_f2(uint32_t addr) {
-    float2 v;
-    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ void st_shared_u4(uint32_t addr, uint4 v) {
-    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-// The power of two that scales up to `most` (bits) are divided by, to be below 2^15: 2^-126 or more.
-constexpr int kTop = 15;
-__device__ __forceinline__ float power_for(uint32_t most) { return __uint_as_float((uint32_t)max((int)(most >> 23) + 1 - kTop, 1) << 23); }
-__device__ __forceinline__ float reciprocal_of_power(float p) { return __uint_as_float(0x7f000000u - __float_as_uint(p)); }
-
-// How the line of steps is shared out: `per` to a CTA, one more to the first `more` of them.
-struct Share {
-    uint32_t per, more, ctas;
-    __device__ uint32_t start(uint32_t cta) const { return per * cta + min(cta, more); }
-    __device__ uint32_t cta_of(uint32_t u) const {
-        const uint32_t first = (per + 1) * more;
-        return u < first ? u / (per + 1) : more + (u - first) / per;
-    }
-};
-
-// A run of steps of one row tile.
-struct Piece {
-    Sequence s;
-    uint32_t seq, head, r0, rows, live;  // rows of the tile; MMA tiles that have some
-    uint32_t step0, steps, all;          // of the `all` steps that the tile has
-    uint32_t line0;                      // where the tile's steps begin in the line
-};
-
-// Steps' worth of time that a row tile takes beside its steps (its queries in, its results out): counted in the line, or the CTAs that have
-// a prompt's first tiles, of one step each, would be done last.
-constexpr uint32_t kStart = 4;
-
-template <uint32_t R, uint32_t N, bool TREE>
-struct Walker {  // through a CTA's pieces; every warp goes its own way
-    Sequence s;
-    uint32_t seq, head, tile, off, now, end;
-
-    static __device__ __forceinline__ uint32_t tiles_of(const Sequence &s, uint32_t group) { return (uint32_t)(((uint64_t)s.rows * group + R - 1) / R); }
-    // (a tile that sees nothing has one step all the same: its results are zeros)
-    static __device__ __forceinline__ uint32_t steps_of(const Sequence &s, const AttentionView &a, uint32_t tile) {
-        const uint32_t last = (uint32_t)min((uint64_t)(tile + 1) * R, (uint64_t)s.rows * a.group) - 1;
-        return max(1u, (seen_end<TREE>(s, a.by_group, last) + N - 1) / N);
-    }
-    __device__ __forceinline__ bool next(const CacheView &c, const BatchView &b, const AttentionView &a, Piece &p) {
-        do {
-            if (!one(c, b, a, p)) return false;
-        } while (p.steps == 0);  // (the end of a share that lies ahead of a tile's first step)
-        return true;
-    }
-    __device__ __forceinline__ bool one(const CacheView &c, const BatchView &b, const AttentionView &a, Piece &p) {
-        if (now >= end) return false;
-        while (tile >= tiles_of(s, a.group)) {  // on to the next head, or the next sequence with rows
-            tile = 0;
-            if (s.rows == 0 || ++head >= c.heads) {
-                head = 0;
-                if (++seq >= b.sequences) return false;
-                s = sequence_of(c, b, seq);
-            }
-        }
-        p.s = s;
-        p.seq = seq;
-        p.head = head;
-        p.r0 = tile * R;
-        p.rows = (uint32_t)min((uint64_t)R, (uint64_t)s.rows * a.group - p.r0);
-        p.live = (p.rows + 127) / 128;
-        p.all = steps_of(s, a, tile);
-        p.line0 = now - off;
-        // of the tile's place in the line [line0, line0 + kStart + all) the steps are behind kStart
-        const uint32_t upto = min(p.all + kStart, end - p.line0);
-        p.step0 = off > kStart ? off - kStart : 0u;
-        p.steps = (upto > kStart ? upto - kStart : 0u) - p.step0;
-        now = p.line0 + upto;
-        off = 0;
-        ++tile;
-        return true;
-    }
-};
-
-// A quantized cache's keys and values expanded to f16 once for all row tiles, by a kernel ahead: a step's tokens of a head are a tile of
-// kTokens rows, zeros behind the sequence's last token.
-struct Dense {
-    uint32_t capacity;        // tiles to a head that there is room for; 0: codes are expanded where they are used
-    const uint32_t *bases;    // [sequences] a sequence's first tile, and behind them [sequences]: all tiles
-    const float2 *powers;     // [tile][head] what K's and V's scales are divided by
-};
-
-// What the join has to know of a row tile that several CTAs have: written by the CTA in whose share it begins, rows 0 by the others.
-struct Split {
-    uint32_t row0, r0, rows, head, more;  // more: CTAs behind the first
-};
-
-// A place in the ring of tiles, and the parity of its barriers' round.
-struct Ring {
-    uint32_t slot = 0, round = 0;
-    __device__ __forceinline__ void on(uint32_t slots) {
-        if (++slot == slots) {
-            slot = 0;
-            ++round;
-        }
-    }
-};
-
-// In which order a piece's tiles of K and V come: K 0, V 0, K 1, V 1, ...; with two places for S K 0, K 1, V 0, K 2, V 1, ..., V n - 1.
-template <uint32_t kPlaces>
-struct Turn {
-    uint32_t values, step;
-    __device__ __forceinline__ Turn(uint32_t turn, uint32_t steps) {
-        if (kPlaces == 1) {
-            values = turn & 1u;
-            step = turn / 2;
-            return;
-        }
-        const bool last = turn + 1 == 2 * steps;
-        values = last || (turn && !(turn & 1u)) ? 1 : 0;
-        step = last ? steps - 1 : values ? turn / 2 - 1 : (turn + 1) / 2;
-    }
-};
-
-template <int D, bool NF4, bool TREE>
+template <int D, bool NF4>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const CacheView c, const BatchView b,
                        const AttentionView a, const Dense dense, uint32_t box_rows, Split *const splits, const FailureRef failure) {
-    using S = Shape<D, NF4, TREE>;
-    using Walk = Walker<S::kRows, S::kTokens, TREE>;
-    constexpr uint32_t kExpandWarp = S::kExpandWarp, kExpandWarps = S::kExpandWarps, kSoftmaxRegs = S::kSoftmaxRegs, kOtherRegs = S::kOtherRegs;
+    using S = Shape<D, NF4>;
+    using Walk = Walker<S::kRows, S::kTokens, kStart, false>;
     // A bf16 cache's pages may be of sixteen tokens, and a warp asks for boxes one after another: four warps share the asking, a tile's
     // columns between two of them (with one, 137 cycles to a box of 2 KB, the MMAs waited for copies)
     constexpr uint32_t kCopies = !NF4 && D >= 128 ? 2 : 1;
@@ -292,12 +103,12 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     if (tid == 0) {
         static_assert(S::kSlots + 1 <= 8);
         for (uint32_t i = 0; i < 8; ++i) {  // (a place more than kSlots may be in use)
-            ptx::mbar_init(full0 + 8 * i, NF4 ? kExpandWarps : kCopies);
+            ptx::mbar_init(full0 + 8 * i, NF4 ? 4 : kCopies);
             ptx::mbar_init(empty0 + 8 * i, 1);
         }
         for (uint32_t i = 0; i < S::kRawSlots; ++i) {
             ptx::mbar_init(raw_full0 + 8 * i, 1);
-            ptx::mbar_init(raw_empty0 + 8 * i, kExpandWarps);
+            ptx::mbar_init(raw_empty0 + 8 * i, 4);
         }
         for (uint32_t i = 0; i < 4; ++i) {
             ptx::mbar_init(s_full0 + 8 * i, 1);
@@ -329,88 +140,8 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
 
     // ---- this CTA's share of the line, and where in it begins ----
     if (warp == 0) {
-        // a lane a sequence: its steps, all heads
-        auto steps_of = [&](uint32_t s0, Sequence &s) -> uint32_t {
-            s = Sequence{0, 0, 0};
-            if (s0 + lane < b.sequences) s = sequence_of(c, b, s0 + lane);
-            const uint32_t tiles = Walk::tiles_of(s, a.group);
-            uint32_t sum = 0;
-            if (tiles <= 8)
-                for (uint32_t t = 0; t < tiles; ++t) sum += kStart + Walk::steps_of(s, a, t);
-            for (uint32_t many = __ballot_sync(0xffffffffu, tiles > 8); many; many &= many - 1) {  // with the whole warp
-                const int l = __ffs(many) - 1;
-                const Sequence o{__shfl_sync(0xffffffffu, s.row0, l), __shfl_sync(0xffffffffu, s.rows, l), __shfl_sync(0xffffffffu, s.length, l)};
-                uint32_t part = 0;
-                for (uint32_t t = lane; t < Walk::tiles_of(o, a.group); t += 32) part += kStart + Walk::steps_of(o, a, t);
-                part = __reduce_add_sync(0xffffffffu, part);
-                if ((int)lane == l) sum = part;
-            }
-            return sum * c.heads;
-        };
-        Sequence s0;
-        const uint32_t own0 = steps_of(0, s0);
-        uint32_t total = own0;
-        for (uint32_t k = 32; k < b.sequences; k += 32) {
-            Sequence s;
-            total += steps_of(k, s);
-        }
-        total = __reduce_add_sync(0xffffffffu, total);
-        Share share;
-        share.ctas = min(gridDim.x, (total + kStart + 1) / (kStart + 2));  // two steps at least
-        share.per = share.ctas ? total / share.ctas : 0;
-        share.more = share.ctas ? total - share.per * share.ctas : 0;
-        const uint32_t first = share.start(blockIdx.x);
-        uint32_t last = blockIdx.x < share.ctas ? share.start(blockIdx.x + 1) : first, before = 0;
-        bool found = false;
-        for (uint32_t k = 0; first < last && k < b.sequences; k += 32) {
-            Sequence s = s0;
-            const uint32_t own = k ? steps_of(k, s) : own0;
-            uint32_t upto = own;
-            #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint32_t o = __shfl_up_sync(0xffffffffu, upto, d);
-                if (lane >= (uint32_t)d) upto += o;
-            }
-            const uint32_t past = __ballot_sync(0xffffffffu, before + upto > first);
-            if (past) {
-                const int l = __ffs(past) - 1;
-                const Sequence o{__shfl_sync(0xffffffffu, s.row0, l), __shfl_sync(0xffffffffu, s.rows, l), __shfl_sync(0xffffffffu, s.length, l)};
-                const uint32_t at = first - before - __shfl_sync(0xffffffffu, upto - own, l), of_head = __shfl_sync(0xffffffffu, own, l) / c.heads;
-                const uint32_t head = of_head ? at / of_head : c.heads;
-                uint32_t left = at - head * of_head, tile = 0;
-                for (uint32_t t0 = 0;; t0 += 32) {
-                    const uint32_t mine = t0 + lane < Walk::tiles_of(o, a.group) ? kStart + Walk::steps_of(o, a, t0 + lane) : 0u;
-                    uint32_t sum = mine;
-                    #pragma unroll
-                    for (int d = 1; d < 32; d <<= 1) {
-                        const uint32_t v = __shfl_up_sync(0xffffffffu, sum, d);
-                        if (lane >= (uint32_t)d) sum += v;
-                    }
-                    const uint32_t in = __ballot_sync(0xffffffffu, sum > left);
-                    if (in) {
-                        const int t = __ffs(in) - 1;
-                        tile = t0 + t;
-                        left -= __shfl_sync(0xffffffffu, sum - mine, t);
-                        found = head < c.heads;
-                        break;
-                    }
-                    if (t0 + 32 >= Walk::tiles_of(o, a.group)) break;  // (not reached where row starts do not decrease: the head has that many steps)
-                    left -= __shfl_sync(0xffffffffu, sum, 31);
-                }
-                if (lane == 0) {
-                    s_first[0] = k + l;
-                    s_first[1] = head;
-                    s_first[2] = tile;
-                    s_first[3] = left;
-                }
-                break;
-            }
-            before += __shfl_sync(0xffffffffu, upto, 31);
-        }
-        if (!found) last = first;  // (row starts that decrease, whose rows are more than the line is counted for: no access by what is not there)
+        const Share share = share_out<Walk>(c, b, a, s_first);
         if (lane == 0) {
-            s_first[4] = first;
-            s_first[5] = last;
             s_share = share;
             splits[blockIdx.x].rows = 0;
         }
@@ -426,7 +157,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
     if (s_first[4] < s_first[5]) {
         Walk walk{sequence_of(c, b, s_first[0]), s_first[0], s_first[1], s_first[2], s_first[3], s_first[4], s_first[5]};
         Piece p;
-        if (warp < S::kSoftmaxWarps) {
+        if (warp < 8) {
             asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
             const uint32_t tile = warp >> 2, r = tid & 127u;
             const uint32_t lanes = (warp & 3u) << 21;  // a warp reaches its quarter of tensor memory's lanes
@@ -482,13 +213,8 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                 // ---- the steps ----
                 const uint32_t row = p.r0 + tile * 128 + r, t_first = p.step0 * N;
                 const bool real = tile * 128 + r < p.rows;
-                const uint32_t token = a.by_group.of(real ? row : p.r0);
-                const int32_t nodes0 = first_node(p.s);
-                const bool blind = !real || (TREE && nodes0 + (int32_t)token < 0);  // a row that sees nothing
-                const uint32_t sees = blind ? 0u : seen_end<TREE>(p.s, a.by_group, row);
-                const uint32_t sees_first = TREE ? (uint32_t)max(nodes0, 0) : visible_end(p.s, a.by_group, p.r0 + tile * 128);
-                const bool idle = TREE && (warp & 3u) * 32 >= p.rows;  // none of the warp's rows is one: its part of S is never looked at
-                const uint32_t steps = p.steps, p_row = p.s.row0 + token;
+                const uint32_t sees = real ? visible_end(p.s, a.by_group, row) : 0u, sees_first = visible_end(p.s, a.by_group, p.r0 + tile * 128);
+                const uint32_t steps = p.steps;
                 const float row_factor = fabsf(a.scale_log2) * (NF4 ? s_qpower[tile * 128 + r] : 1.f);
                 float m = -INFINITY, l = 0.f, ref = 0.f;
                 for (uint32_t j = 0; j < steps; ++j, ++scores) {
@@ -497,10 +223,6 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                         ok = false;
                         if (lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, 23);
                         break;
-                    }
-                    if (idle) {
-                        if (lane == 0) ptx::mbar_arrive(p_ready0 + 8 * place);
-                        continue;
                     }
                     ptx::tc_fence_after();
                     const uint32_t t0 = t_first + j * N, lim = sees > t0 ? sees - t0 : 0u;
@@ -530,10 +252,8 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                             ptx::tmem_wait_ld();
                             if (k + 32 < N) tmem_ld32(ts + k + 32, ahead[k / 32 + 1 & 1]);
                             if (masked) {
-                                uint32_t seen = 0;
-                                if (TREE) seen = seen_nodes(a, p_row, (int32_t)(t0 + k) - nodes0) & low_bits(lim > k ? lim - k : 0u);
                                 #pragma unroll
-                                for (uint32_t i = 0; i < 32; ++i) x[i] = (TREE ? seen >> i & 1u : k + i < lim) ? x[i] : 0xff800000u;
+                                for (uint32_t i = 0; i < 32; ++i) x[i] = k + i < lim ? x[i] : 0xff800000u;
                             }
                             #pragma unroll
                             for (uint32_t i = 0; i < 32; i += 2) {
@@ -653,9 +373,9 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
             }
         } else {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-            if (NF4 && !expanded && warp >= kExpandWarp && warp < kExpandWarp + kExpandWarps) {
+            if (NF4 && !expanded && warp >= kExpandWarp && warp < kExpandWarp + 4) {
                 // ---- codes to f16: a thread has 16 bytes of a token's row, 32 values ----
-                constexpr uint32_t kLanes = D / 32, kPass = 32 * kExpandWarps / kLanes;
+                constexpr uint32_t kLanes = D / 32, kPass = 128 / kLanes;
                 const uint32_t th = tid - 32 * kExpandWarp, q = th % kLanes, lane_word = table | lane * 4u;
                 // In which order a thread takes its four words: so that eight lanes' 16-byte stores hit all banks
                 const uint32_t order = D == 128 ? (q >> 1) * 2 : D == 256 ? q >> 1 : 0u;
@@ -668,7 +388,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                     }
                 };
                 for (; ok && walk.next(c, b, a, p); step += p.steps) {
-                    const uint32_t t_end = min(seen_end<TREE>(p.s, a.by_group, p.r0 + p.rows - 1), (p.step0 + p.steps) * N);
+                    const uint32_t t_end = min(visible_end(p.s, a.by_group, p.r0 + p.rows - 1), (p.step0 + p.steps) * N);
                     #pragma unroll 1
                     for (uint32_t turn = 0; ok && turn < 2 * p.steps; ++turn, ++i, ring.on(slots)) {
                         const Turn<kPlaces> of(turn, p.steps);
@@ -736,7 +456,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                         }
                     }
                 }
-            } else if (NF4 ? warp == kCopyWarp : warp >= kExpandWarp && warp < kExpandWarp + 2 * kCopies) {
+            } else if (NF4 ? warp == kCopyWarp : warp < kExpandWarp + 2 * kCopies) {
                 const uint32_t own = NF4 ? 0u : (warp - kExpandWarp) & 1u, part = NF4 ? 0u : (warp - kExpandWarp) >> 1;  // bf16: K or V, and which columns
                 const uint32_t unit = NF4 ? kGroup : box_rows, units = N / unit;  // tokens that come together, being in one page
                 uint32_t i = 0, tails = 0, step = 0;
@@ -782,7 +502,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
                                 const int32_t row = (int32_t)(((tile0 + j) * c.heads + p.head) * N);
                                 #pragma unroll
                                 for (uint32_t x = 0; x < D / 64; ++x) ptx::tma_load_2d(dst + x * S::kBox, which ? &tmap_v : &tmap_k, (int32_t)(64 * x), row, bar);
-                                for (uint32_t e = 1; e < kExpandWarps; ++e) ptx::mbar_arrive(bar);  // (for the warps that expand)
+                                for (int e = 0; e < 3; ++e) ptx::mbar_arrive(bar);  // (for the four warps that expand)
                             }
                         } else if (NF4) {
                             const uint32_t bar = raw_full0 + 8 * rs, raw = raw0 + rs * S::kRaw;
@@ -923,7 +643,7 @@ attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_
 template <int D>
 __global__ void __launch_bounds__(256)
 expand_kernel(const CacheView c, const BatchView b, uint4 *const k_out, uint4 *const v_out, uint32_t *const bases, float2 *const powers) {
-    constexpr uint32_t N = Shape<D, true, false>::kTokens, kBlocks = D / 64, kGroups = D / 8;  // eight values each
+    constexpr uint32_t N = Shape<D, true>::kTokens, kBlocks = D / 64, kGroups = D / 8;  // eight values each
     __shared__ uint32_t s_pairs[256], s_most[2], s_place[N], s_bad;
     const uint32_t tid = threadIdx.x, lane = tid & 31u;
     s_pairs[tid] = level_pair_f16(tid);
@@ -1003,67 +723,14 @@ expand_kernel(const CacheView c, const BatchView b, uint4 *const k_out, uint4 *c
     }
 }
 
-// The row tiles that several CTAs had: a warp to four rows at a time, the parts in the order of the tokens.
-constexpr uint32_t kJoinRows = 4, kJoinWarps = 8;
-template <int D, uint32_t kRows>
-__global__ void __launch_bounds__(32 * kJoinWarps)
-join_pieces_kernel(const AttentionView a, const Split *const splits) {
-    constexpr uint32_t kWide = D / 32;  // values of a row to a lane
-    ptx::pdl_launch_dependents();
-    ptx::pdl_wait();
-    const Split s = splits[blockIdx.x];
-    const uint32_t r0 = (blockIdx.y * kJoinWarps + threadIdx.x / 32) * kJoinRows, lane = threadIdx.x & 31u;
-    if (r0 >= s.rows) return;
-    auto part = [&](uint32_t i) { return (uint64_t)(2 * (blockIdx.x + i) + (i ? 0 : 1)) * kRows + r0; };
-    float m[kJoinRows], sum[kJoinRows], acc[kJoinRows][kWide];
-    #pragma unroll
-    for (uint32_t r = 0; r < kJoinRows; ++r) {
-        m[r] = -INFINITY;
-        sum[r] = 0.f;
-        #pragma unroll
-        for (uint32_t j = 0; j < kWide; ++j) acc[r][j] = 0.f;
-    }
-    #pragma unroll 2
-    for (uint32_t i = 0; i <= s.more; ++i) {
-        #pragma unroll
-        for (uint32_t r = 0; r < kJoinRows; ++r) {  // (a tile's rows behind its last hold anything; they are not written)
-            const float2 ml = __ldg(a.part_ml + part(i) + r);
-            float v[kWide];
-            const float *const o = a.part_o + (part(i) + r) * D + lane * kWide;
-            #pragma unroll
-            for (uint32_t j = 0; j < kWide; j += 2) {
-                const float2 w = __ldg(reinterpret_cast<const float2 *>(o + j));
-                v[j] = w.x;
-                v[j + 1] = w.y;
-            }
-            const float top = fmaxf(m[r], ml.x), base = top == -INFINITY ? 0.f : top;
-            const float keep = exp2_approx(m[r] - base), f = exp2_approx(ml.x - base);  // (nothing seen: 2^-inf)
-            m[r] = top;
-            sum[r] = fmaf(f, ml.y, sum[r] * keep);
-            #pragma unroll
-            for (uint32_t j = 0; j < kWide; ++j) acc[r][j] = fmaf(f, v[j], acc[r][j] * keep);
-        }
-    }
-    #pragma unroll
-    for (uint32_t r = 0; r < kJoinRows; ++r) {
-        if (r0 + r >= s.rows) break;
-        const float f = sum[r] == 0.f ? 0.f : 1.f / sum[r];
-        const uint32_t q_row = s.r0 + r0 + r, token = a.by_group.of(q_row);
-        __nv_bfloat16 *const out = static_cast<__nv_bfloat16 *>(a.out) + (uint64_t)(s.row0 + token) * a.ldo + (uint64_t)(s.head * a.group + q_row - token * a.group) * D + lane * kWide;
-        #pragma unroll
-        for (uint32_t j = 0; j < kWide; j += 2) *reinterpret_cast<uint32_t *>(out + j) = bf16_pair(acc[r][j] * f, acc[r][j + 1] * f);
-    }
-}
-
-uint64_t rows_of(const AttentionCall &c) { return c.head_dim == 256 || c.tree ? 128 : 256; }
+uint64_t rows_of(const AttentionCall &c) { return c.head_dim == 256 ? 128 : 256; }
 uint64_t tokens_of(const AttentionCall &c) { return c.head_dim == 256 ? 64 : 128; }
 
 // Tiles to a head to be expanded ahead: where the host's bounds say that three row tiles or more of a head go over most tokens (with two
 // the expansion in place, which is slower by half a step, costs what the kernel ahead does), up to 2 GB.
 uint64_t dense_tiles(const AttentionCall &c) {
     if (!c.nf4 || (uint64_t)c.most_rows * c.view.group <= 2 * rows_of(c)) return 0;
-    const uint64_t tiles = (uint64_t)c.batch.sequences * std::max<uint64_t>(1, (c.most_tokens + tokens_of(c) - 1) / tokens_of(c));
-    return tiles * c.cache.heads * tokens_of(c) * c.head_dim * 4 <= 1ull << 31 && tiles * c.cache.heads * tokens_of(c) < 1ull << 31 ? tiles : 0;
+    return attention_expanded_tiles(c);
 }
 
 struct Layout {  // of the workspace
@@ -1087,10 +754,10 @@ struct Layout {  // of the workspace
     }
 };
 
-template <int D, bool NF4, bool TREE>
+template <int D, bool NF4>
 int32_t launch(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) {
-    using S = Shape<D, NF4, TREE>;
-    auto kernel = attention_chunk_kernel<D, NF4, TREE>;
+    using S = Shape<D, NF4>;
+    auto kernel = attention_chunk_kernel<D, NF4>;
     NF4_TRY(ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), S::kSmem));
     const uint64_t pool = (uint64_t)c.cache.pages * c.cache.heads * c.cache.page_size;
     CUtensorMap map_k{}, map_v{};
@@ -1113,14 +780,9 @@ int32_t launch(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) 
         if (dense.capacity) {
             uint32_t *const bases = reinterpret_cast<uint32_t *>(workspace + at.bases);
             float2 *const powers = reinterpret_cast<float2 *>(workspace + at.powers);
-            const uint64_t dense_rows = (uint64_t)dense.capacity * c.cache.heads * S::kTokens;
-            NF4_TRY(make_map(&map_k, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, workspace + at.k, dense_rows, D, 2 * D, S::kTokens, 64, CU_TENSOR_MAP_SWIZZLE_128B));
-            NF4_TRY(make_map(&map_v, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, workspace + at.v, dense_rows, D, 2 * D, S::kTokens, 64, CU_TENSOR_MAP_SWIZZLE_128B));
             dense.bases = bases;
             dense.powers = powers;
-            count_launch();
-            NF4_TRY(launch_maybe_overlapped(expand_kernel<D>, dim3(dense.capacity * c.cache.heads), dim3(256), 0, stream, true, c.cache, c.batch,
-                                            reinterpret_cast<uint4 *>(workspace + at.k), reinterpret_cast<uint4 *>(workspace + at.v), bases, powers));
+            NF4_TRY(attention_expand(c, dense.capacity, workspace + at.k, workspace + at.v, bases, powers, &map_k, &map_v, stream));
         }
     }
     const uint32_t ctas = persistent_ctas();
@@ -1129,16 +791,24 @@ int32_t launch(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) 
     return launch_maybe_overlapped(join_pieces_kernel<D, S::kRows>, dim3(ctas, S::kRows / (kJoinRows * kJoinWarps)), dim3(32 * kJoinWarps), 0, stream, true, view,
                                    static_cast<const Split *>(splits));
 }
-template <bool TREE>
-int32_t launch_of(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) {
-    switch (c.head_dim) {
-        case 64: return c.nf4 ? launch<64, true, TREE>(c, workspace, stream) : launch<64, false, TREE>(c, workspace, stream);
-        case 128: return c.nf4 ? launch<128, true, TREE>(c, workspace, stream) : launch<128, false, TREE>(c, workspace, stream);
-        default: return c.nf4 ? launch<256, true, TREE>(c, workspace, stream) : launch<256, false, TREE>(c, workspace, stream);
-    }
-}
 
 }  // namespace
+
+uint64_t attention_expanded_tiles(const AttentionCall &c) {
+    const uint64_t tiles = (uint64_t)c.batch.sequences * std::max<uint64_t>(1, (c.most_tokens + tokens_of(c) - 1) / tokens_of(c));
+    return tiles * c.cache.heads * tokens_of(c) * c.head_dim * 4 <= 1ull << 31 && tiles * c.cache.heads * tokens_of(c) < 1ull << 31 ? tiles : 0;
+}
+
+int32_t attention_expand(const AttentionCall &c, uint32_t capacity, void *k, void *v, uint32_t *bases, float2 *powers, CUtensorMap *map_k, CUtensorMap *map_v,
+                         cudaStream_t stream) {
+    const uint32_t tokens = (uint32_t)tokens_of(c), dim = c.head_dim;
+    const uint64_t rows = (uint64_t)capacity * c.cache.heads * tokens;
+    NF4_TRY(make_map(map_k, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, k, rows, dim, 2 * dim, tokens, 64, CU_TENSOR_MAP_SWIZZLE_128B));
+    NF4_TRY(make_map(map_v, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, v, rows, dim, 2 * dim, tokens, 64, CU_TENSOR_MAP_SWIZZLE_128B));
+    count_launch();
+    return launch_maybe_overlapped(dim == 64 ? expand_kernel<64> : dim == 128 ? expand_kernel<128> : expand_kernel<256>, dim3(capacity * c.cache.heads), dim3(256), 0,
+                                   stream, true, c.cache, c.batch, static_cast<uint4 *>(k), static_cast<uint4 *>(v), bases, powers);
+}
 
 uint64_t attention_chunk_bytes(const AttentionCall &c) {
     return Layout(c).bytes;
@@ -1152,7 +822,11 @@ bool attention_chunk_counts(const AttentionCall &c) {
 }
 
 int32_t attention_chunk(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) {
-    return c.tree ? launch_of<true>(c, workspace, stream) : launch_of<false>(c, workspace, stream);
+    switch (c.head_dim) {
+        case 64: return c.nf4 ? launch<64, true>(c, workspace, stream) : launch<64, false>(c, workspace, stream);
+        case 128: return c.nf4 ? launch<128, true>(c, workspace, stream) : launch<128, false>(c, workspace, stream);
+        default: return c.nf4 ? launch<256, true>(c, workspace, stream) : launch<256, false>(c, workspace, stream);
+    }
 }
 
 }  // namespace nf4

@@ -1,0 +1,747 @@
+// Attention of trees of drafted tokens over the paged cache on the tensor cores: rows are a tree's nodes, which see their sequence's context and those
+// nodes that their masks have.
+//
+// A tree has some tens of nodes, so that a head of the cache serves 20 to 500 rows, and reading the cache, expanding a quantized one, the exponentials
+// and the MMAs take about as long as one another.  A row tile is one MMA tile of 128 rows (a token's query heads are neighbouring rows), which goes over its
+// tokens 128 (a dim of 256: 64) a step.  The line of steps, its shares, pieces and their join are those of the kernel for many rows (attention_steps.cuh).
+//
+// S = Q K^T has two places in tensor memory, so that a step's scores come while the last one's weights are made.  Two softmax warpgroups have
+// half of a step's tokens each, of the same rows (a thread has a row's 64 scores of a step): with largest exponents, sums and an accumulator of
+// results of their own, which become one when a piece ends, so that they have nothing to say to one another before.  (One warpgroup took 2000 cycles
+// a step of 128 tokens, every scheduler having one warp, where the exponentials are 1024; beside eight expanding warps 2400 to 4000.)  With a dim of
+// 256 tensor memory has no room for a second accumulator: one warpgroup, and 64 tokens a step.
+//
+// A quantized cache's codes come to shared memory by 16-byte copies of three warps (bulk copies of a page's sixteen tokens take 135 cycles each whoever
+// waits, 40 a step: 5300 cycles), which find the powers of two for the scales as well and ask the L2 for the tile after; eight warps expand them.  Where three
+// row tiles or more of a head read the cache it is expanded ahead, as for many rows.  Masks are looked at only in the steps that reach behind the
+// context.  Everything else (weights, f16's range, the order of sums) is as in the kernel for many rows, and said there.
+#include <algorithm>
+
+#include "attention_steps.cuh"
+#include "tmap.cuh"
+
+namespace nf4 {
+
+namespace {
+
+constexpr uint32_t kThreads = 640;
+// warps 0-3 and 4-7: softmax; 8-15: codes to f16 (a bf16 cache: the first of them copies); 16, 18, 19: codes' copies; 17: MMAs
+constexpr uint32_t kExpandWarp = 8, kExpandWarps = 8, kCopyWarp = 16, kMmaWarp = 17, kLoaders = 3;
+
+template <int D, bool NF4>
+struct Shape {
+    static constexpr uint32_t kRows = 128, kTokens = D == 256 ? 64 : 128;  // of a step
+    static constexpr uint32_t kHalves = D == 256 ? 1 : 2, kHalf = kTokens / kHalves, kSoftmaxWarps = 4 * kHalves;
+    static constexpr uint32_t kBlocks = D / 64;
+    static constexpr uint32_t kQTile = 128 * D * 2, kTile = kTokens * D * 2, kBox = kTokens * 128;
+    static constexpr uint32_t kCodes = kTokens * D / 2, kRaw = NF4 ? kCodes + kTokens * kBlocks * 4 : 0, kRawSlots = kLoaders;  // codes, then scales
+    static constexpr uint32_t kSlots = D == 64 ? 7 : D == 128 ? (NF4 ? 4 : 6) : NF4 ? 3 : 5;  // of the ring; one more where the table is not needed
+    // codes, then the table on a multiple of its 32 KB, then Q, then the ring (bf16: Q, then the ring)
+    static constexpr uint32_t kSmem = (NF4 ? 65536 : 2048) - 1024 + kQTile + kSlots * kTile;
+    static constexpr uint32_t kS = 0, kO = 256;  // columns of tensor memory: S's two places, then the halves' O's
+    // 640 threads are launched with 96 registers each; what the softmax warpgroups take more the others leave (480 to a thread of each warpgroup together)
+    static constexpr uint32_t kSoftmaxRegs = kHalves == 2 ? 128 : 152, kOtherRegs = kHalves == 2 ? 72 : 80;
+    static_assert(kHalves * kSoftmaxRegs + (5 - kHalves) * kOtherRegs <= 480 && kSlots + 1 <= 8);
+};
+
+constexpr uint32_t kStart = 4;  // (see Walker)
+
+// The n-th chunk that a lane of a softmax warp brings of the queries and takes of the results: its warp's 32 rows, its half's values.
+template <uint32_t LANES>  // to a row
+__device__ __forceinline__ uint32_t row_of_chunk(uint32_t warp, uint32_t lane, uint32_t n) { return (warp & 3u) * 32 + n * (32 / LANES) + lane / LANES; }
+
+__device__ __forceinline__ void cp_async_16_upto(uint32_t dst_smem, const void *src, uint32_t bytes) {  // of the sixteen, and zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst_smem), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {  // once this thread's copies so far have landed
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+template <int D, bool NF4>
+__global__ void __launch_bounds__(kThreads, 1)
+attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const CacheView c, const BatchView b,
+                      const AttentionView a, const Dense dense, uint32_t box_rows, Split *const splits, const FailureRef failure) {
+    using S = Shape<D, NF4>;
+    using Walk = Walker<S::kRows, S::kTokens, kStart, true>;
+    constexpr uint32_t kCopies = !NF4 && D >= 128 ? 2 : 1;  // (as in the kernel for many rows)
+    constexpr uint32_t N = S::kTokens, kBlocks = S::kBlocks, kHalves = S::kHalves, kHalf = S::kHalf;
+    extern __shared__ uint8_t smem_any[];
+    __shared__ __align__(8) uint64_t s_bars[40];
+    __shared__ uint32_t s_tmem, s_bad[8], s_first[6];  // s_bad: of the last eight pieces, its number + 1 where a page was not there
+    __shared__ Share s_share;
+    __shared__ float s_qpower[NF4 ? kHalves * 128 : 1];
+    __shared__ float2 s_powers[8];  // of the last steps' K and V (who writes them is fewer steps ahead of who reads)
+    const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u;
+    const uint32_t base = ptx::smem_addr(smem_any);
+    const uint32_t raw0 = (base + 15u) & ~15u, table = (raw0 + S::kRawSlots * S::kRaw + 32767u) & ~32767u;
+    const uint32_t q0 = NF4 ? table + 32768u : (base + 1023u) & ~1023u, ring0 = q0 + S::kQTile;
+    // s_full, p_ready: of S's places; pv_done: products that a rescaling waits for; pair: the two warps that have the same rows
+    const uint32_t bars = ptx::smem_addr(s_bars), full0 = bars, empty0 = bars + 64, raw_full0 = bars + 128, raw_empty0 = bars + 152, s_full0 = bars + 176,
+                   p_ready0 = bars + 192, pv_done = bars + 208, q_ready = bars + 216, o_done = bars + 224, tail0 = bars + 232, pair0 = bars + 248;
+    if (ring0 + S::kSlots * S::kTile > base + S::kSmem) {
+        ptx::pdl_wait();
+        if (tid == 0) {
+            NF4_REPORT_FAILURE(*failure.flag, *failure.host, 30);
+            splits[blockIdx.x].rows = 0;
+        }
+        return;
+    }
+    if (tid == 0) {
+        for (uint32_t i = 0; i < 8; ++i) {  // (a place more than kSlots may be in use)
+            ptx::mbar_init(full0 + 8 * i, NF4 ? kExpandWarps : kCopies);
+            ptx::mbar_init(empty0 + 8 * i, 1);
+        }
+        for (uint32_t i = 0; i < S::kRawSlots; ++i) {
+            ptx::mbar_init(raw_full0 + 8 * i, 33);  // each lane's copies, and the powers
+            ptx::mbar_init(raw_empty0 + 8 * i, kExpandWarps);
+        }
+        for (uint32_t i = 0; i < 2; ++i) {
+            ptx::mbar_init(s_full0 + 8 * i, 1);
+            ptx::mbar_init(p_ready0 + 8 * i, S::kSoftmaxWarps);
+            ptx::mbar_init(tail0 + 8 * i, 1);
+        }
+        ptx::mbar_init(pv_done, 1);
+        ptx::mbar_init(q_ready, S::kSoftmaxWarps);
+        ptx::mbar_init(o_done, 1);
+        for (uint32_t i = 0; i < 4; ++i) ptx::mbar_init(pair0 + 8 * i, 2);
+        ptx::fence_mbar_init();
+        ptx::fence_proxy_async();
+    }
+    if (tid < 8) s_bad[tid] = 0;
+    if (NF4) {
+        for (uint32_t i = tid; i < 256 * 8; i += kThreads) {  // the table: an entry's copy to a lane
+            const uint32_t byte = i >> 3, entry = level_pair_f16(byte);
+            st_shared_u4(table + byte * 128u + (i & 7u) * 16u, make_uint4(entry, entry, entry, entry));
+        }
+        ptx::fence_proxy_async();  // (copies may come to this place instead)
+    }
+    if (warp == kMmaWarp) {
+        ptx::tmem_alloc(ptx::smem_addr(&s_tmem), 512);
+        ptx::tmem_relinquish();
+    }
+    ptx::pdl_launch_dependents();
+    ptx::pdl_wait();
+
+    // ---- this CTA's share of the line, and where in it begins ----
+    if (warp == 0) {
+        const Share share = share_out<Walk>(c, b, a, s_first);
+        if (lane == 0) {
+            s_share = share;
+            splits[blockIdx.x].rows = 0;
+        }
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    bool ok = true;
+    const bool expanded = NF4 && dense.capacity && __ldg(dense.bases + b.sequences) <= dense.capacity;  // (more tokens than the host knew of: not)
+    const uint32_t slots = S::kSlots + (expanded ? 1u : 0u);
+    auto place_of = [&](uint32_t slot) -> uint32_t { return slot < S::kSlots ? ring0 + slot * S::kTile : table; };
+    auto wait = [&](uint32_t bar, uint32_t parity, int code) {
+        if (ok && !__all_sync(0xffffffffu, ptx::mbar_wait_suspended(bar, parity))) {
+            ok = false;
+            if (lane == 0) NF4_REPORT_FAILURE(*failure.flag, *failure.host, code);
+        }
+    };
+    if (s_first[4] < s_first[5]) {
+        Walk walk{sequence_of(c, b, s_first[0]), s_first[0], s_first[1], s_first[2], s_first[3], s_first[4], s_first[5]};
+        Piece p;
+        if (warp < S::kSoftmaxWarps) {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftmaxRegs));
+            const uint32_t half = warp >> 2, r = tid & 127u;
+            const uint32_t lanes = (warp & 3u) << 21;  // a warp reaches its quarter of tensor memory's lanes
+            const uint32_t ts0 = tmem + S::kS + half * kHalf + lanes, to0 = tmem + S::kO + lanes, to = to0 + half * D;
+            constexpr uint32_t kWide = D / kHalves, kLanes = kWide / 8;  // values of a row that a warp brings and takes; lanes to them
+            uint32_t scores = 0, finished = 0, step = 0, piece = 0;  // steps and pieces so far
+            for (; ok && walk.next(c, b, a, p); step += p.steps, ++piece) {
+                // ---- Q to shared memory ----
+                constexpr uint32_t kBatch = kLanes < 8 ? kLanes : 8;
+                const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a scale below zero: the rows change sign, so that c is not)
+                #pragma unroll 1
+                for (uint32_t i0 = 0; i0 < kLanes; i0 += kBatch) {
+                    uint4 w[kBatch], w2[kBatch];  // w2: of the row's other half, for the largest magnitude
+                    #pragma unroll
+                    for (uint32_t k = 0; k < kBatch; ++k) {
+                        const uint32_t of_tile = row_of_chunk<kLanes>(warp, lane, i0 + k), row = p.r0 + of_tile, token = a.by_group.of(row);
+                        w[k] = w2[k] = make_uint4(0u, 0u, 0u, 0u);
+                        if (of_tile < p.rows) {
+                            const uint4 *const from = reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.q) + (uint64_t)(p.s.row0 + token) * a.ldq +
+                                                                                      (uint64_t)(p.head * a.group + row - token * a.group) * D) + lane % kLanes;
+                            w[k] = __ldg(from + half * kLanes);
+                            if (NF4 && kHalves == 2) w2[k] = __ldg(from + (1 - half) * kLanes);
+                        }
+                    }
+                    #pragma unroll
+                    for (uint32_t k = 0; k < kBatch; ++k) {
+                        const uint32_t of_tile = row_of_chunk<kLanes>(warp, lane, i0 + k);
+                        uint32_t u[4] = {w[k].x ^ flip, w[k].y ^ flip, w[k].z ^ flip, w[k].w ^ flip};
+                        if (NF4) {
+                            constexpr uint32_t kSize = 0x7fff7fffu;  // (bf16 magnitudes go by their bits)
+                            uint32_t two = __vmaxu2(__vmaxu2(u[0] & kSize, u[1] & kSize), __vmaxu2(u[2] & kSize, u[3] & kSize));
+                            two = __vmaxu2(two, __vmaxu2(__vmaxu2(w2[k].x & kSize, w2[k].y & kSize), __vmaxu2(w2[k].z & kSize, w2[k].w & kSize)));
+                            #pragma unroll
+                            for (uint32_t d = 1; d < kLanes; d <<= 1) two = __vmaxu2(two, __shfl_xor_sync(0xffffffffu, two, d));
+                            const uint32_t most = max(two << 16, two & 0xffff0000u);
+                            // the row's largest magnitude is left in [2^11, 2^12)
+                            const int e2 = most ? min(max((int)(most >> 23) - 127 - 11, -100), 115) : 0;
+                            const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+                            #pragma unroll
+                            for (int e = 0; e < 4; ++e) u[e] = pack<true>(__uint_as_float(u[e] << 16) * down, __uint_as_float(u[e] & 0xffff0000u) * down);
+                            if (lane % kLanes == 0) s_qpower[half * 128 + of_tile] = __uint_as_float((uint32_t)(127 + e2) << 23);
+                        }
+                        st_shared_u4(q0 + chunk_place(of_tile, half * kLanes + lane % kLanes), make_uint4(u[0], u[1], u[2], u[3]));
+                    }
+                }
+                ptx::fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(q_ready);
+
+                // ---- the steps ----
+                const bool idle = (warp & 3u) * 32 >= p.rows;  // none of the warp's rows is one: its part of S is never looked at
+                const bool real = r < p.rows;
+                const uint32_t token = a.by_group.of(real ? p.r0 + r : p.r0), node_row = p.s.row0 + token;
+                const int32_t nodes0 = first_node(p.s);
+                const uint32_t sees = real && nodes0 + (int32_t)token >= 0 ? p.s.length : 0u;  // (a node with a negative token sees nothing)
+                const uint32_t context = (uint32_t)max(nodes0, 0);
+                const float row_factor = fabsf(a.scale_log2) * (NF4 ? s_qpower[half * 128 + r] : 1.f);
+                float m = -INFINITY, l = 0.f, ref = 0.f;
+                for (uint32_t j = 0; j < p.steps; ++j, ++scores) {
+                    const uint32_t place = scores & 1u, ts = ts0 + place * N;
+                    wait(s_full0 + 8 * place, (scores / 2) & 1u, 31);
+                    if (!ok) break;
+                    if (idle) {
+                        if (lane == 0) ptx::mbar_arrive(p_ready0 + 8 * place);
+                        continue;
+                    }
+                    ptx::tc_fence_after();
+                    const uint32_t t0 = (p.step0 + j) * N + half * kHalf, lim = sees > t0 ? sees - t0 : 0u;
+                    const bool masked = t0 + kHalf > context;
+                    // (written before the keys' arrival was made known, which the scores are behind)
+                    const float2 powers = NF4 ? ld_shared_f2(ptx::smem_addr(s_powers + ((step + j) & 7u))) : make_float2(1.f, 1.f);
+                    const float factor = fmaxf(row_factor * powers.x, 1.2e-38f);
+                    const float ref_was = ref;
+                    if (NF4) ref = fmaxf(ref, powers.y);
+                    // the step's values are in units of powers.y, the sums in units of ref: 2^-less of that (a difference that is no more
+                    // than 2^-60 of the largest is made that)
+                    const int less = NF4 ? min((int)(__float_as_uint(ref) >> 23) - (int)(__float_as_uint(powers.y) >> 23), 60) : 0;
+                    bool grown = NF4 && ref != ref_was && j;
+                    // Weights by m as it is, and only then the look at the largest score: where it is out of reach, once or twice a
+                    // row, they are made again.  So nothing waits for a maximum, and S need not be held whole.
+                    uint32_t pw[kHalf / 2];
+                    float2 sum;
+                    for (;;) {
+                        const float from = m == -INFINITY ? 0.f : kRaise<NF4> - m - (float)less;
+                        float top[2] = {-INFINITY, -INFINITY};
+                        sum = make_float2(0.f, 0.f);
+                        uint32_t ahead[2][32];  // 32 scores come while 32 are worked on
+                        tmem_ld32(ts, ahead[0]);
+                        #pragma unroll
+                        for (uint32_t k = 0; k < kHalf; k += 32) {
+                            uint32_t (&x)[32] = ahead[k / 32 & 1];
+                            ptx::tmem_wait_ld();
+                            if (k + 32 < kHalf) tmem_ld32(ts + k + 32, ahead[k / 32 + 1 & 1]);
+                            if (masked) {
+                                const uint32_t seen = seen_nodes(a, node_row, (int32_t)(t0 + k) - nodes0) & low_bits(lim > k ? lim - k : 0u);
+                                #pragma unroll
+                                for (uint32_t i = 0; i < 32; ++i) x[i] = seen >> i & 1u ? x[i] : 0xff800000u;
+                            }
+                            #pragma unroll
+                            for (uint32_t i = 0; i < 32; i += 2) {
+                                top[(i >> 1) & 1] = fmaxf(fmaxf(top[(i >> 1) & 1], __uint_as_float(x[i])), __uint_as_float(x[i + 1]));
+                                const float2 e = fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), factor, from);
+                                const float2 w = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+                                sum = add2(sum, w);
+                                pw[(k + i) / 2] = pack<NF4>(w.x, w.y);
+                            }
+                        }
+                        const float high = fmaxf(top[0], top[1]) * factor;
+                        const bool above = __any_sync(0xffffffffu, high > m + 8.f);
+                        if (!above && !grown) break;
+                        float keep = 1.f;
+                        if (above) {
+                            const float now = fmaxf(m, high);
+                            keep = m == -INFINITY ? 0.f : exp2_approx(m - now);
+                            m = now;
+                            l *= keep;
+                        }
+                        if (grown) keep *= ref_was * reciprocal_of_power(ref);
+                        grown = false;
+                        if (j) {  // once the products so far are done
+                            wait(pv_done, (scores - 1) & 1u, 32);
+                            if (!ok) break;
+                            ptx::tc_fence_after();
+                            #pragma unroll 1
+                            for (uint32_t k = 0; k < D; k += 32) {
+                                uint32_t v[32];
+                                tmem_ld32(to + k, v);
+                                ptx::tmem_wait_ld();
+                                #pragma unroll
+                                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * keep);
+                                tmem_st32(to + k, v);
+                            }
+                        }
+                        if (!above) break;
+                    }
+                    if (!ok) break;
+                    l += (sum.x + sum.y) * (NF4 ? __uint_as_float((uint32_t)(127 + less) << 23) : 1.f);
+                    tmem_st32(ts, pw);
+                    ptx::tmem_wait_st();
+                    ptx::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(p_ready0 + 8 * place);
+                }
+                wait(o_done, finished & 1u, 33);
+                ++finished;
+                if (idle) continue;
+                ptx::tc_fence_after();
+
+                // ---- the row's results, through the place of this warp's part of Q (the products are done) so that whole rows go out ----
+                const bool whole = p.steps == p.all;
+                float w0 = 1.f, w1 = 0.f;  // what the halves' results count
+                if (kHalves == 2) {  // this one's largest exponent and sum to the other's warp, and its to this one
+                    const uint32_t own = q0 + chunk_place(r, half * kLanes), other = q0 + chunk_place(r, (1 - half) * kLanes), bar = pair0 + 8 * (warp & 3u);
+                    st_shared_u4(own, make_uint4(__float_as_uint(m), __float_as_uint(l), 0u, 0u));
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(bar);
+                    wait(bar, 0, 33);
+                    const float2 theirs = ld_shared_f2(other);
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(bar);
+                    wait(bar, 1, 33);  // (both have read: results come to these places)
+                    const float now = fmaxf(m, theirs.x), from = now == -INFINITY ? 0.f : now;
+                    w0 = exp2_approx((half ? theirs.x : m) - from);
+                    w1 = exp2_approx((half ? m : theirs.x) - from);
+                    l = fmaf(half ? l : theirs.y, w1, (half ? theirs.y : l) * w0);
+                    m = now;
+                }
+                if (s_bad[piece & 7u] == piece + 1 || !ok) l = __uint_as_float(0x7fc00000u);  // NaN
+                const uint64_t part = (uint64_t)(2 * blockIdx.x + (p.step0 ? 0 : 1)) * S::kRows;
+                if (!whole && half == 0) a.part_ml[part + r] = make_float2(m, l * kLower<NF4>);
+                const float f = (whole ? l == 0.f ? 0.f : 1.f / l : kLower<NF4>) * (NF4 ? ref : 1.f);
+                #pragma unroll 1
+                for (uint32_t pass = 0; pass < (whole ? 1u : 2u); ++pass) {  // bf16 results, or half of the f32 sums at a time
+                    const uint32_t columns = whole ? kWide : kWide / 2, first = half * kWide + pass * columns;
+                    __syncwarp();
+                    #pragma unroll 1
+                    for (uint32_t k = 0; k < columns; k += 16) {
+                        uint32_t x[16], y[16];
+                        ptx::tmem_ld16(to0 + first + k, x);
+                        if (kHalves == 2) ptx::tmem_ld16(to0 + D + first + k, y);
+                        ptx::tmem_wait_ld();
+                        #pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            float v = __uint_as_float(x[i]);
+                            if (kHalves == 2) v = fmaf(__uint_as_float(y[i]), w1, v * w0);
+                            x[i] = __float_as_uint(v * f);
+                        }
+                        const uint32_t at = half * kLanes + (whole ? k / 8 : k / 4);
+                        if (whole) {
+                            #pragma unroll
+                            for (uint32_t i = 0; i < 2; ++i) {
+                                uint32_t u[4];
+                                #pragma unroll
+                                for (int e = 0; e < 4; ++e) u[e] = bf16_pair(__uint_as_float(x[8 * i + 2 * e]), __uint_as_float(x[8 * i + 2 * e + 1]));
+                                st_shared_u4(q0 + chunk_place(r, at + i), make_uint4(u[0], u[1], u[2], u[3]));
+                            }
+                        } else {
+                            #pragma unroll
+                            for (uint32_t i = 0; i < 4; ++i) st_shared_u4(q0 + chunk_place(r, at + i), make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]));
+                        }
+                    }
+                    __syncwarp();
+                    #pragma unroll 4
+                    for (uint32_t i = 0; i < kLanes; ++i) {
+                        const uint32_t of_tile = row_of_chunk<kLanes>(warp, lane, i), xx = lane % kLanes;
+                        const uint4 v = ld_shared_u4(q0 + chunk_place(of_tile, half * kLanes + xx));
+                        if (of_tile >= p.rows) continue;
+                        if (whole) {
+                            const uint32_t q_row = p.r0 + of_tile, of = a.by_group.of(q_row);
+                            *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(a.out) + (uint64_t)(p.s.row0 + of) * a.ldo +
+                                                       (uint64_t)(p.head * a.group + q_row - of * a.group) * D + first + 8 * xx) = v;
+                        } else {
+                            *reinterpret_cast<uint4 *>(a.part_o + (part + of_tile) * D + first + 4 * xx) = v;
+                        }
+                    }
+                }
+                __syncwarp();  // (the next queries come to the same place)
+                if (!whole && p.step0 == 0 && tid == 0) {
+                    const uint32_t more = min(s_share.cta_of(p.line0 + kStart + p.all - 1) - blockIdx.x, gridDim.x - 1 - blockIdx.x);
+                    splits[blockIdx.x] = Split{p.s.row0, p.r0, p.rows, p.head, more};
+                }
+                ptx::tc_fence_before();
+            }
+        } else {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOtherRegs));
+            if (warp == kMmaWarp) {
+                constexpr uint32_t fmt = NF4 ? 0 : 1;
+                constexpr uint32_t idesc_s = ptx::f16_idesc(fmt, 128, N, false, false), idesc_o = ptx::f16_idesc(fmt, 128, D, false, true);
+                uint32_t made = 0, used = 0, rows_in = 0;  // scores, weights and Q's so far
+                Ring ring;  // the next tile of K or V
+                // (by the elected thread) of the keys in a place of the ring, to the place of the n-th
+                auto scores = [&](uint32_t at, uint32_t n) {
+                    const uint64_t qd = ptx::sw128_desc(q0), kd = ptx::sw128_desc(place_of(at));
+                    #pragma unroll
+                    for (uint32_t k = 0; k < D / 16; ++k)
+                        ptx::mma_ss_f16(tmem + S::kS + (n & 1u) * N, qd + (k >> 2) * (16384 >> 4) + (k & 3u) * 2, kd + (k >> 2) * (S::kBox >> 4) + (k & 3u) * 2, idesc_s, k != 0);
+                    ptx::tc_commit(s_full0 + 8 * (n & 1u));
+                    ptx::tc_commit(empty0 + 8 * at);
+                };
+                while (ok && walk.next(c, b, a, p)) {
+                    for (uint32_t j = 0; j < min(2u, p.steps) && ok; ++j, ring.on(slots)) {  // the first scores
+                        wait(full0 + 8 * ring.slot, ring.round & 1u, 36);
+                        if (j == 0) wait(q_ready, rows_in++ & 1u, 36);
+                        ptx::tc_fence_after();
+                        if (ok && ptx::elect_one()) scores(ring.slot, made);
+                        ++made;
+                        __syncwarp();
+                    }
+                    for (uint32_t j = 0; j < p.steps && ok; ++j) {
+                        const Ring v = ring;
+                        ring.on(slots);
+                        wait(full0 + 8 * v.slot, v.round & 1u, 36);
+                        wait(p_ready0 + 8 * (used & 1u), (used / 2) & 1u, 36);
+                        if (!ok) break;
+                        ptx::tc_fence_after();
+                        if (ptx::elect_one()) {
+                            const uint64_t vd = ptx::sw128_desc(place_of(v.slot), S::kBox);
+                            #pragma unroll
+                            for (uint32_t k = 0; k < N / 16; ++k) {
+                                const uint32_t half = k / (kHalf / 16), of_half = k % (kHalf / 16);
+                                ptx::mma_ts_f16(tmem + S::kO + half * D, tmem + S::kS + (used & 1u) * N + half * kHalf + 8 * of_half, vd + 128 * k, idesc_o, j != 0 || of_half != 0);
+                            }
+                            ptx::tc_commit(pv_done);
+                            ptx::tc_commit(empty0 + 8 * v.slot);
+                            if (j + 1 == p.steps) ptx::tc_commit(o_done);
+                        }
+                        ++used;
+                        __syncwarp();
+                        if (j + 2 >= p.steps) continue;
+                        wait(full0 + 8 * ring.slot, ring.round & 1u, 36);
+                        if (!ok) break;
+                        ptx::tc_fence_after();
+                        if (ptx::elect_one()) scores(ring.slot, made);
+                        ++made;
+                        __syncwarp();
+                        ring.on(slots);
+                    }
+                }
+            } else if (NF4 && !expanded && warp >= kExpandWarp && warp < kExpandWarp + kExpandWarps) {
+                // ---- codes to f16: a thread has 16 bytes of a token's row, 32 values ----
+                constexpr uint32_t kLanes = D / 32, kPass = 32 * kExpandWarps / kLanes, kOwn = N / kPass;
+                const uint32_t th = tid - 32 * kExpandWarp, q = th % kLanes, row = th / kLanes, lane_word = table | lane * 4u;
+                // In which order a thread takes its four words: so that eight lanes' 16-byte stores hit all banks
+                const uint32_t order = D == 128 ? (q >> 1) * 2 : D == 256 ? q >> 1 : 0u;
+                uint32_t i = 0, rs = 0, raw_round = 0, step = 0;  // tiles and steps so far
+                Ring ring;
+                for (; ok && walk.next(c, b, a, p); step += p.steps) {
+                    #pragma unroll 1
+                    for (uint32_t turn = 0; ok && turn < 2 * p.steps; ++turn, ++i, ring.on(slots)) {
+                        const Turn<2> of(turn, p.steps);
+                        const uint32_t slot = ring.slot, raw = raw0 + rs * S::kRaw, dst = place_of(slot) + (q >> 1) * S::kBox;
+                        wait(raw_full0 + 8 * rs, raw_round & 1u, 34);
+                        const float2 powers = ld_shared_f2(ptx::smem_addr(s_powers + ((step + of.step) & 7u)));
+                        const float unit = reciprocal_of_power(of.values ? powers.y : powers.x) * (1.f / kLevelUnit);
+                        uint4 raws[kOwn];
+                        uint32_t factors[kOwn];
+                        #pragma unroll
+                        for (uint32_t pass = 0; pass < kOwn; ++pass) {
+                            const uint32_t t = pass * kPass + row;
+                            raws[pass] = ld_shared_u4(raw + t * (D / 2) + q * 16);
+                            float scale;
+                            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale) : "r"(raw + S::kCodes + (t * kBlocks + (q >> 1)) * 4) : "memory");
+                            factors[pass] = pack<true>(scale * unit, scale * unit);
+                        }
+                        if (ring.round) wait(empty0 + 8 * slot, (ring.round + 1) & 1u, 34);
+                        if (!ok) break;
+                        #pragma unroll
+                        for (uint32_t pass = 0; pass < kOwn; ++pass) {
+                            const uint32_t t = pass * kPass + row, s2 = factors[pass];
+                            uint4 w = raws[pass];
+                            if (order & 2u) w = make_uint4(w.z, w.w, w.x, w.y);
+                            if (order & 1u) w = make_uint4(w.y, w.x, w.w, w.z);
+                            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+                            #pragma unroll
+                            for (uint32_t k = 0; k < 4; ++k) {
+                                uint32_t v[4];
+                                #pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const uint32_t word = words[k], at = ((e == 0 ? word << 7 : word >> (8 * e - 7)) & 0x7f80u) | lane_word;
+                                    asm("ld.shared.u32 %0, [%1];" : "=r"(v[e]) : "r"(at));  // (free to move: the table stands)
+                                    v[e] = mul_f16x2(v[e], s2);
+                                }
+                                const uint32_t chunk = (q & 1u) * 4 + (k ^ order);
+                                st_shared_u4(dst + t * 128 + ((chunk ^ (t & 7u)) << 4), make_uint4(v[0], v[1], v[2], v[3]));
+                            }
+                        }
+                        ptx::fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) {
+                            ptx::mbar_arrive(full0 + 8 * slot);
+                            ptx::mbar_arrive(raw_empty0 + 8 * rs);
+                        }
+                        if (++rs == S::kRawSlots) {
+                            rs = 0;
+                            ++raw_round;
+                        }
+                    }
+                }
+            } else if (NF4 && !expanded && warp >= kCopyWarp) {
+                // ---- codes and scales to shared memory: a warp has every third tile, and a slot of its own ----
+                const uint32_t own = warp == kCopyWarp ? 0u : warp - kMmaWarp, raw = raw0 + own * S::kRaw, full = raw_full0 + 8 * own, empty = raw_empty0 + 8 * own;
+                uint32_t turn = own, step = 0, piece = 0;
+                bool more = walk.next(c, b, a, p);
+                struct Tile {
+                    bool real, values, scarce;  // scarce: a page that there is not
+                    uint32_t info, t0, stored, place, piece;  // place: of group `lane`
+                };
+                // the next tile of this warp, and where its tokens are
+                auto look = [&]() -> Tile {
+                    while (more && turn >= 2 * p.steps) {
+                        turn -= 2 * p.steps;
+                        step += p.steps;
+                        ++piece;
+                        more = walk.next(c, b, a, p);
+                    }
+                    Tile t{more, false, false, 0, 0, 0, 0, piece};
+                    if (!more) return t;
+                    const Turn<2> of(turn, p.steps);
+                    turn += kLoaders;
+                    t.values = of.values;
+                    t.info = step + of.step;
+                    t.t0 = (p.step0 + of.step) * N;
+                    t.stored = p.s.length > t.t0 ? min(p.s.length - t.t0, N) : 0u;
+                    if (lane < N / kGroup && lane * kGroup < t.stored) {
+                        const uint32_t token = t.t0 + lane * kGroup, at = c.by_page.of(token);
+                        const int32_t page = __ldg(b.table + (uint64_t)p.seq * b.width + at);
+                        t.scarce = page < 0 || (uint32_t)page >= c.pages;
+                        t.place = t.scarce ? 0u : ((uint32_t)page * c.heads + p.head) * c.page_size + (token - at * c.page_size);
+                    }
+                    return t;
+                };
+                Tile t = look();
+                for (uint32_t n = 0; ok && t.real; ++n) {
+                    if (t.scarce) s_bad[t.piece & 7u] = t.piece + 1;
+                    if (n) wait(empty, (n + 1) & 1u, 35);
+                    if (!ok) break;
+                    const uint8_t *const pool = static_cast<const uint8_t *>(t.values ? c.v : c.k);
+                    const float *const pool_scales = t.values ? c.v_scales : c.k_scales;
+                    #pragma unroll
+                    for (uint32_t i = 0; i < S::kCodes / 512; ++i) {
+                        constexpr uint32_t kOfGroup = D / 2;  // 16-byte pieces
+                        const uint32_t ch = i * 32 + lane, g = ch / kOfGroup;
+                        const uint64_t at = (uint64_t)__shfl_sync(0xffffffffu, t.place, g) * (D / 2) + (ch % kOfGroup) * 16;
+                        cp_async_16_upto(raw + ch * 16, pool + at, ch * 16 / (D / 2) < t.stored ? 16u : 0u);  // (behind the last token anything may stand: zeros)
+                    }
+                    #pragma unroll
+                    for (uint32_t i = 0; i < N * kBlocks / 128; ++i) {
+                        constexpr uint32_t kOfGroup = 4 * kBlocks;
+                        const uint32_t ch = i * 32 + lane, first = ch * 4;  // scales of the tile
+                        const uint64_t at = (uint64_t)__shfl_sync(0xffffffffu, t.place, ch / kOfGroup) * kBlocks + (ch % kOfGroup) * 4;
+                        const uint32_t there = t.stored * kBlocks;
+                        cp_async_16_upto(raw + S::kCodes + ch * 16, pool_scales + at, there > first ? min((there - first) * 4, 16u) : 0u);
+                    }
+                    cp_async_arrive(full);
+                    const Tile next = look();
+                    if (!t.values) {  // the powers that the step's scales are divided by
+                        uint32_t most[2] = {0, 0};
+                        #pragma unroll
+                        for (uint32_t i = 0; i < N * kBlocks / 128; ++i) {
+                            constexpr uint32_t kOfGroup = 4 * kBlocks;
+                            const uint32_t ch = i * 32 + lane, first = ch * 4, there = t.stored * kBlocks;
+                            const uint64_t at = (uint64_t)__shfl_sync(0xffffffffu, t.place, ch / kOfGroup) * kBlocks + (ch % kOfGroup) * 4;
+                            #pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                if (first >= there) continue;
+                                const uint4 v = __ldg(reinterpret_cast<const uint4 *>((e ? c.v_scales : c.k_scales) + at));
+                                const uint32_t bits[4] = {v.x, v.y, v.z, v.w};
+                                #pragma unroll
+                                for (uint32_t x = 0; x < 4; ++x) most[e] = max(most[e], first + x < there ? bits[x] : 0u);
+                            }
+                        }
+                        const float2 powers = make_float2(power_for(__reduce_max_sync(0xffffffffu, most[0])), power_for(__reduce_max_sync(0xffffffffu, most[1])));
+                        if (lane == 0) s_powers[t.info & 7u] = powers;
+                    }
+                    if (lane == 0) ptx::mbar_arrive(full);
+                    // the L2 asked for the next tile's codes and scales
+                    #pragma unroll
+                    for (uint32_t i = 0; i < S::kCodes / 4096; ++i) {
+                        constexpr uint32_t kOfGroup = D / 16;  // lines
+                        const uint32_t line = i * 32 + lane;
+                        const uint64_t at = (uint64_t)__shfl_sync(0xffffffffu, next.place, line / kOfGroup) * (D / 2) + (line % kOfGroup) * 128;
+                        if (line * 128 / (D / 2) < next.stored) asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t *>(next.values ? c.v : c.k) + at));
+                    }
+                    if (!next.values && lane < N / kGroup && lane * kGroup < next.stored) {
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(c.k_scales + (uint64_t)next.place * kBlocks));
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(c.v_scales + (uint64_t)next.place * kBlocks));
+                    }
+                    t = next;
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+            } else if (NF4 ? warp == kCopyWarp : warp >= kExpandWarp && warp < kExpandWarp + 2 * kCopies) {
+                // ---- tiles as they are: of a bf16 cache's pages, or of what was expanded ahead ----
+                const uint32_t own = NF4 ? 0u : (warp - kExpandWarp) & 1u, part = NF4 ? 0u : (warp - kExpandWarp) >> 1;  // bf16: K or V, and which columns
+                const uint32_t unit = box_rows, units = N / unit;  // tokens that come together, being in one page
+                uint32_t tails = 0, step = 0;
+                Ring ring;
+                for (uint32_t piece = 0; ok && walk.next(c, b, a, p); ++piece, step += p.steps) {
+                    const uint32_t tile0 = expanded ? __ldg(dense.bases + p.seq) + p.step0 : 0u;
+                    const uint32_t stored = min(p.s.length, (p.step0 + p.steps) * N);  // tokens that there are
+                    #pragma unroll 1
+                    for (uint32_t turn = 0; ok && turn < 2 * p.steps; ++turn, ring.on(slots)) {
+                        const Turn<2> of(turn, p.steps);
+                        const uint32_t which = of.values, j = of.step;
+                        if (!NF4 && which != own) continue;
+                        const uint32_t t0 = (p.step0 + j) * N, g = lane % units, box = lane / units, t = t0 + g * unit;
+                        const uint32_t groups = stored > t0 ? min(units, (stored - t0 + unit - 1) / unit) : 0u;
+                        const uint32_t slot = ring.slot, dst = place_of(slot);
+                        uint32_t place = 0;
+                        if (NF4) {
+                            if (!which) {
+                                const float2 powers = __ldg(dense.powers + (uint64_t)(tile0 + j) * c.heads + p.head);
+                                if (powers.x == 0.f) s_bad[piece & 7u] = piece + 1;  // (a page that there is not)
+                                if (lane == 0) s_powers[(step + j) & 7u] = powers;
+                            }
+                        } else if (g < groups) {
+                            const uint32_t at = c.by_page.of(t);
+                            const int32_t page = __ldg(b.table + (uint64_t)p.seq * b.width + at);
+                            if (page >= 0 && (uint32_t)page < c.pages) place = ((uint32_t)page * c.heads + p.head) * c.page_size + (t - at * c.page_size);
+                            else s_bad[piece & 7u] = piece + 1;
+                        }
+                        __syncwarp();
+                        if (ring.round) wait(empty0 + 8 * slot, (ring.round + 1) & 1u, 35);
+                        if (!ok) break;
+                        if (NF4) {
+                            const uint32_t bar = full0 + 8 * slot;
+                            if (lane == 0) {
+                                ptx::mbar_arrive_expect_tx(bar, S::kTile);
+                                const int32_t row = (int32_t)(((tile0 + j) * c.heads + p.head) * N);
+                                #pragma unroll
+                                for (uint32_t x = 0; x < D / 64; ++x) ptx::tma_load_2d(dst + x * S::kBox, which ? &tmap_v : &tmap_k, (int32_t)(64 * x), row, bar);
+                                for (uint32_t e = 1; e < kExpandWarps; ++e) ptx::mbar_arrive(bar);  // (for the warps that expand)
+                            }
+                        } else {
+                            const bool tail = which && t0 + N > p.s.length;  // values that anything may stand behind: zeros, for weights of zero
+                            const uint32_t bar = tail ? tail0 + 8 * part : full0 + 8 * slot;
+                            constexpr uint32_t kColumns = D / 64 / kCopies;  // boxes of 64
+                            if (lane == 0) ptx::mbar_arrive_expect_tx(bar, groups * (unit * 128) * kColumns);
+                            __syncwarp();
+                            if (g < groups && box < kColumns) {
+                                const uint32_t x = part * kColumns + box;
+                                ptx::tma_load_2d(dst + x * S::kBox + g * (unit * 128), which ? &tmap_v : &tmap_k, (int32_t)(64 * x), (int32_t)place, bar);
+                            }
+                            if (tail) {
+                                wait(bar, tails & 1u, 35);
+                                ++tails;
+                                for (uint32_t k = (p.s.length > t0 ? p.s.length - t0 : 0u) * 8 + lane; k < N * 8; k += 32)
+                                    #pragma unroll
+                                    for (uint32_t x = 0; x < kColumns; ++x) st_shared_u4(dst + (part * kColumns + x) * S::kBox + k * 16, make_uint4(0u, 0u, 0u, 0u));
+                                ptx::fence_proxy_async();
+                                __syncwarp();
+                                if (lane == 0) ptx::mbar_arrive(full0 + 8 * slot);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+    }
+    if (!ok) ptx::let_flights_land();
+    __syncwarp();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem, 512);
+    }
+}
+
+constexpr uint64_t kTileRows = 128;
+uint64_t tokens_of(const AttentionCall &c) { return c.head_dim == 256 ? 64 : 128; }
+
+// Tiles to a head to be expanded ahead: where the host's bounds say that three row tiles or more of a head go over most tokens.
+uint64_t dense_tiles(const AttentionCall &c) {
+    if (!c.nf4 || (uint64_t)c.most_rows * c.view.group <= 2 * kTileRows) return 0;
+    return attention_expanded_tiles(c);
+}
+
+struct Layout {  // of the workspace
+    uint64_t splits, ml, o, bases, powers, k, v, bytes;
+    explicit Layout(const AttentionCall &c) {
+        uint64_t at = kAttentionFlagBytes;
+        auto take = [&](uint64_t n) {
+            const uint64_t from = at;
+            at += (n + 255) / 256 * 256;
+            return from;
+        };
+        const uint64_t tiles = dense_tiles(c), expanded = tiles * c.cache.heads * tokens_of(c) * c.head_dim * 2;
+        splits = take(kNumSMs * sizeof(Split));
+        ml = take(2ull * kNumSMs * kTileRows * sizeof(float2));
+        o = take(2ull * kNumSMs * kTileRows * c.head_dim * sizeof(float));
+        bases = take(tiles ? (c.batch.sequences + 1ull) * sizeof(uint32_t) : 0);
+        powers = take(tiles * c.cache.heads * sizeof(float2));
+        k = take(expanded);
+        v = take(expanded);
+        bytes = at;
+    }
+};
+
+template <int D, bool NF4>
+int32_t launch(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) {
+    using S = Shape<D, NF4>;
+    auto kernel = attention_tree_kernel<D, NF4>;
+    NF4_TRY(ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), S::kSmem));
+    const uint64_t pool = (uint64_t)c.cache.pages * c.cache.heads * c.cache.page_size;
+    CUtensorMap map_k{}, map_v{};
+    uint32_t box_rows = kGroup;  // tokens of a page that come in one copy
+    while (box_rows < S::kTokens && c.cache.page_size % (2 * box_rows) == 0) box_rows *= 2;
+    if (!NF4) {
+        NF4_TRY(make_map(&map_k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, c.cache.k, pool, D, 2 * D, box_rows, 64, CU_TENSOR_MAP_SWIZZLE_128B));
+        NF4_TRY(make_map(&map_v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, c.cache.v, pool, D, 2 * D, box_rows, 64, CU_TENSOR_MAP_SWIZZLE_128B));
+    }
+    FailureRef failure;
+    NF4_TRY(prefill_failure_ref(&failure));
+    const Layout at(c);
+    Split *const splits = reinterpret_cast<Split *>(workspace + at.splits);
+    AttentionView view = c.view;
+    view.part_ml = reinterpret_cast<float2 *>(workspace + at.ml);
+    view.part_o = reinterpret_cast<float *>(workspace + at.o);
+    Dense dense{};
+    if (NF4) {
+        dense.capacity = (uint32_t)dense_tiles(c);
+        if (dense.capacity) {
+            uint32_t *const bases = reinterpret_cast<uint32_t *>(workspace + at.bases);
+            float2 *const powers = reinterpret_cast<float2 *>(workspace + at.powers);
+            dense.bases = bases;
+            dense.powers = powers;
+            NF4_TRY(attention_expand(c, dense.capacity, workspace + at.k, workspace + at.v, bases, powers, &map_k, &map_v, stream));
+        }
+    }
+    const uint32_t ctas = persistent_ctas();
+    count_launch(2);
+    NF4_TRY(launch_maybe_overlapped(kernel, dim3(ctas), dim3(kThreads), S::kSmem, stream, true, map_k, map_v, c.cache, c.batch, view, dense, box_rows, splits, failure));
+    return launch_maybe_overlapped(join_pieces_kernel<D, S::kRows>, dim3(ctas, S::kRows / (kJoinRows * kJoinWarps)), dim3(32 * kJoinWarps), 0, stream, true, view,
+                                   static_cast<const Split *>(splits));
+}
+
+}  // namespace
+
+uint64_t attention_tree_bytes(const AttentionCall &c) {
+    return Layout(c).bytes;
+}
+
+// The line of steps is counted in 32 bits, and what the page table has room for bounds it.
+bool attention_tree_counts(const AttentionCall &c) {
+    const uint64_t tiles = ((uint64_t)c.batch.rows * c.view.group / kTileRows + c.batch.sequences) * c.cache.heads;
+    const uint64_t steps = ((uint64_t)c.batch.width * c.cache.page_size + tokens_of(c) - 1) / tokens_of(c);
+    return tiles * (steps + 1 + kStart) < 1ull << 31;
+}
+
+int32_t attention_tree(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) {
+    switch (c.head_dim) {
+        case 64: return c.nf4 ? launch<64, true>(c, workspace, stream) : launch<64, false>(c, workspace, stream);
+        case 128: return c.nf4 ? launch<128, true>(c, workspace, stream) : launch<128, false>(c, workspace, stream);
+        default: return c.nf4 ? launch<256, true>(c, workspace, stream) : launch<256, false>(c, workspace, stream);
+    }
+}
+
+}  // namespace nf4

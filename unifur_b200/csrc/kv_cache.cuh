@@ -169,4 +169,9 @@ bool attention_chunk_counts(const AttentionCall &c);
 uint64_t attention_chunk_bytes(const AttentionCall &c);
 int32_t attention_chunk(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream);
 
+// attention_tree.cu: bf16 tensors whose rows are nodes of trees, likewise
+bool attention_tree_counts(const AttentionCall &c);
+uint64_t attention_tree_bytes(const AttentionCall &c);
+int32_t attention_tree(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream);
+
 }  // namespace nf4
