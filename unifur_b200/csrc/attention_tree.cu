@@ -26,7 +26,7 @@ namespace {
 
 constexpr uint32_t kThreads = 640;
 // warps 0-3 and 4-7: softmax; 8-15: codes to f16 (a bf16 cache: the first of them copies); 16, 18, 19: codes' copies; 17: MMAs
-constexpr uint32_t kExpandWarp = 8, kExpandWarps = 8, kCopyWarp = 16, kMmaWarp = 17, kLoaders = 3;
+constexpr uint32_t kExpandWarp = 8, kExpandWarps = 4, kCopyWarp = 16, kMmaWarp = 17, kLoaders = 3;  // kExpandWarps: to a tile
 
 template <int D, bool NF4>
 struct Shape {
@@ -76,8 +76,8 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     const uint32_t raw0 = (base + 15u) & ~15u, table = (raw0 + S::kRawSlots * S::kRaw + 32767u) & ~32767u;
     const uint32_t q0 = NF4 ? table + 32768u : (base + 1023u) & ~1023u, ring0 = q0 + S::kQTile;
     // s_full, p_ready: of S's places; pv_done: products that a rescaling waits for; pair: the two warps that have the same rows
-    const uint32_t bars = ptx::smem_addr(s_bars), full0 = bars, empty0 = bars + 64, raw_full0 = bars + 128, raw_empty0 = bars + 152, s_full0 = bars + 176,
-                   p_ready0 = bars + 192, pv_done = bars + 208, q_ready = bars + 216, o_done = bars + 224, tail0 = bars + 232, pair0 = bars + 248;
+    const uint32_t bars = ptx::smem_addr(s_bars), full0 = bars, empty0 = bars + 64, raw_full0 = bars + 128, raw_empty0 = bars + 176, s_full0 = bars + 200,
+                   p_ready0 = bars + 216, pv_done = bars + 232, q_ready = bars + 240, o_done = bars + 248, tail0 = bars + 256, pair0 = bars + 272;
     if (ring0 + S::kSlots * S::kTile > base + S::kSmem) {
         ptx::pdl_wait();
         if (tid == 0) {
@@ -92,7 +92,8 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
             ptx::mbar_init(empty0 + 8 * i, 1);
         }
         for (uint32_t i = 0; i < S::kRawSlots; ++i) {
-            ptx::mbar_init(raw_full0 + 8 * i, 33);  // each lane's copies, and the powers
+            ptx::mbar_init(raw_full0 + 16 * i, 33);  // each lane's copies, and the powers
+            ptx::mbar_init(raw_full0 + 16 * i + 8, 33);
             ptx::mbar_init(raw_empty0 + 8 * i, kExpandWarps);
         }
         for (uint32_t i = 0; i < 2; ++i) {
@@ -426,20 +427,24 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                         ring.on(slots);
                     }
                 }
-            } else if (NF4 && !expanded && warp >= kExpandWarp && warp < kExpandWarp + kExpandWarps) {
-                // ---- codes to f16: a thread has 16 bytes of a token's row, 32 values ----
+            } else if (NF4 && !expanded && warp >= kExpandWarp && warp < kCopyWarp) {
+                // ---- codes to f16: a thread has 16 bytes of some tokens' rows, 32 values each ----
+                // Two groups of four warps take every second tile (of a piece, whose tiles are an even number): a tile takes a group as long in
+                // accesses' and barriers' latency as in lookups, which the other's then fill.  (Eight warps to a tile: 3600 cycles a step.)
                 constexpr uint32_t kLanes = D / 32, kPass = 32 * kExpandWarps / kLanes, kOwn = N / kPass;
-                const uint32_t th = tid - 32 * kExpandWarp, q = th % kLanes, row = th / kLanes, lane_word = table | lane * 4u;
+                const uint32_t group = (warp - kExpandWarp) / kExpandWarps, th = tid % (32 * kExpandWarps), q = th % kLanes, row = th / kLanes, lane_word = table | lane * 4u;
                 // In which order a thread takes its four words: so that eight lanes' 16-byte stores hit all banks
                 const uint32_t order = D == 128 ? (q >> 1) * 2 : D == 256 ? q >> 1 : 0u;
-                uint32_t i = 0, rs = 0, raw_round = 0, step = 0;  // tiles and steps so far
+                uint32_t raw6 = group, raw_round = 0, step = 0;  // the tile's number modulo two rounds of the raw ring; steps so far
                 Ring ring;
+                if (group) ring.on(slots);
                 for (; ok && walk.next(c, b, a, p); step += p.steps) {
                     #pragma unroll 1
-                    for (uint32_t turn = 0; ok && turn < 2 * p.steps; ++turn, ++i, ring.on(slots)) {
+                    for (uint32_t turn = group; ok && turn < 2 * p.steps; turn += 2) {
                         const Turn<2> of(turn, p.steps);
+                        const uint32_t rs = raw6 % S::kRawSlots, full = raw_full0 + 16 * rs + 8 * (raw6 & 1u);
                         const uint32_t slot = ring.slot, raw = raw0 + rs * S::kRaw, dst = place_of(slot) + (q >> 1) * S::kBox;
-                        wait(raw_full0 + 8 * rs, raw_round & 1u, 34);
+                        wait(full, raw_round & 1u, 34);
                         const float2 powers = ld_shared_f2(ptx::smem_addr(s_powers + ((step + of.step) & 7u)));
                         const float unit = reciprocal_of_power(of.values ? powers.y : powers.x) * (1.f / kLevelUnit);
                         uint4 raws[kOwn];
@@ -480,15 +485,18 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                             ptx::mbar_arrive(full0 + 8 * slot);
                             ptx::mbar_arrive(raw_empty0 + 8 * rs);
                         }
-                        if (++rs == S::kRawSlots) {
-                            rs = 0;
+                        raw6 += 2;
+                        if (raw6 >= 2 * S::kRawSlots) {
+                            raw6 -= 2 * S::kRawSlots;
                             ++raw_round;
                         }
+                        ring.on(slots);
+                        ring.on(slots);
                     }
                 }
             } else if (NF4 && !expanded && warp >= kCopyWarp) {
                 // ---- codes and scales to shared memory: a warp has every third tile, and a slot of its own ----
-                const uint32_t own = warp == kCopyWarp ? 0u : warp - kMmaWarp, raw = raw0 + own * S::kRaw, full = raw_full0 + 8 * own, empty = raw_empty0 + 8 * own;
+                const uint32_t own = warp == kCopyWarp ? 0u : warp - kMmaWarp, raw = raw0 + own * S::kRaw, empty = raw_empty0 + 8 * own;
                 uint32_t turn = own, step = 0, piece = 0;
                 bool more = walk.next(c, b, a, p);
                 struct Tile {
@@ -524,6 +532,9 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                     if (t.scarce) s_bad[t.piece & 7u] = t.piece + 1;
                     if (n) wait(empty, (n + 1) & 1u, 35);
                     if (!ok) break;
+                    // A slot's rounds have two barriers in turn: a group that takes every second tile comes to every second of them, and one barrier's
+                    // parity would show an earlier round as well.
+                    const uint32_t full = raw_full0 + 16 * own + 8 * ((own + n) & 1u);  // (tile own + 3 n)
                     const uint8_t *const pool = static_cast<const uint8_t *>(t.values ? c.v : c.k);
                     const float *const pool_scales = t.values ? c.v_scales : c.k_scales;
                     #pragma unroll
