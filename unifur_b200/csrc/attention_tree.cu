@@ -457,6 +457,8 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                             asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale) : "r"(raw + S::kCodes + (t * kBlocks + (q >> 1)) * 4) : "memory");
                             factors[pass] = pack<true>(scale * unit, scale * unit);
                         }
+                        __syncwarp();
+                        if (lane == 0) ptx::mbar_arrive(raw_empty0 + 8 * rs);  // (all that the slot had is in registers)
                         if (ring.round) wait(empty0 + 8 * slot, (ring.round + 1) & 1u, 34);
                         if (!ok) break;
                         #pragma unroll
@@ -481,10 +483,7 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                         }
                         ptx::fence_proxy_async();
                         __syncwarp();
-                        if (lane == 0) {
-                            ptx::mbar_arrive(full0 + 8 * slot);
-                            ptx::mbar_arrive(raw_empty0 + 8 * rs);
-                        }
+                        if (lane == 0) ptx::mbar_arrive(full0 + 8 * slot);
                         raw6 += 2;
                         if (raw6 >= 2 * S::kRawSlots) {
                             raw6 -= 2 * S::kRawSlots;
@@ -527,9 +526,38 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                     }
                     return t;
                 };
+                // the scales of a step's tokens, of K and of V
+                constexpr uint32_t kQuads = N * kBlocks / 128;
+                uint4 scales[2][kQuads];
+                auto ask_scales = [&](const Tile &t) {
+                    #pragma unroll
+                    for (uint32_t i = 0; i < kQuads; ++i) {
+                        constexpr uint32_t kOfGroup = 4 * kBlocks;
+                        const uint32_t ch = i * 32 + lane;
+                        const uint64_t at = (uint64_t)__shfl_sync(0xffffffffu, t.place, ch / kOfGroup) * kBlocks + (ch % kOfGroup) * 4;
+                        #pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            scales[e][i] = ch * 4 < t.stored * kBlocks ? __ldg(reinterpret_cast<const uint4 *>((e ? c.v_scales : c.k_scales) + at)) : make_uint4(0u, 0u, 0u, 0u);
+                    }
+                };
                 Tile t = look();
+                if (t.real && !t.values) ask_scales(t);
                 for (uint32_t n = 0; ok && t.real; ++n) {
+                    float2 powers = make_float2(0.f, 0.f);
+                    if (!t.values) {
+                        uint32_t most[2] = {0, 0};
+                        #pragma unroll
+                        for (uint32_t i = 0; i < kQuads; ++i)
+                            #pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const uint32_t bits[4] = {scales[e][i].x, scales[e][i].y, scales[e][i].z, scales[e][i].w};
+                                #pragma unroll
+                                for (uint32_t x = 0; x < 4; ++x) most[e] = max(most[e], (i * 32 + lane) * 4 + x < t.stored * kBlocks ? bits[x] : 0u);
+                            }
+                        powers = make_float2(power_for(__reduce_max_sync(0xffffffffu, most[0])), power_for(__reduce_max_sync(0xffffffffu, most[1])));
+                    }
                     if (t.scarce) s_bad[t.piece & 7u] = t.piece + 1;
+                    const Tile next = look();
                     if (n) wait(empty, (n + 1) & 1u, 35);
                     if (!ok) break;
                     // A slot's rounds have two barriers in turn: a group that takes every second tile comes to every second of them, and one barrier's
@@ -553,28 +581,11 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                         cp_async_16_upto(raw + S::kCodes + ch * 16, pool_scales + at, there > first ? min((there - first) * 4, 16u) : 0u);
                     }
                     cp_async_arrive(full);
-                    const Tile next = look();
-                    if (!t.values) {  // the powers that the step's scales are divided by
-                        uint32_t most[2] = {0, 0};
-                        #pragma unroll
-                        for (uint32_t i = 0; i < N * kBlocks / 128; ++i) {
-                            constexpr uint32_t kOfGroup = 4 * kBlocks;
-                            const uint32_t ch = i * 32 + lane, first = ch * 4, there = t.stored * kBlocks;
-                            const uint64_t at = (uint64_t)__shfl_sync(0xffffffffu, t.place, ch / kOfGroup) * kBlocks + (ch % kOfGroup) * 4;
-                            #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                if (first >= there) continue;
-                                const uint4 v = __ldg(reinterpret_cast<const uint4 *>((e ? c.v_scales : c.k_scales) + at));
-                                const uint32_t bits[4] = {v.x, v.y, v.z, v.w};
-                                #pragma unroll
-                                for (uint32_t x = 0; x < 4; ++x) most[e] = max(most[e], first + x < there ? bits[x] : 0u);
-                            }
-                        }
-                        const float2 powers = make_float2(power_for(__reduce_max_sync(0xffffffffu, most[0])), power_for(__reduce_max_sync(0xffffffffu, most[1])));
-                        if (lane == 0) s_powers[t.info & 7u] = powers;
+                    if (lane == 0) {
+                        if (!t.values) s_powers[t.info & 7u] = powers;
+                        ptx::mbar_arrive(full);
                     }
-                    if (lane == 0) ptx::mbar_arrive(full);
-                    // the L2 asked for the next tile's codes and scales
+                    // the L2 asked for the next tile's codes
                     #pragma unroll
                     for (uint32_t i = 0; i < S::kCodes / 4096; ++i) {
                         constexpr uint32_t kOfGroup = D / 16;  // lines
@@ -582,10 +593,7 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                         const uint64_t at = (uint64_t)__shfl_sync(0xffffffffu, next.place, line / kOfGroup) * (D / 2) + (line % kOfGroup) * 128;
                         if (line * 128 / (D / 2) < next.stored) asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t *>(next.values ? c.v : c.k) + at));
                     }
-                    if (!next.values && lane < N / kGroup && lane * kGroup < next.stored) {
-                        asm volatile("prefetch.global.L2 [%0];" ::"l"(c.k_scales + (uint64_t)next.place * kBlocks));
-                        asm volatile("prefetch.global.L2 [%0];" ::"l"(c.v_scales + (uint64_t)next.place * kBlocks));
-                    }
+                    if (next.real && !next.values) ask_scales(next);
                     t = next;
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
