@@ -46,10 +46,12 @@ struct Shape {
 
 constexpr uint32_t kStart = 4;  // (see Walker)
 
-// The n-th chunk that a lane of a softmax warp brings of the queries and takes of the results: its warp's 32 rows, its half's values.
+// The row of the n-th chunk that a lane of a softmax warp takes of the results: its warp's 32 rows, its half's values.
 template <uint32_t LANES>  // to a row
 __device__ __forceinline__ uint32_t row_of_chunk(uint32_t warp, uint32_t lane, uint32_t n) { return (warp & 3u) * 32 + n * (32 / LANES) + lane / LANES; }
 
+__device__ __forceinline__ void take_columns(uint32_t taddr, uint32_t (&r)[16]) { ptx::tmem_ld16(taddr, r); }
+__device__ __forceinline__ void take_columns(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
 __device__ __forceinline__ void cp_async_16_upto(uint32_t dst_smem, const void *src, uint32_t bytes) {  // of the sixteen, and zeros
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst_smem), "l"(src), "r"(bytes) : "memory");
 }
@@ -69,7 +71,7 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     __shared__ __align__(8) uint64_t s_bars[40];
     __shared__ uint32_t s_tmem, s_bad[8], s_first[6];  // s_bad: of the last eight pieces, its number + 1 where a page was not there
     __shared__ Share s_share;
-    __shared__ float s_qpower[NF4 ? kHalves * 128 : 1];
+    __shared__ float s_qpower[NF4 ? 128 : 1];
     __shared__ float2 s_powers[8];  // of the last steps' K and V (who writes them is fewer steps ahead of who reads)
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u;
     const uint32_t base = ptx::smem_addr(smem_any);
@@ -153,45 +155,54 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
             const uint32_t half = warp >> 2, r = tid & 127u;
             const uint32_t lanes = (warp & 3u) << 21;  // a warp reaches its quarter of tensor memory's lanes
             const uint32_t ts0 = tmem + S::kS + half * kHalf + lanes, to0 = tmem + S::kO + lanes, to = to0 + half * D;
-            constexpr uint32_t kWide = D / kHalves, kLanes = kWide / 8;  // values of a row that a warp brings and takes; lanes to them
+            constexpr uint32_t kWide = D / kHalves, kLanes = kWide / 8;  // values of a row's results that a warp takes; lanes to them
             uint32_t scores = 0, finished = 0, step = 0, piece = 0;  // steps and pieces so far
+            // The two warps that have the same rows meet three times a piece.  left: they are still to meet behind the results.
+            const uint32_t pair = pair0 + 8 * (warp & 3u);
+            uint32_t meets = 0;
+            bool left = false;
+            auto come = [&] {
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(pair);
+            };
+            auto meet = [&] { wait(pair, meets++ & 1u, 33); };
             for (; ok && walk.next(c, b, a, p); step += p.steps, ++piece) {
-                // ---- Q to shared memory ----
-                constexpr uint32_t kBatch = kLanes < 8 ? kLanes : 8;
-                const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a scale below zero: the rows change sign, so that c is not)
-                #pragma unroll 1
-                for (uint32_t i0 = 0; i0 < kLanes; i0 += kBatch) {
-                    uint4 w[kBatch], w2[kBatch];  // w2: of the row's other half, for the largest magnitude
-                    #pragma unroll
-                    for (uint32_t k = 0; k < kBatch; ++k) {
-                        const uint32_t of_tile = row_of_chunk<kLanes>(warp, lane, i0 + k), row = p.r0 + of_tile, token = a.by_group.of(row);
-                        w[k] = w2[k] = make_uint4(0u, 0u, 0u, 0u);
-                        if (of_tile < p.rows) {
-                            const uint4 *const from = reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.q) + (uint64_t)(p.s.row0 + token) * a.ldq +
-                                                                                      (uint64_t)(p.head * a.group + row - token * a.group) * D) + lane % kLanes;
-                            w[k] = __ldg(from + half * kLanes);
-                            if (NF4 && kHalves == 2) w2[k] = __ldg(from + (1 - half) * kLanes);
-                        }
-                    }
-                    #pragma unroll
-                    for (uint32_t k = 0; k < kBatch; ++k) {
-                        const uint32_t of_tile = row_of_chunk<kLanes>(warp, lane, i0 + k);
-                        uint32_t u[4] = {w[k].x ^ flip, w[k].y ^ flip, w[k].z ^ flip, w[k].w ^ flip};
+                // ---- Q to shared memory: half of the pair's rows, as they are, and beside a quantized cache then divided by a power of two ----
+                // (Short loops: code that runs once a piece comes from the L2.  Unrolled, with the loads in registers, this took 11000 cycles.)
+                if (left) meet();  // the other warp has taken its results from these rows' places
+                left = false;
+                constexpr uint32_t kRowLanes = D / 8, kRounds = kRowLanes / kHalves, kRowsOfRound = 32 / kRowLanes;
+                const uint32_t first_row = (warp & 3u) * 32 + half * (32 / kHalves) + lane / kRowLanes, chunk = lane % kRowLanes;
+                #pragma unroll 2
+                for (uint32_t i = 0; i < kRounds; ++i) {
+                    const uint32_t of_tile = first_row + i * kRowsOfRound;
+                    const bool real = of_tile < p.rows;
+                    const uint32_t row = real ? p.r0 + of_tile : p.r0, token = a.by_group.of(row);
+                    const __nv_bfloat16 *const from = static_cast<const __nv_bfloat16 *>(a.q) + (uint64_t)(p.s.row0 + token) * a.ldq + (uint64_t)(p.head * a.group + row - token * a.group) * D;
+                    ptx::cp_async_16_or_zero(q0 + chunk_place(of_tile, chunk), from + 8 * chunk, real);
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                if (NF4 || a.scale_log2 < 0.f) {
+                    const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;  // (a scale below zero: the rows change sign, so that c is not)
+                    #pragma unroll 2
+                    for (uint32_t i = 0; i < kRounds; ++i) {  // (a thread changes what it has brought)
+                        const uint32_t of_tile = first_row + i * kRowsOfRound, at = q0 + chunk_place(of_tile, chunk);
+                        const uint4 w = ld_shared_u4(at);
+                        uint32_t u[4] = {w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip};
                         if (NF4) {
                             constexpr uint32_t kSize = 0x7fff7fffu;  // (bf16 magnitudes go by their bits)
                             uint32_t two = __vmaxu2(__vmaxu2(u[0] & kSize, u[1] & kSize), __vmaxu2(u[2] & kSize, u[3] & kSize));
-                            two = __vmaxu2(two, __vmaxu2(__vmaxu2(w2[k].x & kSize, w2[k].y & kSize), __vmaxu2(w2[k].z & kSize, w2[k].w & kSize)));
                             #pragma unroll
-                            for (uint32_t d = 1; d < kLanes; d <<= 1) two = __vmaxu2(two, __shfl_xor_sync(0xffffffffu, two, d));
+                            for (uint32_t d = 1; d < kRowLanes; d <<= 1) two = __vmaxu2(two, __shfl_xor_sync(0xffffffffu, two, d));
                             const uint32_t most = max(two << 16, two & 0xffff0000u);
                             // the row's largest magnitude is left in [2^11, 2^12)
                             const int e2 = most ? min(max((int)(most >> 23) - 127 - 11, -100), 115) : 0;
                             const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
                             #pragma unroll
                             for (int e = 0; e < 4; ++e) u[e] = pack<true>(__uint_as_float(u[e] << 16) * down, __uint_as_float(u[e] & 0xffff0000u) * down);
-                            if (lane % kLanes == 0) s_qpower[half * 128 + of_tile] = __uint_as_float((uint32_t)(127 + e2) << 23);
+                            if (chunk == 0) s_qpower[of_tile] = __uint_as_float((uint32_t)(127 + e2) << 23);
                         }
-                        st_shared_u4(q0 + chunk_place(of_tile, half * kLanes + lane % kLanes), make_uint4(u[0], u[1], u[2], u[3]));
+                        st_shared_u4(at, make_uint4(u[0], u[1], u[2], u[3]));
                     }
                 }
                 ptx::fence_proxy_async();
@@ -205,7 +216,7 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                 const int32_t nodes0 = first_node(p.s);
                 const uint32_t sees = real && nodes0 + (int32_t)token >= 0 ? p.s.length : 0u;  // (a node with a negative token sees nothing)
                 const uint32_t context = (uint32_t)max(nodes0, 0);
-                const float row_factor = fabsf(a.scale_log2) * (NF4 ? s_qpower[half * 128 + r] : 1.f);
+                float row_factor = fabsf(a.scale_log2);
                 float m = -INFINITY, l = 0.f, ref = 0.f;
                 for (uint32_t j = 0; j < p.steps; ++j, ++scores) {
                     const uint32_t place = scores & 1u, ts = ts0 + place * N;
@@ -216,6 +227,7 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                         continue;
                     }
                     ptx::tc_fence_after();
+                    if (NF4 && j == 0) row_factor *= s_qpower[r];  // (the scores are behind both warps' queries)
                     const uint32_t t0 = (p.step0 + j) * N + half * kHalf, lim = sees > t0 ? sees - t0 : 0u;
                     const bool masked = t0 + kHalf > context;
                     // (written before the keys' arrival was made known, which the scores are behind)
@@ -301,15 +313,12 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                 const bool whole = p.steps == p.all;
                 float w0 = 1.f, w1 = 0.f;  // what the halves' results count
                 if (kHalves == 2) {  // this one's largest exponent and sum to the other's warp, and its to this one
-                    const uint32_t own = q0 + chunk_place(r, half * kLanes), other = q0 + chunk_place(r, (1 - half) * kLanes), bar = pair0 + 8 * (warp & 3u);
-                    st_shared_u4(own, make_uint4(__float_as_uint(m), __float_as_uint(l), 0u, 0u));
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(bar);
-                    wait(bar, 0, 33);
-                    const float2 theirs = ld_shared_f2(other);
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(bar);
-                    wait(bar, 1, 33);  // (both have read: results come to these places)
+                    st_shared_u4(q0 + chunk_place(r, half * kLanes), make_uint4(__float_as_uint(m), __float_as_uint(l), 0u, 0u));
+                    come();
+                    meet();
+                    const float2 theirs = ld_shared_f2(q0 + chunk_place(r, (1 - half) * kLanes));
+                    come();
+                    meet();  // (both have read: results come to these places)
                     const float now = fmaxf(m, theirs.x), from = now == -INFINITY ? 0.f : now;
                     w0 = exp2_approx((half ? theirs.x : m) - from);
                     w1 = exp2_approx((half ? m : theirs.x) - from);
@@ -323,15 +332,16 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                 #pragma unroll 1
                 for (uint32_t pass = 0; pass < (whole ? 1u : 2u); ++pass) {  // bf16 results, or half of the f32 sums at a time
                     const uint32_t columns = whole ? kWide : kWide / 2, first = half * kWide + pass * columns;
+                    constexpr uint32_t kTake = kWide == 32 ? 16 : 32;  // columns at a time
                     __syncwarp();
                     #pragma unroll 1
-                    for (uint32_t k = 0; k < columns; k += 16) {
-                        uint32_t x[16], y[16];
-                        ptx::tmem_ld16(to0 + first + k, x);
-                        if (kHalves == 2) ptx::tmem_ld16(to0 + D + first + k, y);
+                    for (uint32_t k = 0; k < columns; k += kTake) {
+                        uint32_t x[kTake], y[kTake];
+                        take_columns(to0 + first + k, x);
+                        if (kHalves == 2) take_columns(to0 + D + first + k, y);
                         ptx::tmem_wait_ld();
                         #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
+                        for (uint32_t i = 0; i < kTake; ++i) {
                             float v = __uint_as_float(x[i]);
                             if (kHalves == 2) v = fmaf(__uint_as_float(y[i]), w1, v * w0);
                             x[i] = __float_as_uint(v * f);
@@ -339,7 +349,7 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                         const uint32_t at = half * kLanes + (whole ? k / 8 : k / 4);
                         if (whole) {
                             #pragma unroll
-                            for (uint32_t i = 0; i < 2; ++i) {
+                            for (uint32_t i = 0; i < kTake / 8; ++i) {
                                 uint32_t u[4];
                                 #pragma unroll
                                 for (int e = 0; e < 4; ++e) u[e] = bf16_pair(__uint_as_float(x[8 * i + 2 * e]), __uint_as_float(x[8 * i + 2 * e + 1]));
@@ -347,7 +357,7 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                             }
                         } else {
                             #pragma unroll
-                            for (uint32_t i = 0; i < 4; ++i) st_shared_u4(q0 + chunk_place(r, at + i), make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]));
+                            for (uint32_t i = 0; i < kTake / 4; ++i) st_shared_u4(q0 + chunk_place(r, at + i), make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]));
                         }
                     }
                     __syncwarp();
@@ -365,7 +375,11 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                         }
                     }
                 }
-                __syncwarp();  // (the next queries come to the same place)
+                if (kHalves == 2) {  // (the next queries come to the same places)
+                    come();
+                    left = true;
+                }
+                __syncwarp();
                 if (!whole && p.step0 == 0 && tid == 0) {
                     const uint32_t more = min(s_share.cta_of(p.line0 + kStart + p.all - 1) - blockIdx.x, gridDim.x - 1 - blockIdx.x);
                     splits[blockIdx.x] = Split{p.s.row0, p.r0, p.rows, p.head, more};
