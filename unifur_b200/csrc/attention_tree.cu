@@ -482,17 +482,20 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                             if (order & 2u) w = make_uint4(w.z, w.w, w.x, w.y);
                             if (order & 1u) w = make_uint4(w.y, w.x, w.w, w.z);
                             const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+                            // (all lookups ahead of the stores, which none could pass: four at a time took the latency of one each)
+                            uint32_t v[4][4];
                             #pragma unroll
-                            for (uint32_t k = 0; k < 4; ++k) {
-                                uint32_t v[4];
+                            for (uint32_t k = 0; k < 4; ++k)
                                 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
                                     const uint32_t word = words[k], at = ((e == 0 ? word << 7 : word >> (8 * e - 7)) & 0x7f80u) | lane_word;
-                                    asm("ld.shared.u32 %0, [%1];" : "=r"(v[e]) : "r"(at));  // (free to move: the table stands)
-                                    v[e] = mul_f16x2(v[e], s2);
+                                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[k][e]) : "r"(at));
                                 }
+                            #pragma unroll
+                            for (uint32_t k = 0; k < 4; ++k) {
                                 const uint32_t chunk = (q & 1u) * 4 + (k ^ order);
-                                st_shared_u4(dst + t * 128 + ((chunk ^ (t & 7u)) << 4), make_uint4(v[0], v[1], v[2], v[3]));
+                                st_shared_u4(dst + t * 128 + ((chunk ^ (t & 7u)) << 4),
+                                             make_uint4(mul_f16x2(v[k][0], s2), mul_f16x2(v[k][1], s2), mul_f16x2(v[k][2], s2), mul_f16x2(v[k][3], s2)));
                             }
                         }
                         ptx::fence_proxy_async();
