@@ -50,6 +50,11 @@ constexpr uint32_t kStart = 4;  // (see Walker)
 template <uint32_t LANES>  // to a row
 __device__ __forceinline__ uint32_t row_of_chunk(uint32_t warp, uint32_t lane, uint32_t n) { return (warp & 3u) * 32 + n * (32 / LANES) + lane / LANES; }
 
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+                 : "memory");
+}
 __device__ __forceinline__ void take_columns(uint32_t taddr, uint32_t (&r)[16]) { ptx::tmem_ld16(taddr, r); }
 __device__ __forceinline__ void take_columns(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
 __device__ __forceinline__ void cp_async_16_upto(uint32_t dst_smem, const void *src, uint32_t bytes) {  // of the sixteen, and zeros
@@ -227,9 +232,12 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                         continue;
                     }
                     ptx::tc_fence_after();
+                    uint32_t x[2][32];  // the row's scores
+                    static_assert(kHalf == 64);
+                    tmem_ld32(ts, x[0]);
+                    tmem_ld32(ts + 32, x[1]);
                     if (NF4 && j == 0) row_factor *= s_qpower[r];  // (the scores are behind both warps' queries)
                     const uint32_t t0 = (p.step0 + j) * N + half * kHalf, lim = sees > t0 ? sees - t0 : 0u;
-                    const bool masked = t0 + kHalf > context;
                     // (written before the keys' arrival was made known, which the scores are behind)
                     const float2 powers = NF4 ? ld_shared_f2(ptx::smem_addr(s_powers + ((step + j) & 7u))) : make_float2(1.f, 1.f);
                     const float factor = fmaxf(row_factor * powers.x, 1.2e-38f);
@@ -238,39 +246,23 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                     // the step's values are in units of powers.y, the sums in units of ref: 2^-less of that (a difference that is no more
                     // than 2^-60 of the largest is made that)
                     const int less = NF4 ? min((int)(__float_as_uint(ref) >> 23) - (int)(__float_as_uint(powers.y) >> 23), 60) : 0;
-                    bool grown = NF4 && ref != ref_was && j;
-                    // Weights by m as it is, and only then the look at the largest score: where it is out of reach, once or twice a
-                    // row, they are made again.  So nothing waits for a maximum, and S need not be held whole.
-                    uint32_t pw[kHalf / 2];
-                    float2 sum;
-                    for (;;) {
-                        const float from = m == -INFINITY ? 0.f : kRaise<NF4> - m - (float)less;
-                        float top[2] = {-INFINITY, -INFINITY};
-                        sum = make_float2(0.f, 0.f);
-                        uint32_t ahead[2][32];  // 32 scores come while 32 are worked on
-                        tmem_ld32(ts, ahead[0]);
+                    const bool grown = NF4 && ref != ref_was && j;
+                    ptx::tmem_wait_ld();
+                    if (t0 + kHalf > context) {
                         #pragma unroll
-                        for (uint32_t k = 0; k < kHalf; k += 32) {
-                            uint32_t (&x)[32] = ahead[k / 32 & 1];
-                            ptx::tmem_wait_ld();
-                            if (k + 32 < kHalf) tmem_ld32(ts + k + 32, ahead[k / 32 + 1 & 1]);
-                            if (masked) {
-                                const uint32_t seen = seen_nodes(a, node_row, (int32_t)(t0 + k) - nodes0) & low_bits(lim > k ? lim - k : 0u);
-                                #pragma unroll
-                                for (uint32_t i = 0; i < 32; ++i) x[i] = seen >> i & 1u ? x[i] : 0xff800000u;
-                            }
+                        for (uint32_t u = 0; u < 2; ++u) {
+                            const uint32_t seen = seen_nodes(a, node_row, (int32_t)(t0 + 32 * u) - nodes0) & low_bits(lim > 32 * u ? lim - 32 * u : 0u);
                             #pragma unroll
-                            for (uint32_t i = 0; i < 32; i += 2) {
-                                top[(i >> 1) & 1] = fmaxf(fmaxf(top[(i >> 1) & 1], __uint_as_float(x[i])), __uint_as_float(x[i + 1]));
-                                const float2 e = fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), factor, from);
-                                const float2 w = make_float2(exp2_approx(e.x), exp2_approx(e.y));
-                                sum = add2(sum, w);
-                                pw[(k + i) / 2] = pack<NF4>(w.x, w.y);
-                            }
+                            for (uint32_t i = 0; i < 32; ++i) x[u][i] = seen >> i & 1u ? x[u][i] : 0xff800000u;
                         }
-                        const float high = fmaxf(top[0], top[1]) * factor;
-                        const bool above = __any_sync(0xffffffffu, high > m + 8.f);
-                        if (!above && !grown) break;
+                    }
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    #pragma unroll
+                    for (uint32_t i = 0; i < 64; i += 2) top[i / 2 % 4] = fmaxf(fmaxf(top[i / 2 % 4], __uint_as_float(x[i / 32][i % 32])), __uint_as_float(x[i / 32][i % 32 + 1]));
+                    const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * factor;
+                    // m stays up to 8 below the largest score: once or twice a row it is out of reach
+                    const bool above = __any_sync(0xffffffffu, high > m + 8.f);
+                    if (above || grown) {
                         float keep = 1.f;
                         if (above) {
                             const float now = fmaxf(m, high);
@@ -279,26 +271,37 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                             l *= keep;
                         }
                         if (grown) keep *= ref_was * reciprocal_of_power(ref);
-                        grown = false;
                         if (j) {  // once the products so far are done
                             wait(pv_done, (scores - 1) & 1u, 32);
                             if (!ok) break;
                             ptx::tc_fence_after();
                             #pragma unroll 1
-                            for (uint32_t k = 0; k < D; k += 32) {
-                                uint32_t v[32];
-                                tmem_ld32(to + k, v);
+                            for (uint32_t k = 0; k < D; k += 16) {
+                                uint32_t v[16];
+                                ptx::tmem_ld16(to + k, v);
                                 ptx::tmem_wait_ld();
                                 #pragma unroll
-                                for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * keep);
-                                tmem_st32(to + k, v);
+                                for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * keep);
+                                tmem_st16(to + k, v);
                             }
                         }
-                        if (!above) break;
                     }
-                    if (!ok) break;
-                    l += (sum.x + sum.y) * (NF4 ? __uint_as_float((uint32_t)(127 + less) << 23) : 1.f);
-                    tmem_st32(ts, pw);
+                    const float from = m == -INFINITY ? 0.f : kRaise<NF4> - m - (float)less;
+                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                    #pragma unroll
+                    for (uint32_t u = 0; u < 2; ++u) {
+                        uint32_t pw[16];
+                        #pragma unroll
+                        for (uint32_t i = 0; i < 32; i += 2) {
+                            const float2 e = fma2(make_float2(__uint_as_float(x[u][i]), __uint_as_float(x[u][i + 1])), factor, from);
+                            const float2 w = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+                            sum[i / 2 % 2] = add2(sum[i / 2 % 2], w);
+                            pw[i / 2] = pack<NF4>(w.x, w.y);
+                        }
+                        tmem_st16(ts + 16 * u, pw);  // (over scores that all of the row's are read of)
+                    }
+                    sum[0] = add2(sum[0], sum[1]);
+                    l += (sum[0].x + sum[0].y) * (NF4 ? __uint_as_float((uint32_t)(127 + less) << 23) : 1.f);
                     ptx::tmem_wait_st();
                     ptx::tc_fence_before();
                     __syncwarp();
