@@ -141,6 +141,35 @@ def test_results_are_the_same_every_time_and_beside_other_sequences(quantized):
     assert all(torch.equal(o, first) for o in outs)
 
 
+@pytest.mark.parametrize("heads,group,dim,page_size", [(4, 4, 128, 32), (2, 16, 64, 16), (2, 5, 256, 48)])
+@pytest.mark.parametrize("quantized", [True, False])
+def test_pieces_of_every_number_of_steps_are_the_same_every_time(quantized, heads, group, dim, page_size):
+    """Sequences of one step, of few, and ones that the shares cut anywhere, between others of unlike scales: what a piece takes of the one before it
+    or after it is none of its own."""
+    rng = np.random.default_rng(6)
+    specs = [(int(n), int(min(n, k))) for n, k in zip(rng.choice([60, 128, 129, 300, 700], 90), rng.integers(20, 60, 90))]
+    batch, pages = batch_of(specs, page_size, seed=1)
+    cache = filled_cache(pages, page_size, heads, dim, quantized, seed=2)
+    for i, (table, length) in enumerate(zip(batch.page_table.tolist(), batch.lengths.tolist())):
+        used = table[:-(-length // page_size)]
+        for t in (cache.k_scales, cache.v_scales) if quantized else (cache.k, cache.v):
+            t[used] *= 2.0 ** float(rng.integers(-12, 12))
+    masks = masks_of("tree", specs, batch, rng)
+    q = torch.randn(batch.rows, heads * group, dim, device=DEV).bfloat16()
+    first = cache.tree_attention(q, masks, batch)
+    ref, spread, reach = tree_reference(cache, batch, q, masks, dim ** -0.5)
+    off = np.abs(first.cpu().double().numpy() - ref)
+    # Keys of such sizes make scores whose errors e = 2 * 2^-11 * reach (a level's rounding and its product's with the scale) are not small, as
+    # `tolerance` takes them to be.  A weight is exp(score) over the sum of all: with scores off by up to e it is between exp(-2 e) and exp(2 e) times
+    # what it should be, so that a result is off by up to (exp(2 e) - 1) * sum(weight * |value|), of which `tolerance` has 2 e.
+    two_e = np.minimum(4 * 2.0 ** -11 * reach[..., None], 50.0)
+    may = tolerance(ref, spread, reach, dim, 700, False, largest(cache)) + (np.expm1(two_e) - two_e) * spread
+    worst = np.unravel_index(np.argmax(off / may), off.shape)
+    assert bool((off <= may).all()), f"{int((off > may).sum())} of {off.size}, {worst}: off by {off[worst]} where {may[worst]} is allowed, 2 e {two_e[worst[:2]]}"
+    for _ in range(60):
+        assert torch.equal(cache.tree_attention(q, masks, batch), first)
+
+
 def test_no_words_no_rows_no_sequences():
     specs = [(50, 3), (7, 7)]
     batch, pages = batch_of(specs, 16)

@@ -317,6 +317,13 @@ bool takes_decode(const AttentionCall &c) {
         return (double)std::min<uint64_t>(all, c.batch.sequences * (((uint64_t)c.most_rows * group + rows - 1) / rows));
     };
     const double steps = c.most_tokens / 128 + 1, heads = c.cache.heads;
+    if (c.tree) {
+        // Likewise, trees having a kernel of their own for many rows (us, first / second; 16 sequences of 8192 tokens, 8 heads of 128, NF4: 16 rows of a head 62 /
+        // 103, 32 rows 112 / 103, 64 rows 209 / 107; bf16: 94 / 98, 174 / 98, 32 rows of 64 81 / 83 and 89 / 72; one sequence, 4 heads, 112 rows, NF4: 8192 tokens
+        // 21 / 20, 65536 93 / 41, four of 512 10 / 18)
+        static constexpr double kTreeStream[2][3] = {{7, 14, 36}, {7, 9, 45}}, kTreeMany[2][3] = {{11, 14, 50}, {13, 16, 55}};
+        return tiles(16) * heads * (32 + steps * kTreeStream[c.nf4][of_dim]) <= tiles(128) * heads * (64 + steps * kTreeMany[c.nf4][of_dim]) + kNumSMs * 90;
+    }
     const double stream = tiles(16) * heads * (32 + steps * kStream[c.nf4][of_dim]);
     const double many = tiles(c.head_dim == 256 ? 128 : 256) * heads * (90 + steps * kMany[c.nf4][of_dim]) + kNumSMs * (c.nf4 ? 200 : 150);
     return stream <= many;

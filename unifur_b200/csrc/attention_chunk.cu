@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 attention_chunk_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const CacheView c, const BatchView b,
                        const AttentionView a, const Dense dense, uint32_t box_rows, Split *const splits, const FailureRef failure) {
     using S = Shape<D, NF4>;
-    using Walk = Walker<S::kRows, S::kTokens, kStart, false>;
+    using Walk = Walker<S::kRows, S::kTokens, kStart, kStart + 2, 0, false>;
     // A bf16 cache's pages may be of sixteen tokens, and a warp asks for boxes one after another: four warps share the asking, a tile's
     // columns between two of them (with one, 137 cycles to a box of 2 KB, the MMAs waited for copies)
     constexpr uint32_t kCopies = !NF4 && D >= 128 ? 2 : 1;

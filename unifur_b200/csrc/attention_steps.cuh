@@ -110,10 +110,11 @@ struct Piece {
 
 // Through a CTA's pieces; every warp goes its own way.  R rows to a tile, N tokens to a step; START: steps' worth of time that a row tile takes beside
 // its steps (its queries in, its results out), counted in the line, or the CTAs that have a prompt's first tiles, of one step each, would be done
-// last; TREE: rows are nodes of trees.
-template <uint32_t R, uint32_t N, uint32_t START, bool TREE>
+// last; LEAST: what a CTA has of the line at least, and where
+// no tile has more than WHOLE a whole tile; TREE: rows are nodes of trees.
+template <uint32_t R, uint32_t N, uint32_t START, uint32_t LEAST, uint32_t WHOLE, bool TREE>
 struct Walker {
-    static constexpr uint32_t kStart = START;
+    static constexpr uint32_t kStart = START, kLeast = LEAST, kWhole = WHOLE;
     Sequence s;
     uint32_t seq, head, tile, off, now, end;
 
@@ -204,11 +205,13 @@ struct Turn {
 template <class Walk>
 __device__ __forceinline__ Share share_out(const CacheView &c, const BatchView &b, const AttentionView &a, uint32_t *first_of) {
     const uint32_t lane = threadIdx.x & 31u;
+    uint32_t longest = 0;  // what a tile has of the line at most
     // a lane a sequence: its steps, all heads
     auto steps_of = [&](uint32_t s0, Sequence &s) -> uint32_t {
         s = Sequence{0, 0, 0};
         if (s0 + lane < b.sequences) s = sequence_of(c, b, s0 + lane);
         const uint32_t tiles = Walk::tiles_of(s, a.group);
+        if (Walk::kWhole && tiles) longest = max(longest, Walk::kStart + Walk::steps_of(s, a, tiles - 1));
         uint32_t sum = 0;
         if (tiles <= 8)
             for (uint32_t t = 0; t < tiles; ++t) sum += Walk::kStart + Walk::steps_of(s, a, t);
@@ -230,8 +233,10 @@ __device__ __forceinline__ Share share_out(const CacheView &c, const BatchView &
         total += steps_of(k, s);
     }
     total = __reduce_add_sync(0xffffffffu, total);
+    if (Walk::kWhole) longest = __reduce_max_sync(0xffffffffu, longest);
     Share share;
-    share.ctas = min(gridDim.x, (total + Walk::kStart + 1) / (Walk::kStart + 2));  // two steps at least
+    const uint32_t least = Walk::kWhole && longest <= Walk::kWhole ? max(longest, Walk::kLeast) : Walk::kLeast;
+    share.ctas = min(gridDim.x, (total + least - 1) / least);
     share.per = share.ctas ? total / share.ctas : 0;
     share.more = share.ctas ? total - share.per * share.ctas : 0;
     const uint32_t first = share.start(blockIdx.x);

@@ -12,7 +12,7 @@
 // 256 tensor memory has no room for a second accumulator: one warpgroup, and 64 tokens a step.
 //
 // A quantized cache's codes come to shared memory by 16-byte copies of three warps (bulk copies of a page's sixteen tokens take 135 cycles each whoever
-// waits, 40 a step: 5300 cycles), which find the powers of two for the scales as well and ask the L2 for the tile after; eight warps expand them.  Where three
+// waits, 40 a step: 5300 cycles), which find the powers of two for the scales as well and ask the L2 for the tile after; eight warps expand them.  Where nine
 // row tiles or more of a head read the cache it is expanded ahead, as for many rows.  Masks are looked at only in the steps that reach behind the
 // context.  Everything else (weights, f16's range, the order of sums) is as in the kernel for many rows, and said there.
 #include <algorithm>
@@ -44,7 +44,7 @@ struct Shape {
     static_assert(kHalves * kSoftmaxRegs + (5 - kHalves) * kOtherRegs <= 480 && kSlots + 1 <= 8);
 };
 
-constexpr uint32_t kStart = 4;  // (see Walker)
+constexpr uint32_t kStart = 4, kLeast = 3, kWhole = 7;  // (see Walker)
 
 // The row of the n-th chunk that a lane of a softmax warp takes of the results: its warp's 32 rows, its half's values.
 template <uint32_t LANES>  // to a row
@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, const CacheView c, const BatchView b,
                       const AttentionView a, const Dense dense, uint32_t box_rows, Split *const splits, const FailureRef failure) {
     using S = Shape<D, NF4>;
-    using Walk = Walker<S::kRows, S::kTokens, kStart, true>;
+    using Walk = Walker<S::kRows, S::kTokens, kStart, kLeast, kWhole, true>;
     constexpr uint32_t kCopies = !NF4 && D >= 128 ? 2 : 1;  // (as in the kernel for many rows)
     constexpr uint32_t N = S::kTokens, kBlocks = S::kBlocks, kHalves = S::kHalves, kHalf = S::kHalf;
     extern __shared__ uint8_t smem_any[];
@@ -77,7 +77,8 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     __shared__ uint32_t s_tmem, s_bad[8], s_first[6];  // s_bad: of the last eight pieces, its number + 1 where a page was not there
     __shared__ Share s_share;
     __shared__ float s_qpower[NF4 ? 128 : 1];
-    __shared__ float2 s_powers[8];  // of the last steps' K and V (who writes them is fewer steps ahead of who reads)
+    __shared__ float2 s_powers[8];  // of the last steps' K and V, for the softmax (who writes them is fewer steps ahead of who reads)
+    __shared__ float s_raw_powers[S::kRawSlots];  // of the tiles in the raw ring
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u;
     const uint32_t base = ptx::smem_addr(smem_any);
     const uint32_t raw0 = (base + 15u) & ~15u, table = (raw0 + S::kRawSlots * S::kRaw + 32767u) & ~32767u;
@@ -452,18 +453,16 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                 const uint32_t group = (warp - kExpandWarp) / kExpandWarps, th = tid % (32 * kExpandWarps), q = th % kLanes, row = th / kLanes, lane_word = table | lane * 4u;
                 // In which order a thread takes its four words: so that eight lanes' 16-byte stores hit all banks
                 const uint32_t order = D == 128 ? (q >> 1) * 2 : D == 256 ? q >> 1 : 0u;
-                uint32_t raw6 = group, raw_round = 0, step = 0;  // the tile's number modulo two rounds of the raw ring; steps so far
+                uint32_t raw6 = group, raw_round = 0;  // the tile's number modulo two rounds of the raw ring
                 Ring ring;
                 if (group) ring.on(slots);
-                for (; ok && walk.next(c, b, a, p); step += p.steps) {
+                while (ok && walk.next(c, b, a, p)) {
                     #pragma unroll 1
                     for (uint32_t turn = group; ok && turn < 2 * p.steps; turn += 2) {
-                        const Turn<2> of(turn, p.steps);
                         const uint32_t rs = raw6 % S::kRawSlots, full = raw_full0 + 16 * rs + 8 * (raw6 & 1u);
                         const uint32_t slot = ring.slot, raw = raw0 + rs * S::kRaw, dst = place_of(slot) + (q >> 1) * S::kBox;
                         wait(full, raw_round & 1u, 34);
-                        const float2 powers = ld_shared_f2(ptx::smem_addr(s_powers + ((step + of.step) & 7u)));
-                        const float unit = reciprocal_of_power(of.values ? powers.y : powers.x) * (1.f / kLevelUnit);
+                        const float unit = reciprocal_of_power(s_raw_powers[rs]) * (1.f / kLevelUnit);
                         uint4 raws[kOwn];
                         uint32_t factors[kOwn];
                         #pragma unroll
@@ -546,7 +545,8 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                     }
                     return t;
                 };
-                // the scales of a step's tokens, of K and of V
+                // The scales of a step's tokens, of K and of V; with the keys for both, whose powers the softmax takes, and with the values again for theirs:
+                // the step's keys may be another warp's, of which this one knows nothing.
                 constexpr uint32_t kQuads = N * kBlocks / 128;
                 uint4 scales[2][kQuads];
                 auto ask_scales = [&](const Tile &t) {
@@ -557,25 +557,22 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                         const uint64_t at = (uint64_t)__shfl_sync(0xffffffffu, t.place, ch / kOfGroup) * kBlocks + (ch % kOfGroup) * 4;
                         #pragma unroll
                         for (int e = 0; e < 2; ++e)
-                            scales[e][i] = ch * 4 < t.stored * kBlocks ? __ldg(reinterpret_cast<const uint4 *>((e ? c.v_scales : c.k_scales) + at)) : make_uint4(0u, 0u, 0u, 0u);
+                            scales[e][i] = ch * 4 < t.stored * kBlocks && (e || !t.values) ? __ldg(reinterpret_cast<const uint4 *>((e ? c.v_scales : c.k_scales) + at)) : make_uint4(0u, 0u, 0u, 0u);
                     }
                 };
                 Tile t = look();
-                if (t.real && !t.values) ask_scales(t);
+                if (t.real) ask_scales(t);
                 for (uint32_t n = 0; ok && t.real; ++n) {
-                    float2 powers = make_float2(0.f, 0.f);
-                    if (!t.values) {
-                        uint32_t most[2] = {0, 0};
+                    uint32_t most[2] = {0, 0};
+                    #pragma unroll
+                    for (uint32_t i = 0; i < kQuads; ++i)
                         #pragma unroll
-                        for (uint32_t i = 0; i < kQuads; ++i)
+                        for (int e = 0; e < 2; ++e) {
+                            const uint32_t bits[4] = {scales[e][i].x, scales[e][i].y, scales[e][i].z, scales[e][i].w};
                             #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const uint32_t bits[4] = {scales[e][i].x, scales[e][i].y, scales[e][i].z, scales[e][i].w};
-                                #pragma unroll
-                                for (uint32_t x = 0; x < 4; ++x) most[e] = max(most[e], (i * 32 + lane) * 4 + x < t.stored * kBlocks ? bits[x] : 0u);
-                            }
-                        powers = make_float2(power_for(__reduce_max_sync(0xffffffffu, most[0])), power_for(__reduce_max_sync(0xffffffffu, most[1])));
-                    }
+                            for (uint32_t x = 0; x < 4; ++x) most[e] = max(most[e], (i * 32 + lane) * 4 + x < t.stored * kBlocks ? bits[x] : 0u);
+                        }
+                    const float2 powers = make_float2(power_for(__reduce_max_sync(0xffffffffu, most[0])), power_for(__reduce_max_sync(0xffffffffu, most[1])));
                     if (t.scarce) s_bad[t.piece & 7u] = t.piece + 1;
                     const Tile next = look();
                     if (n) wait(empty, (n + 1) & 1u, 35);
@@ -602,6 +599,7 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                     }
                     cp_async_arrive(full);
                     if (lane == 0) {
+                        s_raw_powers[own] = t.values ? powers.y : powers.x;
                         if (!t.values) s_powers[t.info & 7u] = powers;
                         ptx::mbar_arrive(full);
                     }
@@ -613,7 +611,7 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                         const uint64_t at = (uint64_t)__shfl_sync(0xffffffffu, next.place, line / kOfGroup) * (D / 2) + (line % kOfGroup) * 128;
                         if (line * 128 / (D / 2) < next.stored) asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t *>(next.values ? c.v : c.k) + at));
                     }
-                    if (next.real && !next.values) ask_scales(next);
+                    if (next.real) ask_scales(next);
                     t = next;
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
@@ -697,10 +695,66 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
 constexpr uint64_t kTileRows = 128;
 uint64_t tokens_of(const AttentionCall &c) { return c.head_dim == 256 ? 64 : 128; }
 
-// Tiles to a head to be expanded ahead: where the host's bounds say that three row tiles or more of a head go over most tokens.
+// Tiles to a head to be expanded ahead: where the host's bounds say that nine row tiles or more of a head go over most tokens.  Expanding 128 tokens of a head
+// ahead takes 29 ns, and saves 3.5 of a row tile's 10.
 uint64_t dense_tiles(const AttentionCall &c) {
-    if (!c.nf4 || (uint64_t)c.most_rows * c.view.group <= 2 * kTileRows) return 0;
+    if (!c.nf4 || (uint64_t)c.most_rows * c.view.group <= 8 * kTileRows) return 0;
     return attention_expanded_tiles(c);
+}
+
+// The row tiles that several CTAs had: a warp to a row.  Its parts' largest exponents and sums come together, a lane to each, and then their results, eight
+// parts asked for at a time and added in the order of the tokens.
+constexpr uint32_t kJoinWarpsOfTree = 8;
+template <int D>
+__global__ void __launch_bounds__(32 * kJoinWarpsOfTree)
+join_rows_kernel(const AttentionView a, const Split *const splits) {
+    constexpr uint32_t kWide = D / 32, kAtOnce = 8;  // values of a row to a lane; parts in flight
+    ptx::pdl_launch_dependents();
+    ptx::pdl_wait();
+    const Split s = splits[blockIdx.x];
+    const uint32_t lane = threadIdx.x & 31u, parts = s.more + 1;
+    const uint32_t r = blockIdx.y * kJoinWarpsOfTree + threadIdx.x / 32;
+    if (r >= s.rows) return;
+    auto part = [&](uint32_t i) { return (uint64_t)(2 * (blockIdx.x + i) + (i ? 0 : 1)) * kTileRows + r; };
+    float m = -INFINITY;
+    for (uint32_t i = lane; i < parts; i += 32) m = fmaxf(m, __ldg(&a.part_ml[part(i)].x));
+    #pragma unroll
+    for (uint32_t d = 1; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    const float from = m == -INFINITY ? 0.f : m;  // (nothing seen: 2^-inf)
+    float sum = 0.f, acc[kWide] = {};
+    for (uint32_t i0 = 0; i0 < parts; i0 += 32) {
+        const float2 ml = i0 + lane < parts ? __ldg(a.part_ml + part(i0 + lane)) : make_float2(-INFINITY, 0.f);
+        const float counts = exp2_approx(ml.x - from);
+        sum = fmaf(counts, ml.y, sum);
+        for (uint32_t i = i0; i < min(parts, i0 + 32); i += kAtOnce) {
+            float v[kAtOnce][kWide];
+            #pragma unroll
+            for (uint32_t k = 0; k < kAtOnce; ++k) {
+                if (i + k >= parts) continue;
+                const float2 *const o = reinterpret_cast<const float2 *>(a.part_o + part(i + k) * D + lane * kWide);
+                #pragma unroll
+                for (uint32_t j = 0; j < kWide; j += 2) {
+                    const float2 w = __ldg(o + j / 2);
+                    v[k][j] = w.x;
+                    v[k][j + 1] = w.y;
+                }
+            }
+            #pragma unroll
+            for (uint32_t k = 0; k < kAtOnce; ++k) {
+                if (i + k >= parts) continue;
+                const float f = __shfl_sync(0xffffffffu, counts, (i + k) & 31u);
+                #pragma unroll
+                for (uint32_t j = 0; j < kWide; ++j) acc[j] = fmaf(f, v[k][j], acc[j]);
+            }
+        }
+    }
+    #pragma unroll
+    for (uint32_t d = 1; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    const float f = sum == 0.f ? 0.f : 1.f / sum;
+    const uint32_t q_row = s.r0 + r, token = a.by_group.of(q_row);
+    __nv_bfloat16 *const out = static_cast<__nv_bfloat16 *>(a.out) + (uint64_t)(s.row0 + token) * a.ldo + (uint64_t)(s.head * a.group + q_row - token * a.group) * D + lane * kWide;
+    #pragma unroll
+    for (uint32_t j = 0; j < kWide; j += 2) *reinterpret_cast<uint32_t *>(out + j) = bf16_pair(acc[j] * f, acc[j + 1] * f);
 }
 
 struct Layout {  // of the workspace
@@ -758,7 +812,7 @@ int32_t launch(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) 
     const uint32_t ctas = persistent_ctas();
     count_launch(2);
     NF4_TRY(launch_maybe_overlapped(kernel, dim3(ctas), dim3(kThreads), S::kSmem, stream, true, map_k, map_v, c.cache, c.batch, view, dense, box_rows, splits, failure));
-    return launch_maybe_overlapped(join_pieces_kernel<D, S::kRows>, dim3(ctas, S::kRows / (kJoinRows * kJoinWarps)), dim3(32 * kJoinWarps), 0, stream, true, view,
+    return launch_maybe_overlapped(join_rows_kernel<D>, dim3(ctas, S::kRows / kJoinWarpsOfTree), dim3(32 * kJoinWarpsOfTree), 0, stream, true, view,
                                    static_cast<const Split *>(splits));
 }
 
