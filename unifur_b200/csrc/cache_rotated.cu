@@ -16,7 +16,7 @@ namespace {
 
 constexpr uint32_t kMostThreads = 256;
 constexpr uint32_t kStarts = 1024;                 // row_starts that a CTA holds; of more, every second, third, ...
-constexpr uint32_t kMostRows = kMostThreads / 4;   // of a CTA
+constexpr uint32_t kMostRows = 96;                 // of a CTA
 
 struct Rotated {
     const void *k, *v, *q;
@@ -26,8 +26,8 @@ struct Rotated {
     const int32_t *positions;
     uint32_t table_positions, rotary_dim, q_heads;
     bool pairs;
-    // CTAs take `abreast` rows (blockIdx.x) and of each `width` vectors at a time, `batch` times (blockIdx.y: which)
-    uint32_t width, abreast;
+    // CTAs take `rounds` times `abreast` rows (blockIdx.x) and of each `width` vectors at a time, BATCH times (blockIdx.y: which)
+    uint32_t width, abreast, rounds;
 };
 
 // Two groups of eight values turned.  pairs: neighbours, with four cosines and sines to a group.
@@ -46,8 +46,8 @@ append_rotated_kernel(const CacheView c, const BatchView b, const Rotated t) {
     __shared__ int64_t s_places[kMostRows];
     __shared__ int32_t s_positions[kMostRows];
     const uint32_t tid = threadIdx.x, lane = tid % L, slot = tid / L, of_cta = slot / t.width, first = blockIdx.y * t.width * BATCH + (slot - of_cta * t.width);
-    const uint32_t row0 = blockIdx.x * t.abreast, row = row0 + of_cta, vectors = t.q_heads + 2 * c.heads;
-    const bool any = of_cta < t.abreast && row < b.rows;
+    const uint32_t rows = t.abreast * t.rounds, row0 = blockIdx.x * rows, vectors = t.q_heads + 2 * c.heads;
+    const bool any = of_cta < t.abreast;
     if (NF4)
         for (uint32_t i = tid; i < kCellWords; i += blockDim.x) s_cells[i] = c_cell_table[i];
     // the thread's groups; turned[]: whether the rotation has them
@@ -68,12 +68,11 @@ append_rotated_kernel(const CacheView c, const BatchView b, const Rotated t) {
     ptx::pdl_wait();
     ptx::pdl_launch_dependents();
 
-    // ---- all that the thread takes is asked for ----
+    // ---- all that the thread takes of a row is asked for: of the first ahead of the rows' places, of the next ones as registers become free ----
     uint4 raw[BATCH][2][kQuads];
-    #pragma unroll
-    for (uint32_t u = 0; u < BATCH; ++u) {
+    auto ask = [&](uint32_t u, uint32_t row) {
         const uint32_t vec = first + u * t.width;
-        if (!any || vec >= vectors) continue;
+        if (!any || vec >= vectors || row >= b.rows) return;
         const bool is_q = vec < t.q_heads, is_v = vec >= t.q_heads + c.heads;
         const uint32_t head = is_q ? vec : is_v ? vec - t.q_heads - c.heads : vec - t.q_heads;
         const uint8_t *const from = static_cast<const uint8_t *>(is_q ? t.q : is_v ? t.v : t.k) + ((uint64_t)row * (is_q ? t.ldq : is_v ? t.ldv : t.ldk) + (uint64_t)head * D) * kBytes;
@@ -81,144 +80,151 @@ append_rotated_kernel(const CacheView c, const BatchView b, const Rotated t) {
         for (int e = 0; e < 2; ++e)
             #pragma unroll
             for (uint32_t k = 0; k < kQuads; ++k) raw[u][e][k] = __ldcs(reinterpret_cast<const uint4 *>(from + group[e] * 8 * kBytes) + k);
-    }
+    };
+    #pragma unroll
+    for (uint32_t u = 0; u < BATCH; ++u) ask(u, row0 + of_cta);
     // ---- the rows' places and positions (while the values come) ----
     const uint32_t step = (b.sequences + kStarts - 1) / kStarts;
     for (uint32_t i = tid; i * step < b.sequences; i += blockDim.x) s_starts[i] = __ldg(b.starts + i * step);
     __syncthreads();
-    if (tid < t.abreast) {
+    for (uint32_t i = tid; i < rows; i += blockDim.x) {
         int64_t place = kNoRow, token = -1;
         int32_t position = -1;
-        if (row0 + tid < b.rows) {
-            if (t.positions) position = __ldg(t.positions + row0 + tid);
-            place = place_of_row(c, b, s_starts, step, row0 + tid, token);
+        if (row0 + i < b.rows) {
+            if (t.positions) position = __ldg(t.positions + row0 + i);
+            place = place_of_row(c, b, s_starts, step, row0 + i, token);
             if (!t.positions) position = (int32_t)token;
         }
         const bool there = position >= 0 && (uint32_t)position < t.table_positions;
-        s_positions[tid] = there ? position : -1;
-        s_places[tid] = there || place == kNoRow ? place : kNowhere;
+        s_positions[i] = there ? position : -1;
+        s_places[i] = there || place == kNoRow ? place : kNowhere;
     }
     __syncthreads();
-    const int64_t place = any ? s_places[of_cta] : kNoRow;
-    const int32_t position = any ? s_positions[of_cta] : -1;
-    float cosines[8], sines[8];  // halves: of the two groups' pairs; neighbours: four to a group
-    #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        cosines[i] = 1.f;
-        sines[i] = 0.f;
-    }
-    if (position >= 0 && place != kNoRow) {
-        const float *const angles = t.table + (uint64_t)position * t.rotary_dim;
-        auto four = [&](float *to, const float *from) {
-            const float4 w = __ldg(reinterpret_cast<const float4 *>(from));
-            to[0] = w.x; to[1] = w.y; to[2] = w.z; to[3] = w.w;
-        };
-        if (t.pairs) {
-            #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                if (turned[e]) {
-                    four(cosines + 4 * e, angles + 4 * group[e]);
-                    four(sines + 4 * e, angles + t.rotary_dim / 2 + 4 * group[e]);
-                }
-        } else if (turned[0]) {
-            #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                four(cosines + 4 * e, angles + 8 * group[0] + 4 * e);
-                four(sines + 4 * e, angles + t.rotary_dim / 2 + 8 * group[0] + 4 * e);
-            }
-        }
-    }
-
-    #pragma unroll
-    for (uint32_t u = 0; u < BATCH; ++u) {
-        const uint32_t vec = first + u * t.width;
-        const bool here = any && vec < vectors && place != kNoRow;
-        const bool is_q = vec < t.q_heads, is_v = vec >= t.q_heads + c.heads;
-        const uint32_t head = is_q ? vec : is_v ? vec - t.q_heads - c.heads : vec - t.q_heads;
-        const bool turns = here && !is_v;
-        float v[2][8];
+    for (uint32_t round = 0; round < t.rounds; ++round) {  // (by all of a warp's threads)
+        const uint32_t in_cta = of_cta + round * t.abreast, row = row0 + in_cta;
+        if (__all_sync(0xffffffffu, row >= b.rows)) break;
+        const int64_t place = any ? s_places[in_cta] : kNoRow;
+        const int32_t position = any ? s_positions[in_cta] : -1;
+        float cosines[8], sines[8];  // halves: of the two groups' pairs; neighbours: four to a group
         #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            #pragma unroll
-            for (int i = 0; i < 8; ++i) v[e][i] = 0.f;
-            if (!here) continue;
-            if constexpr (BF16) {
-                values_of_bf16(raw[u][e][0], v[e]);
-            } else {
-                #pragma unroll
-                for (uint32_t k = 0; k < kQuads; ++k) {
-                    v[e][4 * k] = __uint_as_float(raw[u][e][k].x); v[e][4 * k + 1] = __uint_as_float(raw[u][e][k].y);
-                    v[e][4 * k + 2] = __uint_as_float(raw[u][e][k].z); v[e][4 * k + 3] = __uint_as_float(raw[u][e][k].w);
-                }
-            }
+        for (int i = 0; i < 8; ++i) {
+            cosines[i] = 1.f;
+            sines[i] = 0.f;
         }
-        if (turns) {
+        if (position >= 0 && place != kNoRow) {
+            const float *const angles = t.table + (uint64_t)position * t.rotary_dim;
+            auto four = [&](float *to, const float *from) {
+                const float4 w = __ldg(reinterpret_cast<const float4 *>(from));
+                to[0] = w.x; to[1] = w.y; to[2] = w.z; to[3] = w.w;
+            };
             if (t.pairs) {
                 #pragma unroll
                 for (int e = 0; e < 2; ++e)
-                    if (turned[e])
-                        #pragma unroll
-                        for (int i = 0; i < 4; ++i) turn(v[e][2 * i], v[e][2 * i + 1], cosines[4 * e + i], sines[4 * e + i]);
+                    if (turned[e]) {
+                        four(cosines + 4 * e, angles + 4 * group[e]);
+                        four(sines + 4 * e, angles + t.rotary_dim / 2 + 4 * group[e]);
+                    }
             } else if (turned[0]) {
                 #pragma unroll
-                for (int i = 0; i < 8; ++i) turn(v[0][i], v[1][i], cosines[i], sines[i]);
-            }
-        }
-        if (here && is_q) {
-            uint8_t *const to = static_cast<uint8_t *>(t.q_out) + ((uint64_t)row * t.ldo + (uint64_t)head * D) * kBytes;
-            #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                if (position < 0)
-                    #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[e][i] = __uint_as_float(0x7fc00000u);  // NaN
-                uint4 *const at = reinterpret_cast<uint4 *>(to + group[e] * 8 * kBytes);
-                if constexpr (BF16) {
-                    *at = make_uint4(bf16_pair(v[e][0], v[e][1]), bf16_pair(v[e][2], v[e][3]), bf16_pair(v[e][4], v[e][5]), bf16_pair(v[e][6], v[e][7]));
-                } else {
-                    #pragma unroll
-                    for (int k = 0; k < 2; ++k)
-                        reinterpret_cast<float4 *>(at)[k] = make_float4(v[e][4 * k], v[e][4 * k + 1], v[e][4 * k + 2], v[e][4 * k + 3]);
+                for (int e = 0; e < 2; ++e) {
+                    four(cosines + 4 * e, angles + 8 * group[0] + 4 * e);
+                    four(sines + 4 * e, angles + t.rotary_dim / 2 + 8 * group[0] + 4 * e);
                 }
             }
         }
-        const bool stored = here && !is_q && place >= 0;
-        const uint64_t to = ((uint64_t)place + (uint64_t)head * c.page_size) * (D / 8);  // in groups
-        void *const pool = const_cast<void *>(is_v ? c.v : c.k);
-        if (!NF4) {
-            #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                if (stored)
-                    static_cast<uint4 *>(pool)[to + group[e]] =
-                        make_uint4(bf16_pair(v[e][0], v[e][1]), bf16_pair(v[e][2], v[e][3]), bf16_pair(v[e][4], v[e][5]), bf16_pair(v[e][6], v[e][7]));
-            continue;
-        }
-        if (!__any_sync(0xffffffffu, stored)) continue;
-        // a block's largest magnitude is its groups', which its vector's lanes have
-        float most[kBlocks];
+
         #pragma unroll
-        for (uint32_t k = 0; k < kBlocks; ++k) most[k] = 0.f;
-        #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            float m = 0.f;  // (NaNs drop out)
+        for (uint32_t u = 0; u < BATCH; ++u) {
+            const uint32_t vec = first + u * t.width;
+            const bool here = any && vec < vectors && place != kNoRow;
+            const bool is_q = vec < t.q_heads, is_v = vec >= t.q_heads + c.heads;
+            const uint32_t head = is_q ? vec : is_v ? vec - t.q_heads - c.heads : vec - t.q_heads;
+            const bool turns = here && !is_v;
+            float v[2][8];
             #pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[e][i]));
+            for (int e = 0; e < 2; ++e) {
+                #pragma unroll
+                for (int i = 0; i < 8; ++i) v[e][i] = 0.f;
+                if (!here) continue;
+                if constexpr (BF16) {
+                    values_of_bf16(raw[u][e][0], v[e]);
+                } else {
+                    #pragma unroll
+                    for (uint32_t k = 0; k < kQuads; ++k) {
+                        v[e][4 * k] = __uint_as_float(raw[u][e][k].x); v[e][4 * k + 1] = __uint_as_float(raw[u][e][k].y);
+                        v[e][4 * k + 2] = __uint_as_float(raw[u][e][k].z); v[e][4 * k + 3] = __uint_as_float(raw[u][e][k].w);
+                    }
+                }
+            }
+            if (round + 1 < t.rounds) ask(u, row + t.abreast);
+            if (turns) {
+                if (t.pairs) {
+                    #pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        if (turned[e])
+                            #pragma unroll
+                            for (int i = 0; i < 4; ++i) turn(v[e][2 * i], v[e][2 * i + 1], cosines[4 * e + i], sines[4 * e + i]);
+                } else if (turned[0]) {
+                    #pragma unroll
+                    for (int i = 0; i < 8; ++i) turn(v[0][i], v[1][i], cosines[i], sines[i]);
+                }
+            }
+            if (here && is_q) {
+                uint8_t *const to = static_cast<uint8_t *>(t.q_out) + ((uint64_t)row * t.ldo + (uint64_t)head * D) * kBytes;
+                #pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if (position < 0)
+                        #pragma unroll
+                        for (int i = 0; i < 8; ++i) v[e][i] = __uint_as_float(0x7fc00000u);  // NaN
+                    uint4 *const at = reinterpret_cast<uint4 *>(to + group[e] * 8 * kBytes);
+                    if constexpr (BF16) {
+                        *at = make_uint4(bf16_pair(v[e][0], v[e][1]), bf16_pair(v[e][2], v[e][3]), bf16_pair(v[e][4], v[e][5]), bf16_pair(v[e][6], v[e][7]));
+                    } else {
+                        #pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            reinterpret_cast<float4 *>(at)[k] = make_float4(v[e][4 * k], v[e][4 * k + 1], v[e][4 * k + 2], v[e][4 * k + 3]);
+                    }
+                }
+            }
+            const bool stored = here && !is_q && place >= 0;
+            const uint64_t to = ((uint64_t)place + (uint64_t)head * c.page_size) * (D / 8);  // in groups
+            void *const pool = const_cast<void *>(is_v ? c.v : c.k);
+            if (!NF4) {
+                #pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (stored)
+                        static_cast<uint4 *>(pool)[to + group[e]] =
+                            make_uint4(bf16_pair(v[e][0], v[e][1]), bf16_pair(v[e][2], v[e][3]), bf16_pair(v[e][4], v[e][5]), bf16_pair(v[e][6], v[e][7]));
+                continue;
+            }
+            if (!__any_sync(0xffffffffu, stored)) continue;
+            // a block's largest magnitude is its groups', which its vector's lanes have
+            float most[kBlocks];
+            #pragma unroll
+            for (uint32_t k = 0; k < kBlocks; ++k) most[k] = 0.f;
+            #pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float m = 0.f;  // (NaNs drop out)
+                #pragma unroll
+                for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(v[e][i]));
+                #pragma unroll
+                for (uint32_t k = 0; k < kBlocks; ++k)
+                    if (group[e] / 8 == k) most[k] = fmaxf(most[k], m);
+            }
             #pragma unroll
             for (uint32_t k = 0; k < kBlocks; ++k)
-                if (group[e] / 8 == k) most[k] = fmaxf(most[k], m);
-        }
-        #pragma unroll
-        for (uint32_t k = 0; k < kBlocks; ++k)
+                #pragma unroll
+                for (uint32_t d = 1; d < L; d <<= 1) most[k] = fmaxf(most[k], __shfl_xor_sync(0xffffffffu, most[k], d));
+            if (!stored) continue;
+            float *const scales = const_cast<float *>(is_v ? c.v_scales : c.k_scales);
             #pragma unroll
-            for (uint32_t d = 1; d < L; d <<= 1) most[k] = fmaxf(most[k], __shfl_xor_sync(0xffffffffu, most[k], d));
-        if (!stored) continue;
-        float *const scales = const_cast<float *>(is_v ? c.v_scales : c.k_scales);
-        #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            float m = most[0];
-            #pragma unroll
-            for (uint32_t k = 1; k < kBlocks; ++k) m = group[e] / 8 == k ? most[k] : m;
-            static_cast<uint32_t *>(pool)[to + group[e]] = codes_of_group(v[e], m, s_cells);
-            if ((group[e] & 7u) == 0) scales[(to + group[e]) / 8] = m;
+            for (int e = 0; e < 2; ++e) {
+                float m = most[0];
+                #pragma unroll
+                for (uint32_t k = 1; k < kBlocks; ++k) m = group[e] / 8 == k ? most[k] : m;
+                static_cast<uint32_t *>(pool)[to + group[e]] = codes_of_group(v[e], m, s_cells);
+                if ((group[e] & 7u) == 0) scales[(to + group[e]) / 8] = m;
+            }
         }
     }
 }
@@ -262,15 +268,20 @@ int32_t nf4_cache_append_rotated_dev(const nf4_cache *cache, const nf4_cache_bat
         NF4_TRY(check_rows(what, "q_out", q_out, &ldo, q_width, io_dtype));
         if (q == q_out && ldq != ldo) return fail(NF4_ERR_INVALID_ARG, "%s: q_out is q with another row stride", what);
     }
-    Rotated t{k, v, q, q_out, ldk, ldv, ldq, ldo, rotation->table, rotation->positions, rotation->table_positions, rotation->rotary_dim, q_heads, rotation->pairs != 0, 0, 0};
+    Rotated t{k, v, q, q_out, ldk, ldv, ldq, ldo, rotation->table, rotation->positions, rotation->table_positions, rotation->rotary_dim, q_heads, rotation->pairs != 0, 0, 0, 1};
     const uint32_t lanes = cache->head_dim / 16, slots = kMostThreads / lanes, vectors = q_heads + 2 * cache->heads;
     // One vector to a thread where that leaves no SM more than two CTAs: such a call takes what its chain of loads takes.  Else four.
     const uint32_t batch_of = (uint64_t)batch->rows * vectors <= 2ull * kNumSMs * slots ? 1 : 4;
     const uint32_t across = (vectors + slots * batch_of - 1) / (slots * batch_of);  // CTAs to a row
     t.width = (vectors + across * batch_of - 1) / (across * batch_of);
     t.abreast = std::max(1u, slots / t.width);
-    const uint32_t threads = (t.abreast * t.width * lanes + 31) / 32 * 32;
-    const dim3 grid((batch->rows + t.abreast - 1) / t.abreast, across);
+    // A CTA finds its rows' places once, a chain of four loads: so many rounds that the CTAs which an SM has registers for (128 a thread) do all (measured with 7,345
+    // rows of 28 + 8 heads of 128, NF4 / bf16: one round to a CTA 46 / 39 us, as many as that 29 / 25)
+    const uint32_t threads = (t.abreast * t.width * lanes + 31) / 32 * 32, ctas = kNumSMs * std::max(1u, 512u / threads);
+    const uint64_t in_turn = ((uint64_t)batch->rows + t.abreast - 1) / t.abreast * across;
+    t.rounds = (uint32_t)std::min<uint64_t>(kMostRows / t.abreast, (in_turn + ctas - 1) / ctas);
+    const uint32_t rows_of_cta = t.abreast * t.rounds;
+    const dim3 grid((batch->rows + rows_of_cta - 1) / rows_of_cta, across);
     const bool nf4 = cache->form == NF4_CACHE_NF4, bf16 = io_dtype == NF4_DTYPE_BF16;
     count_launch();
     return launch_maybe_overlapped(cache->head_dim == 64 ? kernel_of<64>(nf4, bf16, batch_of) : cache->head_dim == 128 ? kernel_of<128>(nf4, bf16, batch_of) : kernel_of<256>(nf4, bf16, batch_of),

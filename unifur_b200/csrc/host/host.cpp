@@ -718,24 +718,26 @@ PyObject *cache_append_rotated(PyObject *, PyObject *const *v, Py_ssize_t n) {
     });
 }
 
-// cache_tree(<cache, batch>, parents, masks, positions)
+// cache_tree(<cache, batch>, parents, masks or None, positions or None) -> (masks, positions)
 PyObject *cache_tree(PyObject *, PyObject *const *v, Py_ssize_t n) {
     return guarded([&]() -> PyObject * {
         expect(n, kCacheArgs + 3);
         const CacheCall c = cache_call(v);
-        const Tensor &masks = tensor(v[kCacheArgs + 1]);
         const int64_t rows = c.batch.rows;
         const int32_t *parents = words_of(tensor(v[kCacheArgs]), c, {rows}, "parents");
+        const Tensor *given[2] = {tensor_or_none(v[kCacheArgs + 1]), tensor_or_none(v[kCacheArgs + 2])};
+        Place place(c.k->device());
+        const int64_t words = ((int64_t)(c.batch.max_rows ? c.batch.max_rows : c.batch.rows) + 31) / 32;
+        Tensor masks = given[0] ? *given[0] : empty({rows, words}, at::kInt, place), positions = given[1] ? *given[1] : empty({rows}, at::kInt, place);
         require(masks.dim() == 2 && masks.size(1) < 1ll << 31, "masks is [rows, words]");
         uint32_t *m = reinterpret_cast<uint32_t *>(words_of(masks, c, {rows, masks.size(1)}, "masks"));
-        int32_t *p = words_of(tensor(v[kCacheArgs + 2]), c, {rows}, "positions");
-        Place place(c.k->device());
+        int32_t *p = words_of(positions, c, {rows}, "positions");
         check(unlocked([&] { return nf4_cache_tree_dev(&c.cache, &c.batch, parents, m, (uint32_t)masks.size(1), p, place.stream); }));
-        Py_RETURN_NONE;
+        return pair(std::move(masks), std::move(positions));
     });
 }
 
-// cache_keep(<cache, batch>, kept, counts, lengths)
+// cache_keep(<cache, batch>, kept, counts, lengths or None) -> lengths
 PyObject *cache_keep(PyObject *, PyObject *const *v, Py_ssize_t n) {
     return guarded([&]() -> PyObject * {
         expect(n, kCacheArgs + 3);
@@ -744,10 +746,12 @@ PyObject *cache_keep(PyObject *, PyObject *const *v, Py_ssize_t n) {
         const int64_t sequences = c.batch.sequences;
         require(kept.dim() == 2 && kept.size(1) < 1ll << 31, "kept is [sequences, nodes]");
         const int32_t *path = words_of(kept, c, {sequences, kept.size(1)}, "kept"), *counts = words_of(tensor(v[kCacheArgs + 1]), c, {sequences}, "counts");
-        int32_t *lengths = words_of(tensor(v[kCacheArgs + 2]), c, {sequences}, "out");
+        const Tensor *given = tensor_or_none(v[kCacheArgs + 2]);
         Place place(c.k->device());
-        check(unlocked([&] { return nf4_cache_keep_dev(&c.cache, &c.batch, path, (uint32_t)kept.size(1), counts, lengths, place.stream); }));
-        Py_RETURN_NONE;
+        Tensor lengths = given ? *given : empty({sequences}, at::kInt, place);
+        int32_t *to = words_of(lengths, c, {sequences}, "out");
+        check(unlocked([&] { return nf4_cache_keep_dev(&c.cache, &c.batch, path, (uint32_t)kept.size(1), counts, to, place.stream); }));
+        return THPVariable_Wrap(std::move(lengths));
     });
 }
 

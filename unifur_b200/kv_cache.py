@@ -146,12 +146,8 @@ class PagedKvCache:
         ``j % 32`` of word ``j / 32`` for node ``j``: the node itself and its ancestors) and positions (int32 ``[rows]``: the
         context's length and the node's depth).  There are as many words as ``max_rows`` (or ``rows``) needs, or as ``out`` has: nodes behind
         them are seen by none.  Rows of no sequence are left as ``out`` has them, and without ``out`` undefined."""
-        if out is None:
-            words = ((batch.max_rows or batch.rows) + 31) // 32
-            out = (torch.empty(batch.rows, words, dtype=torch.int32, device=self.k.device),
-                   torch.empty(batch.rows, dtype=torch.int32, device=self.k.device))
-        _lib.host().cache_tree(*self._args(), *batch._args(), parents, *out)
-        return out
+        masks, positions = out if out is not None else (None, None)
+        return _lib.host().cache_tree(*self._args(), *batch._args(), parents, masks, positions)
 
     def tree_attention(self, q: torch.Tensor, masks: torch.Tensor, batch: CacheBatch, scale: Optional[float] = None,
                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -167,7 +163,4 @@ class PagedKvCache:
         increase along it, move to the places behind the context.  Returns the sequences' new lengths, the context's and ``counts`` (in ``out``,
         which may be ``batch.lengths`` where no other cache is still to be moved).  A path ends ahead of the first entry that is not above the
         one before it, or that is no node."""
-        if out is None:
-            out = torch.empty_like(batch.lengths)
-        _lib.host().cache_keep(*self._args(), *batch._args(), kept, counts, out)
-        return out
+        return _lib.host().cache_keep(*self._args(), *batch._args(), kept, counts, out)
