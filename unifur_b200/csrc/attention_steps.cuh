@@ -93,6 +93,7 @@ __device__ __forceinline__ float reciprocal_of_power(float p) { return __uint_as
 // How the line of steps is shared out: `per` to a CTA, one more to the first `more` of them.
 struct Share {
     uint32_t per, more, ctas;
+    bool whole;  // a tile belongs to the CTA in whose share it begins
     __device__ uint32_t start(uint32_t cta) const { return per * cta + min(cta, more); }
     __device__ uint32_t cta_of(uint32_t u) const {
         const uint32_t first = (per + 1) * more;
@@ -110,13 +111,15 @@ struct Piece {
 
 // Through a CTA's pieces; every warp goes its own way.  R rows to a tile, N tokens to a step; START: steps' worth of time that a row tile takes beside
 // its steps (its queries in, its results out), counted in the line, or the CTAs that have a prompt's first tiles, of one step each, would be done
-// last; LEAST: what a CTA has of the line at least, and where
-// no tile has more than WHOLE a whole tile; TREE: rows are nodes of trees.
+// last; LEAST: what a CTA has of the line at least; WHOLE: how much
+// more than its share a CTA may have where no row tile is divided then, in place of the second start and the join (0: tiles are divided); TREE: rows
+// are nodes of trees.
 template <uint32_t R, uint32_t N, uint32_t START, uint32_t LEAST, uint32_t WHOLE, bool TREE>
 struct Walker {
     static constexpr uint32_t kStart = START, kLeast = LEAST, kWhole = WHOLE;
     Sequence s;
     uint32_t seq, head, tile, off, now, end;
+    bool whole;
 
     static __device__ __forceinline__ uint32_t tiles_of(const Sequence &s, uint32_t group) { return (uint32_t)(((uint64_t)s.rows * group + R - 1) / R); }
     // (a tile that sees nothing has one step all the same: its results are zeros)
@@ -149,7 +152,7 @@ struct Walker {
         p.all = steps_of(s, a, tile);
         p.line0 = now - off;
         // of the tile's place in the line [line0, line0 + kStart + all) the steps are behind kStart
-        const uint32_t upto = min(p.all + kStart, end - p.line0);
+        const uint32_t upto = WHOLE && whole ? p.all + kStart : min(p.all + kStart, end - p.line0);
         p.step0 = off > kStart ? off - kStart : 0u;
         p.steps = (upto > kStart ? upto - kStart : 0u) - p.step0;
         now = p.line0 + upto;
@@ -205,13 +208,17 @@ struct Turn {
 template <class Walk>
 __device__ __forceinline__ Share share_out(const CacheView &c, const BatchView &b, const AttentionView &a, uint32_t *first_of) {
     const uint32_t lane = threadIdx.x & 31u;
-    uint32_t longest = 0;  // what a tile has of the line at most
+    uint32_t longest = 0, shortest = 0xffffffffu, all_tiles = 0;  // what a tile has of the line at most and at least
     // a lane a sequence: its steps, all heads
     auto steps_of = [&](uint32_t s0, Sequence &s) -> uint32_t {
         s = Sequence{0, 0, 0};
         if (s0 + lane < b.sequences) s = sequence_of(c, b, s0 + lane);
         const uint32_t tiles = Walk::tiles_of(s, a.group);
-        if (Walk::kWhole && tiles) longest = max(longest, Walk::kStart + Walk::steps_of(s, a, tiles - 1));
+        if (Walk::kWhole && tiles) {
+            longest = max(longest, Walk::kStart + Walk::steps_of(s, a, tiles - 1));
+            shortest = min(shortest, Walk::kStart + Walk::steps_of(s, a, 0));
+            all_tiles += tiles * c.heads;
+        }
         uint32_t sum = 0;
         if (tiles <= 8)
             for (uint32_t t = 0; t < tiles; ++t) sum += Walk::kStart + Walk::steps_of(s, a, t);
@@ -233,14 +240,20 @@ __device__ __forceinline__ Share share_out(const CacheView &c, const BatchView &
         total += steps_of(k, s);
     }
     total = __reduce_add_sync(0xffffffffu, total);
-    if (Walk::kWhole) longest = __reduce_max_sync(0xffffffffu, longest);
     Share share;
-    const uint32_t least = Walk::kWhole && longest <= Walk::kWhole ? max(longest, Walk::kLeast) : Walk::kLeast;
-    share.ctas = min(gridDim.x, (total + least - 1) / least);
+    share.ctas = min(gridDim.x, (total + Walk::kLeast - 1) / Walk::kLeast);
+    share.whole = false;
+    if (Walk::kWhole) {
+        longest = __reduce_max_sync(0xffffffffu, longest);
+        shortest = __reduce_min_sync(0xffffffffu, shortest);
+        all_tiles = __reduce_add_sync(0xffffffffu, all_tiles);
+        // (no share is as long as a tile then, so that none has two that begin in it)
+        share.whole = all_tiles <= gridDim.x && (uint64_t)shortest * share.ctas >= total && (uint64_t)(longest - min(longest, Walk::kWhole)) * share.ctas <= total;
+    }
     share.per = share.ctas ? total / share.ctas : 0;
     share.more = share.ctas ? total - share.per * share.ctas : 0;
     const uint32_t first = share.start(blockIdx.x);
-    uint32_t last = blockIdx.x < share.ctas ? share.start(blockIdx.x + 1) : first, before = 0;
+    uint32_t last = blockIdx.x < share.ctas ? share.start(blockIdx.x + 1) : first, before = 0, skipped = 0;
     bool found = false;
     for (uint32_t k = 0; first < last && k < b.sequences; k += 32) {
         Sequence s = s0;
@@ -277,6 +290,11 @@ __device__ __forceinline__ Share share_out(const CacheView &c, const BatchView &
                 if (t0 + 32 >= Walk::tiles_of(o, a.group)) break;  // (not reached where row starts do not decrease: the head has that many steps)
                 left -= __shfl_sync(0xffffffffu, sum, 31);
             }
+            if (Walk::kWhole && share.whole && left) {  // on to the next tile's beginning
+                skipped = Walk::kStart + Walk::steps_of(o, a, tile) - left;
+                left = 0;
+                ++tile;
+            }
             if (lane == 0) {
                 first_of[0] = k + l;
                 first_of[1] = head;
@@ -289,7 +307,7 @@ __device__ __forceinline__ Share share_out(const CacheView &c, const BatchView &
     }
     if (!found) last = first;  // (row starts that decrease, whose rows are more than the line is counted for: no access by what is not there)
     if (lane == 0) {
-        first_of[4] = first;
+        first_of[4] = first + skipped;
         first_of[5] = last;
     }
     return share;
