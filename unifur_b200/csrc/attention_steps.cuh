@@ -112,7 +112,7 @@ struct Piece {
 // Through a CTA's pieces; every warp goes its own way.  R rows to a tile, N tokens to a step; START: steps' worth of time that a row tile takes beside
 // its steps (its queries in, its results out), counted in the line, or the CTAs that have a prompt's first tiles, of one step each, would be done
 // last; LEAST: what a CTA has of the line at least; WHOLE: how much
-// more than its share a CTA may have where no row tile is divided then, in place of the second start and the join (0: tiles are divided); TREE: rows
+// more than its share a CTA may have at least where no row tile is divided then, in place of the second start and the join (0: tiles are divided); TREE: rows
 // are nodes of trees.
 template <uint32_t R, uint32_t N, uint32_t START, uint32_t LEAST, uint32_t WHOLE, bool TREE>
 struct Walker {
@@ -248,7 +248,8 @@ __device__ __forceinline__ Share share_out(const CacheView &c, const BatchView &
         shortest = __reduce_min_sync(0xffffffffu, shortest);
         all_tiles = __reduce_add_sync(0xffffffffu, all_tiles);
         // (no share is as long as a tile then, so that none has two that begin in it)
-        share.whole = all_tiles <= gridDim.x && (uint64_t)shortest * share.ctas >= total && (uint64_t)(longest - min(longest, Walk::kWhole)) * share.ctas <= total;
+        const uint32_t of_share = share.ctas ? total / share.ctas : 0, more = Walk::kWhole + min(4u, of_share / 12);  // (a long tile's start and results are more, too)
+        share.whole = all_tiles <= gridDim.x && (uint64_t)shortest * share.ctas >= total && (uint64_t)(longest - min(longest, more)) * share.ctas <= total;
     }
     share.per = share.ctas ? total / share.ctas : 0;
     share.more = share.ctas ? total - share.per * share.ctas : 0;

@@ -44,7 +44,7 @@ struct Shape {
     static_assert(kHalves * kSoftmaxRegs + (5 - kHalves) * kOtherRegs <= 480 && kSlots + 1 <= 8);
 };
 
-constexpr uint32_t kStart = 4, kLeast = 3, kWhole = 7;  // (see Walker)
+constexpr uint32_t kStart = 4, kLeast = 3, kWhole = 6;  // (see Walker)
 
 // The row of the n-th chunk that a lane of a softmax warp takes of the results: its warp's 32 rows, its half's values.
 template <uint32_t LANES>  // to a row
