@@ -7,14 +7,19 @@
 //
 // S = Q K^T has two places in tensor memory, so that a step's scores come while the last one's weights are made.  Two softmax warpgroups have
 // half of a step's tokens each, of the same rows (a thread has a row's 64 scores of a step): with largest exponents, sums and an accumulator of
-// results of their own, which become one when a piece ends, so that they have nothing to say to one another before.  (One warpgroup took 2000 cycles
-// a step of 128 tokens, every scheduler having one warp, where the exponentials are 1024; beside eight expanding warps 2400 to 4000.)  With a dim of
-// 256 tensor memory has no room for a second accumulator: one warpgroup, and 64 tokens a step.
+// results of their own, which become one when a piece ends, so that they have nothing to say to one another before.  (One warpgroup: 2000 cycles a step of 128
+// tokens over a bf16 cache, where the exponentials and the MMAs are 1024 each, and 2400 to 4000 beside eight warps that expand; two: 1700 and 2500.)  With a
+// dim of 256 tensor memory has no room for a second accumulator: one warpgroup, and 64 tokens a step.
 //
 // A quantized cache's codes come to shared memory by 16-byte copies of three warps (bulk copies of a page's sixteen tokens take 135 cycles each whoever
 // waits, 40 a step: 5300 cycles), which find the powers of two for the scales as well and ask the L2 for the tile after; eight warps expand them.  Where nine
 // row tiles or more of a head read the cache it is expanded ahead, as for many rows.  Masks are looked at only in the steps that reach behind the
-// context.  Everything else (weights, f16's range, the order of sums) is as in the kernel for many rows, and said there.
+// context.
+//
+// Measured (16 sequences of 8192 tokens, 8 heads of 128): bf16, 16 to 64 rows of a head, 89 us = 6.0 TB/s; NF4, 16 to 128 rows, 97 to 99 us, 2800 cycles a step,
+// in which a scheduler issues 2000 instructions for two softmax and two expanding warps.  Tried for those, with no gain: a fourth of the words expanded by byte permutes of
+// the levels' bytes in place of lookups, half of the exponentials by FMA, a step's first scores asked for during the last one's weights, up to 64 rows in
+// the tile twice with a softmax warp to each scheduler.  Everything else (weights, f16's range, the order of sums) is as in the kernel for many rows, and said there.
 #include <algorithm>
 
 #include "attention_steps.cuh"
@@ -35,9 +40,14 @@ struct Shape {
     static constexpr uint32_t kBlocks = D / 64;
     static constexpr uint32_t kQTile = 128 * D * 2, kTile = kTokens * D * 2, kBox = kTokens * 128;
     static constexpr uint32_t kCodes = kTokens * D / 2, kRaw = NF4 ? kCodes + kTokens * kBlocks * 4 : 0, kRawSlots = kLoaders;  // codes, then scales
-    static constexpr uint32_t kSlots = D == 64 ? 7 : D == 128 ? (NF4 ? 4 : 6) : NF4 ? 3 : 5;  // of the ring; one more where the table is not needed
-    // codes, then the table on a multiple of its 32 KB, then Q, then the ring (bf16: Q, then the ring)
-    static constexpr uint32_t kSmem = (NF4 ? 65536 : 2048) - 1024 + kQTile + kSlots * kTile;
+    // A table entry's copies to the lanes are 256 bytes apart where there is room, so that a byte permute makes a whole address (a dim of 128: 3 % of the
+    // time, though the ring has a place less), else 128.
+    static constexpr bool kApart = NF4 && D <= 128;
+    static constexpr uint32_t kStride = kApart ? 256 : 128, kTable = 256 * kStride;
+    static constexpr uint32_t kSlots = D == 64 ? (NF4 ? 6 : 7) : D == 128 ? (NF4 ? 3 : 6) : NF4 ? 3 : 5;  // of the ring; one more where the table is not needed
+    // Q and codes, then the table on a multiple of its 64 KB, then the ring; or codes, then the table on a multiple of its 32 KB, then Q, then the ring;
+    // or (bf16) Q, then the ring
+    static constexpr uint32_t kSmem = (kApart ? 131072 : (NF4 ? 65536 : 2048) + kQTile) - 1024 + kSlots * kTile;
     static constexpr uint32_t kS = 0, kO = 256;  // columns of tensor memory: S's two places, then the halves' O's
     // 640 threads are launched with 96 registers each; what the softmax warpgroups take more the others leave (480 to a thread of each warpgroup together)
     static constexpr uint32_t kSoftmaxRegs = kHalves == 2 ? 128 : 152, kOtherRegs = kHalves == 2 ? 72 : 80;
@@ -81,8 +91,9 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     __shared__ float s_raw_powers[S::kRawSlots];  // of the tiles in the raw ring
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31u;
     const uint32_t base = ptx::smem_addr(smem_any);
-    const uint32_t raw0 = (base + 15u) & ~15u, table = (raw0 + S::kRawSlots * S::kRaw + 32767u) & ~32767u;
-    const uint32_t q0 = NF4 ? table + 32768u : (base + 1023u) & ~1023u, ring0 = q0 + S::kQTile;
+    const uint32_t aligned = (base + 1023u) & ~1023u, raw0 = S::kApart ? aligned + S::kQTile : (base + 15u) & ~15u;
+    const uint32_t table = (raw0 + S::kRawSlots * S::kRaw + S::kTable - 1) & ~(S::kTable - 1);
+    const uint32_t q0 = NF4 && !S::kApart ? table + S::kTable : aligned, ring0 = S::kApart ? table + S::kTable : q0 + S::kQTile;
     // s_full, p_ready: of S's places; pv_done: products that a rescaling waits for; pair: the two warps that have the same rows
     const uint32_t bars = ptx::smem_addr(s_bars), full0 = bars, empty0 = bars + 64, raw_full0 = bars + 128, raw_empty0 = bars + 176, s_full0 = bars + 200,
                    p_ready0 = bars + 216, pv_done = bars + 232, q_ready = bars + 240, o_done = bars + 248, tail0 = bars + 256, pair0 = bars + 272;
@@ -120,7 +131,7 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     if (NF4) {
         for (uint32_t i = tid; i < 256 * 8; i += kThreads) {  // the table: an entry's copy to a lane
             const uint32_t byte = i >> 3, entry = level_pair_f16(byte);
-            st_shared_u4(table + byte * 128u + (i & 7u) * 16u, make_uint4(entry, entry, entry, entry));
+            st_shared_u4(table + byte * S::kStride + (i & 7u) * 16u, make_uint4(entry, entry, entry, entry));
         }
         ptx::fence_proxy_async();  // (copies may come to this place instead)
     }
@@ -448,7 +459,7 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
             } else if (NF4 && !expanded && warp >= kExpandWarp && warp < kCopyWarp) {
                 // ---- codes to f16: a thread has 16 bytes of some tokens' rows, 32 values each ----
                 // Two groups of four warps take every second tile (of a piece, whose tiles are an even number): a tile takes a group as long in
-                // accesses' and barriers' latency as in lookups, which the other's then fill.  (Eight warps to a tile: 3600 cycles a step.)
+                // accesses' and barriers' latency as in lookups, which the other's then fill.  (Eight warps to a tile: 126 us in place of 120 for the case above, as it was then.)
                 constexpr uint32_t kLanes = D / 32, kPass = 32 * kExpandWarps / kLanes, kOwn = N / kPass;
                 const uint32_t group = (warp - kExpandWarp) / kExpandWarps, th = tid % (32 * kExpandWarps), q = th % kLanes, row = th / kLanes, lane_word = table | lane * 4u;
                 // In which order a thread takes its four words: so that eight lanes' 16-byte stores hit all banks
@@ -490,7 +501,8 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                             for (uint32_t k = 0; k < 4; ++k)
                                 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
-                                    const uint32_t word = words[k], at = ((e == 0 ? word << 7 : word >> (8 * e - 7)) & 0x7f80u) | lane_word;
+                                    const uint32_t word = words[k], at = S::kApart ? __byte_perm(word, lane_word, 0x7604u | ((uint32_t)e << 4))
+                                                                                   : ((e == 0 ? word << 7 : word >> (8 * e - 7)) & 0x7f80u) | lane_word;
                                     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[k][e]) : "r"(at));
                                 }
                             #pragma unroll
