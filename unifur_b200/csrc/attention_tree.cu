@@ -474,24 +474,22 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                         const uint32_t slot = ring.slot, raw = raw0 + rs * S::kRaw, dst = place_of(slot) + (q >> 1) * S::kBox;
                         wait(full, raw_round & 1u, 34);
                         const float unit = reciprocal_of_power(s_raw_powers[rs]) * (1.f / kLevelUnit);
-                        uint4 raws[kOwn];
-                        uint32_t factors[kOwn];
-                        #pragma unroll
-                        for (uint32_t pass = 0; pass < kOwn; ++pass) {
-                            const uint32_t t = pass * kPass + row;
-                            raws[pass] = ld_shared_u4(raw + t * (D / 2) + q * 16);
-                            float scale;
-                            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale) : "r"(raw + S::kCodes + (t * kBlocks + (q >> 1)) * 4) : "memory");
-                            factors[pass] = pack<true>(scale * unit, scale * unit);
-                        }
-                        __syncwarp();
-                        if (lane == 0) ptx::mbar_arrive(raw_empty0 + 8 * rs);  // (all that the slot had is in registers)
+                        uint32_t from = raw + row * (D / 2) + q * 16, scale_at = raw + S::kCodes + (row * kBlocks + (q >> 1)) * 4, to = dst + row * 128;
+                        uint4 next = ld_shared_u4(from);
+                        float scale;
+                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale) : "r"(scale_at) : "memory");
                         if (ring.round) wait(empty0 + 8 * slot, (ring.round + 1) & 1u, 34);
                         if (!ok) break;
-                        #pragma unroll
+                        #pragma unroll 1
                         for (uint32_t pass = 0; pass < kOwn; ++pass) {
-                            const uint32_t t = pass * kPass + row, s2 = factors[pass];
-                            uint4 w = raws[pass];
+                            const uint32_t s2 = pack<true>(scale * unit, scale * unit);
+                            uint4 w = next;
+                            from += kPass * (D / 2);
+                            scale_at += kPass * kBlocks * 4;
+                            if (pass + 1 < kOwn) {
+                                next = ld_shared_u4(from);
+                                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(scale) : "r"(scale_at) : "memory");
+                            }
                             if (order & 2u) w = make_uint4(w.z, w.w, w.x, w.y);
                             if (order & 1u) w = make_uint4(w.y, w.x, w.w, w.z);
                             const uint32_t words[4] = {w.x, w.y, w.z, w.w};
@@ -508,13 +506,17 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                             #pragma unroll
                             for (uint32_t k = 0; k < 4; ++k) {
                                 const uint32_t chunk = (q & 1u) * 4 + (k ^ order);
-                                st_shared_u4(dst + t * 128 + ((chunk ^ (t & 7u)) << 4),
+                                st_shared_u4(to + ((chunk ^ (row & 7u)) << 4),
                                              make_uint4(mul_f16x2(v[k][0], s2), mul_f16x2(v[k][1], s2), mul_f16x2(v[k][2], s2), mul_f16x2(v[k][3], s2)));
                             }
+                            to += kPass * 128;
                         }
                         ptx::fence_proxy_async();
                         __syncwarp();
-                        if (lane == 0) ptx::mbar_arrive(full0 + 8 * slot);
+                        if (lane == 0) {
+                            ptx::mbar_arrive(full0 + 8 * slot);
+                            ptx::mbar_arrive(raw_empty0 + 8 * rs);
+                        }
                         raw6 += 2;
                         if (raw6 >= 2 * S::kRawSlots) {
                             raw6 -= 2 * S::kRawSlots;
