@@ -723,6 +723,58 @@ expand_kernel(const CacheView c, const BatchView b, uint4 *const k_out, uint4 *c
     }
 }
 
+// The row tiles that several CTAs had: a warp to four rows at a time, the parts in the order of the tokens.
+constexpr uint32_t kJoinRows = 4, kJoinWarps = 8;
+template <int D, bool NF4>
+__global__ void __launch_bounds__(32 * kJoinWarps)
+join_pieces_kernel(const AttentionView a, const Split *const splits) {
+    constexpr uint32_t kRows = Shape<D, NF4>::kRows, kWide = D / 32;  // values of a row to a lane
+    ptx::pdl_launch_dependents();
+    ptx::pdl_wait();
+    const Split s = splits[blockIdx.x];
+    const uint32_t r0 = (blockIdx.y * kJoinWarps + threadIdx.x / 32) * kJoinRows, lane = threadIdx.x & 31u;
+    if (r0 >= s.rows) return;
+    auto part = [&](uint32_t i) { return (uint64_t)(2 * (blockIdx.x + i) + (i ? 0 : 1)) * kRows + r0; };
+    float m[kJoinRows], sum[kJoinRows], acc[kJoinRows][kWide];
+    #pragma unroll
+    for (uint32_t r = 0; r < kJoinRows; ++r) {
+        m[r] = -INFINITY;
+        sum[r] = 0.f;
+        #pragma unroll
+        for (uint32_t j = 0; j < kWide; ++j) acc[r][j] = 0.f;
+    }
+    #pragma unroll 2
+    for (uint32_t i = 0; i <= s.more; ++i) {
+        #pragma unroll
+        for (uint32_t r = 0; r < kJoinRows; ++r) {  // (a tile's rows behind its last hold anything; they are not written)
+            const float2 ml = __ldg(a.part_ml + part(i) + r);
+            float v[kWide];
+            const float *const o = a.part_o + (part(i) + r) * D + lane * kWide;
+            #pragma unroll
+            for (uint32_t j = 0; j < kWide; j += 2) {
+                const float2 w = __ldg(reinterpret_cast<const float2 *>(o + j));
+                v[j] = w.x;
+                v[j + 1] = w.y;
+            }
+            const float top = fmaxf(m[r], ml.x), base = top == -INFINITY ? 0.f : top;
+            const float keep = exp2_approx(m[r] - base), f = exp2_approx(ml.x - base);  // (nothing seen: 2^-inf)
+            m[r] = top;
+            sum[r] = fmaf(f, ml.y, sum[r] * keep);
+            #pragma unroll
+            for (uint32_t j = 0; j < kWide; ++j) acc[r][j] = fmaf(f, v[j], acc[r][j] * keep);
+        }
+    }
+    #pragma unroll
+    for (uint32_t r = 0; r < kJoinRows; ++r) {
+        if (r0 + r >= s.rows) break;
+        const float f = sum[r] == 0.f ? 0.f : 1.f / sum[r];
+        const uint32_t q_row = s.r0 + r0 + r, token = a.by_group.of(q_row);
+        __nv_bfloat16 *const out = static_cast<__nv_bfloat16 *>(a.out) + (uint64_t)(s.row0 + token) * a.ldo + (uint64_t)(s.head * a.group + q_row - token * a.group) * D + lane * kWide;
+        #pragma unroll
+        for (uint32_t j = 0; j < kWide; j += 2) *reinterpret_cast<uint32_t *>(out + j) = bf16_pair(acc[r][j] * f, acc[r][j + 1] * f);
+    }
+}
+
 uint64_t rows_of(const AttentionCall &c) { return c.head_dim == 256 ? 128 : 256; }
 uint64_t tokens_of(const AttentionCall &c) { return c.head_dim == 256 ? 64 : 128; }
 
@@ -788,7 +840,7 @@ int32_t launch(const AttentionCall &c, uint8_t *workspace, cudaStream_t stream) 
     const uint32_t ctas = persistent_ctas();
     count_launch(2);
     NF4_TRY(launch_maybe_overlapped(kernel, dim3(ctas), dim3(kThreads), S::kSmem, stream, true, map_k, map_v, c.cache, c.batch, view, dense, box_rows, splits, failure));
-    return launch_maybe_overlapped(join_pieces_kernel<D, S::kRows>, dim3(ctas, S::kRows / (kJoinRows * kJoinWarps)), dim3(32 * kJoinWarps), 0, stream, true, view,
+    return launch_maybe_overlapped(join_pieces_kernel<D, NF4>, dim3(ctas, S::kRows / (kJoinRows * kJoinWarps)), dim3(32 * kJoinWarps), 0, stream, true, view,
                                    static_cast<const Split *>(splits));
 }
 
