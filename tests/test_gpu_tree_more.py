@@ -187,3 +187,40 @@ def test_rows_of_larger_tensors_at_odd_places():
     out = torch.zeros(batch.rows, 2, 8, 64, dtype=BF16, device=DEV)
     assert torch.equal(caches[0].tree_attention(q.unflatten(1, (8, 64)), masks, batch, out=out[:, 1]), caches[1].tree_attention(q.contiguous(), masks, batch).view(-1, 8, 64))
     assert bool((out[:, 0] == 0).all())
+
+
+@pytest.mark.parametrize("heads,group,dim,page_size", [(2, 4, 128, 16), (2, 8, 64, 48), (1, 4, 256, 16)])
+def test_a_page_that_there_is_not_among_small_ones(heads, group, dim, page_size):
+    """Each head's and each step's: pages -1 and behind the pool, in the first and the last steps of the sequence."""
+    specs = [(700, 30), (900, 30), (500, 30), (300, 30)]
+    batch, pages = batch_of(specs, page_size)
+    cache = filled_cache(pages, page_size, heads, dim, False)
+    batch.page_table[0, 0] = -1
+    batch.page_table[2, (500 - 31) // page_size] = pages
+    q = torch.randn(batch.rows, heads * group, dim, device=DEV).bfloat16()
+    out = cache.tree_attention(q, masks_of("tree", specs, batch, np.random.default_rng(0)), batch)
+    for s in range(4):
+        rows = out[30 * s:30 * s + 30]
+        assert bool(torch.isnan(rows).all()) if s in (0, 2) else bool(torch.isfinite(rows).all())
+
+
+@pytest.mark.parametrize("heads,group,dim,page_size", [(4, 4, 128, 16), (2, 8, 64, 16), (2, 8, 64, 112), (2, 5, 256, 16)])
+def test_small_pages_are_as_large_ones(heads, group, dim, page_size):
+    """A bf16 cache of the same tokens in small pages and in large ones: sequences of one step to many, every time the same bits."""
+    rng = np.random.default_rng(8)
+    specs = [(int(n), int(min(n, k))) for n, k in zip(rng.choice([1, 60, 128, 129, 300, 700, 2500], 60), rng.integers(10, 50, 60))]
+    outs = []
+    for size in (page_size, 128):
+        batch, pages = batch_of(specs, size)
+        cache = filled_cache(pages, size, heads, dim, False)
+        cache.k.zero_(), cache.v.zero_()
+        for s, (n, _) in enumerate(specs):
+            g = torch.Generator(device=DEV).manual_seed(s)
+            k, v = (torch.randn(n, heads, dim, device=DEV, generator=g).bfloat16() for _ in range(2))
+            for t0 in range(0, n, size):
+                page, some = int(batch.page_table[s, t0 // size]), min(size, n - t0)
+                cache.k[page, :, :some], cache.v[page, :, :some] = k[t0:t0 + some].transpose(0, 1), v[t0:t0 + some].transpose(0, 1)
+        q = torch.randn(batch.rows, heads * group, dim, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1000)).bfloat16()
+        masks = masks_of("tree", specs, batch, np.random.default_rng(3))
+        outs.append([cache.tree_attention(q, masks, batch) for _ in range(5)])
+    assert all(torch.equal(o, outs[0][0]) for o in outs[0] + outs[1])

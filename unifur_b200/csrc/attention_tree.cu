@@ -30,7 +30,7 @@ namespace nf4 {
 namespace {
 
 constexpr uint32_t kThreads = 640;
-// warps 0-3 and 4-7: softmax; 8-15: codes to f16 (a bf16 cache: the first of them copies); 16, 18, 19: codes' copies; 17: MMAs
+// warps 0-3 and 4-7: softmax; 8-15: codes to f16 (a bf16 cache: the first of them copy, all where pages are small); 16, 18, 19: codes' copies; 17: MMAs
 constexpr uint32_t kExpandWarp = 8, kExpandWarps = 4, kCopyWarp = 16, kMmaWarp = 17, kLoaders = 3;  // kExpandWarps: to a tile
 
 template <int D, bool NF4>
@@ -81,6 +81,8 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     using S = Shape<D, NF4>;
     using Walk = Walker<S::kRows, S::kTokens, kStart, kLeast, kWhole, true>;
     constexpr uint32_t kCopies = !NF4 && D >= 128 ? 2 : 1;  // (as in the kernel for many rows)
+    constexpr uint32_t kSmallCopies = 4;               // warps to a tile whose pages are of sixteen tokens
+    const bool small_pages = !NF4 && box_rows == kGroup;
     constexpr uint32_t N = S::kTokens, kBlocks = S::kBlocks, kHalves = S::kHalves, kHalf = S::kHalf;
     extern __shared__ uint8_t smem_any[];
     __shared__ __align__(8) uint64_t s_bars[40];
@@ -107,7 +109,7 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     }
     if (tid == 0) {
         for (uint32_t i = 0; i < 8; ++i) {  // (a place more than kSlots may be in use)
-            ptx::mbar_init(full0 + 8 * i, NF4 ? kExpandWarps : kCopies);
+            ptx::mbar_init(full0 + 8 * i, NF4 ? kExpandWarps : small_pages ? kSmallCopies : kCopies);
             ptx::mbar_init(empty0 + 8 * i, 1);
         }
         for (uint32_t i = 0; i < S::kRawSlots; ++i) {
@@ -629,6 +631,62 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                     t = next;
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
+            } else if (!NF4 && small_pages) {
+                // ---- a bf16 cache whose pages hold sixteen tokens (or an odd number of them): 16-byte copies of four warps to K's tiles and four to V's ----
+                // (With TMA, boxes of sixteen tokens: 16 sequences of 8192 tokens, 8 heads of 128, pages of 16, 64 rows a head 106 to 109 us,
+                // so 96 to 98; heads of 64 98 to 121 us, so 76 to 90; pages of 48 are as fast either way, larger boxes stay with TMA.)
+                if (warp < kCopyWarp && warp >= kExpandWarp) {
+                    constexpr uint32_t kRows = N / kSmallCopies, kChunks = D / 8, kRound = 32 / kChunks;  // tokens of a warp; 16-byte pieces of a row; tokens at a time
+                    const uint32_t own = warp & 1u, first = ((warp - kExpandWarp) >> 1) * kRows, x = lane % kChunks;
+                    const __nv_bfloat16 *const pool = static_cast<const __nv_bfloat16 *>(own ? c.v : c.k);
+                    uint32_t pending = 0;  // the barrier of the tile whose copies are under way, or 0
+                    auto deliver = [&] {   // (its copies are done)
+                        ptx::fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) ptx::mbar_arrive(pending);
+                        pending = 0;
+                    };
+                    Ring ring;
+                    for (uint32_t piece = 0; ok && walk.next(c, b, a, p); ++piece) {
+                        #pragma unroll 1
+                        for (uint32_t turn = 0; ok && turn < 2 * p.steps; ++turn, ring.on(slots)) {
+                            const Turn<2> of(turn, p.steps);
+                            if (of.values != own) continue;
+                            const uint32_t t0 = (p.step0 + of.step) * N + first, slot = ring.slot, dst = place_of(slot);
+                            const uint32_t stored = p.s.length > t0 ? min(p.s.length - t0, kRows) : 0u;  // of the warp's tokens
+                            uint32_t place = 0;  // of group `lane`
+                            if (lane * kGroup < stored) {
+                                const uint32_t t = t0 + lane * kGroup, at = c.by_page.of(t);
+                                const int32_t page = __ldg(b.table + (uint64_t)p.seq * b.width + at);
+                                if (page >= 0 && (uint32_t)page < c.pages) place = ((uint32_t)page * c.heads + p.head) * c.page_size + (t - at * c.page_size);
+                                else s_bad[piece & 7u] = piece + 1;
+                            }
+                            __syncwarp();
+                            if (ring.round && !__all_sync(0xffffffffu, ptx::mbar_try_wait(empty0 + 8 * slot, (ring.round + 1) & 1u))) {
+                                if (pending) {  // (before a wait that may be for what it holds back)
+                                    asm volatile("cp.async.wait_all;" ::: "memory");
+                                    deliver();
+                                }
+                                wait(empty0 + 8 * slot, (ring.round + 1) & 1u, 35);
+                            }
+                            if (!ok) break;
+                            #pragma unroll
+                            for (uint32_t i = 0; i < kRows / kRound; ++i) {
+                                const uint32_t t = i * kRound + lane / kChunks, row = first + t;
+                                const uint64_t at = (uint64_t)__shfl_sync(0xffffffffu, place, i * kRound / kGroup) + t % kGroup;
+                                ptx::cp_async_16_or_zero(dst + (x >> 3) * S::kBox + row * 128 + (((x & 7u) ^ (row & 7u)) << 4), pool + at * D + x * 8, t < stored);
+                            }
+                            asm volatile("cp.async.commit_group;" ::: "memory");
+                            if (pending) {
+                                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                                deliver();
+                            }
+                            pending = full0 + 8 * slot;
+                        }
+                    }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    if (ok && pending) deliver();
+                }
             } else if (NF4 ? warp == kCopyWarp : warp >= kExpandWarp && warp < kExpandWarp + 2 * kCopies) {
                 // ---- tiles as they are: of a bf16 cache's pages, or of what was expanded ahead ----
                 const uint32_t own = NF4 ? 0u : (warp - kExpandWarp) & 1u, part = NF4 ? 0u : (warp - kExpandWarp) >> 1;  // bf16: K or V, and which columns
