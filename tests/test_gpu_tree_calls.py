@@ -55,6 +55,30 @@ def test_a_long_chain():
     assert positions.tolist() == list(range(n))
 
 
+@pytest.mark.parametrize("near,words", [(1, None), (3, None), (40, 130), (5000, None), (40, 7), (2, 100)])
+@pytest.mark.parametrize("hints", [True, False])
+def test_deep_trees_of_thousands_of_nodes(near, words, hints):
+    """Ways that go through most words of a row, or leap over many; with masks for fewer nodes and for more."""
+    specs = [(4500, 4300), (3, 3), (2049, 2049), (257, 256)]
+    rng = np.random.default_rng(near)
+    batch, pages = batch_of(specs, 64, spare_rows=(1, 1), hints=hints)
+    cache = filled_cache(pages, 64, 1, 64, True)
+    starts = batch.row_starts.tolist()
+    parents = np.zeros(batch.rows, np.int32)
+    for s, (_, n) in enumerate(specs):
+        i = np.arange(n)
+        parents[starts[s]:starts[s + 1]] = np.where(i == 0, -1, np.maximum(i - rng.integers(1, near + 1, n), -1))
+    words = words or -(-4300 // 32)
+    out = (torch.full((batch.rows, words), 5, dtype=torch.int32, device=DEV), torch.full((batch.rows,), 5, dtype=torch.int32, device=DEV))
+    masks, positions = (t.cpu().numpy() for t in cache.tree_masks(torch.from_numpy(parents).to(DEV), batch, out=out))
+    for t in (masks, positions):
+        assert (t[0] == 5).all() and (t[-1] == 5).all()
+    for s, (length, n) in enumerate(specs):
+        seen, depth = ancestors(parents, starts[s], n)
+        rows = slice(starts[s], starts[s + 1])
+        assert (masks[rows] == packed(seen, words)).all() and (positions[rows] == length - n + depth).all()
+
+
 # ---- appending with rotation --------------------------------------------------------------------
 def turned(x, positions, table, pairs):
     """In f32, each product and sum rounded; and a sum of magnitudes for tolerances."""

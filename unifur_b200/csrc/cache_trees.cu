@@ -10,41 +10,57 @@ namespace nf4 {
 namespace {
 
 // ---- masks and positions ----------------------------------------------------------------------------
-// A thread to a row, which goes up from its node to the root.  Parents come before their children, so the bits are met from the highest down: a
-// word of the mask is whole when the way leaves it, and is held in a register until then.  (The way of a node is its depth long, a
-// load from L1 a step: 45 ns.  A chain of 1000 nodes takes 45 us; trees are shallow.)
-constexpr uint32_t kTreeThreads = 128;
+// A parent comes before its children, so a node's ancestors within its own word of 32 nodes follow from that word alone: a warp finds
+// them for its lanes' nodes by doubling (after k exchanges a lane has its 2^k nearest ancestors and knows the next one), and the ancestor
+// at which the way leaves the word.  A thread to a row then goes up a word at a time, and writes words from the highest down.
+// (A node at a time, lanes leaving their words at different steps: 118 ns a node of the way, chains of 64 / 250 / 1000 nodes 7.7 / 27 / 113 us;
+// so 1.7 / 2.4 / 6.7, and trees with two children to a node 1.7 / 2.4 / 6.8 where they took 1.9 / 2.8 / 4.9.)
+// Nodes are prepared kWindow at a time, from the highest that the CTA's rows have, until no row has a way left.
+constexpr uint32_t kTreeThreads = 256, kWindow = 2048;
+static_assert(kWindow % 32 == 0);
 
 __global__ void __launch_bounds__(kTreeThreads)
 tree_kernel(const CacheView c, const BatchView b, const int32_t *const parents, uint32_t *const masks, uint32_t words, int32_t *const positions) {
+    __shared__ uint2 s_nodes[kWindow];  // itself and its ancestors in its word; the parent of the first of them, or -1
+    const uint32_t tid = threadIdx.x, lane = tid & 31u;
     ptx::pdl_launch_dependents();
     ptx::pdl_wait();
     const Sequence s = sequence_of(c, b, blockIdx.x);
-    for (uint32_t i = blockIdx.y * kTreeThreads + threadIdx.x; i < s.rows; i += gridDim.y * kTreeThreads) {
-        uint32_t *const mask = masks ? masks + (uint64_t)(s.row0 + i) * words : nullptr;
-        uint32_t node = i, depth = 0, word = i / 32, bits = 0;
-        if (mask)
-            for (uint32_t w = word + 1; w < words; ++w) mask[w] = 0;
-        for (;;) {
-            if (node / 32 != word) {
-                if (mask) {
-                    if (word < words) mask[word] = bits;
-                    for (uint32_t w = node / 32 + 1; w < min(word, words); ++w) mask[w] = 0;
+    for (uint32_t r0 = blockIdx.y * kTreeThreads; r0 < s.rows; r0 += gridDim.y * kTreeThreads) {
+        const uint32_t i = r0 + tid, end = min(s.rows, r0 + kTreeThreads);
+        uint32_t *const mask = masks && i < end ? masks + (uint64_t)(s.row0 + i) * words : nullptr;
+        int32_t node = i < end ? (int32_t)i : -1;
+        uint32_t met = 0, done = words;  // nodes on the way so far; words from here on are written
+        for (int32_t w0 = (int32_t)((end - 1) / kWindow * kWindow); w0 >= 0; w0 -= (int32_t)kWindow) {
+            if (!__syncthreads_or(node >= 0)) break;
+            const uint32_t last = min(end, (uint32_t)w0 + kWindow);
+            for (uint32_t at = (uint32_t)w0 + tid; at - lane < last; at += kTreeThreads) {
+                int32_t up = at < last ? __ldg(parents + s.row0 + at) : -1;
+                if (up < 0 || (uint32_t)up >= at) up = -1;
+                uint32_t bits = 1u << lane, next = up >= (int32_t)(at - lane) ? (uint32_t)up & 31u : lane;
+                #pragma unroll
+                for (uint32_t k = 0; k < 5; ++k) {
+                    bits |= __shfl_sync(0xffffffffu, bits, next);
+                    next = __shfl_sync(0xffffffffu, next, next);
                 }
-                word = node / 32;
-                bits = 0;
+                s_nodes[at - (uint32_t)w0] = make_uint2(bits, (uint32_t)__shfl_sync(0xffffffffu, up, next));
             }
-            bits |= 1u << (node & 31u);
-            const int32_t up = __ldg(parents + s.row0 + node);
-            if (up < 0 || (uint32_t)up >= node) break;
-            node = (uint32_t)up;
-            ++depth;
+            __syncthreads();
+            while (node >= w0) {
+                const uint2 of = s_nodes[node - w0];
+                const uint32_t word = (uint32_t)node / 32;
+                if (mask) {
+                    for (uint32_t w = word + 1; w < done; ++w) mask[w] = 0;
+                    if (word < done) mask[word] = of.x;
+                }
+                done = min(done, word);
+                met += __popc(of.x);
+                node = (int32_t)of.y;
+            }
         }
-        if (mask) {
-            if (word < words) mask[word] = bits;
-            for (uint32_t w = 0; w < min(word, words); ++w) mask[w] = 0;
-        }
-        if (positions) positions[s.row0 + i] = (int32_t)s.length - (int32_t)s.rows + (int32_t)depth;
+        if (mask)
+            for (uint32_t w = 0; w < done; ++w) mask[w] = 0;
+        if (positions && i < end) positions[s.row0 + i] = (int32_t)s.length - (int32_t)s.rows + (int32_t)met - 1;
     }
 }
 
