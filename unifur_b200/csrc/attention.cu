@@ -319,8 +319,8 @@ bool takes_decode(const AttentionCall &c) {
     const double steps = c.most_tokens / 128 + 1, heads = c.cache.heads;
     if (c.tree) {
         // Likewise, trees having a kernel of their own for many rows (us, first / second; 16 sequences of 8192 tokens, 8 heads of 128, NF4: 16 rows of a head 62 /
-        // 103, 32 rows 112 / 103, 64 rows 209 / 107; bf16: 94 / 98, 174 / 98, 32 rows of 64 81 / 83 and 89 / 72; one sequence, 4 heads, 112 rows, NF4: 8192 tokens
-        // 21 / 20, 65536 93 / 41, four of 512 10 / 18)
+        // 97, 32 rows 112 / 97, 64 rows 209 / 97; bf16: 94 / 90, 174 / 90, 32 rows of 64 81 / 86 and 89 / 75; one sequence, 4 heads, 112 rows, NF4: 8192 tokens
+        // 21 / 20, 65536 93 / 40, four of 512 10 / 18)
         static constexpr double kTreeStream[2][3] = {{7, 14, 36}, {7, 9, 45}}, kTreeMany[2][3] = {{11, 14, 50}, {13, 16, 55}};
         return tiles(16) * heads * (32 + steps * kTreeStream[c.nf4][of_dim]) <= tiles(128) * heads * (64 + steps * kTreeMany[c.nf4][of_dim]) + kNumSMs * 90;
     }

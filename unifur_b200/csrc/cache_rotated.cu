@@ -276,7 +276,7 @@ int32_t nf4_cache_append_rotated_dev(const nf4_cache *cache, const nf4_cache_bat
     t.width = (vectors + across * batch_of - 1) / (across * batch_of);
     t.abreast = std::max(1u, slots / t.width);
     // A CTA finds its rows' places once, a chain of four loads: so many rounds that the CTAs which an SM has registers for (128 a thread) do all (measured with 7,345
-    // rows of 28 + 8 heads of 128, NF4 / bf16: one round to a CTA 46 / 39 us, as many as that 29 / 25)
+    // rows of 28 + 8 heads of 128, NF4 / bf16: one round to a CTA 42 / 36 us, as many as that 29 / 25)
     const uint32_t threads = (t.abreast * t.width * lanes + 31) / 32 * 32, ctas = kNumSMs * std::max(1u, 512u / threads);
     const uint64_t in_turn = ((uint64_t)batch->rows + t.abreast - 1) / t.abreast * across;
     t.rounds = (uint32_t)std::min<uint64_t>(kMostRows / t.abreast, (in_turn + ctas - 1) / ctas);
