@@ -523,13 +523,17 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
                     for (int e = 0; e < 4; ++e) x[u][nt][e] *= factor[nt][e & 1];
             }
             if (t0 + G * kGroup > sees_first) {  // some row does not see all of it
-                uint32_t window[NT][2];  // TREE: bit i: the column's row sees token t0 + i
+                uint32_t window[NT][2], some = 0;  // TREE: bit i: the column's row sees token t0 + i; some row of the tile does
                 if (TREE) {
                     #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
                         #pragma unroll
-                        for (int j = 0; j < 2; ++j)
+                        for (int j = 0; j < 2; ++j) {
                             window[nt][j] = sees[nt][j] == kBlind ? 0u : seen_nodes(a, sees[nt][j], (int32_t)t0 - first_node(s)) & low_bits(limit - t0);
+                            some |= window[nt][j];
+                        }
+                    some |= __shfl_xor_sync(0xffffffffu, some, 1);
+                    some |= __shfl_xor_sync(0xffffffffu, some, 2);
                 }
                 #pragma unroll
                 for (uint32_t u = 0; u < G; ++u) {
@@ -544,7 +548,8 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
                                 x[u][nt][2 * h + j] = seen ? x[u][nt][2 * h + j] : -INFINITY;
                             }
                         #pragma unroll
-                        for (uint32_t kb = 0; NF4 && kb < kBlocks; ++kb) vs[u][h][kb] = tok + 8 * h < limit ? vs[u][h][kb] : 0.f;  // (anything may stand there)
+                        for (uint32_t kb = 0; NF4 && kb < kBlocks; ++kb)  // (anything may stand behind; a node that the tile's rows do not see has no say in `ref`)
+                            vs[u][h][kb] = (TREE ? some >> (tok + 8 * h - t0) & 1u : tok + 8 * h < limit) ? vs[u][h][kb] : 0.f;
                     }
                 }
             }
