@@ -579,8 +579,9 @@ NF4_API int32_t nf4_cache_tree_dev(const nf4_cache *cache, const nf4_cache_batch
 /* nf4_cache_attention_dev for such rows: row i sees its sequence's context, and the nodes that its mask has, whether they come before it or not.
  * A row that sees nothing becomes zeros, as does a row whose own token is negative (a node with a negative token is seen by none).  Values of all tokens
  * of the sequences that have rows are finite, those of nodes that a row's mask hides among them.  With bf16 tensors over an
- * NF4 cache a token's part of a result is off by up to 2^-31 of the largest value that the row, or one of 15 on either side of it, sees.  All else is as
- * there, with these three for its workspace. */
+ * NF4 cache a token's part of a result is off by up to 2^-31 of the largest value that the row, or one of 15 on either side of it, sees; with many rows by
+ * 2^-28 of its own value, down to 2^-92 of the largest among the tokens that the row sees or that stand with them.  All else is as there, with
+ * these three for its workspace. */
 NF4_API uint64_t nf4_cache_tree_attention_workspace_bytes(const nf4_cache *cache, const nf4_cache_batch *batch, uint32_t q_heads,
                                                           int32_t io_dtype);
 NF4_API uint64_t nf4_cache_tree_attention_call_flag_bytes(const nf4_cache *cache, const nf4_cache_batch *batch, uint32_t q_heads,

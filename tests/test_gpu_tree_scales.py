@@ -69,3 +69,34 @@ def test_few_rows_beside_a_larger_node_of_another_branch(context, n, group, k_by
     for name, by in zip("kv", factors):
         tokens_scaled(cache, batch, 16, name, by)
     check(cache, batch, rows(batch, 2 * group, dim), branches(n, [5], np.random.default_rng(n)), 16, False)
+
+
+# the last: expanded ahead
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("k_by,v_by", [(0, 0), (0, 25), (0, 40), (0, 100), (15, 20), (0, -30), (0, -100)])
+@pytest.mark.parametrize("context,n,group", [(0, 300, 2), (128, 400, 1), (128, 290, 3), (0, 300, 4)])
+def test_many_rows_beside_larger_nodes_of_another_branch(context, n, group, k_by, v_by, dim):
+    """Larger nodes in a step whose nodes most others do not see, ahead of the steps that these see."""
+    batch, pages = batch_of([(context + n, n)], 16, width=4096, hints=False)
+    cache = filled_cache(pages, 16, 2, dim, True)
+    step, large = 64 if dim == 256 else 128, [3, 7]
+    factors = np.ones((2, context + n))
+    for node in large:
+        factors[0, context + node], factors[1, context + node] = 2.0 ** k_by, 2.0 ** v_by
+    for name, by in zip("kv", factors):
+        tokens_scaled(cache, batch, 16, name, by)
+    check(cache, batch, rows(batch, 2 * group, dim), branches(n, large, np.random.default_rng(n), step), 16, True)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("by", [[0, 100, 0, -100, 60, -20], [-110, 90, 0, 50, -60, 90], [0, -3, -6, -9, -12, -15], [100, 40, -20, -80, -110, 10], [-110, -50, 10, 70, 100, 100]])
+def test_steps_that_rise_and_fall(by, dim):
+    """Each step of tokens of another size, up and down over the whole range of f32; rows see some steps, and others not."""
+    step, n = 64 if dim == 256 else 128, 6 * (64 if dim == 256 else 128)
+    batch, pages = batch_of([(n, n)], 16, width=4096, hints=False)
+    cache = filled_cache(pages, 16, 1, dim, True)
+    tokens_scaled(cache, batch, 16, "v", np.repeat(2.0 ** np.array(by), step))
+    rng = np.random.default_rng(2)
+    bits = np.repeat(rng.random((n, 6)) < 0.4, step, 1) & (rng.random((n, n)) < 0.5)
+    bits[np.arange(n), np.arange(n)] = True
+    check(cache, batch, rows(batch, 2, dim, 0.5), torch.from_numpy(packed(bits, -(-n // 32))).to(DEV), 16, True)

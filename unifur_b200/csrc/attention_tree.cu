@@ -19,7 +19,8 @@
 // Measured (16 sequences of 8192 tokens, 8 heads of 128): bf16, 16 to 64 rows of a head, 89 us = 6.0 TB/s; NF4, 16 to 128 rows, 97 to 99 us, 2800 cycles a step,
 // in which a scheduler issues 2000 instructions for two softmax and two expanding warps.  Tried for those, with no gain: a fourth of the words expanded by byte permutes of
 // the levels' bytes in place of lookups, half of the exponentials by FMA, a step's first scores asked for during the last one's weights, up to 64 rows in
-// the tile twice with a softmax warp to each scheduler.  Everything else (weights, f16's range, the order of sums) is as in the kernel for many rows, and said there.
+// the tile twice with a softmax warp to each scheduler.  Everything else (weights, f16's range, the order of sums) is as in the kernel for many rows, and said there,
+// but for the unit of a row's sums over a quantized cache: a step that a row sees nothing of may hold far larger values, of other branches, and has no say in it.
 #include <algorithm>
 
 #include "attention_steps.cuh"
@@ -55,6 +56,7 @@ struct Shape {
 };
 
 constexpr uint32_t kStart = 4, kLeast = 3, kWhole = 6;  // (see Walker)
+constexpr uint32_t kMostLess = 4;  // by how many powers of two a step may be below a row's unit
 
 // The row of the n-th chunk that a lane of a softmax warp takes of the results: its warp's 32 rows, its half's values.
 template <uint32_t LANES>  // to a row
@@ -65,6 +67,7 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
                  "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
                  : "memory");
 }
+__device__ __forceinline__ float power_of_two(int e) { return e < -126 ? 0.f : __uint_as_float((uint32_t)(127 + e) << 23); }  // up to 127
 __device__ __forceinline__ void take_columns(uint32_t taddr, uint32_t (&r)[16]) { ptx::tmem_ld16(taddr, r); }
 __device__ __forceinline__ void take_columns(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
 __device__ __forceinline__ void cp_async_16_upto(uint32_t dst_smem, const void *src, uint32_t bytes) {  // of the sixteen, and zeros
@@ -236,7 +239,8 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                 const uint32_t sees = real && nodes0 + (int32_t)token >= 0 ? p.s.length : 0u;  // (a node with a negative token sees nothing)
                 const uint32_t context = (uint32_t)max(nodes0, 0);
                 float row_factor = fabsf(a.scale_log2);
-                float m = -INFINITY, l = 0.f, ref = 0.f;
+                float m = -INFINITY, l = 0.f;
+                int unit = 0, top_unit = 0;  // NF4: exponents of what the row's sums are in units of, and of the largest of a step that it saw something of
                 for (uint32_t j = 0; j < p.steps; ++j, ++scores) {
                     const uint32_t place = scores & 1u, ts = ts0 + place * N;
                     wait(s_full0 + 8 * place, (scores / 2) & 1u, 31);
@@ -255,12 +259,6 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                     // (written before the keys' arrival was made known, which the scores are behind)
                     const float2 powers = NF4 ? ld_shared_f2(ptx::smem_addr(s_powers + ((step + j) & 7u))) : make_float2(1.f, 1.f);
                     const float factor = fmaxf(row_factor * powers.x, 1.2e-38f);
-                    const float ref_was = ref;
-                    if (NF4) ref = fmaxf(ref, powers.y);
-                    // the step's values are in units of powers.y, the sums in units of ref: 2^-less of that (a difference that is no more
-                    // than 2^-60 of the largest is made that)
-                    const int less = NF4 ? min((int)(__float_as_uint(ref) >> 23) - (int)(__float_as_uint(powers.y) >> 23), 60) : 0;
-                    const bool grown = NF4 && ref != ref_was && j;
                     ptx::tmem_wait_ld();
                     if (t0 + kHalf > context) {
                         #pragma unroll
@@ -274,17 +272,27 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                     #pragma unroll
                     for (uint32_t i = 0; i < 64; i += 2) top[i / 2 % 4] = fmaxf(fmaxf(top[i / 2 % 4], __uint_as_float(x[i / 32][i % 32])), __uint_as_float(x[i / 32][i % 32 + 1]));
                     const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * factor;
-                    // m stays up to 8 below the largest score: once or twice a row it is out of reach
-                    const bool above = __any_sync(0xffffffffu, high > m + 8.f);
-                    if (above || grown) {
-                        float keep = 1.f;
-                        if (above) {
-                            const float now = fmaxf(m, high);
-                            keep = m == -INFINITY ? 0.f : exp2_approx(m - now);
-                            m = now;
-                            l *= keep;
+                    // The step's values are in units of powers.y, a row's sums in units of 2^unit of which that is 2^-less.  A step that the row sees nothing of leaves its
+                    // unit, and one whose power is below it or far above takes it along, so that `less` costs a weight few of its bits (no further down than
+                    // 2^-60 of the largest, so that the sums do not overflow; from there on weights lose theirs, and a value below 2^-120 of the largest is made that).
+                    int shift = 0, less = 0;
+                    if (NF4) {
+                        const int of_step = (int)(__float_as_uint(powers.y) >> 23);
+                        if ((uint32_t)(unit - of_step) > kMostLess && high != -INFINITY) {
+                            top_unit = max(top_unit, of_step);
+                            const int now = max(of_step, top_unit - 60);
+                            shift = unit - now;
+                            unit = now;
                         }
-                        if (grown) keep *= ref_was * reciprocal_of_power(ref);
+                        less = min(max(unit - of_step, 0), 60);
+                    }
+                    // m stays up to 8 below the largest score: once or twice a row it is out of reach
+                    if (__any_sync(0xffffffffu, high > m + 8.f || shift)) {
+                        const float now = fmaxf(m, high);
+                        float keep = m == -INFINITY ? 0.f : exp2_approx(m - now);
+                        m = now;
+                        l *= keep;
+                        if (NF4) keep *= power_of_two(shift);
                         if (j) {  // once the products so far are done
                             wait(pv_done, (scores - 1) & 1u, 32);
                             if (!ok) break;
@@ -330,10 +338,11 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                 const bool whole = p.steps == p.all;
                 float w0 = 1.f, w1 = 0.f;  // what the halves' results count
                 if (kHalves == 2) {  // this one's largest exponent and sum to the other's warp, and its to this one
-                    st_shared_u4(q0 + chunk_place(r, half * kLanes), make_uint4(__float_as_uint(m), __float_as_uint(l), 0u, 0u));
+                    st_shared_u4(q0 + chunk_place(r, half * kLanes), make_uint4(__float_as_uint(m), __float_as_uint(l), (uint32_t)unit, 0u));
                     come();
                     meet();
-                    const float2 theirs = ld_shared_f2(q0 + chunk_place(r, (1 - half) * kLanes));
+                    const uint4 got = ld_shared_u4(q0 + chunk_place(r, (1 - half) * kLanes));
+                    const float2 theirs = make_float2(__uint_as_float(got.x), __uint_as_float(got.y));
                     come();
                     meet();  // (both have read: results come to these places)
                     const float now = fmaxf(m, theirs.x), from = now == -INFINITY ? 0.f : now;
@@ -341,11 +350,17 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                     w1 = exp2_approx((half ? m : theirs.x) - from);
                     l = fmaf(half ? l : theirs.y, w1, (half ? theirs.y : l) * w0);
                     m = now;
+                    if (NF4) {  // and to one unit
+                        const int larger = max(unit, (int)got.z), mine = unit - larger, other = (int)got.z - larger;
+                        w0 *= power_of_two(half ? other : mine);
+                        w1 *= power_of_two(half ? mine : other);
+                        unit = larger;
+                    }
                 }
                 if (s_bad[piece & 7u] == piece + 1 || !ok) l = __uint_as_float(0x7fc00000u);  // NaN
                 const uint64_t part = (uint64_t)(2 * blockIdx.x + (p.step0 ? 0 : 1)) * S::kRows;
                 if (!whole && half == 0) a.part_ml[part + r] = make_float2(m, l * kLower<NF4>);
-                const float f = (whole ? l == 0.f ? 0.f : 1.f / l : kLower<NF4>) * (NF4 ? ref : 1.f);
+                const float f = (whole ? l == 0.f ? 0.f : 1.f / l : kLower<NF4>) * (NF4 ? __uint_as_float((uint32_t)unit << 23) : 1.f);
                 #pragma unroll 1
                 for (uint32_t pass = 0; pass < (whole ? 1u : 2u); ++pass) {  // bf16 results, or half of the f32 sums at a time
                     const uint32_t columns = whole ? kWide : kWide / 2, first = half * kWide + pass * columns;
