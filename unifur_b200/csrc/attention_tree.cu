@@ -163,6 +163,7 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     const bool expanded = NF4 && dense.capacity && __ldg(dense.bases + b.sequences) <= dense.capacity;  // (more tokens than the host knew of: not)
     const uint32_t slots = S::kSlots + (expanded ? 1u : 0u);
     auto place_of = [&](uint32_t slot) -> uint32_t { return slot < S::kSlots ? ring0 + slot * S::kTile : table; };
+    // codes: 30 shared memory; 31 scores, 32 sums to be rescaled, 33 results, 37 the warp of the same rows; 34 expanding; 35 copies; 36 MMAs
     auto wait = [&](uint32_t bar, uint32_t parity, int code) {
         if (ok && !__all_sync(0xffffffffu, ptx::mbar_wait_suspended(bar, parity))) {
             ok = false;
@@ -187,7 +188,7 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(pair);
             };
-            auto meet = [&] { wait(pair, meets++ & 1u, 33); };
+            auto meet = [&] { wait(pair, meets++ & 1u, 37); };
             for (; ok && walk.next(c, b, a, p); step += p.steps, ++piece) {
                 // ---- Q to shared memory: half of the pair's rows, as they are, and beside a quantized cache then divided by a power of two ----
                 // (Short loops: code that runs once a piece comes from the L2.  Unrolled, with the loads in registers, this took 11000 cycles.)
