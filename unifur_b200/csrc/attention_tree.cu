@@ -89,7 +89,7 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     constexpr uint32_t N = S::kTokens, kBlocks = S::kBlocks, kHalves = S::kHalves, kHalf = S::kHalf;
     extern __shared__ uint8_t smem_any[];
     __shared__ __align__(8) uint64_t s_bars[40];
-    __shared__ uint32_t s_tmem, s_bad[8], s_first[6];  // s_bad: of the last eight pieces, its number + 1 where a page was not there
+    __shared__ uint32_t s_tmem, s_bad[8], s_first[6];  // s_bad: of the last eight pieces, its number + 1 where a page was not there (it is marked up to six pieces ahead)
     __shared__ Share s_share;
     __shared__ float s_qpower[NF4 ? 128 : 1];
     __shared__ float2 s_powers[8];  // of the last steps' K and V, for the softmax (who writes them is fewer steps ahead of who reads)
@@ -630,6 +630,7 @@ attention_tree_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
                         cp_async_16_upto(raw + S::kCodes + ch * 16, pool_scales + at, there > first ? min((there - first) * 4, 16u) : 0u);
                     }
                     cp_async_arrive(full);
+                    __syncwarp();  // (another lane's s_bad is ahead of the arrival)
                     if (lane == 0) {
                         s_raw_powers[own] = t.values ? powers.y : powers.x;
                         if (!t.values) s_powers[t.info & 7u] = powers;
