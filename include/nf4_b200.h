@@ -543,7 +543,7 @@ NF4_API int32_t nf4_cache_attention_dev(const nf4_cache *cache, const nf4_cache_
  * place in shared memory, or a negative status.  For inspection and tests. */
 NF4_API int32_t nf4_cache_attention_row_place(uint32_t head_dim, uint32_t thread, uint32_t chunk, int32_t results);
 
-/* The same with the positions' rotation on the way: neighbouring values (pairs) or the two halves of a head's first `rotary_dim`
+/* nf4_cache_append_dev with the positions' rotation on the way: neighbouring values (pairs) or the two halves of a head's first `rotary_dim`
  * values are turned by the angles of the row's position,
  *     a' = a cos - b sin,  b' = b cos + a sin,
  * with pair i's cosine at table[position][i] and its sine at table[position][rotary_dim / 2 + i] (f32, 16-byte aligned): the two are values i and
@@ -577,8 +577,8 @@ NF4_API int32_t nf4_cache_tree_dev(const nf4_cache *cache, const nf4_cache_batch
                                    uint32_t mask_words, int32_t *positions, void *stream);
 
 /* nf4_cache_attention_dev for such rows: row i sees its sequence's context, and the nodes that its mask has, whether they come before it or not.
- * A row that sees nothing becomes zeros, as does a row whose own token is negative (a node with a negative token is seen by none).  Values of all tokens
- * of the sequences that have rows are finite, those of nodes that a row's mask hides among them.  With bf16 tensors over an
+ * A row that sees nothing becomes zeros, as does a row whose own token is negative (a node with a negative token is seen by none).  Keys and values of all
+ * tokens of the sequences that have rows are finite, those of nodes that a row's mask hides among them.  With bf16 tensors over an
  * NF4 cache a token's part of a result is off by up to 2^-31 of the largest value that the row, or one of 15 on either side of it, sees; with many rows by
  * 2^-28 of its own value, down to 2^-92 of the largest among the tokens that the row sees or that stand with them.  All else is as there, with
  * these three for its workspace. */

@@ -23,7 +23,8 @@ class CacheBatch:
     int32 tensors on the cache's device (``[sequences, pages]``, ``[sequences]``, ``[sequences + 1]``); their values may change
     between replays of a captured graph.  ``rows``: rows of the call's tensors; those of no sequence are not written.
     ``max_rows``, ``max_length``: the most rows and tokens of a sequence where the program knows them; they choose kernels and
-    how work is shared out, and results hold without them.  Sequences may share the pages of a common prefix, but a token that a
+    how work is shared out, and results hold without them and where they are wrong.  One call takes its word from them: the masks that
+    ``tree_masks`` makes without ``out`` have the words that ``max_rows`` nodes need.  Sequences may share the pages of a common prefix, but a token that a
     call appends is in a page of its sequence alone."""
 
     __slots__ = ("page_table", "lengths", "row_starts", "rows", "max_rows", "max_length")
@@ -145,7 +146,7 @@ class PagedKvCache:
         number of an earlier node of the row's sequence, anything else (-1) makes it a root.  Returns masks (int32 ``[rows, words]``, bit
         ``j % 32`` of word ``j / 32`` for node ``j``: the node itself and its ancestors) and positions (int32 ``[rows]``: the
         context's length and the node's depth).  There are as many words as ``max_rows`` (or ``rows``) needs, or as ``out`` has: nodes behind
-        them are seen by none.  Rows of no sequence are left as ``out`` has them, and without ``out`` undefined."""
+        them are seen by none, not by themselves, so that ``max_rows`` is no less than any sequence's rows here, or 0.  Rows of no sequence are left as ``out`` has them, and without ``out`` undefined."""
         masks, positions = out if out is not None else (None, None)
         return _lib.host().cache_tree(*self._args(), *batch._args(), parents, masks, positions)
 
@@ -153,7 +154,7 @@ class PagedKvCache:
                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``attention`` of the nodes of trees: each row sees its sequence's context (what is cached ahead of the sequence's rows) and those
         of its nodes that ``masks`` (int32 ``[rows, words]``, as ``tree_masks`` makes them) has for it, whether they come before it or not.
-        A row that sees nothing becomes zeros.  Values of all the sequences' tokens are finite, of hidden nodes too."""
+        A row that sees nothing becomes zeros.  Keys and values of all the sequences' tokens are finite, of hidden nodes too."""
         if scale is None:
             scale = 1.0 / math.sqrt(self.head_dim())
         return _lib.host().cache_attention(*self._args(), *batch._args(), q, scale, out, masks)
