@@ -248,7 +248,7 @@ __device__ __forceinline__ Share share_out(const CacheView &c, const BatchView &
         shortest = __reduce_min_sync(0xffffffffu, shortest);
         all_tiles = __reduce_add_sync(0xffffffffu, all_tiles);
         // (no share is as long as a tile then, so that none has two that begin in it)
-        const uint32_t of_share = share.ctas ? total / share.ctas : 0, more = Walk::kWhole + min(4u, of_share / 12);  // (a long tile's start and results are more, too)
+        const uint32_t of_share = share.ctas ? total / share.ctas : 0, more = Walk::kWhole + min(4u, of_share / 12);  // (measured: see kWhole)
         share.whole = all_tiles <= gridDim.x && (uint64_t)shortest * share.ctas >= total && (uint64_t)(longest - min(longest, more)) * share.ctas <= total;
     }
     share.per = share.ctas ? total / share.ctas : 0;

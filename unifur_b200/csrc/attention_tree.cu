@@ -55,6 +55,10 @@ struct Shape {
     static_assert(kHalves * kSoftmaxRegs + (5 - kHalves) * kOtherRegs <= 480 && kSlots + 1 <= 8);
 };
 
+// kWhole: up to that many steps more than a share, and a share's twelfth but no more than four, row tiles stay whole.  Measured on both sides, tiles of one length,
+// as many as given for 148 CTAs, us divided / whole (heads of 128, 64 rows).  NF4: 8 steps, 144 tiles 30 / 25, 80 27.5 / 24.5; 16 steps, 112 40 / 36, 96 35 / 36; 32 steps, 120 59 / 59,
+// 112 56 / 58; 64 steps, 136 110 / 106, 128 104 / 105; 128 steps, 140 199 / 196, 136 195 / 196; 256 steps, 140 390 / 386, 128 355 / 377: as long at 5.5 to 7, 7, 7, 8, 10 and 20 steps
+// more than a share.  A bf16 cache, bound by its bytes, could go on for longer: 16 steps, 96 tiles 35 / 30, 80 28 / 29; 64 steps, 112 92 / 83, 96 81 / 82.
 constexpr uint32_t kStart = 4, kLeast = 3, kWhole = 6;  // (see Walker)
 constexpr uint32_t kMostLess = 4;  // by how many powers of two a step may be below a row's unit
 
