@@ -532,8 +532,10 @@ attention_decode_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
                             window[nt][j] = sees[nt][j] == kBlind ? 0u : seen_nodes(a, sees[nt][j], (int32_t)t0 - first_node(s)) & low_bits(limit - t0);
                             some |= window[nt][j];
                         }
-                    some |= __shfl_xor_sync(0xffffffffu, some, 1);
-                    some |= __shfl_xor_sync(0xffffffffu, some, 2);
+                    if (NF4) {
+                        some |= __shfl_xor_sync(0xffffffffu, some, 1);
+                        some |= __shfl_xor_sync(0xffffffffu, some, 2);
+                    }
                 }
                 #pragma unroll
                 for (uint32_t u = 0; u < G; ++u) {
